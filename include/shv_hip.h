@@ -131,6 +131,11 @@ enum {
     SHV_OP_ARGMAX_STATIC = 18, /* shv_argmax_static as an op, so that a recorded sequence can hold it */
     SHV_OP_ATTN_CELLS = 19,    /* shv_attn_decode_args: the rows' cells alone */
     SHV_OP_DN_PASS = 20,
+    SHV_OP_ATTN_TREE = 21,
+    SHV_OP_ATTN_KEEP = 22,
+    SHV_OP_DN_TREE = 23,
+    SHV_OP_DN_KEEP = 24,
+    SHV_OP_TREE_ACCEPT = 25,
     SHV_OP__COUNT
 };
 
@@ -566,6 +571,146 @@ typedef struct {
     int32_t hist_slots, reserved;
 } shv_dn_pass_args;
 
+/* ---- verification of a tree of drafted tokens --------------------------------------------------
+ * The reference verifies a chain of drafts (llm/spec.go:221-857).  Here a pass may carry several candidates a position: the
+ * rows of a sequence form a tree, row 0 the token the sequence goes on with and every other row one that may follow its parent.
+ *   parent [n_seq][rows]: the row each row follows, a lower one.  A parent that is not (-1 by custom) makes the row follow the
+ *     sequence's last kept token, as row 0 does; such a row is computed but never accepted.  NULL: a chain, parent[i] = i - 1.
+ *   count [n_seq]: rows in use, 0 .. rows; a larger number means rows, a negative one 0.  NULL: all.  Of rows past it nothing
+ *     is read and nothing is written.
+ *   pos, slot as in the other ops: sequence s has kept pos[s] tokens (NULL: none) and owns cache or state slot slot[s] (NULL: s).
+ * A row sits at position pos + its depth.  The pass itself changes neither cache, ring nor state: shv_attn_tree and shv_dn_tree
+ * leave beside their outputs what is needed to keep a branch, shv_tree_accept finds the branch, shv_attn_keep and
+ * shv_dn_keep (one call a layer) write it into cache, ring and state.  A call's sequences have different slots, all ops take
+ * 1 .. SHV_TREE_MAX_ROWS rows a sequence, and nothing an op writes may overlap anything it reads unless it is said to. */
+#define SHV_TREE_MAX_ROWS 64
+
+/* Gated full attention of a tree's rows over a sequence's cells and their own ancestors.  qkv rows, norms, rotary table and
+ * caches as shv_attn_decode has them, for head_dim 64, 128 or 256, any number of query heads per KV head up to 64, and any even
+ * rope_dims up to head_dim.  Row i sees cell c < pos and each row on its way to the root, itself included, and with window > 0
+ * only those of them whose position p is below sinks (the first tokens, which stay visible) or within the last `window`
+ * positions up to the row's own, position(i) - p < window.  Cells at pos and behind it are not looked at.
+ * kcells / vcells [n_seq][rows][n_head_kv][head_dim] binary16 receive each row's key (normed and rotated; formed in
+ * float64 and rounded through float32, so that it does not depend on the order of a sum) and value; a value beyond
+ * binary16's range becomes infinite there as in the cache, and reaches those rows that see its row and no others.  NaN and infinities in cells a row
+ * does not see never reach it.  out [n_seq][rows][n_head*head_dim], before the sigmoid gate.
+ * A sequence with pos < 0 or pos + rows in use > max_cells is left alone: nothing of it is written.
+ * partial: n_seq*rows*n_head*n_splits*(head_dim+2) floats of scratch; n_splits 1..512 is how many ways the cells may be split. */
+typedef struct {
+    const float *qkv;
+    const float *q_norm;
+    const float *k_norm;
+    const float *rope;       /* row p: cos[rope_dims/2] then sin[rope_dims/2], max_cells rows; may be NULL with rope_dims 0 */
+    const void *kcache;
+    const void *vcache;
+    void *kcells;
+    void *vcells;
+    float *partial;
+    float *out;
+    const int32_t *pos;
+    const int32_t *slot;
+    const int32_t *parent;
+    const int32_t *count;
+    int32_t n_seq, rows;
+    int32_t n_head, n_head_kv, head_dim, rope_dims;
+    int32_t max_cells, qkv_stride, n_splits;
+    int32_t window, sinks;
+    float eps;
+} shv_attn_tree_args;
+
+/* The kept branch's cells into a layer's cache: cell pos + j from row path[s][j] of kcells / vcells, for j < n_keep[s]
+ * (at most rows); a path entry that is no row (-1 by custom), and a cell outside the cache, are passed over. */
+typedef struct {
+    const void *kcells;
+    const void *vcells;
+    void *kcache;
+    void *vcache;
+    const int32_t *path;     /* [n_seq][rows] */
+    const int32_t *n_keep;   /* [n_seq] */
+    const int32_t *pos;
+    const int32_t *slot;
+    int32_t n_seq, rows;
+    int32_t n_head_kv, head_dim, max_cells;
+} shv_attn_keep_args;
+
+/* The gated delta rule of shv_dn_step over a tree's rows: a row's conv taps meet its ancestors (behind the root the ring's rows
+ * at pos-1, pos-2, pos-3, zeros before the sequence's start) and its state is its parent's, S_i = g_i S_parent + k_i delta_i^T with
+ * delta_i = beta_i (v_i - g_i S_parent^T k_i); out_i = S_i^T q_i / sqrt(d).  x [n_seq][rows] holds the fused projection rows (shv_dn_step's row
+ * layout), x_stride floats apart; ring [n_slots][ring_slots][ring_stride] holds the history and state [n_slots][n_planes][hv][d][d] the
+ * committed state in plane plane[slot] (n_planes 0 or 1, plane NULL: the only one; 0); both are only read.  No row's state is formed: the
+ * rows are solved together, (I + A) delta = B with A[i][j] = beta_i e^(G_i - G_j) (k_j . k_i) where j is an ancestor of i, G_i
+ * the sum of log g from the root to row i.
+ * Beside out [n_seq][rows][hv*d] the call leaves kn [n_seq][rows][hk*d] (the normed keys), delta [n_seq][rows][hv*d] and
+ * decay [n_seq][rows][hv] (G) for shv_dn_keep.  head_dim 128, conv 4, n_head_v a multiple of n_head_k, ring_slots >= 3. */
+typedef struct {
+    const float *x;
+    const float *ring;
+    const float *conv1d;
+    const float *a;
+    const float *dt_bias;
+    const float *state;
+    float *out;
+    float *kn;
+    float *delta;
+    float *decay;
+    const int32_t *pos;
+    const int32_t *slot;
+    const int32_t *plane;
+    const int32_t *parent;
+    const int32_t *count;
+    int32_t n_seq, rows;
+    int32_t n_head_k, n_head_v, head_dim, conv;
+    int32_t x_stride, ring_slots, ring_stride;
+    int32_t n_planes, qk_norm_max;
+    float eps;
+} shv_dn_tree_args;
+
+/* The state behind the kept branch, S' = e^(G_last) S + sum_j e^(G_last - G_j) k_j delta_j^T over the rows path[s][0 .. n_keep[s]), from what
+ * shv_dn_tree left, into plane (plane[slot] + 1) % n_planes (in place with n_planes 0 or 1; with n_keep 0 the state as it is), and the conv
+ * channels (2*hk*d + hv*d floats) of its last three rows from x into the ring's rows at their positions.  With planes the
+ * caller makes the new one the committed one, plane[slot] = (plane[slot] + 1) % n_planes.  n_keep counts at most rows; path entries that
+ * are no row are passed over. */
+typedef struct {
+    const float *x;
+    const float *kn;
+    const float *delta;
+    const float *decay;
+    float *state;
+    float *ring;
+    const int32_t *path;
+    const int32_t *n_keep;
+    const int32_t *pos;
+    const int32_t *slot;
+    const int32_t *plane;
+    int32_t n_seq, rows;
+    int32_t n_head_k, n_head_v, head_dim, conv;
+    int32_t x_stride, ring_slots, ring_stride;
+    int32_t n_planes;
+} shv_dn_keep_args;
+
+/* The branch the model agrees with: best [n_seq][rows] receives each row's arg-max over logits [n_seq*rows][n] (logits_stride
+ * floats apart; shv_argmax's order: first maximum, NaN never wins), then from row 0 on the walk goes to the child whose id is the best of the
+ * row it stands on, the lowest such row if there are several, until there is none.  path [n_seq][rows] receives the rows of the way, -1
+ * behind them, n_keep [n_seq] their number, next [n_seq] the best of the last: the token after the branch.  logits NULL: best is read
+ * instead (tokens the caller drew for each row).  With count 0 n_keep is 0 and next -1.  ids [n_seq][rows] are the rows' tokens.
+ * pos and base (both or neither; [n_seq]): base receives pos and pos moves on by n_keep, so that what keeps the branch takes base for its
+ * pos and the next pass finds pos where it belongs.  At most SHV_TREE_ACCEPT_MAX_ROWS rows and 1024 sequences a call. */
+#define SHV_TREE_ACCEPT_MAX_ROWS 16384
+typedef struct {
+    const float *logits;
+    const int32_t *ids;
+    const int32_t *parent;
+    const int32_t *count;
+    int32_t *best;
+    int32_t *path;
+    int32_t *n_keep;
+    int32_t *next;
+    int32_t *pos;
+    int32_t *base;
+    int32_t n_seq, rows;
+    int32_t n, logits_stride;
+} shv_tree_accept_args;
+
 typedef struct {
     uint32_t kind;
     uint32_t flags;          /* bit 0: may overlap the previous op (MultiDispatch.Overlap) */
@@ -617,6 +762,11 @@ int shv_advance(shv_ctx *ctx, const shv_advance_args *a);
 int shv_ring_rows(shv_ctx *ctx, const shv_ring_rows_args *a);
 int shv_router_fold(shv_ctx *ctx, const shv_router_fold_args *a);
 int shv_qsa_index(shv_ctx *ctx, const shv_qsa_index_args *a);
+int shv_attn_tree(shv_ctx *ctx, const shv_attn_tree_args *a);
+int shv_attn_keep(shv_ctx *ctx, const shv_attn_keep_args *a);
+int shv_dn_tree(shv_ctx *ctx, const shv_dn_tree_args *a);
+int shv_dn_keep(shv_ctx *ctx, const shv_dn_keep_args *a);
+int shv_tree_accept(shv_ctx *ctx, const shv_tree_accept_args *a);
 
 /* shv_argmax for callers that cannot allocate (code under HIP graph capture, tight serving loops,
  * harnesses that forbid hipMalloc).  No counterpart in the reference.  Same arguments and

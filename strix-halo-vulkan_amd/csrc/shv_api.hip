@@ -83,6 +83,10 @@ int shv_init(int device, shv_ctx **out) {
     if (e == hipSuccess) e = hipMalloc(reinterpret_cast<void **>(&ctx->gemm_part), shv_ctx::kGemmPartBytes);
     if (e == hipSuccess) e = hipMalloc(reinterpret_cast<void **>(&ctx->argmax_val), shv_ctx::kArgmaxBlocks * sizeof(float));
     if (e == hipSuccess) e = hipMalloc(reinterpret_cast<void **>(&ctx->argmax_idx), shv_ctx::kArgmaxBlocks * sizeof(int32_t));
+    if (e == hipSuccess) e = hipMalloc(reinterpret_cast<void **>(&ctx->tree_val), shv_ctx::kTreePairs * sizeof(float));
+    if (e == hipSuccess) e = hipMalloc(reinterpret_cast<void **>(&ctx->tree_idx), shv_ctx::kTreePairs * sizeof(int32_t));
+    if (e == hipSuccess) e = hipMalloc(reinterpret_cast<void **>(&ctx->tree_counters), shv_ctx::kTreeSeqs * shv_ctx::kTreeCounterStep * sizeof(int32_t));
+    if (e == hipSuccess) e = hipMemset(ctx->tree_counters, 0, shv_ctx::kTreeSeqs * shv_ctx::kTreeCounterStep * sizeof(int32_t));
     if (e == hipSuccess) e = hipMalloc(reinterpret_cast<void **>(&ctx->gemv_amax_val), shv_ctx::kGemvAmaxBlocks * sizeof(float));
     if (e == hipSuccess) e = hipMalloc(reinterpret_cast<void **>(&ctx->gemv_amax_idx), shv_ctx::kGemvAmaxBlocks * sizeof(int32_t));
     if (e != hipSuccess) {
@@ -115,6 +119,9 @@ void shv_destroy(shv_ctx *ctx) {
     if (ctx->gemm_part) (void)hipFree(ctx->gemm_part);
     if (ctx->argmax_val) (void)hipFree(ctx->argmax_val);
     if (ctx->argmax_idx) (void)hipFree(ctx->argmax_idx);
+    if (ctx->tree_val) (void)hipFree(ctx->tree_val);
+    if (ctx->tree_idx) (void)hipFree(ctx->tree_idx);
+    if (ctx->tree_counters) (void)hipFree(ctx->tree_counters);
     if (ctx->gemv_amax_val) (void)hipFree(ctx->gemv_amax_val);
     if (ctx->gemv_amax_idx) (void)hipFree(ctx->gemv_amax_idx);
     if (ctx->up_ring) (void)hipHostFree(ctx->up_ring);
@@ -310,6 +317,11 @@ static int dispatch_one(shv_ctx *ctx, uint32_t kind, const void *args, size_t by
         case SHV_OP_ROUTER_FOLD: return run_as<shv_router_fold_args>(ctx, args, bytes, shv_launch_router_fold, "router_fold");
         case SHV_OP_QSA_INDEX: return run_as<shv_qsa_index_args>(ctx, args, bytes, shv_launch_qsa_index, "qsa_index");
         case SHV_OP_ARGMAX_STATIC: return run_as<shv_argmax_args>(ctx, args, bytes, shv_launch_argmax_static, "argmax_static");
+        case SHV_OP_ATTN_TREE: return run_as<shv_attn_tree_args>(ctx, args, bytes, shv_launch_attn_tree, "attn_tree");
+        case SHV_OP_ATTN_KEEP: return run_as<shv_attn_keep_args>(ctx, args, bytes, shv_launch_attn_keep, "attn_keep");
+        case SHV_OP_DN_TREE: return run_as<shv_dn_tree_args>(ctx, args, bytes, shv_launch_dn_tree, "dn_tree");
+        case SHV_OP_DN_KEEP: return run_as<shv_dn_keep_args>(ctx, args, bytes, shv_launch_dn_keep, "dn_keep");
+        case SHV_OP_TREE_ACCEPT: return run_as<shv_tree_accept_args>(ctx, args, bytes, shv_launch_tree_accept, "tree_accept");
         default: return shv_set_error(SHV_E_INVALID, "shv_enqueue: unknown op kind %u", kind);
     }
 }
@@ -488,6 +500,11 @@ int shv_advance(shv_ctx *ctx, const shv_advance_args *a) { return dispatch_one(c
 int shv_ring_rows(shv_ctx *ctx, const shv_ring_rows_args *a) { return dispatch_one(ctx, SHV_OP_RING_ROWS, a, sizeof(*a)); }
 int shv_router_fold(shv_ctx *ctx, const shv_router_fold_args *a) { return dispatch_one(ctx, SHV_OP_ROUTER_FOLD, a, sizeof(*a)); }
 int shv_qsa_index(shv_ctx *ctx, const shv_qsa_index_args *a) { return dispatch_one(ctx, SHV_OP_QSA_INDEX, a, sizeof(*a)); }
+int shv_attn_tree(shv_ctx *ctx, const shv_attn_tree_args *a) { return dispatch_one(ctx, SHV_OP_ATTN_TREE, a, sizeof(*a)); }
+int shv_attn_keep(shv_ctx *ctx, const shv_attn_keep_args *a) { return dispatch_one(ctx, SHV_OP_ATTN_KEEP, a, sizeof(*a)); }
+int shv_dn_tree(shv_ctx *ctx, const shv_dn_tree_args *a) { return dispatch_one(ctx, SHV_OP_DN_TREE, a, sizeof(*a)); }
+int shv_dn_keep(shv_ctx *ctx, const shv_dn_keep_args *a) { return dispatch_one(ctx, SHV_OP_DN_KEEP, a, sizeof(*a)); }
+int shv_tree_accept(shv_ctx *ctx, const shv_tree_accept_args *a) { return dispatch_one(ctx, SHV_OP_TREE_ACCEPT, a, sizeof(*a)); }
 
 int shv_argmax_static(shv_ctx *ctx, const shv_argmax_args *a) {
     SHV_REQUIRE(ctx && a, "shv_argmax_static: NULL argument");

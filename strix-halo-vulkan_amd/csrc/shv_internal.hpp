@@ -79,6 +79,11 @@ struct shv_ctx {
     float *gemv_amax_val = nullptr;
     int32_t *gemv_amax_idx = nullptr;
     enum { kGemvAmaxBlocks = 2048 };
+    // per-block (value, index) pairs of a tree's rows, and the arrival counters of its sequences, a line apart (tree_accept)
+    float *tree_val = nullptr;
+    int32_t *tree_idx = nullptr;
+    int32_t *tree_counters = nullptr;
+    enum { kTreePairs = SHV_TREE_ACCEPT_MAX_ROWS, kTreeSeqs = 1024, kTreeCounterStep = 32 };
     // device address of this GPU's copy of the library's static scratch array (misc.hip), for the
     // entry point that allocates nothing
     void *static_scratch = nullptr;
@@ -213,6 +218,12 @@ int shv_launch_advance(shv_ctx *ctx, const shv_advance_args *a);
 int shv_launch_ring_rows(shv_ctx *ctx, const shv_ring_rows_args *a);
 int shv_launch_router_fold(shv_ctx *ctx, const shv_router_fold_args *a);
 int shv_launch_qsa_index(shv_ctx *ctx, const shv_qsa_index_args *a);
+// verification of a tree of drafted tokens (attn_tree.hip, dn_tree.hip, tree_accept.hip)
+int shv_launch_attn_tree(shv_ctx *ctx, const shv_attn_tree_args *a);
+int shv_launch_attn_keep(shv_ctx *ctx, const shv_attn_keep_args *a);
+int shv_launch_dn_tree(shv_ctx *ctx, const shv_dn_tree_args *a);
+int shv_launch_dn_keep(shv_ctx *ctx, const shv_dn_keep_args *a);
+int shv_launch_tree_accept(shv_ctx *ctx, const shv_tree_accept_args *a);
 bool shv_dn_chunk_covers(const shv_dn_step_args &a);
 int shv_launch_dn_chunk(shv_ctx *ctx, const shv_dn_step_args &a, float *hist, int hist_slots);
 int shv_launch_copy_spans(shv_ctx *ctx, const shv_span *spans, int n);

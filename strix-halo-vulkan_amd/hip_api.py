@@ -12,6 +12,8 @@ OP_GEMV_Q4K, OP_DEQUANT_Q4K, OP_QUANTIZE_Q4K, OP_FILL_NORMAL = 1, 2, 3, 4
 OP_MOE_ROUTER, OP_MOE_UP, OP_MOE_DOWN, OP_DN_STEP, OP_ATTN_DECODE = 5, 6, 7, 8, 9
 OP_EMBED, OP_ARGMAX, OP_ADVANCE, OP_DEQUANT, OP_GEMV, OP_RING_ROWS, OP_ROUTER_FOLD, OP_QSA_INDEX = 10, 11, 12, 13, 14, 15, 16, 17
 OP_ARGMAX_STATIC, OP_ATTN_CELLS, OP_DN_PASS = 18, 19, 20
+OP_ATTN_TREE, OP_ATTN_KEEP, OP_DN_TREE, OP_DN_KEEP, OP_TREE_ACCEPT = 21, 22, 23, 24, 25
+TREE_MAX_ROWS, TREE_ACCEPT_MAX_ROWS = 64, 16384
 PRO_NONE, PRO_RMSNORM, PRO_GATED_NORM, PRO_MUL_SIGMOID, PRO_RMSNORM_PAIR = 0, 1, 2, 3, 4
 
 
@@ -132,6 +134,44 @@ class QsaIndexArgs(C.Structure):
                 ("rope_dims", C.c_int32), ("max_cells", C.c_int32), ("mask_stride", C.c_int32), ("eps", C.c_float)]
 
 
+class AttnTreeArgs(C.Structure):
+    _fields_ = [("qkv", C.c_void_p), ("q_norm", C.c_void_p), ("k_norm", C.c_void_p), ("rope", C.c_void_p), ("kcache", C.c_void_p),
+                ("vcache", C.c_void_p), ("kcells", C.c_void_p), ("vcells", C.c_void_p), ("partial", C.c_void_p), ("out", C.c_void_p),
+                ("pos", C.c_void_p), ("slot", C.c_void_p), ("parent", C.c_void_p), ("count", C.c_void_p), ("n_seq", C.c_int32),
+                ("rows", C.c_int32), ("n_head", C.c_int32), ("n_head_kv", C.c_int32), ("head_dim", C.c_int32), ("rope_dims", C.c_int32),
+                ("max_cells", C.c_int32), ("qkv_stride", C.c_int32), ("n_splits", C.c_int32), ("window", C.c_int32), ("sinks", C.c_int32),
+                ("eps", C.c_float)]
+
+
+class AttnKeepArgs(C.Structure):
+    _fields_ = [("kcells", C.c_void_p), ("vcells", C.c_void_p), ("kcache", C.c_void_p), ("vcache", C.c_void_p), ("path", C.c_void_p),
+                ("n_keep", C.c_void_p), ("pos", C.c_void_p), ("slot", C.c_void_p), ("n_seq", C.c_int32), ("rows", C.c_int32),
+                ("n_head_kv", C.c_int32), ("head_dim", C.c_int32), ("max_cells", C.c_int32)]
+
+
+class DnTreeArgs(C.Structure):
+    _fields_ = [("x", C.c_void_p), ("ring", C.c_void_p), ("conv1d", C.c_void_p), ("a", C.c_void_p), ("dt_bias", C.c_void_p),
+                ("state", C.c_void_p), ("out", C.c_void_p), ("kn", C.c_void_p), ("delta", C.c_void_p), ("decay", C.c_void_p),
+                ("pos", C.c_void_p), ("slot", C.c_void_p), ("plane", C.c_void_p), ("parent", C.c_void_p), ("count", C.c_void_p),
+                ("n_seq", C.c_int32), ("rows", C.c_int32), ("n_head_k", C.c_int32), ("n_head_v", C.c_int32), ("head_dim", C.c_int32),
+                ("conv", C.c_int32), ("x_stride", C.c_int32), ("ring_slots", C.c_int32), ("ring_stride", C.c_int32), ("n_planes", C.c_int32),
+                ("qk_norm_max", C.c_int32), ("eps", C.c_float)]
+
+
+class DnKeepArgs(C.Structure):
+    _fields_ = [("x", C.c_void_p), ("kn", C.c_void_p), ("delta", C.c_void_p), ("decay", C.c_void_p), ("state", C.c_void_p),
+                ("ring", C.c_void_p), ("path", C.c_void_p), ("n_keep", C.c_void_p), ("pos", C.c_void_p), ("slot", C.c_void_p),
+                ("plane", C.c_void_p), ("n_seq", C.c_int32), ("rows", C.c_int32), ("n_head_k", C.c_int32), ("n_head_v", C.c_int32),
+                ("head_dim", C.c_int32), ("conv", C.c_int32), ("x_stride", C.c_int32), ("ring_slots", C.c_int32), ("ring_stride", C.c_int32),
+                ("n_planes", C.c_int32)]
+
+
+class TreeAcceptArgs(C.Structure):
+    _fields_ = [("logits", C.c_void_p), ("ids", C.c_void_p), ("parent", C.c_void_p), ("count", C.c_void_p), ("best", C.c_void_p),
+                ("path", C.c_void_p), ("n_keep", C.c_void_p), ("next", C.c_void_p), ("pos", C.c_void_p), ("base", C.c_void_p),
+                ("n_seq", C.c_int32), ("rows", C.c_int32), ("n", C.c_int32), ("logits_stride", C.c_int32)]
+
+
 class EmbedArgs(C.Structure):
     _fields_ = [("table", C.c_void_p), ("ids", C.c_void_p), ("pos", C.c_void_p), ("x", C.c_void_p),
                 ("n_tok", C.c_int32), ("n_embd", C.c_int32), ("vocab", C.c_int32),
@@ -184,6 +224,7 @@ SYMBOLS = [
     "shv_prerecorded_destroy", "shv_gemv_q4k", "shv_dequant_q4k", "shv_dequant", "shv_gemv", "shv_quantize_q4k",
     "shv_fill_normal", "shv_moe_router", "shv_moe_up", "shv_moe_down", "shv_dn_step", "shv_dn_pass", "shv_attn_decode", "shv_embed", "shv_argmax", "shv_advance",
     "shv_argmax_static", "shv_ring_rows", "shv_router_fold", "shv_qsa_index",
+    "shv_attn_tree", "shv_attn_keep", "shv_dn_tree", "shv_dn_keep", "shv_tree_accept",
 ]
 
 _lib = None
@@ -251,6 +292,11 @@ def load():
     L.shv_ring_rows.argtypes = [vp, C.POINTER(RingRowsArgs)]
     L.shv_router_fold.argtypes = [vp, C.POINTER(RouterFoldArgs)]
     L.shv_qsa_index.argtypes = [vp, C.POINTER(QsaIndexArgs)]
+    L.shv_attn_tree.argtypes = [vp, C.POINTER(AttnTreeArgs)]
+    L.shv_attn_keep.argtypes = [vp, C.POINTER(AttnKeepArgs)]
+    L.shv_dn_tree.argtypes = [vp, C.POINTER(DnTreeArgs)]
+    L.shv_dn_keep.argtypes = [vp, C.POINTER(DnKeepArgs)]
+    L.shv_tree_accept.argtypes = [vp, C.POINTER(TreeAcceptArgs)]
     _lib = L
     return L
 

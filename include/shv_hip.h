@@ -586,8 +586,8 @@ typedef struct {
 #define SHV_TREE_MAX_ROWS 64
 
 /* Gated full attention of a tree's rows over a sequence's cells and their own ancestors.  qkv rows, norms, rotary table and
- * caches as shv_attn_decode has them, for head_dim 64, 128 or 256, any number of query heads per KV head up to 64, and any even
- * rope_dims up to head_dim.  Row i sees cell c < pos and each row on its way to the root, itself included, and with window > 0
+ * caches as shv_attn_decode has them, for head_dim 64, 128 or 256, any number of query heads per KV head up to 64, and rope_dims
+ * any multiple of head_dim / 32 up to head_dim.  Row i sees cell c < pos and each row on its way to the root, itself included, and with window > 0
  * only those of them whose position p is below sinks (the first tokens, which stay visible) or within the last `window`
  * positions up to the row's own, position(i) - p < window.  Cells at pos and behind it are not looked at.
  * kcells / vcells [n_seq][rows][n_head_kv][head_dim] binary16 receive each row's key (normed and rotated; formed in

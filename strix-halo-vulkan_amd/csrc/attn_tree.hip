@@ -17,10 +17,30 @@ constexpr int kMaxSplits = 512;
 __device__ __forceinline__ bool fits(int pos, int n, int max_cells) { return n > 0 && pos >= 0 && pos <= max_cells - n; }
 
 // Sum over a wave, in every lane.
+template <int CTRL, int ROW_MASK = 0xF>
+__device__ __forceinline__ double dpp_f64(double v) {
+    const uint64_t b = __builtin_bit_cast(uint64_t, v);
+    const uint32_t lo = __builtin_amdgcn_update_dpp(0, static_cast<int>(b), CTRL, ROW_MASK, 0xF, false);
+    const uint32_t hi = __builtin_amdgcn_update_dpp(0, static_cast<int>(b >> 32), CTRL, ROW_MASK, 0xF, false);
+    return __builtin_bit_cast(double, static_cast<uint64_t>(hi) << 32 | lo);
+}
 __device__ __forceinline__ double wave_sum_f64(double v) {
-#pragma unroll
-    for (int off = 32; off >= 1; off >>= 1) v += __shfl_xor(v, off, 64);
-    return v;
+    v += dpp_f64<kDppXor1>(v);
+    v += dpp_f64<kDppXor2>(v);
+    v += dpp_f64<kDppHalfMirror>(v);
+    v += dpp_f64<kDppMirror>(v);
+    v += dpp_f64<kDppBcast15, 0xA>(v);
+    v += dpp_f64<kDppBcast31, 0xC>(v);
+    const uint64_t b = __builtin_bit_cast(uint64_t, v);
+    const uint32_t lo = __builtin_amdgcn_readlane(static_cast<int>(b), 63), hi = __builtin_amdgcn_readlane(static_cast<int>(b >> 32), 63);
+    return __builtin_bit_cast(double, static_cast<uint64_t>(hi) << 32 | lo);
+}
+// 1 / sqrt(x) to the last places: the instruction's estimate and two Newton steps (of 0 and infinity the estimate is the result).
+__device__ __forceinline__ double rsqrt_f64(double x) {
+    const double e = __builtin_amdgcn_rsq(x);
+    double y = fma(e * 0.5, fma(-x * e, e, 1.0), e);
+    y = fma(y * 0.5, fma(-x * y, y, 1.0), y);
+    return x == 0.0 || x == static_cast<double>(INFINITY) ? e : y;
 }
 
 // A cell's value in binary16, by way of float32 (the compiler would fold the two conversions into one).
@@ -31,11 +51,16 @@ __device__ __forceinline__ __half cell_value(double v) {
 }
 
 typedef _Float16 half8_t __attribute__((ext_vector_type(8)));
+typedef _Float16 half2_t __attribute__((ext_vector_type(2)));
 typedef float float4_t __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) void *lds_ptr_t;
 
 constexpr int kChunk = 64 * 16;
 constexpr int kStages = 4, kAhead = kStages - 1;
+// Weights are e^(s - m) 2^kLift, and m stands until a score is more than 2^kSlack above it: up to 2^15, which the larger half holds, and down to
+// 2^-31 of the largest with the smaller half's last place (at a lift of 0 2^-24, 6e-6 of a weight of a hundredth).
+constexpr float kLift = 7.f, kSlack = 8.f;
+constexpr int kMergeMany = 1024;  // 64-dim pieces of rows and heads from which one wave joins the slices of each
 constexpr int kMinTiles = 4;  // tiles a slice gets at least
 
 // Which tiles of 32 cells a sequence's rows look at: the sinks', then those the window of the first row reaches.
@@ -53,34 +78,43 @@ struct Tiles {
     __device__ __forceinline__ int at(int i) const { return i < sinks ? i : i - sinks + first; }
 };
 
+// What the launcher works out once.
+struct Plan {
+    int q_blocks;        // blocks that share a slice, 16 query rows a wave
+    int slots;           // slices of the cache that all sequences have together: as many blocks as the chip holds at once
+    uint32_t rep_magic;  // r / rep = r * rep_magic >> 20 for r < 4096 and rep <= 64: off by less than r / 2^20 <= 1 / 256 before it is cut
+};
+__device__ __forceinline__ int over_rep(const Plan &plan, int r) { return static_cast<int>(static_cast<uint32_t>(r) * plan.rep_magic >> 20); }
+
 // How a call's sequences are cut: slices of `len` tiles as many as the call has blocks for, and behind them one for the rows
 // themselves; where a call has one slice, it holds both.
 struct Cut {
     int len, cache, all;  // tiles of a slice, slices of the cache, slices
     __device__ __forceinline__ Cut(const shv_attn_tree_args &a, int tiles, int slots, int lane) {
-        long long total = 0;
-        for (int s0 = 0; s0 < a.n_seq; s0 += 64) {
-            const int s = s0 + lane;
-            int t = 0;
-            if (s < a.n_seq) {
-                const int pos = a.pos ? a.pos[s] : 0;
-                const int n = tree_rows(a.count, s, a.rows);
-                t = fits(pos, n, a.max_cells) ? Tiles(a, pos).all : 0;
-            }
-            int sum = t;
-#pragma unroll
-            for (int off = 32; off >= 1; off >>= 1) sum += __shfl_xor(sum, off, 64);
-            total += sum;
-        }
         if (a.n_splits == 1) {
             len = tiles;
             cache = 0;
             all = 1;
             return;
         }
-        len = max(kMinTiles, static_cast<int>((total + slots - 1) / slots));
-        len = max(len, (tiles + a.n_splits - 2) / (a.n_splits - 1));
-        cache = (tiles + len - 1) / len;
+        uint32_t total = tiles;
+        if (a.n_seq > 1) {
+            total = 0;
+            for (int s0 = 0; s0 < a.n_seq; s0 += 64) {
+                const int s = min(s0 + lane, a.n_seq - 1);
+                const int pos = a.pos ? a.pos[s] : 0;
+                uint32_t sum = s0 + lane < a.n_seq && fits(pos, tree_rows(a.count, s, a.rows), a.max_cells) ? Tiles(a, pos).all : 0;
+#pragma unroll
+                for (int off = 32; off >= 1; off >>= 1) sum += __shfl_xor(sum, off, 64);
+                total = min(total + sum, 1u << 30);  // (64 sequences have at most 2^32 / 2^6 tiles)
+            }
+        }
+        total = __builtin_amdgcn_readfirstlane(total);
+        const uint32_t share = (total + slots - 1) / slots, room = a.n_splits - 1;
+        uint32_t l = share > kMinTiles ? share : kMinTiles;
+        if (l * static_cast<uint64_t>(room) < static_cast<uint32_t>(tiles)) l = (tiles + room - 1) / room;
+        len = l;
+        cache = (tiles + l - 1) / l;
         all = cache + 1;
     }
 };
@@ -102,32 +136,31 @@ struct Row {  // a lane's dims of one head's row: VEC * lane ..
     }
 };
 
-// The rotary factors of a lane's dims, of a position.
+// The rotation of a lane's dims at a position, x' = x c + other s: of a pair the first is x0 cos - x1 sin, the second x1 cos + x0 sin, and
+// a dim that does not turn has c = 1, s = 0.  (Lanes without a rotated dim read the first's factors: no branch around loads.)
 template <int D>
 struct Turn {
     static constexpr int VEC = D / 64;
-    float c[VEC], s[VEC];
-    int partner;
+    Row<D> c, s;
+    int partner, at;
     bool turns, first;
     __device__ __forceinline__ Turn(int rope_dims, int lane) {
         const int half = rope_dims / 2, e = VEC * lane;
         turns = e < rope_dims;
         first = e < half;
-        partner = !turns ? lane : first ? lane + half / VEC : lane - half / VEC;
+        at = !turns ? 0 : first ? lane : lane - half / VEC;
+        partner = !turns ? lane : first ? lane + half / VEC : at;
     }
-    __device__ __forceinline__ void load(const float *table, int rope_dims, int lane) {
-        const int half = rope_dims / 2, e = VEC * lane;
+    __device__ __forceinline__ void load(const float *table, int rope_dims) {
+        c.load(table, at);
+        s.load(table + rope_dims / 2, at);
+    }
+    __device__ __forceinline__ void settle() {
 #pragma unroll
         for (int v = 0; v < VEC; v++) {
-            c[v] = turns ? table[(first ? e : e - half) + v] : 1.f;
-            s[v] = turns ? table[(first ? e + half : e) + v] : 0.f;
+            c.x[v] = turns ? c.x[v] : 1.f;
+            s.x[v] = turns ? (first ? -s.x[v] : s.x[v]) : 0.f;
         }
-    }
-    template <typename T>
-    __device__ __forceinline__ T of(T x, T other, int v) const {
-        // first of the pair: x0' = x0 cos - x1 sin; second: x1' = x0 sin + x1 cos
-        const T r = first ? x * static_cast<T>(c[v]) - other * static_cast<T>(s[v]) : other * static_cast<T>(s[v]) + x * static_cast<T>(c[v]);
-        return turns ? r : x;
     }
 };
 
@@ -144,6 +177,20 @@ __device__ __forceinline__ int v_byte(int cell, int dim) {
     return (D / 16 + (dim >> 4)) * kChunk + (16 * (cell >> 3) + (dim & 15)) * 16 + (cell & 7) * 2;
 }
 
+// Largest and sum over the four lanes (n, 0..3) that share a query row.
+__device__ __forceinline__ float max_over_q(float v) {
+    auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+    r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float sum_over_q(float v) {
+    auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+    r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+
 template <int N>
 __device__ __forceinline__ void wait_loads() { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory"); }
 
@@ -156,7 +203,7 @@ struct TreeSmem {
 // grid: (slices rounded up to 8, times query blocks; n_head_kv; n_seq), W waves.  A wave holds 16 query rows: query row r of a KV head is
 // head r % rep of tree row r / rep.
 template <int D, int W>
-__global__ __launch_bounds__(64 * W, D == 256 ? 2 : 4) void tree_attn_kernel(shv_attn_tree_args a, int q_blocks, int slots) {
+__global__ __launch_bounds__(64 * W, D == 256 ? 2 : 4) void tree_attn_kernel(shv_attn_tree_args a, Plan plan) {
     constexpr int VEC = D / 64, KI = D / 32, DB = D / 16;
     constexpr int kPer = D / 8 / W;  // chunks of a tile a wave asks for
     extern __shared__ __align__(16) char raw[];
@@ -164,14 +211,32 @@ __global__ __launch_bounds__(64 * W, D == 256 ? 2 : 4) void tree_attn_kernel(shv
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int n = lane & 15, q = lane >> 4;
     // blocks of one slice lie on one die (workgroups go to the dies in turn) and find its tiles in the die's L2
-    const int split = blockIdx.x / (8 * q_blocks) * 8 + (blockIdx.x & 7), qb = blockIdx.x / 8 % q_blocks;
+    const int group = blockIdx.x >> 3, of_group = static_cast<int>(static_cast<uint32_t>(group) / static_cast<uint32_t>(plan.q_blocks));
+    const int split = of_group * 8 + (blockIdx.x & 7), qb = group - of_group * plan.q_blocks;
     const int kvh = blockIdx.y, seq = blockIdx.z;
     const int rep = a.n_head / a.n_head_kv;
-    const int slot = a.slot ? a.slot[seq] : seq, pos = a.pos ? a.pos[seq] : 0;
-    const TreeRow t = tree_row(a.parent, a.count, seq, a.rows, lane);
-    if (!fits(pos, t.n, a.max_cells) || qb * W * 16 >= t.n * rep) return;
+    const TreeWords words(a.count, a.pos, a.slot, a.parent, a.q_norm, seq, a.rows, lane);
+    // ---- what depends on nothing: the first query rows this wave prepares.  Four waves share the rows of all of them (there are at most four
+    //      groups of 16, often one), four rows of a group each; eight take their own group's ----
+    constexpr bool kShared = W == 4;
+    const int fours = kShared ? (a.rows * rep + 15) / 16 : 4;  // of rows the wave prepares
+    const auto row_of = [&](int f, int u) { return kShared ? 16 * f + 4 * u + wave : (qb * W + wave) * 16 + 4 * f + u; };
+    const float *qkv = a.qkv + static_cast<size_t>(seq) * a.rows * a.qkv_stride;
+    const auto load_four = [&](Row<D>(&x)[4], int f) {
+#pragma unroll
+        for (int u = 0; u < 4; u++) {
+            const int r = min(row_of(f, u), a.rows * rep - 1), tr = over_rep(plan, r);  // (rows past the last repeat it and are dropped)
+            x[u].load(qkv + static_cast<size_t>(tr) * a.qkv_stride + static_cast<size_t>(kvh * rep + r - tr * rep) * 2 * D, lane);
+        }
+    };
+    Row<D> qx[4];
+    load_four(qx, 0);
+    Row<D> gq;
+    gq.load(a.q_norm, lane);
+    const int slot = words.slot, pos = __builtin_amdgcn_readfirstlane(words.pos), rows = __builtin_amdgcn_readfirstlane(words.count);
+    if (!fits(pos, rows, a.max_cells) || qb * W * 16 >= rows * rep) return;
     const Tiles tiles(a, pos);
-    const Cut cut(a, tiles.all, slots, lane);
+    const Cut cut(a, tiles.all, plan.slots, lane);
     if (split >= cut.all) return;
     const bool with_rows = split == cut.all - 1;
     const int t0 = with_rows && cut.all > 1 ? 0 : split * cut.len;
@@ -180,18 +245,6 @@ __global__ __launch_bounds__(64 * W, D == 256 ? 2 : 4) void tree_attn_kernel(shv
     const size_t kvw = static_cast<size_t>(a.n_head_kv) * D;
     const uint16_t *kc = static_cast<const uint16_t *>(a.kcache) + static_cast<size_t>(slot) * a.max_cells * kvw + kvh * D;
     const uint16_t *vc = static_cast<const uint16_t *>(a.vcache) + static_cast<size_t>(slot) * a.max_cells * kvw + static_cast<size_t>(kvh) * D * kTile;
-
-    // ---- the wave's query rows are asked for, then the first two tiles ----
-    const int r0 = (qb * W + wave) * 16, r_end = t.n * rep;  // rows past the last repeat it and are dropped
-    Row<D> qx[16];
-    const float *qkv = a.qkv + static_cast<size_t>(seq) * a.rows * a.qkv_stride;
-#pragma unroll
-    for (int i = 0; i < 16; i++) {
-        const int r = min(r0 + i, r_end - 1), tr = r / rep;
-        qx[i].load(qkv + static_cast<size_t>(tr) * a.qkv_stride + static_cast<size_t>(kvh * rep + r - tr * rep) * 2 * D, lane);
-    }
-    Row<D> gq;
-    gq.load(a.q_norm, lane);
     const bool keys = wave < W / 2;
     const int first = (keys ? wave : wave - W / 2) * kPer;  // of the wave's chunks among K's or V's
     const uint32_t from = keys ? static_cast<uint32_t>((8 * (n >> 2) + 4 * (first / KI) + (n & 3)) * kvw + 32 * (first % KI) + 8 * q) * 2
@@ -204,66 +257,132 @@ __global__ __launch_bounds__(64 * W, D == 256 ? 2 : 4) void tree_attn_kernel(shv
         for (int u = 0; u < kPer; u++)
             __builtin_amdgcn_raw_ptr_buffer_load_lds(bytes, (lds_ptr_t)(to + u * kChunk), 16, from, u * (keys ? 64 : 1024), 0, 0);
     };
-    if (t0 < t1) ask(t0);
-    if (t0 + 1 < t1) ask(t0 + 1);
-
-    // ---- queries: norm, rotation, operand order by way of the last two stages, half of the dims at a time ----
-    half8_t qh[KI], ql[KI];
-    {
-        const Turn<D> shape(a.rope_dims, lane);
+    if (!with_rows) {
+        ask(t0);
+        if (t0 + 1 < t1) ask(t0 + 1);
+    }
+    const TreeRow t = tree_row(rows, words.parent, a.rows, lane);
+    const Turn<D> shape(a.rope_dims, lane);
+    const int n_own = with_rows ? (rows + kTile - 1) / kTile : 0;  // tiles of the rows' own cells
+    if (with_rows) {
+        // ---- the rows' own cells: normed, rotated and rounded into the first two stages, and left for whoever keeps them ----
+        if (rows % kTile != 0) {
+            // behind the last row the second product wants something finite
+            uint4 *v = reinterpret_cast<uint4 *>(sm.ring[n_own - 1] + 2 * KI * kChunk);
+            for (int i = tid; i < DB * 64; i += 64 * W) v[i] = make_uint4(0, 0, 0, 0);
+            __syncthreads();
+        }
+        Row<D> gk, k, val;
+        gk.load(a.k_norm, lane);
         Turn<D> turn = shape;
-        int at_row = -1;
+        const auto load = [&](int j) {
+            const float *src = qkv + static_cast<size_t>(j) * a.qkv_stride + static_cast<size_t>(a.n_head) * 2 * D + kvh * D;
+            k.load(src, lane);
+            val.load(src + kvw, lane);
+            if (a.rope_dims > 0) turn.load(a.rope + static_cast<size_t>(pos + __builtin_amdgcn_readlane(t.depth, j)) * a.rope_dims, a.rope_dims);
+        };
+        if (wave < rows) load(wave);
+        for (int j = wave; j < rows; j += W) {
+            if (a.rope_dims > 0) turn.settle();
+            uint16_t kx[VEC], vx[VEC];
+            double ss = 0;
 #pragma unroll
-        for (int i = 0; i < 16; i++) {
-            const int r = min(r0 + i, r_end - 1), tr = r / rep;
-            if (tr != at_row && a.rope_dims > 0) turn.load(a.rope + static_cast<size_t>(pos + __builtin_amdgcn_readlane(t.depth, tr)) * a.rope_dims, a.rope_dims, lane);
-            at_row = tr;
-            float ss = 0.f;
-#pragma unroll
-            for (int v = 0; v < VEC; v++) ss = fmaf(qx[i].x[v], qx[i].x[v], ss);
-            const float sc = 1.f / sqrtf(wave_sum_all(ss) / static_cast<float>(D) + a.eps);
-            float y[VEC], o[VEC];
+            for (int v = 0; v < VEC; v++) ss = fma(static_cast<double>(k.x[v]), static_cast<double>(k.x[v]), ss);
+            const double sc = rsqrt_f64(fma(wave_sum_f64(ss), 1.0 / D, static_cast<double>(a.eps)));
 #pragma unroll
             for (int v = 0; v < VEC; v++) {
-                y[v] = qx[i].x[v] * sc * gq.x[v];
-                o[v] = __shfl(y[v], turn.partner, 64);
+                double y = k.x[v] * sc * gk.x[v];
+                if (a.rope_dims > 0) y = y * turn.c.x[v] + __shfl(y, shape.partner, 64) * turn.s.x[v];
+                kx[v] = __half_as_ushort(cell_value(y));
+                vx[v] = __half_as_ushort(__float2half_rn(val.x[v]));
             }
-#pragma unroll
-            for (int v = 0; v < VEC; v++) qx[i].x[v] = a.rope_dims > 0 ? turn.of(y[v], o[v], v) : y[v];
-        }
-        // a wave's share: [dim step of the half][hi, lo][lane] 16 bytes
-        char *mine = sm.ring[2] + wave * (KI / 2 * 2 * kChunk);
-        static_assert(W * KI * kChunk <= 2 * (D / 8) * kChunk, "the last two stages hold all waves' shares");
-#pragma unroll
-        for (int h = 0; h < 2; h++) {
-            if ((lane >> 5) == h) {
-                const int e = VEC * (lane & 31);  // dim within the half
-#pragma unroll
-                for (int i = 0; i < 16; i++) {
-                    _Float16 hi[VEC], lo[VEC];
-#pragma unroll
-                    for (int v = 0; v < VEC; v++) {
-                        hi[v] = static_cast<_Float16>(qx[i].x[v]);
-                        lo[v] = static_cast<_Float16>(qx[i].x[v] - static_cast<float>(hi[v]));
-                    }
-                    char *dst = mine + (e / 32) * 2 * kChunk + (16 * ((e & 31) >> 3) + i) * 16 + (e & 7) * 2;
-                    __builtin_memcpy(__builtin_assume_aligned(dst, 2 * VEC), hi, sizeof(hi));
-                    __builtin_memcpy(__builtin_assume_aligned(dst + kChunk, 2 * VEC), lo, sizeof(lo));
-                }
+            if (j + W < rows) load(j + W);  // under the rest of this one
+            if (qb == 0) {
+                const size_t cell = (static_cast<size_t>(seq) * a.rows + j) * kvw + kvh * D + VEC * lane;
+                __builtin_memcpy(__builtin_assume_aligned(static_cast<uint16_t *>(a.kcells) + cell, 2 * VEC), kx, sizeof(kx));
+                __builtin_memcpy(__builtin_assume_aligned(static_cast<uint16_t *>(a.vcells) + cell, 2 * VEC), vx, sizeof(vx));
             }
-            __builtin_amdgcn_wave_barrier();
+            char *to = sm.ring[j / kTile];
+            __builtin_memcpy(__builtin_assume_aligned(to + k_byte<D>(j % kTile, VEC * lane), 2 * VEC), kx, sizeof(kx));
 #pragma unroll
-            for (int i = 0; i < KI / 2; i++) {
-                qh[h * (KI / 2) + i] = *reinterpret_cast<const half8_t *>(mine + (2 * i) * kChunk + lane * 16);
-                ql[h * (KI / 2) + i] = *reinterpret_cast<const half8_t *>(mine + (2 * i + 1) * kChunk + lane * 16);
-            }
-            __builtin_amdgcn_wave_barrier();
+            for (int v = 0; v < VEC; v++) *reinterpret_cast<uint16_t *>(to + v_byte<D>(j % kTile, VEC * lane + v)) = vx[v];
         }
     }
+
+    // ---- queries: norm, rotation, and operand order by way of the last two stages ----
+    half8_t qh[KI], ql[KI];
+    {
+        // [dim step][lane] 16 bytes of a group's large halves, then of their small ones; eight waves' groups pass eight rows at a time, with
+        // eight rows' room
+        constexpr int kRowsHere = kShared ? 16 : 8;
+        constexpr int kPart = KI * 4 * kRowsHere * 16;
+        static_assert(2 * W * kPart <= 2 * (D / 8) * kChunk, "the last two stages hold all groups' operands");
+        char *stage = sm.ring[2];
+        const auto read = [&]() {
+            const char *mine = stage + 2 * wave * kPart + (kRowsHere * q + (n & (kRowsHere - 1))) * 16;
+#pragma unroll
+            for (int i = 0; i < KI; i++) {
+                qh[i] = *reinterpret_cast<const half8_t *>(mine + i * 4 * kRowsHere * 16);
+                ql[i] = *reinterpret_cast<const half8_t *>(mine + kPart + i * 4 * kRowsHere * 16);
+            }
+        };
+        Turn<D> turn = shape;
+        int turned = -1;
+        for (int f = 0; f < fours; f++) {
+            Row<D> next[4];
+            if (f + 1 < fours) load_four(next, f + 1);
+#pragma unroll
+            for (int u = 0; u < 4; u++) {
+                const int r = row_of(f, u), tr = min(over_rep(plan, r), rows - 1);
+                if (a.rope_dims > 0 && tr != turned) {  // (the heads of a row turn alike)
+                    turn.load(a.rope + static_cast<size_t>(pos + __builtin_amdgcn_readlane(t.depth, tr)) * a.rope_dims, a.rope_dims);
+                    turn.settle();
+                    turned = tr;
+                }
+                float ss = 0.f;
+#pragma unroll
+                for (int v = 0; v < VEC; v++) ss = fmaf(qx[u].x[v], qx[u].x[v], ss);
+                const float sc = __builtin_amdgcn_rsqf(fmaf(wave_sum_all(ss), 1.f / static_cast<float>(D), a.eps));
+                _Float16 hi[VEC], lo[VEC];
+#pragma unroll
+                for (int v = 0; v < VEC; v++) {
+                    float y = qx[u].x[v] * sc * gq.x[v];
+                    if (a.rope_dims > 0) y = fmaf(__shfl(y, shape.partner, 64), turn.s.x[v], y * turn.c.x[v]);
+                    hi[v] = static_cast<_Float16>(y);
+                    lo[v] = static_cast<_Float16>(fmaf(static_cast<float>(hi[v]), -1.f, y));
+                }
+                const int e = VEC * lane, i = kShared ? 4 * u + wave : 4 * f + u;  // the row within its group
+                char *dst = stage + 2 * (kShared ? f : wave) * kPart + (e / 32) * 4 * kRowsHere * 16 + (kRowsHere * ((e & 31) >> 3) + (i & (kRowsHere - 1))) * 16 + (e & 7) * 2;
+                __builtin_memcpy(__builtin_assume_aligned(dst, 2 * VEC), hi, sizeof(hi));
+                __builtin_memcpy(__builtin_assume_aligned(dst + kPart, 2 * VEC), lo, sizeof(lo));
+            }
+            if (!kShared && (f & 1)) {
+                __builtin_amdgcn_wave_barrier();
+                if ((n >> 3) == (f >> 1)) read();
+                __builtin_amdgcn_wave_barrier();
+            }
+#pragma unroll
+            for (int u = 0; u < 4; u++) qx[u] = next[u];
+        }
+        if (kShared) {
+            __syncthreads();
+            read();
+        }
+    }
+    const int r0 = (qb * W + wave) * 16, r_end = rows * rep;
     const bool working = r0 < r_end;
-    const int my_tr = min(r0 + n, r_end - 1) / rep;                 // the lane's query row's tree row
+    const int my_tr = over_rep(plan, min(r0 + n, r_end - 1));       // the lane's query row's tree row
     const int my_pos = pos + __shfl(t.depth, my_tr, 64);
     const int my_first = a.window > 0 ? my_pos - a.window + 1 : 0;  // sees sinks and positions from here on
+    uint64_t mates = static_cast<uint64_t>(__shfl(static_cast<uint32_t>(t.ancestors >> 32), my_tr, 64)) << 32 | __shfl(static_cast<uint32_t>(t.ancestors), my_tr, 64);
+    if (a.window > 0 && a.window < rows) {
+        uint64_t in = 0;
+        for (int j = 0; j < rows; j++) {
+            const int p = pos + __builtin_amdgcn_readlane(t.depth, j);
+            in |= p < a.sinks || p >= my_first ? 1ull << j : 0ull;
+        }
+        mates &= in;
+    }
     const float c2 = 1.44269504088896f / sqrtf(static_cast<float>(D));
 
     float4_t o[DB];
@@ -271,71 +390,105 @@ __global__ __launch_bounds__(64 * W, D == 256 ? 2 : 4) void tree_attn_kernel(shv
     for (int db = 0; db < DB; db++) o[db] = float4_t{0.f, 0.f, 0.f, 0.f};
     float m_run = -INFINITY, l_run = 0.f;  // of the scores as they are, before their scale
 
-    // one tile; sees(c): whether the lane's row sees cell c of it, asked where `part` says that some row may not see some cell
-    auto tile = [&](const char *kt, bool part, auto sees) {
+    // ---- the rows' own tiles, then the slice's: three of these on their way while one is multiplied, one barrier a tile ----
+    __syncthreads();  // every wave holds its queries, the rows' cells are there; the last two stages are free
+    if (!with_rows && t0 + 2 < t1) ask(t0 + 2);
+    for (int i = t0 - n_own; i < t1; i++) {
+        const char *kt;
+        uint32_t seen = 0xFF;  // which of the lane's eight cells its query row sees
+        bool part;
+        if (i < t0) {
+            kt = sm.ring[i - t0 + n_own];
+            part = true;
+            seen = static_cast<uint32_t>(mates >> (kTile * (i - t0 + n_own) + 8 * q)) & 0xFF;
+        } else {
+            if (i == t0 && with_rows) {
+                __syncthreads();  // the rows' tiles have been read
+                ask(t0);
+                if (t0 + 1 < t1) ask(t0 + 1);
+                if (t0 + 2 < t1) ask(t0 + 2);
+            }
+            // a wave's loads complete in order: this tile's have landed when no more are out than those behind it
+            if (i + 2 < t1) wait_loads<2 * kPer>();
+            else if (i + 1 < t1) wait_loads<kPer>();
+            else wait_loads<0>();
+            asm volatile("s_barrier" ::: "memory");  // everyone's: this tile is whole, and the stage of the one before is free
+            if (i + kAhead < t1) ask(i + kAhead);
+            kt = sm.ring[(i - t0) & (kStages - 1)];
+            const int c0 = tiles.at(i) * kTile;
+            part = c0 + kTile > pos || (a.window > 0 && c0 + kTile > a.sinks && c0 < pos + rows - a.window);
+            if (part) {
+                seen = 0;
+#pragma unroll
+                for (int e = 0; e < 8; e++) {
+                    const int c = c0 + 8 * q + e;
+                    seen |= c < pos && (a.window == 0 || c < a.sinks || c >= my_first) ? 1u << e : 0u;
+                }
+            }
+        }
+        if (!working) continue;
         const char *vt = kt + 2 * KI * kChunk;
+        // operands come from LDS four reads ahead of the products that use them
         float4_t st[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}}, lo[2] = {st[0], st[0]};
+        half8_t kb[2][4];
+        const auto read_k = [&](half8_t(&to)[4], int g) {
 #pragma unroll
-        for (int i = 0; i < KI; i++)
+            for (int e = 0; e < 4; e++) to[e] = *reinterpret_cast<const half8_t *>(kt + ((e & 1) * KI + 2 * g + (e >> 1)) * kChunk + lane * 16);
+        };
+        read_k(kb[0], 0);
 #pragma unroll
-            for (int T = 0; T < 2; T++) {
-                const half8_t k = *reinterpret_cast<const half8_t *>(kt + (T * KI + i) * kChunk + lane * 16);
-                st[T] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, qh[i], st[T], 0, 0, 0);
-                lo[T] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, ql[i], lo[T], 0, 0, 0);
+        for (int g = 0; g < KI / 2; g++) {
+            if (g + 1 < KI / 2) read_k(kb[(g + 1) & 1], g + 1);
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                st[e & 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kb[g & 1][e], qh[2 * g + (e >> 1)], st[e & 1], 0, 0, 0);
+                lo[e & 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kb[g & 1][e], ql[2 * g + (e >> 1)], lo[e & 1], 0, 0, 0);
             }
-        float mx = -INFINITY;
-        uint32_t seen = 0xFF;
+        }
+        float mx = -INFINITY, s[8];
+#pragma unroll
+        for (int e = 0; e < 8; e++) s[e] = st[e >> 2][e & 3] + lo[e >> 2][e & 3];
         if (part) {
-            seen = 0;
 #pragma unroll
-            for (int T = 0; T < 2; T++)
-#pragma unroll
-                for (int i = 0; i < 4; i++) seen |= sees(8 * q + 4 * T + i) ? 1u << (4 * T + i) : 0u;
+            for (int e = 0; e < 8; e++) s[e] = seen >> e & 1 ? s[e] : -INFINITY;
         }
 #pragma unroll
-        for (int T = 0; T < 2; T++)
-#pragma unroll
-            for (int i = 0; i < 4; i++) {
-                st[T][i] += lo[T][i];
-                if (part) st[T][i] = seen >> (4 * T + i) & 1 ? st[T][i] : -INFINITY;
-                mx = fmaxf(mx, st[T][i]);
-            }
-        mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
-        mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
-        const float m_new = fmaxf(m_run, mx);
-        const float m_use = m_new == -INFINITY ? 0.f : m_new;
-        const float m2 = m_use * c2;
-        float sum = 0.f, pv[8];
-#pragma unroll
-        for (int e = 0; e < 8; e++) {
-            pv[e] = __builtin_amdgcn_exp2f(fmaf(st[e >> 2][e & 3], c2, -m2));
-            sum += pv[e];
-        }
-        sum += __shfl_xor(sum, 16, 64);
-        sum += __shfl_xor(sum, 32, 64);
-        const float alpha = __builtin_amdgcn_exp2f(fmaf(m_run, c2, -m2));
-        l_run = l_run * alpha + sum;
-        m_run = m_new;
-        if (__ballot(alpha != 1.f) != 0ull) {
+        for (int e = 0; e < 8; e++) mx = fmaxf(mx, s[e]);
+        mx = max_over_q(mx);
+        // the sums are rescaled a few times a slice instead of whenever some row's maximum moves
+        const bool moves = mx * c2 > fmaf(m_run, c2, kSlack);
+        if (__ballot(moves) != 0ull) {
+            const float m_new = moves ? mx : m_run;
+            const float alpha = m_new == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((m_run - m_new) * c2);
+            l_run *= alpha;
+            m_run = m_new;
             float av[4];
 #pragma unroll
-            for (int i = 0; i < 4; i++) av[i] = __shfl(alpha, 4 * q + i, 64);
+            for (int e = 0; e < 4; e++) av[e] = __shfl(alpha, 4 * q + e, 64);
 #pragma unroll
             for (int db = 0; db < DB; db++)
 #pragma unroll
-                for (int i = 0; i < 4; i++) o[db][i] *= av[i];
+                for (int e = 0; e < 4; e++) o[db][e] *= av[e];
+        }
+        const float m2 = fmaf(m_run == -INFINITY ? 0.f : m_run, c2, -kLift);
+        float pv[8];
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+            pv[e] = __builtin_amdgcn_exp2f(fmaf(s[e], c2, -m2));
+            l_run += pv[e];
         }
         if (part) {
-            // a value that is not finite meets the weight 0 of rows that do not see it: such a tile is multiplied by hand
-            bool odd = false;
+            // a value that is not finite would meet the weight 0 of rows that do not see it: such a tile is multiplied by hand
+            uint32_t odd = 0;
 #pragma unroll
             for (int db = 0; db < DB; db++) {
                 const uint4 v = *reinterpret_cast<const uint4 *>(vt + db * kChunk + lane * 16);
                 const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-                for (int e = 0; e < 4; e++) odd = odd || (w[e] & 0x7C00u) == 0x7C00u || (w[e] & 0x7C000000u) == 0x7C000000u;
+                for (int e = 0; e < 4; e++) odd |= ((w[e] & 0x7C007C00u) + 0x04000400u) & 0x80008000u;  // an exponent of ones carries into the sign
             }
-            if (__ballot(odd) != 0ull) {
+            if (__ballot(odd != 0) != 0ull) {
                 float *p = sm.p[wave];
 #pragma unroll
                 for (int e = 0; e < 8; e++) p[n * kTile + 8 * q + e] = seen >> e & 1 ? pv[e] : -1.f;
@@ -343,102 +496,44 @@ __global__ __launch_bounds__(64 * W, D == 256 ? 2 : 4) void tree_attn_kernel(shv
                 for (int c = 0; c < kTile; c++) {
                     float w[4];
 #pragma unroll
-                    for (int i = 0; i < 4; i++) w[i] = p[(4 * q + i) * kTile + c];
+                    for (int e = 0; e < 4; e++) w[e] = p[(4 * q + e) * kTile + c];
 #pragma unroll
                     for (int db = 0; db < DB; db++) {
                         const float v = static_cast<float>(*reinterpret_cast<const _Float16 *>(vt + db * kChunk + (16 * (c >> 3) + n) * 16 + (c & 7) * 2));
 #pragma unroll
-                        for (int i = 0; i < 4; i++) o[db][i] = w[i] < 0.f ? o[db][i] : fmaf(w[i], v, o[db][i]);
+                        for (int e = 0; e < 4; e++) o[db][e] = w[e] < 0.f ? o[db][e] : fmaf(w[e], v, o[db][e]);
                     }
                 }
                 __builtin_amdgcn_wave_barrier();
-                return;
+                continue;
             }
         }
+        // weights as two halves, the large one cut off and not rounded: the small one holds the rest either way
         half8_t ph, pl;
 #pragma unroll
-        for (int e = 0; e < 8; e++) {
-            ph[e] = static_cast<_Float16>(pv[e]);
-            pl[e] = static_cast<_Float16>(pv[e] - static_cast<float>(ph[e]));
+        for (int e = 0; e < 8; e += 2) {
+            const half2_t h = __builtin_bit_cast(half2_t, __builtin_amdgcn_cvt_pkrtz(pv[e], pv[e + 1]));
+            const half2_t r = __builtin_bit_cast(half2_t, __builtin_amdgcn_cvt_pkrtz(fmaf(static_cast<float>(h[0]), -1.f, pv[e]), fmaf(static_cast<float>(h[1]), -1.f, pv[e + 1])));
+            ph[e] = h[0]; ph[e + 1] = h[1];
+            pl[e] = r[0]; pl[e + 1] = r[1];
         }
+        half8_t vb[2][4];
 #pragma unroll
-        for (int db = 0; db < DB; db++) {
-            const half8_t v = *reinterpret_cast<const half8_t *>(vt + db * kChunk + lane * 16);
-            o[db] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ph, v, o[db], 0, 0, 0);
-            o[db] = __builtin_amdgcn_mfma_f32_16x16x32_f16(pl, v, o[db], 0, 0, 0);
-        }
-    };
-
-    // ---- the slice's tiles: three on their way while one is multiplied; one barrier a tile ----
-    __syncthreads();  // every wave holds its queries: the last two stages are free
-    if (t0 + 2 < t1) ask(t0 + 2);
-    for (int i = t0; i < t1; i++) {
-        // a wave's loads complete in order: this tile's have landed when no more are out than those behind it
-        if (i + 2 < t1) wait_loads<2 * kPer>();
-        else if (i + 1 < t1) wait_loads<kPer>();
-        else wait_loads<0>();
-        asm volatile("s_barrier" ::: "memory");  // everyone's: this tile is whole, and the stage of the one before is free
-        if (i + kAhead < t1) ask(i + kAhead);
-        if (!working) continue;
-        const int c0 = tiles.at(i) * kTile;
-        const bool part = c0 + kTile > pos || (a.window > 0 && c0 + kTile > a.sinks && c0 < pos + t.n - a.window);
-        tile(sm.ring[(i - t0) & (kStages - 1)], part, [&](int c) {
-            c += c0;
-            return c < pos && (a.window == 0 || c < a.sinks || c >= my_first);
-        });
-    }
-    if (with_rows) {
-        // ---- the rows' own cells: normed, rotated and rounded into two more tiles, and left for whoever keeps them ----
-        __syncthreads();
-        const int n_tiles = (t.n + kTile - 1) / kTile;
-        const Turn<D> shape(a.rope_dims, lane);
-        Row<D> gk;
-        gk.load(a.k_norm, lane);
-        for (int j = wave; j < n_tiles * kTile; j += W) {
-            char *to = sm.ring[j / kTile];
-            uint16_t kx[VEC], vx[VEC];
+        for (int e = 0; e < 4; e++) vb[0][e] = *reinterpret_cast<const half8_t *>(vt + e * kChunk + lane * 16);
 #pragma unroll
-            for (int v = 0; v < VEC; v++) kx[v] = vx[v] = 0;
-            if (j < t.n) {
-                const float *src = qkv + static_cast<size_t>(j) * a.qkv_stride + static_cast<size_t>(a.n_head) * 2 * D + kvh * D;
-                Row<D> k, val;
-                k.load(src, lane);
-                val.load(src + kvw, lane);
-                Turn<D> turn = shape;
-                if (a.rope_dims > 0) turn.load(a.rope + static_cast<size_t>(pos + __builtin_amdgcn_readlane(t.depth, j)) * a.rope_dims, a.rope_dims, lane);
-                double ss = 0;
+        for (int g = 0; g < DB / 4; g++) {
+            if (g + 1 < DB / 4) {
 #pragma unroll
-                for (int v = 0; v < VEC; v++) ss += static_cast<double>(k.x[v]) * k.x[v];
-                const double sc = 1.0 / sqrt(wave_sum_f64(ss) / D + a.eps);
-#pragma unroll
-                for (int v = 0; v < VEC; v++) {
-                    const double y = k.x[v] * sc * gk.x[v], other = __shfl(y, turn.partner, 64);
-                    kx[v] = __half_as_ushort(cell_value(a.rope_dims > 0 ? turn.of(y, other, v) : y));
-                    vx[v] = __half_as_ushort(__float2half_rn(val.x[v]));
-                }
-                if (qb == 0) {
-                    const size_t cell = (static_cast<size_t>(seq) * a.rows + j) * kvw + kvh * D + VEC * lane;
-                    __builtin_memcpy(__builtin_assume_aligned(static_cast<uint16_t *>(a.kcells) + cell, 2 * VEC), kx, sizeof(kx));
-                    __builtin_memcpy(__builtin_assume_aligned(static_cast<uint16_t *>(a.vcells) + cell, 2 * VEC), vx, sizeof(vx));
-                }
+                for (int e = 0; e < 4; e++) vb[(g + 1) & 1][e] = *reinterpret_cast<const half8_t *>(vt + (4 * (g + 1) + e) * kChunk + lane * 16);
             }
-            __builtin_memcpy(__builtin_assume_aligned(to + k_byte<D>(j % kTile, VEC * lane), 2 * VEC), kx, sizeof(kx));
+            __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-            for (int v = 0; v < VEC; v++) *reinterpret_cast<uint16_t *>(to + v_byte<D>(j % kTile, VEC * lane + v)) = vx[v];
+            for (int e = 0; e < 4; e++) o[4 * g + e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ph, vb[g & 1][e], o[4 * g + e], 0, 0, 0);
+#pragma unroll
+            for (int e = 0; e < 4; e++) o[4 * g + e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(pl, vb[g & 1][e], o[4 * g + e], 0, 0, 0);
         }
-        __syncthreads();
-        uint64_t see = static_cast<uint64_t>(__shfl(static_cast<uint32_t>(t.ancestors >> 32), my_tr, 64)) << 32 | __shfl(static_cast<uint32_t>(t.ancestors), my_tr, 64);
-        if (a.window > 0 && a.window < t.n) {
-            uint64_t in = 0;
-            for (int j = 0; j < t.n; j++) {
-                const int p = pos + __builtin_amdgcn_readlane(t.depth, j);
-                in |= p < a.sinks || p >= my_first ? 1ull << j : 0ull;
-            }
-            see &= in;
-        }
-        if (working)
-            for (int i = 0; i < n_tiles; i++) tile(sm.ring[i], true, [&](int c) { return (see >> (i * kTile + c) & 1) != 0; });
     }
+    l_run = sum_over_q(l_run);
     if (!working) return;
     if (cut.all == 1) {
         float lr[4];
@@ -446,7 +541,7 @@ __global__ __launch_bounds__(64 * W, D == 256 ? 2 : 4) void tree_attn_kernel(shv
         for (int i = 0; i < 4; i++) lr[i] = __shfl(l_run, 4 * q + i, 64);
 #pragma unroll
         for (int i = 0; i < 4; i++) {
-            const int r = r0 + 4 * q + i, tr = r / rep;
+            const int r = r0 + 4 * q + i, tr = over_rep(plan, r);
             if (r >= r_end) continue;
             float *dst = a.out + ((static_cast<size_t>(seq) * a.rows + tr) * a.n_head + kvh * rep + r - tr * rep) * D;
 #pragma unroll
@@ -466,12 +561,12 @@ __global__ __launch_bounds__(64 * W, D == 256 ? 2 : 4) void tree_attn_kernel(shv
     if (q == 0 && r0 + n < r_end) *reinterpret_cast<float2 *>(rec + static_cast<size_t>(r0 + n) * (D + 2) + D) = make_float2(m_run, l_run);
 }
 
-// grid: (n_head * D / 64, rows, n_seq), a block 64 dims of a row's head: its waves share the slices' records, each folds its share with all of a
-// batch's loads on their way together, and the first wave folds their results.
-constexpr int kMergeWaves = 8;
-template <int D>
-__global__ __launch_bounds__(64 * kMergeWaves) void tree_merge_kernel(shv_attn_tree_args a, int slots) {
-    __shared__ float red[3][kMergeWaves][64];
+// The slices' records of a row and head joined, a thread a dim.  NW waves share the records of 64 dims, each folds its share with all of a
+// batch's loads on their way together, and the first wave folds their results: eight waves where a call has few rows and heads, one
+// otherwise.  grid: (n_head * D / 64, rows, n_seq).
+template <int D, int NW>
+__global__ __launch_bounds__(64 * NW) void tree_merge_kernel(shv_attn_tree_args a, int slots) {
+    __shared__ float red[3][NW][64];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int head = blockIdx.x / (D / 64), d = blockIdx.x % (D / 64) * 64 + lane, row = blockIdx.y, seq = blockIdx.z;
     const int rep = a.n_head / a.n_head_kv, kvh = head / rep;
@@ -484,12 +579,12 @@ __global__ __launch_bounds__(64 * kMergeWaves) void tree_merge_kernel(shv_attn_t
     const float *from = a.partial + (static_cast<size_t>(seq) * a.n_head_kv + kvh) * a.n_splits * step + static_cast<size_t>(row * rep + head % rep) * (D + 2);
     constexpr int MB = 16;
     float num = 0.f, den = 0.f, M = -INFINITY;
-    for (int s0 = wave; s0 < cut.all; s0 += kMergeWaves * MB) {
+    for (int s0 = wave; s0 < cut.all; s0 += NW * MB) {
         float v[MB];
         float2 ml[MB];
 #pragma unroll
         for (int u = 0; u < MB; u++) {
-            const int s = s0 + kMergeWaves * u < cut.all ? s0 + kMergeWaves * u : s0;
+            const int s = s0 + NW * u < cut.all ? s0 + NW * u : s0;
             v[u] = from[s * step + d];
             ml[u] = *reinterpret_cast<const float2 *>(from + s * step + D);
         }
@@ -497,13 +592,18 @@ __global__ __launch_bounds__(64 * kMergeWaves) void tree_merge_kernel(shv_attn_t
         for (int u = 0; u < MB; u++) asm volatile("" : "+v"(v[u]));  // asked for together, not each behind the one before's test
 #pragma unroll
         for (int u = 0; u < MB; u++) {
-            if (s0 + kMergeWaves * u >= cut.all || (ml[u].x == -INFINITY && ml[u].y == 0.f)) continue;  // (sees nothing; a sum of NaN stays)
+            if (s0 + NW * u >= cut.all || (ml[u].x == -INFINITY && ml[u].y == 0.f)) continue;  // (sees nothing; a sum of NaN stays)
             const float Mn = fmaxf(M, ml[u].x);
             const float shrink = __builtin_amdgcn_exp2f((M - Mn) * c2), w = __builtin_amdgcn_exp2f((ml[u].x - Mn) * c2);
             den = fmaf(den, shrink, w * ml[u].y);
             num = fmaf(num, shrink, w * v[u]);
             M = Mn;
         }
+    }
+    float *out = a.out + ((static_cast<size_t>(seq) * a.rows + row) * a.n_head + head) * D + d;
+    if constexpr (NW == 1) {
+        *out = num / den;
+        return;
     }
     red[0][wave][lane] = M;
     red[1][wave][lane] = den;
@@ -512,27 +612,28 @@ __global__ __launch_bounds__(64 * kMergeWaves) void tree_merge_kernel(shv_attn_t
     if (wave != 0) return;
     float Mt = red[0][0][lane];
 #pragma unroll
-    for (int k = 1; k < kMergeWaves; k++) Mt = fmaxf(Mt, red[0][k][lane]);
+    for (int k = 1; k < NW; k++) Mt = fmaxf(Mt, red[0][k][lane]);
     float nt = 0.f, dt = 0.f;
 #pragma unroll
-    for (int k = 0; k < kMergeWaves; k++) {
+    for (int k = 0; k < NW; k++) {
         const float mk = red[0][k][lane];
         if (mk == -INFINITY && red[1][k][lane] == 0.f) continue;
         const float w = __builtin_amdgcn_exp2f((mk - Mt) * c2);
         dt = fmaf(w, red[1][k][lane], dt);
         nt = fmaf(w, red[2][k][lane], nt);
     }
-    a.out[((static_cast<size_t>(seq) * a.rows + row) * a.n_head + head) * D + d] = nt / dt;
+    *out = nt / dt;
 }
 
 template <int D, int W>
 int launch_tree(shv_ctx *ctx, const shv_attn_tree_args &a) {
     const int rep = a.n_head / a.n_head_kv;
-    const int q_blocks = (a.rows * rep + 16 * W - 1) / (16 * W);
     constexpr int kBlocksPerUnit = D == 256 ? 1 : 2;
-    // slices of the cache all sequences have together: as many blocks as the chip holds at once
-    int slots = ctx->prop.multiProcessorCount * kBlocksPerUnit / (a.n_head_kv * q_blocks) - a.n_seq;
-    if (slots < 1) slots = 1;
+    Plan plan;
+    plan.q_blocks = (a.rows * rep + 16 * W - 1) / (16 * W);
+    plan.slots = ctx->prop.multiProcessorCount * kBlocksPerUnit / (a.n_head_kv * plan.q_blocks) - a.n_seq;
+    if (plan.slots < 1) plan.slots = 1;
+    plan.rep_magic = ((1u << 20) + rep - 1) / rep;
     static std::atomic<uint64_t> raised{0};  // by device
     const uint64_t bit = 1ull << (ctx->device & 63);
     if (!(raised.load(std::memory_order_acquire) & bit)) {
@@ -540,11 +641,15 @@ int launch_tree(shv_ctx *ctx, const shv_attn_tree_args &a) {
         raised.fetch_or(bit, std::memory_order_release);
     }
     // a sequence may have all the slices of the cache to itself, and those its share leaves over
-    const int most = a.n_splits < slots + 1 + a.n_seq ? a.n_splits : slots + 1 + a.n_seq;
+    const int most = a.n_splits < plan.slots + 1 + a.n_seq ? a.n_splits : plan.slots + 1 + a.n_seq;
     shv_attn_tree_args b = a;
     b.n_splits = most;
-    SHV_LAUNCH(ctx, (tree_attn_kernel<D, W>), dim3((most + 7) / 8 * 8 * q_blocks, a.n_head_kv, a.n_seq), dim3(64 * W), sizeof(TreeSmem<D, W>), b, q_blocks, slots);
-    if (most > 1) SHV_LAUNCH(ctx, tree_merge_kernel<D>, dim3(a.n_head * (D / 64), a.rows, a.n_seq), dim3(64 * kMergeWaves), 0, b, slots);
+    SHV_LAUNCH(ctx, (tree_attn_kernel<D, W>), dim3((most + 7) / 8 * 8 * plan.q_blocks, a.n_head_kv, a.n_seq), dim3(64 * W), sizeof(TreeSmem<D, W>), b, plan);
+    if (most > 1) {
+        const dim3 grid(a.n_head * (D / 64), a.rows, a.n_seq);
+        if (a.n_head * (D / 64) * a.rows * a.n_seq < kMergeMany) SHV_LAUNCH(ctx, (tree_merge_kernel<D, 8>), grid, dim3(512), 0, b, plan.slots);
+        else SHV_LAUNCH(ctx, (tree_merge_kernel<D, 1>), grid, dim3(64), 0, b, plan.slots);
+    }
     return SHV_OK;
 }
 
@@ -583,6 +688,7 @@ int shv_launch_attn_tree(shv_ctx *ctx, const shv_attn_tree_args *pa) {
     SHV_REQUIRE(a.rope_dims >= 0 && a.rope_dims <= a.head_dim && a.rope_dims % (a.head_dim / 32) == 0,
                 "attn_tree: rope_dims %d; a multiple of %d up to %d", a.rope_dims, a.head_dim / 32, a.head_dim);
     SHV_REQUIRE(a.rope || a.rope_dims == 0, "attn_tree: NULL rotary table");
+    SHV_REQUIRE(shv_aligned16(a.rope), "attn_tree: the rotary table must be 16-byte aligned");
     SHV_REQUIRE(a.max_cells >= kTile && a.max_cells % kTile == 0, "attn_tree: max_cells %d; a multiple of %d", a.max_cells, kTile);
     SHV_REQUIRE(a.qkv_stride >= (a.n_head + a.n_head_kv) * 2 * a.head_dim && a.qkv_stride % 4 == 0, "attn_tree: qkv_stride %d", a.qkv_stride);
     SHV_REQUIRE(a.n_splits >= 1 && a.n_splits <= kMaxSplits, "attn_tree: %d slices; 1..%d", a.n_splits, kMaxSplits);

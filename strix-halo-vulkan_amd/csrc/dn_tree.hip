@@ -43,8 +43,9 @@ __global__ __launch_bounds__(kBlock) void dn_tree_kernel(shv_dn_tree_args a) {
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int col0 = blockIdx.x * kCols, h = blockIdx.y, seq = blockIdx.z, hk = h % a.n_head_k;
     const int qk = a.n_head_k * kD, vw = a.n_head_v * kD;
-    const int slot = a.slot ? a.slot[seq] : seq, pos = a.pos ? a.pos[seq] : 0;
-    const TreeRow t = tree_row(a.parent, a.count, seq, a.rows, lane);
+    const TreeWords words(a.count, a.pos, a.slot, a.parent, a.conv1d, seq, a.rows, lane);
+    const int slot = words.slot, pos = words.pos;
+    const TreeRow t = tree_row(words.count, words.parent, a.rows, lane);
     const int n = t.n;
     if (n == 0) return;
     const float *x = a.x + static_cast<size_t>(seq) * a.rows * a.x_stride;
@@ -71,7 +72,7 @@ __global__ __launch_bounds__(kBlock) void dn_tree_kernel(shv_dn_tree_args a) {
             const int next = __shfl(t.parent, up < 0 ? 0 : up, 64);
             up = up < 0 ? -1 : next;
         }
-        const float G = tree_sum(t, g, lane);
+        const float G = tree_sum(t, g, a.rows, lane);
         if (wave == 0) {
             L.G[lane] = G;
             L.beta[lane] = b;

@@ -19,25 +19,38 @@ __device__ __forceinline__ int tree_rows(const int32_t *count, int seq, int rows
     return n < 0 ? 0 : n > rows ? rows : n;
 }
 
-__device__ __forceinline__ int tree_parent(const int32_t *parent, int seq, int rows, int n, int lane) {
-    if (lane >= n) return -1;
-    const int p = parent ? parent[static_cast<size_t>(seq) * rows + lane] : lane - 1;
-    return p >= 0 && p < lane ? p : -1;
-}
+// What memory says of a sequence and its tree, as words that are asked for together and branch nowhere: an absent array's word is
+// read from `any`, which is readable, and not used.
+struct TreeWords {
+    int count, pos, slot, parent;
+    __device__ __forceinline__ TreeWords(const int32_t *counts, const int32_t *positions, const int32_t *slots, const int32_t *parents, const void *any, int seq, int rows,
+                                         int lane) {
+        const int32_t *a = static_cast<const int32_t *>(any);
+        const int at = lane < rows ? lane : rows - 1;
+        parent = *(parents ? parents + static_cast<size_t>(seq) * rows + at : a);
+        count = *(counts ? counts + seq : a);
+        pos = *(positions ? positions + seq : a);
+        slot = *(slots ? slots + seq : a);
+        count = counts ? (count < 0 ? 0 : count > rows ? rows : count) : rows;
+        pos = positions ? pos : 0;
+        slot = slots ? slot : seq;
+        parent = parents ? parent : lane - 1;
+    }
+};
 
-// The ancestors by doubling: after step k a lane holds those up to 2^k rows away, and the row 2^k away.  64 rows: six steps.
-__device__ __forceinline__ TreeRow tree_row(const int32_t *parent, const int32_t *count, int seq, int rows, int lane) {
+// The ancestors by doubling: after step k a lane holds those up to 2^k rows away, and the row 2^k away.  log2(rows) steps.
+__device__ __forceinline__ TreeRow tree_row(int n, int parent, int rows, int lane) {
     TreeRow t;
-    t.n = tree_rows(count, seq, rows);
-    t.parent = tree_parent(parent, seq, rows, t.n, lane);
-    uint32_t lo = lane < t.n && lane < 32 ? 1u << lane : 0, hi = lane < t.n && lane >= 32 ? 1u << (lane - 32) : 0;
+    t.n = n;
+    t.parent = lane < n && parent >= 0 && parent < lane ? parent : -1;
+    uint32_t lo = lane < n && lane < 32 ? 1u << lane : 0, hi = lane < n && lane >= 32 ? 1u << (lane - 32) : 0;
     int up = t.parent;
-#pragma unroll
-    for (int k = 0; k < 6; k++) {
+    for (int far = 1; far < rows; far *= 2) {
         const int from = up < 0 ? lane : up;  // a row without one that far asks itself
-        lo |= __shfl(lo, from, 64);
-        hi |= __shfl(hi, from, 64);
+        const uint32_t more_lo = __shfl(lo, from, 64), more_hi = rows > 32 ? __shfl(hi, from, 64) : 0;
         const int next = __shfl(up, from, 64);
+        lo |= more_lo;
+        hi |= more_hi;
         up = up < 0 ? -1 : next;
     }
     t.ancestors = static_cast<uint64_t>(hi) << 32 | lo;
@@ -46,10 +59,9 @@ __device__ __forceinline__ TreeRow tree_row(const int32_t *parent, const int32_t
 }
 
 // Sum of v over a lane's row and the rows on its way to the root.
-__device__ __forceinline__ float tree_sum(const TreeRow &t, float v, int lane) {
+__device__ __forceinline__ float tree_sum(const TreeRow &t, float v, int rows, int lane) {
     int up = t.parent;
-#pragma unroll
-    for (int k = 0; k < 6; k++) {
+    for (int far = 1; far < rows; far *= 2) {
         const int from = up < 0 ? lane : up;
         const float more = __shfl(v, from, 64);
         const int next = __shfl(up, from, 64);

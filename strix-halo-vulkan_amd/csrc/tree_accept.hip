@@ -20,14 +20,14 @@ constexpr int kBlocksWanted = 4096;
 __device__ __forceinline__ void walk(const shv_tree_accept_args &a, int seq, int best_of, int lane) {
     const size_t base = static_cast<size_t>(seq) * a.rows;
     const int n = tree_rows(a.count, seq, a.rows);
-    const int parent = tree_parent(a.parent, seq, a.rows, n, lane);
+    const int parent = lane >= n ? -1 : a.parent ? a.parent[base + lane] : lane - 1;
     const int id = lane < n ? a.ids[base + lane] : 0;
     int kept = 0, at = 0, row_here = -1, next = -1;
     while (n > 0) {
         if (lane == kept) row_here = at;
         kept++;
         next = __builtin_amdgcn_readlane(best_of, at);
-        const uint64_t follow = __ballot(lane < n && parent == at && id == next);
+        const uint64_t follow = __ballot(lane < n && lane > at && parent == at && id == next);
         if (follow == 0) break;  // a child is a higher row than its parent: at most n steps
         at = __builtin_amdgcn_readfirstlane(__ffsll(static_cast<unsigned long long>(follow)) - 1);
     }

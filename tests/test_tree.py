@@ -45,7 +45,7 @@ def _refused(fn, args, match):
 
 @pytest.mark.parametrize("bad,match", [
     *[({k: None}, "NULL") for k in ("qkv", "q_norm", "k_norm", "rope", "kcache", "vcache", "kcells", "vcells", "partial", "out")],
-    *[({k: P + 4}, "aligned") for k in ("qkv", "q_norm", "k_norm", "kcache", "vcache", "kcells", "vcells", "partial", "out")],
+    *[({k: P + 4}, "aligned") for k in ("rope", "qkv", "q_norm", "k_norm", "kcache", "vcache", "kcells", "vcells", "partial", "out")],
     ({"rows": 0}, "rows"), ({"rows": 65}, "rows"), ({"n_seq": 0}, "sequences"), ({"n_seq": 70000}, "sequences"), ({"head_dim": 96}, "head_dim"),
     ({"head_dim": 512}, "head_dim"), ({"n_head": 15}, "heads"), ({"n_head_kv": 0}, "heads"), ({"n_head": 130}, "heads"), ({"n_head": -16}, "heads"),
     ({"n_head": 1026, "n_head_kv": 1026}, "heads"), ({"rope_dims": 63}, "rope_dims"), ({"rope_dims": 60}, "rope_dims"), ({"rope_dims": 258}, "rope_dims"), ({"rope_dims": -2}, "rope_dims"),

@@ -257,12 +257,22 @@ __global__ __launch_bounds__(64 * W, D == 256 ? 2 : 4) void tree_attn_kernel(shv
         for (int u = 0; u < kPer; u++)
             __builtin_amdgcn_raw_ptr_buffer_load_lds(bytes, (lds_ptr_t)(to + u * kChunk), 16, from, u * (keys ? 64 : 1024), 0, 0);
     };
+    // (loads complete in order: what the prologue needs goes out before the tiles do)
+    const TreeRow t = tree_row(rows, words.parent, a.rows, lane);
+    const Turn<D> shape(a.rope_dims, lane);
+    const auto tree_row_of = [&](int f, int u) { return min(over_rep(plan, row_of(f, u)), rows - 1); };
+    const auto load_turn = [&](Turn<D> &turn, int row) { turn.load(a.rope + static_cast<size_t>(pos + __builtin_amdgcn_readlane(t.depth, row)) * a.rope_dims, a.rope_dims); };
+    const auto turn_four = [&](Turn<D>(&turn)[4], int f) {
+        if (a.rope_dims == 0) return;
+#pragma unroll
+        for (int u = 0; u < 4; u++) load_turn(turn[u], tree_row_of(f, u));
+    };
+    Turn<D> q_turn[4] = {shape, shape, shape, shape};
+    turn_four(q_turn, 0);
     if (!with_rows) {
         ask(t0);
         if (t0 + 1 < t1) ask(t0 + 1);
     }
-    const TreeRow t = tree_row(rows, words.parent, a.rows, lane);
-    const Turn<D> shape(a.rope_dims, lane);
     const int n_own = with_rows ? (rows + kTile - 1) / kTile : 0;  // tiles of the rows' own cells
     if (with_rows) {
         // ---- the rows' own cells: normed, rotated and rounded into the first two stages, and left for whoever keeps them ----
@@ -279,7 +289,7 @@ __global__ __launch_bounds__(64 * W, D == 256 ? 2 : 4) void tree_attn_kernel(shv
             const float *src = qkv + static_cast<size_t>(j) * a.qkv_stride + static_cast<size_t>(a.n_head) * 2 * D + kvh * D;
             k.load(src, lane);
             val.load(src + kvw, lane);
-            if (a.rope_dims > 0) turn.load(a.rope + static_cast<size_t>(pos + __builtin_amdgcn_readlane(t.depth, j)) * a.rope_dims, a.rope_dims);
+            if (a.rope_dims > 0) load_turn(turn, j);
         };
         if (wave < rows) load(wave);
         for (int j = wave; j < rows; j += W) {
@@ -318,41 +328,56 @@ __global__ __launch_bounds__(64 * W, D == 256 ? 2 : 4) void tree_attn_kernel(shv
         constexpr int kPart = KI * 4 * kRowsHere * 16;
         static_assert(2 * W * kPart <= 2 * (D / 8) * kChunk, "the last two stages hold all groups' operands");
         char *stage = sm.ring[2];
+        // row i's 16 bytes of dims 32 d + 8 q ..: turned on among the rows' places, since a row, written at once, would ask the same few banks
+        const auto place = [&](int i, int d, int q) { return (kRowsHere * q + ((i + (kRowsHere == 16 ? 4 * d + q : 2 * d + (q >> 1))) & (kRowsHere - 1))) * 16; };
         const auto read = [&]() {
-            const char *mine = stage + 2 * wave * kPart + (kRowsHere * q + (n & (kRowsHere - 1))) * 16;
+            const char *mine = stage + 2 * wave * kPart;
 #pragma unroll
             for (int i = 0; i < KI; i++) {
-                qh[i] = *reinterpret_cast<const half8_t *>(mine + i * 4 * kRowsHere * 16);
-                ql[i] = *reinterpret_cast<const half8_t *>(mine + kPart + i * 4 * kRowsHere * 16);
+                qh[i] = *reinterpret_cast<const half8_t *>(mine + i * 4 * kRowsHere * 16 + place(n, i, q));
+                ql[i] = *reinterpret_cast<const half8_t *>(mine + kPart + i * 4 * kRowsHere * 16 + place(n, i, q));
             }
         };
-        Turn<D> turn = shape;
-        int turned = -1;
         for (int f = 0; f < fours; f++) {
             Row<D> next[4];
-            if (f + 1 < fours) load_four(next, f + 1);
+            Turn<D> next_turn[4] = {shape, shape, shape, shape};
+            if (f + 1 < fours) {
+                load_four(next, f + 1);
+                turn_four(next_turn, f + 1);
+            }
+            float y[4][VEC], other[4][VEC];
 #pragma unroll
             for (int u = 0; u < 4; u++) {
-                const int r = row_of(f, u), tr = min(over_rep(plan, r), rows - 1);
-                if (a.rope_dims > 0 && tr != turned) {  // (the heads of a row turn alike)
-                    turn.load(a.rope + static_cast<size_t>(pos + __builtin_amdgcn_readlane(t.depth, tr)) * a.rope_dims, a.rope_dims);
-                    turn.settle();
-                    turned = tr;
-                }
                 float ss = 0.f;
 #pragma unroll
                 for (int v = 0; v < VEC; v++) ss = fmaf(qx[u].x[v], qx[u].x[v], ss);
                 const float sc = __builtin_amdgcn_rsqf(fmaf(wave_sum_all(ss), 1.f / static_cast<float>(D), a.eps));
+#pragma unroll
+                for (int v = 0; v < VEC; v++) y[u][v] = qx[u].x[v] * sc * gq.x[v];
+            }
+            if (a.rope_dims > 0) {
+#pragma unroll
+                for (int u = 0; u < 4; u++) {
+#pragma unroll
+                    for (int v = 0; v < VEC; v++) other[u][v] = __shfl(y[u][v], shape.partner, 64);
+                }
+#pragma unroll
+                for (int u = 0; u < 4; u++) {
+                    q_turn[u].settle();
+#pragma unroll
+                    for (int v = 0; v < VEC; v++) y[u][v] = fmaf(other[u][v], q_turn[u].s.x[v], y[u][v] * q_turn[u].c.x[v]);
+                }
+            }
+#pragma unroll
+            for (int u = 0; u < 4; u++) {
                 _Float16 hi[VEC], lo[VEC];
 #pragma unroll
                 for (int v = 0; v < VEC; v++) {
-                    float y = qx[u].x[v] * sc * gq.x[v];
-                    if (a.rope_dims > 0) y = fmaf(__shfl(y, shape.partner, 64), turn.s.x[v], y * turn.c.x[v]);
-                    hi[v] = static_cast<_Float16>(y);
-                    lo[v] = static_cast<_Float16>(fmaf(static_cast<float>(hi[v]), -1.f, y));
+                    hi[v] = static_cast<_Float16>(y[u][v]);
+                    lo[v] = static_cast<_Float16>(fmaf(static_cast<float>(hi[v]), -1.f, y[u][v]));
                 }
                 const int e = VEC * lane, i = kShared ? 4 * u + wave : 4 * f + u;  // the row within its group
-                char *dst = stage + 2 * (kShared ? f : wave) * kPart + (e / 32) * 4 * kRowsHere * 16 + (kRowsHere * ((e & 31) >> 3) + (i & (kRowsHere - 1))) * 16 + (e & 7) * 2;
+                char *dst = stage + 2 * (kShared ? f : wave) * kPart + (e / 32) * 4 * kRowsHere * 16 + place(i, e / 32, (e & 31) >> 3) + (e & 7) * 2;
                 __builtin_memcpy(__builtin_assume_aligned(dst, 2 * VEC), hi, sizeof(hi));
                 __builtin_memcpy(__builtin_assume_aligned(dst + kPart, 2 * VEC), lo, sizeof(lo));
             }
@@ -362,7 +387,7 @@ __global__ __launch_bounds__(64 * W, D == 256 ? 2 : 4) void tree_attn_kernel(shv
                 __builtin_amdgcn_wave_barrier();
             }
 #pragma unroll
-            for (int u = 0; u < 4; u++) qx[u] = next[u];
+            for (int u = 0; u < 4; u++) qx[u] = next[u], q_turn[u] = next_turn[u];
         }
         if (kShared) {
             __syncthreads();

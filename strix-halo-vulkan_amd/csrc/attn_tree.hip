@@ -194,16 +194,107 @@ __device__ __forceinline__ float sum_over_q(float v) {
 template <int N>
 __device__ __forceinline__ void wait_loads() { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory"); }
 
+// ---- the same work for the launch before a wide call's, and inside a narrow one's --------------------------------------------------
+// A row's key, normed and rotated, as the lane's dims' halves.
+template <int D>
+__device__ __forceinline__ void cell_key(const Row<D> &k, const Row<D> &gamma, const Turn<D> &turn, int rope_dims, float eps, uint16_t (&out)[D / 64]) {
+    double ss = 0;
+#pragma unroll
+    for (int v = 0; v < D / 64; v++) ss = fma(static_cast<double>(k.x[v]), static_cast<double>(k.x[v]), ss);
+    const double sc = rsqrt_f64(fma(wave_sum_f64(ss), 1.0 / D, static_cast<double>(eps)));
+#pragma unroll
+    for (int v = 0; v < D / 64; v++) {
+        double y = k.x[v] * sc * gamma.x[v];
+        if (rope_dims > 0) y = y * turn.c.x[v] + __shfl(y, turn.partner, 64) * turn.s.x[v];
+        out[v] = __half_as_ushort(cell_value(y));
+    }
+}
+// A query row as large and small halves.
+template <int D>
+__device__ __forceinline__ void split_row(const float (&y)[D / 64], _Float16 (&hi)[D / 64], _Float16 (&lo)[D / 64]) {
+#pragma unroll
+    for (int v = 0; v < D / 64; v++) {
+        hi[v] = static_cast<_Float16>(y[v]);
+        lo[v] = static_cast<_Float16>(fmaf(static_cast<float>(hi[v]), -1.f, y[v]));
+    }
+}
+template <int BYTES, typename T>
+__device__ __forceinline__ void put_bytes(void *to, const T *from) { __builtin_memcpy(__builtin_assume_aligned(to, BYTES), from, BYTES); }
+
+// Where the rows' operands of a wide call lie: of group g (16 query rows, fewer in a KV head's last) of a KV head, [dim step][large, small]
+// [dims 8 q ..][row] 16 bytes.  As many bytes as the rows have floats.
+__device__ __forceinline__ char *staged(char *stage, const shv_attn_tree_args &a, int seq, int kvh, int rows, int rep, int g, int D) {
+    return stage + (static_cast<size_t>(seq) * a.rows * a.n_head + static_cast<size_t>(kvh) * rows * rep + 16 * g) * D * 4;
+}
+
+// grid: (ceil((rows * n_head + rows * n_head_kv) / 4), n_seq), a wave a query row or a row's cell of a KV head.
+template <int D>
+__global__ __launch_bounds__(256) void tree_prep_kernel(shv_attn_tree_args a, Plan plan, char *stage) {
+    constexpr int VEC = D / 64, KI = D / 32;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), seq = blockIdx.y;
+    const int rep = a.n_head / a.n_head_kv;
+    const TreeWords words(a.count, a.pos, a.slot, a.parent, a.q_norm, seq, a.rows, lane);
+    const int item = blockIdx.x * 4 + wave, cell0 = a.rows * a.n_head;
+    if (item >= cell0 + a.rows * a.n_head_kv) return;
+    const bool query = item < cell0;
+    const int per = query ? a.n_head : a.n_head_kv, i = query ? item : item - cell0;
+    const int row = static_cast<int>(static_cast<uint32_t>(i) / static_cast<uint32_t>(per)), head = i - row * per;
+    const float *src = a.qkv + (static_cast<size_t>(seq) * a.rows + row) * a.qkv_stride + static_cast<size_t>(query ? head : a.n_head) * 2 * D + (query ? 0 : head * D);
+    Row<D> x, gamma, val;
+    x.load(src, lane);
+    val.load(query ? src : src + static_cast<size_t>(a.n_head_kv) * D, lane);
+    gamma.load(query ? a.q_norm : a.k_norm, lane);
+    const int pos = __builtin_amdgcn_readfirstlane(words.pos), rows = __builtin_amdgcn_readfirstlane(words.count);
+    if (row >= rows || !fits(pos, rows, a.max_cells)) return;
+    const TreeRow t = tree_row(rows, words.parent, a.rows, lane);
+    Turn<D> turn(a.rope_dims, lane);
+    if (a.rope_dims > 0) {
+        turn.load(a.rope + static_cast<size_t>(pos + __builtin_amdgcn_readlane(t.depth, row)) * a.rope_dims, a.rope_dims);
+        turn.settle();
+    }
+    if (!query) {
+        uint16_t kx[VEC], vx[VEC];
+        cell_key<D>(x, gamma, turn, a.rope_dims, a.eps, kx);
+#pragma unroll
+        for (int v = 0; v < VEC; v++) vx[v] = __half_as_ushort(__float2half_rn(val.x[v]));
+        const size_t cell = ((static_cast<size_t>(seq) * a.rows + row) * a.n_head_kv + head) * D + VEC * lane;
+        put_bytes<2 * VEC>(static_cast<uint16_t *>(a.kcells) + cell, kx);
+        put_bytes<2 * VEC>(static_cast<uint16_t *>(a.vcells) + cell, vx);
+        return;
+    }
+    float ss = 0.f, y[VEC];
+#pragma unroll
+    for (int v = 0; v < VEC; v++) ss = fmaf(x.x[v], x.x[v], ss);
+    const float sc = __builtin_amdgcn_rsqf(fmaf(wave_sum_all(ss), 1.f / static_cast<float>(D), a.eps));
+#pragma unroll
+    for (int v = 0; v < VEC; v++) {
+        y[v] = x.x[v] * sc * gamma.x[v];
+        if (a.rope_dims > 0) y[v] = fmaf(__shfl(y[v], turn.partner, 64), turn.s.x[v], y[v] * turn.c.x[v]);
+    }
+    _Float16 hi[VEC], lo[VEC];
+    split_row<D>(y, hi, lo);
+    const int kvh = over_rep(plan, head), r = row * rep + head - kvh * rep, g = r >> 4, here = min(16, rows * rep - 16 * g), e = VEC * lane;
+    char *dst = staged(stage, a, seq, kvh, rows, rep, g, D) + ((e / 32) * 8 + ((e & 31) >> 3)) * here * 16 + (r & 15) * 16 + (e & 7) * 2;
+    put_bytes<2 * VEC>(dst, hi);
+    put_bytes<2 * VEC>(dst + 4 * here * 16, lo);
+    static_assert(KI * 32 == D, "whole steps");
+}
+
 template <int D, int W>
 struct TreeSmem {
     char ring[kStages][D / 8 * kChunk];
     float p[W][16 * kTile];  // a wave's weights of a tile, where its values are not all finite
 };
 
-// grid: (slices rounded up to 8, times query blocks; n_head_kv; n_seq), W waves.  A wave holds 16 query rows: query row r of a KV head is
-// head r % rep of tree row r / rep.
+// grid: (slices rounded up to 8, times query blocks; n_head_kv; n_seq), four waves.  A wave holds GW groups of 16 query rows: query row r of a KV
+// head is head r % rep of tree row r / rep.  GW 1: calls of up to 64 query rows a KV head, whose rows are normed and turned here, by every
+// block; GW 2: wider ones, whose rows a launch before (tree_prep_kernel) has left as operands: there every block has 128 rows to prepare,
+// 5 us before its first product, and the launch costs 4.
+// What bounds a wide call is the matrix cores and the LDS reads that feed them: a key's and a value's operand read once serves both
+// groups, and one group's exponentials run under the other's products.
 template <int D, int W>
-__global__ __launch_bounds__(64 * W, D == 256 ? 2 : 4) void tree_attn_kernel(shv_attn_tree_args a, Plan plan) {
+__global__ __launch_bounds__(64 * W, W == 4 || D == 256 ? 2 : 4) void tree_attn_kernel(shv_attn_tree_args a, Plan plan, char *stage) {
+    constexpr bool kWide = W == 8;
     constexpr int VEC = D / 64, KI = D / 32, DB = D / 16;
     constexpr int kPer = D / 8 / W;  // chunks of a tile a wave asks for
     extern __shared__ __align__(16) char raw[];
@@ -211,17 +302,16 @@ __global__ __launch_bounds__(64 * W, D == 256 ? 2 : 4) void tree_attn_kernel(shv
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int n = lane & 15, q = lane >> 4;
     // blocks of one slice lie on one die (workgroups go to the dies in turn) and find its tiles in the die's L2
-    const int group = blockIdx.x >> 3, of_group = static_cast<int>(static_cast<uint32_t>(group) / static_cast<uint32_t>(plan.q_blocks));
-    const int split = of_group * 8 + (blockIdx.x & 7), qb = group - of_group * plan.q_blocks;
+    const int eight = blockIdx.x >> 3, of_eight = static_cast<int>(static_cast<uint32_t>(eight) / static_cast<uint32_t>(plan.q_blocks));
+    const int split = of_eight * 8 + (blockIdx.x & 7), qb = eight - of_eight * plan.q_blocks;
     const int kvh = blockIdx.y, seq = blockIdx.z;
     const int rep = a.n_head / a.n_head_kv;
     const TreeWords words(a.count, a.pos, a.slot, a.parent, a.q_norm, seq, a.rows, lane);
-    // ---- what depends on nothing: the first query rows this wave prepares.  Four waves share the rows of all of them (there are at most four
-    //      groups of 16, often one), four rows of a group each; eight take their own group's ----
-    constexpr bool kShared = W == 4;
-    const int fours = kShared ? (a.rows * rep + 15) / 16 : 4;  // of rows the wave prepares
-    const auto row_of = [&](int f, int u) { return kShared ? 16 * f + 4 * u + wave : (qb * W + wave) * 16 + 4 * f + u; };
     const float *qkv = a.qkv + static_cast<size_t>(seq) * a.rows * a.qkv_stride;
+    // ---- GW 1: what depends on nothing, the first query rows this wave prepares.  The waves share the rows of all groups (there is often one),
+    //      four rows of a group each ----
+    const int groups_here = !kWide ? (a.rows * rep + 15) / 16 : 0;
+    const auto row_of = [&](int f, int u) { return 16 * f + 4 * u + wave; };
     const auto load_four = [&](Row<D>(&x)[4], int f) {
 #pragma unroll
         for (int u = 0; u < 4; u++) {
@@ -229,12 +319,14 @@ __global__ __launch_bounds__(64 * W, D == 256 ? 2 : 4) void tree_attn_kernel(shv
             x[u].load(qkv + static_cast<size_t>(tr) * a.qkv_stride + static_cast<size_t>(kvh * rep + r - tr * rep) * 2 * D, lane);
         }
     };
-    Row<D> qx[4];
-    load_four(qx, 0);
-    Row<D> gq;
-    gq.load(a.q_norm, lane);
+    Row<D> qx[4], gq;
+    if constexpr (!kWide) {
+        load_four(qx, 0);
+        gq.load(a.q_norm, lane);
+    }
     const int slot = words.slot, pos = __builtin_amdgcn_readfirstlane(words.pos), rows = __builtin_amdgcn_readfirstlane(words.count);
-    if (!fits(pos, rows, a.max_cells) || qb * W * 16 >= rows * rep) return;
+    const int r_end = rows * rep;
+    if (!fits(pos, rows, a.max_cells) || qb * W * 16 >= r_end) return;
     const Tiles tiles(a, pos);
     const Cut cut(a, tiles.all, plan.slots, lane);
     if (split >= cut.all) return;
@@ -249,99 +341,107 @@ __global__ __launch_bounds__(64 * W, D == 256 ? 2 : 4) void tree_attn_kernel(shv
     const int first = (keys ? wave : wave - W / 2) * kPer;  // of the wave's chunks among K's or V's
     const uint32_t from = keys ? static_cast<uint32_t>((8 * (n >> 2) + 4 * (first / KI) + (n & 3)) * kvw + 32 * (first % KI) + 8 * q) * 2
                                : static_cast<uint32_t>((16 * first + n) * kTile + 8 * q) * 2;
-    auto ask = [&](int i) {
-        const size_t at = static_cast<size_t>(tiles.at(i)) * kTile * kvw;
+    // The block's tiles in a row: the rows' own, n_own of them, then the slice's.  Tile j lies in stage j % kStages.
+    const int n_own = with_rows ? (rows + kTile - 1) / kTile : 0, n_tiles = n_own + t1 - t0;
+    const auto ask = [&](int j) {
+        const size_t at = static_cast<size_t>(tiles.at(t0 + j - n_own)) * kTile * kvw;
         const __amdgpu_buffer_rsrc_t bytes = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t *>((keys ? kc : vc) + at), 0, static_cast<uint32_t>(kTile * kvw) * 2, 0x00027000);
-        char *to = sm.ring[(i - t0) & (kStages - 1)] + (wave * kPer) * kChunk;
+        char *to = sm.ring[j & (kStages - 1)] + (wave * kPer) * kChunk;
 #pragma unroll
         for (int u = 0; u < kPer; u++)
             __builtin_amdgcn_raw_ptr_buffer_load_lds(bytes, (lds_ptr_t)(to + u * kChunk), 16, from, u * (keys ? 64 : 1024), 0, 0);
     };
     // (loads complete in order: what the prologue needs goes out before the tiles do)
+    const int r0 = (qb * W + wave) * 16;
+    const bool working = r0 < r_end;
+    half8_t qh[KI], ql[KI];
+    if constexpr (kWide) {
+        // a group that is not there is the last one again, and dropped
+        const int g = min(r0, r_end - 1) / 16, here = min(16, r_end - 16 * g);
+        const char *mine = staged(stage, a, seq, kvh, rows, rep, g, D) + (q * here + min(n, here - 1)) * 16;
+#pragma unroll
+        for (int i = 0; i < KI; i++) {
+            qh[i] = *reinterpret_cast<const half8_t *>(mine + (i * 8) * here * 16);
+            ql[i] = *reinterpret_cast<const half8_t *>(mine + (i * 8 + 4) * here * 16);
+        }
+    }
     const TreeRow t = tree_row(rows, words.parent, a.rows, lane);
     const Turn<D> shape(a.rope_dims, lane);
-    const auto tree_row_of = [&](int f, int u) { return min(over_rep(plan, row_of(f, u)), rows - 1); };
     const auto load_turn = [&](Turn<D> &turn, int row) { turn.load(a.rope + static_cast<size_t>(pos + __builtin_amdgcn_readlane(t.depth, row)) * a.rope_dims, a.rope_dims); };
     const auto turn_four = [&](Turn<D>(&turn)[4], int f) {
         if (a.rope_dims == 0) return;
 #pragma unroll
-        for (int u = 0; u < 4; u++) load_turn(turn[u], tree_row_of(f, u));
+        for (int u = 0; u < 4; u++) load_turn(turn[u], min(over_rep(plan, row_of(f, u)), rows - 1));
     };
     Turn<D> q_turn[4] = {shape, shape, shape, shape};
-    turn_four(q_turn, 0);
+    if constexpr (!kWide) turn_four(q_turn, 0);
     if (!with_rows) {
-        ask(t0);
-        if (t0 + 1 < t1) ask(t0 + 1);
+        ask(0);
+        if (1 < n_tiles) ask(1);
     }
-    const int n_own = with_rows ? (rows + kTile - 1) / kTile : 0;  // tiles of the rows' own cells
     if (with_rows) {
-        // ---- the rows' own cells: normed, rotated and rounded into the first two stages, and left for whoever keeps them ----
+        // ---- the rows' own cells go into the first two stages; GW 1: normed, rotated and rounded here, and left for whoever keeps them ----
         if (rows % kTile != 0) {
             // behind the last row the second product wants something finite
             uint4 *v = reinterpret_cast<uint4 *>(sm.ring[n_own - 1] + 2 * KI * kChunk);
             for (int i = tid; i < DB * 64; i += 64 * W) v[i] = make_uint4(0, 0, 0, 0);
             __syncthreads();
         }
-        Row<D> gk, k, val;
-        gk.load(a.k_norm, lane);
-        Turn<D> turn = shape;
-        const auto load = [&](int j) {
-            const float *src = qkv + static_cast<size_t>(j) * a.qkv_stride + static_cast<size_t>(a.n_head) * 2 * D + kvh * D;
-            k.load(src, lane);
-            val.load(src + kvw, lane);
-            if (a.rope_dims > 0) load_turn(turn, j);
-        };
-        if (wave < rows) load(wave);
-        for (int j = wave; j < rows; j += W) {
-            if (a.rope_dims > 0) turn.settle();
-            uint16_t kx[VEC], vx[VEC];
-            double ss = 0;
-#pragma unroll
-            for (int v = 0; v < VEC; v++) ss = fma(static_cast<double>(k.x[v]), static_cast<double>(k.x[v]), ss);
-            const double sc = rsqrt_f64(fma(wave_sum_f64(ss), 1.0 / D, static_cast<double>(a.eps)));
-#pragma unroll
-            for (int v = 0; v < VEC; v++) {
-                double y = k.x[v] * sc * gk.x[v];
-                if (a.rope_dims > 0) y = y * turn.c.x[v] + __shfl(y, shape.partner, 64) * turn.s.x[v];
-                kx[v] = __half_as_ushort(cell_value(y));
-                vx[v] = __half_as_ushort(__float2half_rn(val.x[v]));
-            }
-            if (j + W < rows) load(j + W);  // under the rest of this one
-            if (qb == 0) {
-                const size_t cell = (static_cast<size_t>(seq) * a.rows + j) * kvw + kvh * D + VEC * lane;
-                __builtin_memcpy(__builtin_assume_aligned(static_cast<uint16_t *>(a.kcells) + cell, 2 * VEC), kx, sizeof(kx));
-                __builtin_memcpy(__builtin_assume_aligned(static_cast<uint16_t *>(a.vcells) + cell, 2 * VEC), vx, sizeof(vx));
-            }
+        const auto place = [&](int j, const uint16_t(&kx)[VEC], const uint16_t(&vx)[VEC]) {
             char *to = sm.ring[j / kTile];
-            __builtin_memcpy(__builtin_assume_aligned(to + k_byte<D>(j % kTile, VEC * lane), 2 * VEC), kx, sizeof(kx));
+            put_bytes<2 * VEC>(to + k_byte<D>(j % kTile, VEC * lane), kx);
 #pragma unroll
             for (int v = 0; v < VEC; v++) *reinterpret_cast<uint16_t *>(to + v_byte<D>(j % kTile, VEC * lane + v)) = vx[v];
+        };
+        const size_t cell0 = static_cast<size_t>(seq) * a.rows * kvw + kvh * D + VEC * lane;
+        if constexpr (kWide) {
+            for (int j0 = wave; j0 < rows; j0 += 4 * W) {
+                uint16_t kx[4][VEC], vx[4][VEC];
+#pragma unroll
+                for (int u = 0; u < 4; u++) {
+                    const size_t cell = cell0 + min(j0 + u * W, rows - 1) * kvw;
+                    put_bytes<2 * VEC>(kx[u], static_cast<const uint16_t *>(__builtin_assume_aligned(static_cast<const uint16_t *>(a.kcells) + cell, 2 * VEC)));
+                    put_bytes<2 * VEC>(vx[u], static_cast<const uint16_t *>(__builtin_assume_aligned(static_cast<const uint16_t *>(a.vcells) + cell, 2 * VEC)));
+                }
+#pragma unroll
+                for (int u = 0; u < 4; u++)
+                    if (j0 + u * W < rows) place(j0 + u * W, kx[u], vx[u]);
+            }
+        } else {
+            Row<D> gk, k, val;
+            gk.load(a.k_norm, lane);
+            Turn<D> turn = shape;
+            const auto load = [&](int j) {
+                const float *src = qkv + static_cast<size_t>(j) * a.qkv_stride + static_cast<size_t>(a.n_head) * 2 * D + kvh * D;
+                k.load(src, lane);
+                val.load(src + kvw, lane);
+                if (a.rope_dims > 0) load_turn(turn, j);
+            };
+            if (wave < rows) load(wave);
+            for (int j = wave; j < rows; j += W) {
+                if (a.rope_dims > 0) turn.settle();
+                uint16_t kx[VEC], vx[VEC];
+                cell_key<D>(k, gk, turn, a.rope_dims, a.eps, kx);
+#pragma unroll
+                for (int v = 0; v < VEC; v++) vx[v] = __half_as_ushort(__float2half_rn(val.x[v]));
+                if (j + W < rows) load(j + W);  // under the rest of this one
+                put_bytes<2 * VEC>(static_cast<uint16_t *>(a.kcells) + cell0 + j * kvw, kx);
+                put_bytes<2 * VEC>(static_cast<uint16_t *>(a.vcells) + cell0 + j * kvw, vx);
+                place(j, kx, vx);
+            }
         }
     }
-
-    // ---- queries: norm, rotation, and operand order by way of the last two stages ----
-    half8_t qh[KI], ql[KI];
-    {
-        // [dim step][lane] 16 bytes of a group's large halves, then of their small ones; eight waves' groups pass eight rows at a time, with
-        // eight rows' room
-        constexpr int kRowsHere = kShared ? 16 : 8;
-        constexpr int kPart = KI * 4 * kRowsHere * 16;
+    if constexpr (!kWide) {
+        // ---- queries: norm, rotation, and operand order by way of the last two stages: [group][large, small][dim step][dims 8 q ..][row] 16 bytes ----
+        constexpr int kPart = KI * kChunk;
         static_assert(2 * W * kPart <= 2 * (D / 8) * kChunk, "the last two stages hold all groups' operands");
-        char *stage = sm.ring[2];
+        char *here = sm.ring[2];
         // row i's 16 bytes of dims 32 d + 8 q ..: turned on among the rows' places, since a row, written at once, would ask the same few banks
-        const auto place = [&](int i, int d, int q) { return (kRowsHere * q + ((i + (kRowsHere == 16 ? 4 * d + q : 2 * d + (q >> 1))) & (kRowsHere - 1))) * 16; };
-        const auto read = [&]() {
-            const char *mine = stage + 2 * wave * kPart;
-#pragma unroll
-            for (int i = 0; i < KI; i++) {
-                qh[i] = *reinterpret_cast<const half8_t *>(mine + i * 4 * kRowsHere * 16 + place(n, i, q));
-                ql[i] = *reinterpret_cast<const half8_t *>(mine + kPart + i * 4 * kRowsHere * 16 + place(n, i, q));
-            }
-        };
-        for (int f = 0; f < fours; f++) {
+        const auto place = [&](int i, int d, int q) { return (16 * q + ((i + 4 * d + q) & 15)) * 16; };
+        for (int f = 0; f < groups_here; f++) {
             Row<D> next[4];
             Turn<D> next_turn[4] = {shape, shape, shape, shape};
-            if (f + 1 < fours) {
+            if (f + 1 < groups_here) {
                 load_four(next, f + 1);
                 turn_four(next_turn, f + 1);
             }
@@ -371,76 +471,64 @@ __global__ __launch_bounds__(64 * W, D == 256 ? 2 : 4) void tree_attn_kernel(shv
 #pragma unroll
             for (int u = 0; u < 4; u++) {
                 _Float16 hi[VEC], lo[VEC];
-#pragma unroll
-                for (int v = 0; v < VEC; v++) {
-                    hi[v] = static_cast<_Float16>(y[u][v]);
-                    lo[v] = static_cast<_Float16>(fmaf(static_cast<float>(hi[v]), -1.f, y[u][v]));
-                }
-                const int e = VEC * lane, i = kShared ? 4 * u + wave : 4 * f + u;  // the row within its group
-                char *dst = stage + 2 * (kShared ? f : wave) * kPart + (e / 32) * 4 * kRowsHere * 16 + place(i, e / 32, (e & 31) >> 3) + (e & 7) * 2;
-                __builtin_memcpy(__builtin_assume_aligned(dst, 2 * VEC), hi, sizeof(hi));
-                __builtin_memcpy(__builtin_assume_aligned(dst + kPart, 2 * VEC), lo, sizeof(lo));
-            }
-            if (!kShared && (f & 1)) {
-                __builtin_amdgcn_wave_barrier();
-                if ((n >> 3) == (f >> 1)) read();
-                __builtin_amdgcn_wave_barrier();
+                split_row<D>(y[u], hi, lo);
+                const int e = VEC * lane;
+                char *dst = here + 2 * f * kPart + (e / 32) * kChunk + place(4 * u + wave, e / 32, (e & 31) >> 3) + (e & 7) * 2;
+                put_bytes<2 * VEC>(dst, hi);
+                put_bytes<2 * VEC>(dst + kPart, lo);
             }
 #pragma unroll
             for (int u = 0; u < 4; u++) qx[u] = next[u], q_turn[u] = next_turn[u];
         }
-        if (kShared) {
-            __syncthreads();
-            read();
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < KI; i++) {
+            qh[i] = *reinterpret_cast<const half8_t *>(here + 2 * wave * kPart + i * kChunk + place(n, i, q));
+            ql[i] = *reinterpret_cast<const half8_t *>(here + (2 * wave + 1) * kPart + i * kChunk + place(n, i, q));
         }
     }
-    const int r0 = (qb * W + wave) * 16, r_end = rows * rep;
-    const bool working = r0 < r_end;
-    const int my_tr = over_rep(plan, min(r0 + n, r_end - 1));       // the lane's query row's tree row
-    const int my_pos = pos + __shfl(t.depth, my_tr, 64);
-    const int my_first = a.window > 0 ? my_pos - a.window + 1 : 0;  // sees sinks and positions from here on
-    uint64_t mates = static_cast<uint64_t>(__shfl(static_cast<uint32_t>(t.ancestors >> 32), my_tr, 64)) << 32 | __shfl(static_cast<uint32_t>(t.ancestors), my_tr, 64);
-    if (a.window > 0 && a.window < rows) {
-        uint64_t in = 0;
-        for (int j = 0; j < rows; j++) {
-            const int p = pos + __builtin_amdgcn_readlane(t.depth, j);
-            in |= p < a.sinks || p >= my_first ? 1ull << j : 0ull;
+    int my_first;    // the first position the lane's row sees, but for the sinks
+    uint64_t mates;  // the rows it sees
+    {
+        const int tr = over_rep(plan, min(r0 + n, r_end - 1));
+        my_first = a.window > 0 ? pos + __shfl(t.depth, tr, 64) - a.window + 1 : 0;
+        mates = static_cast<uint64_t>(__shfl(static_cast<uint32_t>(t.ancestors >> 32), tr, 64)) << 32 | __shfl(static_cast<uint32_t>(t.ancestors), tr, 64);
+        if (a.window > 0 && a.window < rows) {
+            uint64_t in = 0;
+            for (int j = 0; j < rows; j++) {
+                const int p = pos + __builtin_amdgcn_readlane(t.depth, j);
+                in |= p < a.sinks || p >= my_first ? 1ull << j : 0ull;
+            }
+            mates &= in;
         }
-        mates &= in;
     }
     const float c2 = 1.44269504088896f / sqrtf(static_cast<float>(D));
 
     float4_t o[DB];
+    float m_run, l_run;  // of the scores as they are, before their scale; the sums of a lane's own cells
 #pragma unroll
     for (int db = 0; db < DB; db++) o[db] = float4_t{0.f, 0.f, 0.f, 0.f};
-    float m_run = -INFINITY, l_run = 0.f;  // of the scores as they are, before their scale
+    m_run = -INFINITY;
+    l_run = 0.f;
 
     // ---- the rows' own tiles, then the slice's: three of these on their way while one is multiplied, one barrier a tile ----
     __syncthreads();  // every wave holds its queries, the rows' cells are there; the last two stages are free
-    if (!with_rows && t0 + 2 < t1) ask(t0 + 2);
-    for (int i = t0 - n_own; i < t1; i++) {
-        const char *kt;
+    for (int j = with_rows ? n_own : 2; j < min(n_tiles, 3); j++) ask(j);
+    for (int j = 0; j < n_tiles; j++) {
+        const char *kt = sm.ring[j & (kStages - 1)];
         uint32_t seen = 0xFF;  // which of the lane's eight cells its query row sees
         bool part;
-        if (i < t0) {
-            kt = sm.ring[i - t0 + n_own];
+        // a wave's loads complete in order: this tile's have landed when no more are out than those behind it
+        if (j + 2 < n_tiles) wait_loads<2 * kPer>();
+        else if (j + 1 < n_tiles) wait_loads<kPer>();
+        else wait_loads<0>();
+        asm volatile("s_barrier" ::: "memory");  // everyone's: this tile is whole, and the stage of the one before is free
+        if (j + kAhead < n_tiles && j + kAhead >= n_own) ask(j + kAhead);
+        if (j < n_own) {
             part = true;
-            seen = static_cast<uint32_t>(mates >> (kTile * (i - t0 + n_own) + 8 * q)) & 0xFF;
+            seen = static_cast<uint32_t>(mates >> (kTile * j + 8 * q)) & 0xFF;
         } else {
-            if (i == t0 && with_rows) {
-                __syncthreads();  // the rows' tiles have been read
-                ask(t0);
-                if (t0 + 1 < t1) ask(t0 + 1);
-                if (t0 + 2 < t1) ask(t0 + 2);
-            }
-            // a wave's loads complete in order: this tile's have landed when no more are out than those behind it
-            if (i + 2 < t1) wait_loads<2 * kPer>();
-            else if (i + 1 < t1) wait_loads<kPer>();
-            else wait_loads<0>();
-            asm volatile("s_barrier" ::: "memory");  // everyone's: this tile is whole, and the stage of the one before is free
-            if (i + kAhead < t1) ask(i + kAhead);
-            kt = sm.ring[(i - t0) & (kStages - 1)];
-            const int c0 = tiles.at(i) * kTile;
+            const int c0 = tiles.at(t0 + j - n_own) * kTile;
             part = c0 + kTile > pos || (a.window > 0 && c0 + kTile > a.sinks && c0 < pos + rows - a.window);
             if (part) {
                 seen = 0;
@@ -558,12 +646,12 @@ __global__ __launch_bounds__(64 * W, D == 256 ? 2 : 4) void tree_attn_kernel(shv
             for (int e = 0; e < 4; e++) o[4 * g + e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(pl, vb[g & 1][e], o[4 * g + e], 0, 0, 0);
         }
     }
-    l_run = sum_over_q(l_run);
     if (!working) return;
+    const float sum = sum_over_q(l_run);
     if (cut.all == 1) {
         float lr[4];
 #pragma unroll
-        for (int i = 0; i < 4; i++) lr[i] = __shfl(l_run, 4 * q + i, 64);
+        for (int i = 0; i < 4; i++) lr[i] = __shfl(sum, 4 * q + i, 64);
 #pragma unroll
         for (int i = 0; i < 4; i++) {
             const int r = r0 + 4 * q + i, tr = over_rep(plan, r);
@@ -583,7 +671,7 @@ __global__ __launch_bounds__(64 * W, D == 256 ? 2 : 4) void tree_attn_kernel(shv
 #pragma unroll
         for (int db = 0; db < DB; db++) rec[static_cast<size_t>(r) * (D + 2) + 16 * db + n] = o[db][i];
     }
-    if (q == 0 && r0 + n < r_end) *reinterpret_cast<float2 *>(rec + static_cast<size_t>(r0 + n) * (D + 2) + D) = make_float2(m_run, l_run);
+    if (q == 0 && r0 + n < r_end) *reinterpret_cast<float2 *>(rec + static_cast<size_t>(r0 + n) * (D + 2) + D) = make_float2(m_run, sum);
 }
 
 // The slices' records of a row and head joined, a thread a dim.  NW waves share the records of 64 dims, each folds its share with all of a
@@ -665,12 +753,21 @@ int launch_tree(shv_ctx *ctx, const shv_attn_tree_args &a) {
         SHV_HIP_CHECK(hipFuncSetAttribute(reinterpret_cast<const void *>(&tree_attn_kernel<D, W>), hipFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(sizeof(TreeSmem<D, W>))));
         raised.fetch_or(bit, std::memory_order_release);
     }
-    // a sequence may have all the slices of the cache to itself, and those its share leaves over
-    const int most = a.n_splits < plan.slots + 1 + a.n_seq ? a.n_splits : plan.slots + 1 + a.n_seq;
+    // A sequence may have all the slices of the cache to itself, and those its share leaves over.  Of a wide call the last slice's records
+    // (all there are, with one slice) are where the rows' operands lie: D floats of each record's D + 2.
     shv_attn_tree_args b = a;
-    b.n_splits = most;
-    SHV_LAUNCH(ctx, (tree_attn_kernel<D, W>), dim3((most + 7) / 8 * 8 * plan.q_blocks, a.n_head_kv, a.n_seq), dim3(64 * W), sizeof(TreeSmem<D, W>), b, plan);
-    if (most > 1) {
+    char *stage = nullptr;
+    if (W == 8) {
+        b.n_splits = a.n_splits > 1 ? a.n_splits - 1 : 1;
+        const size_t records = static_cast<size_t>(a.n_seq) * a.rows * a.n_head * (D + 2) * (a.n_splits - 1);
+        stage = reinterpret_cast<char *>((reinterpret_cast<uintptr_t>(a.partial + records) + 15) & ~static_cast<uintptr_t>(15));
+        const int items = a.rows * (a.n_head + a.n_head_kv);
+        SHV_LAUNCH(ctx, tree_prep_kernel<D>, dim3((items + 3) / 4, a.n_seq), dim3(256), 0, a, plan, stage);
+    }
+    const int most = plan.slots + 1 + a.n_seq;
+    if (b.n_splits > most) b.n_splits = most;
+    SHV_LAUNCH(ctx, (tree_attn_kernel<D, W>), dim3((b.n_splits + 7) / 8 * 8 * plan.q_blocks, a.n_head_kv, a.n_seq), dim3(64 * W), sizeof(TreeSmem<D, W>), b, plan, stage);
+    if (b.n_splits > 1) {
         const dim3 grid(a.n_head * (D / 64), a.rows, a.n_seq);
         if (a.n_head * (D / 64) * a.rows * a.n_seq < kMergeMany) SHV_LAUNCH(ctx, (tree_merge_kernel<D, 8>), grid, dim3(512), 0, b, plan.slots);
         else SHV_LAUNCH(ctx, (tree_merge_kernel<D, 1>), grid, dim3(64), 0, b, plan.slots);

@@ -60,8 +60,8 @@ constexpr int kStages = 4, kAhead = kStages - 1;
 // Weights are e^(s - m) 2^kLift, and m stands until a score is more than 2^kSlack above it: up to 2^15, which the larger half holds, and down to
 // 2^-31 of the largest with the smaller half's last place (at a lift of 0 2^-24, 6e-6 of a weight of a hundredth).
 constexpr float kLift = 7.f, kSlack = 8.f;
+constexpr int kLeastNarrow = 2, kLeastWide = 3;
 constexpr int kMergeMany = 1024;  // 64-dim pieces of rows and heads from which one wave joins the slices of each
-constexpr int kMinTiles = 4;  // tiles a slice gets at least
 
 // Which tiles of 32 cells a sequence's rows look at: the sinks', then those the window of the first row reaches.
 struct Tiles {
@@ -81,6 +81,7 @@ struct Tiles {
 // What the launcher works out once.
 struct Plan {
     int q_blocks;        // blocks that share a slice, 16 query rows a wave
+    int least;           // tiles a slice gets at least
     int slots;           // slices of the cache that all sequences have together: as many blocks as the chip holds at once
     uint32_t rep_magic;  // r / rep = r * rep_magic >> 20 for r < 4096 and rep <= 64: off by less than r / 2^20 <= 1 / 256 before it is cut
 };
@@ -90,7 +91,7 @@ __device__ __forceinline__ int over_rep(const Plan &plan, int r) { return static
 // themselves; where a call has one slice, it holds both.
 struct Cut {
     int len, cache, all;  // tiles of a slice, slices of the cache, slices
-    __device__ __forceinline__ Cut(const shv_attn_tree_args &a, int tiles, int slots, int lane) {
+    __device__ __forceinline__ Cut(const shv_attn_tree_args &a, int tiles, const Plan &plan, int lane) {
         if (a.n_splits == 1) {
             len = tiles;
             cache = 0;
@@ -110,8 +111,8 @@ struct Cut {
             }
         }
         total = __builtin_amdgcn_readfirstlane(total);
-        const uint32_t share = (total + slots - 1) / slots, room = a.n_splits - 1;
-        uint32_t l = share > kMinTiles ? share : kMinTiles;
+        const uint32_t slots = plan.slots, least = plan.least, share = (total + slots - 1) / slots, room = a.n_splits - 1;
+        uint32_t l = share > least ? share : least;
         if (l * static_cast<uint64_t>(room) < static_cast<uint32_t>(tiles)) l = (tiles + room - 1) / room;
         len = l;
         cache = (tiles + l - 1) / l;
@@ -328,7 +329,7 @@ __global__ __launch_bounds__(64 * W, W == 4 || D == 256 ? 2 : 4) void tree_attn_
     const int r_end = rows * rep;
     if (!fits(pos, rows, a.max_cells) || qb * W * 16 >= r_end) return;
     const Tiles tiles(a, pos);
-    const Cut cut(a, tiles.all, plan.slots, lane);
+    const Cut cut(a, tiles.all, plan, lane);
     if (split >= cut.all) return;
     const bool with_rows = split == cut.all - 1;
     const int t0 = with_rows && cut.all > 1 ? 0 : split * cut.len;
@@ -678,14 +679,14 @@ __global__ __launch_bounds__(64 * W, W == 4 || D == 256 ? 2 : 4) void tree_attn_
 // batch's loads on their way together, and the first wave folds their results: eight waves where a call has few rows and heads, one
 // otherwise.  grid: (n_head * D / 64, rows, n_seq).
 template <int D, int NW>
-__global__ __launch_bounds__(64 * NW) void tree_merge_kernel(shv_attn_tree_args a, int slots) {
+__global__ __launch_bounds__(64 * NW) void tree_merge_kernel(shv_attn_tree_args a, Plan plan) {
     __shared__ float red[3][NW][64];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int head = blockIdx.x / (D / 64), d = blockIdx.x % (D / 64) * 64 + lane, row = blockIdx.y, seq = blockIdx.z;
     const int rep = a.n_head / a.n_head_kv, kvh = head / rep;
     const int pos = a.pos ? a.pos[seq] : 0, rows = tree_rows(a.count, seq, a.rows);
     if (row >= rows || !fits(pos, rows, a.max_cells)) return;
-    const Cut cut(a, Tiles(a, pos).all, slots, lane);
+    const Cut cut(a, Tiles(a, pos).all, plan, lane);
     if (cut.all == 1) return;  // put straight out
     const float c2 = 1.44269504088896f / sqrtf(static_cast<float>(D));
     const size_t step = static_cast<size_t>(a.rows) * rep * (D + 2);
@@ -746,6 +747,8 @@ int launch_tree(shv_ctx *ctx, const shv_attn_tree_args &a) {
     plan.q_blocks = (a.rows * rep + 16 * W - 1) / (16 * W);
     plan.slots = ctx->prop.multiProcessorCount * kBlocksPerUnit / (a.n_head_kv * plan.q_blocks) - a.n_seq;
     if (plan.slots < 1) plan.slots = 1;
+    // A tile more to a slice costs a narrow call 1.2 us and a wide one 1.4; of a slice more the merge reads a record more of every row.
+    plan.least = W == 4 ? kLeastNarrow : kLeastWide;
     plan.rep_magic = ((1u << 20) + rep - 1) / rep;
     static std::atomic<uint64_t> raised{0};  // by device
     const uint64_t bit = 1ull << (ctx->device & 63);
@@ -769,8 +772,8 @@ int launch_tree(shv_ctx *ctx, const shv_attn_tree_args &a) {
     SHV_LAUNCH(ctx, (tree_attn_kernel<D, W>), dim3((b.n_splits + 7) / 8 * 8 * plan.q_blocks, a.n_head_kv, a.n_seq), dim3(64 * W), sizeof(TreeSmem<D, W>), b, plan, stage);
     if (b.n_splits > 1) {
         const dim3 grid(a.n_head * (D / 64), a.rows, a.n_seq);
-        if (a.n_head * (D / 64) * a.rows * a.n_seq < kMergeMany) SHV_LAUNCH(ctx, (tree_merge_kernel<D, 8>), grid, dim3(512), 0, b, plan.slots);
-        else SHV_LAUNCH(ctx, (tree_merge_kernel<D, 1>), grid, dim3(64), 0, b, plan.slots);
+        if (a.n_head * (D / 64) * a.rows * a.n_seq < kMergeMany) SHV_LAUNCH(ctx, (tree_merge_kernel<D, 8>), grid, dim3(512), 0, b, plan);
+        else SHV_LAUNCH(ctx, (tree_merge_kernel<D, 1>), grid, dim3(64), 0, b, plan);
     }
     return SHV_OK;
 }

@@ -19,142 +19,404 @@ using namespace shv;
 constexpr int kBlock = 256;
 constexpr int kD = 128;
 constexpr int kRows = SHV_TREE_MAX_ROWS;
-constexpr int kCols = 32;  // value columns of a block
+constexpr int kWaves = 8;
+
+typedef _Float16 half4_t __attribute__((ext_vector_type(4)));
+typedef _Float16 half8_t __attribute__((ext_vector_type(8)));
+typedef float float4_t __attribute__((ext_vector_type(4)));
+typedef float float4_u __attribute__((ext_vector_type(4), aligned(4)));  // rows may lie any number of floats apart
+typedef float float2_u __attribute__((ext_vector_type(2), aligned(4)));
 
 __device__ __forceinline__ float softplus_ref(float x) {
     // the add inside the log is float32 on purpose, as in the step's kernels: below about -16.6 it returns exactly 0
     return x > 20.f ? x : logf(1.f + expf(x));
 }
 
-struct TreeLds {
-    float q[kRows][kD + 4], k[kRows][kD + 4];
-    float s[kCols][kD + 4];
-    float a[kRows][kRows + 1], m[kRows][kRows + 1];
-    float d[kRows][kCols + 1], o[kRows][kCols + 1];
-    float G[kRows], beta[kRows];
-    uint32_t anc[kRows][2];
-    const float *src[kRows][4];  // the rows a row's taps meet, NULL before the sequence's start
+// float32 operands enter the matrix cores as two binary16 values, the small one scaled by 2^11 so that it stays normal, three products
+// a term: about 22 bits of each operand, accumulated in float32.
+constexpr float kLoScale = 2048.f, kLoInv = 1.f / 2048.f;
+__device__ __forceinline__ void split(float x, _Float16 &hi, _Float16 &lo) {
+    hi = static_cast<_Float16>(x);
+    lo = static_cast<_Float16>((x - static_cast<float>(hi)) * kLoScale);
+}
+__device__ __forceinline__ void mma32(half8_t xh, half8_t xl, half8_t yh, half8_t yl, float4_t &main, float4_t &low) {
+    main = __builtin_amdgcn_mfma_f32_16x16x32_f16(xh, yh, main, 0, 0, 0);
+    low = __builtin_amdgcn_mfma_f32_16x16x32_f16(xh, yl, low, 0, 0, 0);
+    low = __builtin_amdgcn_mfma_f32_16x16x32_f16(xl, yh, low, 0, 0, 0);
+}
+__device__ __forceinline__ void mma16(half4_t xh, half4_t xl, half4_t yh, half4_t yl, float4_t &main, float4_t &low) {
+    main = __builtin_amdgcn_mfma_f32_16x16x16f16(xh, yh, main, 0, 0, 0);
+    low = __builtin_amdgcn_mfma_f32_16x16x16f16(xh, yl, low, 0, 0, 0);
+    low = __builtin_amdgcn_mfma_f32_16x16x16f16(xl, yh, low, 0, 0, 0);
+}
+__device__ __forceinline__ float max_over_g(float v) {
+    auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+    r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ uint32_t or_over_g(uint32_t v) {
+    auto r = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+    v = r[0] | r[1];
+    r = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+    return r[0] | r[1];
+}
+// Sum over each half of the wave, in every lane of it.
+__device__ __forceinline__ float sum32(float v) {
+    v += dpp_f32<kDppXor1>(v);
+    v += dpp_f32<kDppXor2>(v);
+    v += dpp_f32<kDppHalfMirror>(v);
+    v += dpp_f32<kDppMirror>(v);
+    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+// The power of two that brings values of up to m to 1 and below (of 0 and of what is no number, 1), and its inverse.
+struct Scale {
+    float down, up;
+    __device__ __forceinline__ explicit Scale(float m) {
+        int e = static_cast<int>(__float_as_uint(m) >> 23) - 126;  // m < 2^e
+        e = m > 0.f && m < INFINITY ? max(e, -120) : 0;
+        down = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
+        up = __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
+    }
 };
 
-// grid: (128 / kCols, n_head_v, n_seq)
-__global__ __launch_bounds__(kBlock) void dn_tree_kernel(shv_dn_tree_args a) {
+constexpr int kKS = kD + 8;      // halves between rows of the [64][128] operands (272 B: 16 rows cover all banks)
+constexpr int kAS = kRows + 8;   // halves between rows of the [64][64] ones
+constexpr int kTS = 24;          // halves between rows of a 16 x 16 inverse
+template <int CT>
+struct TreeLds {
+    _Float16 kh[kRows][kKS], kl[kRows][kKS], qh[kRows][kKS], ql[kRows][kKS];
+    _Float16 ah[kRows][kAS], al[kRows][kAS], mh[kRows][kAS], ml[kRows][kAS];  // -A, strictly below the diagonal blocks' diagonals, and M
+    _Float16 th[4][16][kTS], tl[4][16][kTS];                                  // the inverses of the diagonal blocks of I + A
+    float adiag[4][16][17];
+    float v[kRows][16 * CT + 4];
+    float G[kRows], beta[kRows];
+    uint64_t anc[kRows];
+    int lost[kRows];  // bit 0: A's row holds what is no number, bit 1: M's
+};
+
+// grid: (8 / CT, n_head_v, n_seq), eight waves: a value head's rows against CT tiles of 16 of its 128 value columns.
+//   1  conv, SiLU and norm of q and k, conv and SiLU of v, a row a wave at a time, into LDS as operands
+//   2  P = K K^T and R = Q K^T in tiles of 16 x 16 on and below the diagonal, A and M from them where the column's row is an
+//      ancestor of the row's; the diagonal blocks of I + A inverted by substitution, a lane a column; and, a column tile a wave,
+//      K and Q against the state, which goes from memory to registers once
+//   3  a column tile a wave: the block rows' solve, the outputs.  A product's result is laid out as the next one's second operand,
+//      so a column tile never leaves its wave
+// A row whose delta is no number must reach its descendants alone, and the products are of whole tiles: A, M and B are cleaned of such values
+// first, and the outputs of rows that stand on one are made NaN at the end.  v, the state and B enter the products scaled by a power of two a column: any
+// float32.
+template <int CT>
+__global__ __launch_bounds__(64 * kWaves, 2) void dn_tree_kernel(shv_dn_tree_args a) {
     extern __shared__ __align__(16) char raw[];
-    TreeLds &L = *reinterpret_cast<TreeLds *>(raw);
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const int col0 = blockIdx.x * kCols, h = blockIdx.y, seq = blockIdx.z, hk = h % a.n_head_k;
+    TreeLds<CT> &L = *reinterpret_cast<TreeLds<CT> *>(raw);
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int n = lane & 15, g = lane >> 4;
+    const int slab = blockIdx.x, h = blockIdx.y, seq = blockIdx.z, hk = h % a.n_head_k;
     const int qk = a.n_head_k * kD, vw = a.n_head_v * kD;
     const TreeWords words(a.count, a.pos, a.slot, a.parent, a.conv1d, seq, a.rows, lane);
-    const int slot = words.slot, pos = words.pos;
-    const TreeRow t = tree_row(words.count, words.parent, a.rows, lane);
-    const int n = t.n;
-    if (n == 0) return;
     const float *x = a.x + static_cast<size_t>(seq) * a.rows * a.x_stride;
+    // asked for before anything is known: each lane's row's gates, the convs' taps, the state's columns
+    const float *gates = x + static_cast<size_t>(lane < a.rows ? lane : 0) * a.x_stride + 2 * qk + 2 * vw;
+    const float alpha = gates[h], write = gates[a.n_head_v + h], dt_bias = load_in_turn(a.dt_bias + h), decay = load_in_turn(a.a + h);
+    const int ch = lane < 32 ? hk * kD + 4 * lane : qk + hk * kD + 4 * (lane - 32);
+    constexpr int VC = CT == 8 ? 2 : 1;  // columns of v a lane takes
+    const int vcol = VC * (CT == 8 ? lane : lane & (16 * CT - 1)), vch = 2 * qk + h * kD + slab * 16 * CT + vcol;
+    float4_t tap[4], vtap[VC];
+#pragma unroll
+    for (int c = 0; c < 4; c++) tap[c] = *reinterpret_cast<const float4_t *>(a.conv1d + static_cast<size_t>(ch + c) * 4);
+#pragma unroll
+    for (int c = 0; c < VC; c++) vtap[c] = *reinterpret_cast<const float4_t *>(a.conv1d + static_cast<size_t>(vch + c) * 4);
+    const int slot = __builtin_amdgcn_readfirstlane(words.slot), pos = __builtin_amdgcn_readfirstlane(words.pos), rows = __builtin_amdgcn_readfirstlane(words.count);
+    if (rows == 0) return;
+    const int planes = a.n_planes > 1 ? a.n_planes : 1;
+    const int cur = a.plane && planes > 1 ? static_cast<int>(static_cast<unsigned>(a.plane[slot]) % static_cast<unsigned>(planes)) : 0;
+    const bool has_tile = wave < CT;  // of value columns
+    float4_t S[4][2];
+    if (has_tile) {
+        const float *state = a.state + ((static_cast<size_t>(slot) * planes + cur) * a.n_head_v + h) * kD * kD + static_cast<size_t>((slab * CT + wave) * 16 + n) * kD + 8 * g;
+#pragma unroll
+        for (int ks = 0; ks < 4; ks++)
+#pragma unroll
+            for (int e = 0; e < 2; e++) S[ks][e] = *reinterpret_cast<const float4_t *>(state + 32 * ks + 4 * e);
+    }
+    const TreeRow t = tree_row(rows, words.parent, a.rows, lane);
+    const int tiles = (rows + 15) / 16;
     const float *ring = a.ring + static_cast<size_t>(slot) * a.ring_slots * a.ring_stride;
-    {
-        // every wave forms the tables, the first one stores them
-        int up = lane < n ? lane : -1, above = 0;
-        float g = 0.f, b = 0.f;
-        if (lane < n) {
-            const float *row = x + static_cast<size_t>(lane) * a.x_stride + 2 * qk + 2 * vw;
-            g = softplus_ref(row[h] + a.dt_bias[h]) * a.a[h];
-            b = sigmoid_exact(row[a.n_head_v + h]);
-        }
-        const float *src[4];
+
+    // ---- 1 ----
+    struct Taps {
+        float4_t qk[4];
+        float v[4][VC];
+    };
+    // the row, its parent, grandparent and the one above it; behind the root the ring's rows, zeros before the start
+    const auto load = [&](Taps &f, int r) {
+        int up = r, back = 0;
 #pragma unroll
         for (int k = 0; k < 4; k++) {
+            const float *row;
+            bool there = true;
             if (up >= 0) {
-                src[k] = x + static_cast<size_t>(up) * a.x_stride;
+                row = x + static_cast<size_t>(up) * a.x_stride;
+                up = __builtin_amdgcn_readlane(t.parent, up);
             } else {
-                above++;
-                const int p = pos - above;
-                src[k] = p >= 0 ? ring + static_cast<size_t>(p % a.ring_slots) * a.ring_stride : nullptr;
+                const int p = pos - ++back;
+                there = p >= 0;
+                row = ring + static_cast<size_t>(there ? static_cast<uint32_t>(p) % static_cast<uint32_t>(a.ring_slots) : 0) * a.ring_stride;
             }
-            const int next = __shfl(t.parent, up < 0 ? 0 : up, 64);
-            up = up < 0 ? -1 : next;
+            f.qk[k] = *reinterpret_cast<const float4_u *>(row + ch);
+            if constexpr (VC == 2) {
+                const float2_u v = *reinterpret_cast<const float2_u *>(row + vch);
+                f.v[k][0] = v.x;
+                f.v[k][1] = v.y;
+            } else {
+                f.v[k][0] = row[vch];
+            }
+            if (!there) {
+                f.qk[k] = float4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int c = 0; c < VC; c++) f.v[k][c] = 0.f;
+            }
         }
-        const float G = tree_sum(t, g, a.rows, lane);
+    };
+    Taps now;
+    if (wave < rows) load(now, wave);
+    {
+        const float G = tree_sum(t, lane < rows ? softplus_ref(alpha + dt_bias) * decay : 0.f, a.rows, lane);
         if (wave == 0) {
             L.G[lane] = G;
-            L.beta[lane] = b;
-            L.anc[lane][0] = static_cast<uint32_t>(t.ancestors);
-            L.anc[lane][1] = static_cast<uint32_t>(t.ancestors >> 32);
+            L.beta[lane] = lane < rows ? sigmoid_exact(write) : 0.f;
+            L.anc[lane] = t.ancestors;
+            L.lost[lane] = 0;
+            if (slab == 0 && lane < rows) a.decay[(static_cast<size_t>(seq) * a.rows + lane) * a.n_head_v + h] = G;
+        }
+    }
+    const auto silu = [](float c) { return c * __builtin_amdgcn_rcpf(1.f + __expf(-c)); };
+    for (int r = wave; r < 16 * tiles; r += kWaves) {
+        float y[4], v[VC];
+        if (r < rows) {
+            float ss = 0.f;
 #pragma unroll
-            for (int k = 0; k < 4; k++) L.src[lane][k] = src[k];
-        }
-    }
-    const int planes = a.n_planes > 1 ? a.n_planes : 1;
-    const int cur = a.plane ? static_cast<int>(static_cast<unsigned>(a.plane[slot]) % static_cast<unsigned>(planes)) : 0;
-    const float *state = a.state + ((static_cast<size_t>(slot) * planes + cur) * a.n_head_v + h) * kD * kD + static_cast<size_t>(col0) * kD;
-    for (int i = tid; i < kCols * kD; i += kBlock) L.s[i / kD][i % kD] = state[i];
-    __syncthreads();
-    const auto conv = [&](int r, int ch) {
-        const float4 tp = *reinterpret_cast<const float4 *>(a.conv1d + static_cast<size_t>(ch) * 4);
-        const float w[4] = {tp.w, tp.z, tp.y, tp.x};
-        float c = 0.f;
-        for (int k = 3; k >= 0; k--) c += (L.src[r][k] ? L.src[r][k][ch] : 0.f) * w[k];
-        return c * sigmoid_exact(c);
-    };
-    for (int r = 0; r < n; r++) (tid < kD ? L.q : L.k)[r][tid & (kD - 1)] = conv(r, tid < kD ? hk * kD + tid : qk + hk * kD + tid - kD);
-    __syncthreads();
-    for (int v = wave; v < 2 * n; v += 4) {
-        float *row = v < n ? L.q[v] : L.k[v - n];
-        const float x0 = row[lane], x1 = row[lane + 64];
-        const float ss = wave_sum_all(fmaf(x0, x0, x1 * x1));
-        const float nrm = a.qk_norm_max ? 1.f / fmaxf(sqrtf(ss), a.eps) : 1.f / sqrtf(ss + a.eps);
-        row[lane] = x0 * nrm;
-        row[lane + 64] = x1 * nrm;
-    }
-    __syncthreads();
-    if (col0 == 0 && h < a.n_head_k)
-        for (int i = tid; i < n * kD; i += kBlock) a.kn[(static_cast<size_t>(seq) * a.rows + i / kD) * qk + hk * kD + i % kD] = L.k[i / kD][i % kD];
-    if (col0 == 0 && tid < n) a.decay[(static_cast<size_t>(seq) * a.rows + tid) * a.n_head_v + h] = L.G[tid];
-    for (int e = tid; e < n * n; e += kBlock) {
-        const int i = e / n, j = e % n;
-        float av = 0.f, mv = 0.f;
-        if (L.anc[i][j >> 5] >> (j & 31) & 1) {
-            float kk = 0.f, kq = 0.f;
-            for (int c = 0; c < kD; c++) {
-                kk = fmaf(L.k[i][c], L.k[j][c], kk);
-                kq = fmaf(L.q[i][c], L.k[j][c], kq);
+            for (int c = 0; c < 4; c++) {
+                float s = now.qk[3][c] * tap[c].x;
+                s = fmaf(now.qk[2][c], tap[c].y, s);
+                s = fmaf(now.qk[1][c], tap[c].z, s);
+                y[c] = silu(fmaf(now.qk[0][c], tap[c].w, s));
+                ss = fmaf(y[c], y[c], ss);
             }
-            const float fall = expf(L.G[i] - L.G[j]);
-            av = i == j ? 0.f : L.beta[i] * fall * kk;
-            mv = fall * kq;
+#pragma unroll
+            for (int c = 0; c < VC; c++) {
+                float s = now.v[3][c] * vtap[c].x;
+                s = fmaf(now.v[2][c], vtap[c].y, s);
+                s = fmaf(now.v[1][c], vtap[c].z, s);
+                v[c] = silu(fmaf(now.v[0][c], vtap[c].w, s));
+            }
+            if (r + kWaves < rows) load(now, r + kWaves);  // under the rest of this one
+            ss = sum32(ss);
+            const float nrm = a.qk_norm_max ? 1.f / fmaxf(sqrtf(ss), a.eps) : __builtin_amdgcn_rsqf(ss + a.eps);
+#pragma unroll
+            for (int c = 0; c < 4; c++) y[c] *= nrm;
+            if (slab == 0 && h < a.n_head_k && lane >= 32)
+                *reinterpret_cast<float4_t *>(a.kn + (static_cast<size_t>(seq) * a.rows + r) * qk + hk * kD + 4 * (lane - 32)) = float4_t{y[0], y[1], y[2], y[3]};
+        } else {
+#pragma unroll
+            for (int c = 0; c < 4; c++) y[c] = 0.f;
+#pragma unroll
+            for (int c = 0; c < VC; c++) v[c] = 0.f;
         }
-        L.a[i][j] = av;
-        L.m[i][j] = mv;
-    }
-    for (int e = tid; e < n * kCols; e += kBlock) {
-        const int i = e / kCols, c = e % kCols;
-        float sk = 0.f, sq = 0.f;
-        for (int u = 0; u < kD; u++) {
-            sk = fmaf(L.s[c][u], L.k[i][u], sk);
-            sq = fmaf(L.s[c][u], L.q[i][u], sq);
+        half4_t hi, lo;
+#pragma unroll
+        for (int c = 0; c < 4; c++) {
+            _Float16 p, q;
+            split(y[c], p, q);
+            hi[c] = p;
+            lo[c] = q;
         }
-        const float fall = expf(L.G[i]);
-        L.d[i][c] = L.beta[i] * (conv(i, 2 * qk + h * kD + col0 + c) - fall * sk);
-        L.o[i][c] = fall * sq;
+        *reinterpret_cast<half4_t *>(lane < 32 ? &L.qh[r][4 * lane] : &L.kh[r][4 * (lane - 32)]) = hi;
+        *reinterpret_cast<half4_t *>(lane < 32 ? &L.ql[r][4 * lane] : &L.kl[r][4 * (lane - 32)]) = lo;
+        if (CT == 8 || lane < 16 * CT) {
+#pragma unroll
+            for (int c = 0; c < VC; c++) L.v[r][vcol + c] = v[c];
+        }
     }
     __syncthreads();
-    if (tid < kCols) {
-        for (int i = 1; i < n; i++) {
-            float d = L.d[i][tid];
-            for (int j = 0; j < i; j++)
-                if (L.anc[i][j >> 5] >> (j & 31) & 1) d = fmaf(-L.a[i][j], L.d[j][tid], d);  // (another row's delta may be NaN)
-            L.d[i][tid] = d;
+
+    // ---- 2 ----
+    const auto tile = [&](int tt, int st) {
+        float4_t pm = {0.f, 0.f, 0.f, 0.f}, pl = pm, rm = pm, rl = pm;
+#pragma unroll
+        for (int ks = 0; ks < 4; ks++) {
+            const int c = 32 * ks + 8 * g;
+            const half8_t bh = *reinterpret_cast<const half8_t *>(&L.kh[16 * st + n][c]), bl = *reinterpret_cast<const half8_t *>(&L.kl[16 * st + n][c]);
+            mma32(*reinterpret_cast<const half8_t *>(&L.kh[16 * tt + n][c]), *reinterpret_cast<const half8_t *>(&L.kl[16 * tt + n][c]), bh, bl, pm, pl);
+            mma32(*reinterpret_cast<const half8_t *>(&L.qh[16 * tt + n][c]), *reinterpret_cast<const half8_t *>(&L.ql[16 * tt + n][c]), bh, bl, rm, rl);
+        }
+        const int s = 16 * st + n;
+        const float Gs = L.G[s];
+#pragma unroll
+        for (int r = 0; r < 4; r++) {
+            const int row = 16 * tt + 4 * g + r;
+            const bool above = (L.anc[row] >> s & 1) != 0;
+            const float dec = __expf(L.G[row] - Gs);
+            float av = above && s != row ? L.beta[row] * dec * fmaf(pl[r], kLoInv, pm[r]) : 0.f;
+            float mv = above ? dec * fmaf(rl[r], kLoInv, rm[r]) : 0.f;
+            if (!(fabsf(av) < INFINITY)) {
+                atomicOr(&L.lost[row], 1);
+                av = 0.f;
+            }
+            if (!(fabsf(mv) < INFINITY)) {
+                atomicOr(&L.lost[row], 2);
+                mv = 0.f;
+            }
+            _Float16 hi, lo;
+            split(-av, hi, lo);
+            L.ah[row][s] = hi;
+            L.al[row][s] = lo;
+            split(mv, hi, lo);
+            L.mh[row][s] = hi;
+            L.ml[row][s] = lo;
+            if (st == tt) L.adiag[tt][4 * g + r][n] = av;
+        }
+    };
+    if (wave < tiles) tile(wave, wave);
+    __syncthreads();
+    if (wave == kWaves - 1) {
+        // lane (block g, column n): its column of (I + A_gg)^-1, by forward substitution
+        if (g < tiles) {
+            float T[16];
+#pragma unroll
+            for (int i = 0; i < 16; i++) {
+                float s0 = i == n ? 1.f : 0.f, s1 = 0.f;
+#pragma unroll
+                for (int j = 0; j < i; j++) {
+                    const float av = L.adiag[g][i][j];
+                    if (j & 1) s1 = fmaf(-av, T[j], s1);
+                    else s0 = fmaf(-av, T[j], s0);
+                }
+                T[i] = s0 + s1;
+                _Float16 hi, lo;
+                split(T[i], hi, lo);
+                L.th[g][i][n] = hi;
+                L.tl[g][i][n] = lo;
+            }
+        }
+    } else {
+        // the tiles below the diagonal: (1,0) (2,0) (2,1) (3,0) (3,1) (3,2), one a wave
+        const int tt = wave < 1 ? 1 : wave < 3 ? 2 : 3, st = wave < 1 ? 0 : wave < 3 ? wave - 1 : wave - 3;
+        if (wave < 6 && tt < tiles) tile(tt, st);
+    }
+    float4_t B[4], O[4];  // of a row tile: B, and e^G Q S0
+    uint32_t bad_lo = 0, bad_hi = 0;
+    if (has_tile) {
+        float m = 0.f;
+#pragma unroll
+        for (int ks = 0; ks < 4; ks++)
+#pragma unroll
+            for (int e = 0; e < 8; e++) m = fmaxf(m, fabsf(S[ks][e >> 2][e & 3]));
+        const Scale scale(max_over_g(m));
+        half8_t sh[4], sl[4];
+#pragma unroll
+        for (int ks = 0; ks < 4; ks++)
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                _Float16 hi, lo;
+                split(S[ks][e >> 2][e & 3] * scale.down, hi, lo);
+                sh[ks][e] = hi;
+                sl[ks][e] = lo;
+            }
+#pragma unroll
+        for (int tt = 0; tt < 4; tt++) {
+            B[tt] = O[tt] = float4_t{0.f, 0.f, 0.f, 0.f};
+            if (tt >= tiles) continue;
+            float4_t km = {0.f, 0.f, 0.f, 0.f}, kl = km, qm = km, ql = km;
+#pragma unroll
+            for (int ks = 0; ks < 4; ks++) {
+                const int c = 32 * ks + 8 * g;
+                mma32(*reinterpret_cast<const half8_t *>(&L.kh[16 * tt + n][c]), *reinterpret_cast<const half8_t *>(&L.kl[16 * tt + n][c]), sh[ks], sl[ks], km, kl);
+                mma32(*reinterpret_cast<const half8_t *>(&L.qh[16 * tt + n][c]), *reinterpret_cast<const half8_t *>(&L.ql[16 * tt + n][c]), sh[ks], sl[ks], qm, ql);
+            }
+#pragma unroll
+            for (int r = 0; r < 4; r++) {
+                const int row = 16 * tt + 4 * g + r;
+                const float fall = __expf(L.G[row]) * scale.up;
+                float b = L.beta[row] * (L.v[row][16 * wave + n] - fall * fmaf(kl[r], kLoInv, km[r]));
+                if (!(fabsf(b) < INFINITY)) {
+                    if (row < 32) bad_lo |= 1u << row;
+                    else bad_hi |= 1u << (row - 32);
+                    b = 0.f;
+                }
+                B[tt][r] = b;
+                O[tt][r] = fall * fmaf(ql[r], kLoInv, qm[r]);
+            }
         }
     }
     __syncthreads();
-    const float scale = 1.f / sqrtf(static_cast<float>(kD));
-    for (int e = tid; e < n * kCols; e += kBlock) {
-        const int i = e / kCols, c = e % kCols;
-        float o = L.o[i][c];
-        for (int j = 0; j <= i; j++)
-            if (L.anc[i][j >> 5] >> (j & 31) & 1) o = fmaf(L.m[i][j], L.d[j][c], o);
-        const size_t at = (static_cast<size_t>(seq) * a.rows + i) * vw + static_cast<size_t>(h) * kD + col0 + c;
-        a.out[at] = o * scale;
-        a.delta[at] = L.d[i][c];
+    if (!has_tile) return;
+
+    // ---- 3 ----
+    const int lost_here = L.lost[lane];
+    const uint64_t bad = (static_cast<uint64_t>(or_over_g(bad_hi)) << 32 | or_over_g(bad_lo)) | __ballot((lost_here & 1) != 0), bad_out = __ballot((lost_here & 2) != 0);
+    float m = 0.f;
+#pragma unroll
+    for (int tt = 0; tt < 4; tt++)
+#pragma unroll
+        for (int r = 0; r < 4; r++) m = fmaxf(m, fabsf(B[tt][r]));
+    const Scale scale(max_over_g(m));
+    half4_t uh[4], ul[4];
+    const float root = 1.f / sqrtf(static_cast<float>(kD));
+#pragma unroll
+    for (int tt = 0; tt < 4; tt++) {
+        if (tt >= tiles) continue;
+        // U_t = T_tt (B_t - sum over s < t of A_ts U_s)
+        float4_t am = {0.f, 0.f, 0.f, 0.f}, alo = am;
+#pragma unroll
+        for (int st = 0; st < tt; st++)
+            mma16(*reinterpret_cast<const half4_t *>(&L.ah[16 * tt + n][16 * st + 4 * g]), *reinterpret_cast<const half4_t *>(&L.al[16 * tt + n][16 * st + 4 * g]), uh[st], ul[st], am, alo);
+        half4_t bh, bl;
+#pragma unroll
+        for (int r = 0; r < 4; r++) {
+            _Float16 hi, lo;
+            split(fmaf(B[tt][r], scale.down, fmaf(alo[r], kLoInv, am[r])), hi, lo);
+            bh[r] = hi;
+            bl[r] = lo;
+        }
+        float4_t um = {0.f, 0.f, 0.f, 0.f}, ulo = um;
+        mma16(*reinterpret_cast<const half4_t *>(&L.th[tt][n][4 * g]), *reinterpret_cast<const half4_t *>(&L.tl[tt][n][4 * g]), bh, bl, um, ulo);
+        float4_t u;
+#pragma unroll
+        for (int r = 0; r < 4; r++) {
+            u[r] = fmaf(ulo[r], kLoInv, um[r]);
+            _Float16 hi, lo;
+            split(u[r], hi, lo);
+            uh[tt][r] = hi;
+            ul[tt][r] = lo;
+        }
+        float4_t om = {0.f, 0.f, 0.f, 0.f}, olo = om;
+#pragma unroll
+        for (int st = 0; st <= tt; st++)
+            mma16(*reinterpret_cast<const half4_t *>(&L.mh[16 * tt + n][16 * st + 4 * g]), *reinterpret_cast<const half4_t *>(&L.ml[16 * tt + n][16 * st + 4 * g]), uh[st], ul[st], om, olo);
+#pragma unroll
+        for (int r = 0; r < 4; r++) {
+            const int row = 16 * tt + 4 * g + r;
+            if (row >= rows) continue;
+            const bool lost = (L.anc[row] & bad) != 0, lost_out = lost || (bad_out >> row & 1) != 0;
+            const size_t at = (static_cast<size_t>(seq) * a.rows + row) * vw + static_cast<size_t>(h) * kD + (slab * CT + wave) * 16 + n;
+            a.out[at] = lost_out ? __int_as_float(0x7fc00000) : fmaf(fmaf(olo[r], kLoInv, om[r]), scale.up, O[tt][r]) * root;
+            a.delta[at] = lost ? __int_as_float(0x7fc00000) : u[r] * scale.up;
+        }
     }
+}
+
+template <int CT>
+int launch_tree(shv_ctx *ctx, const shv_dn_tree_args &a) {
+    static std::atomic<uint64_t> raised{0};  // by device
+    const uint64_t bit = 1ull << (ctx->device & 63);
+    if (!(raised.load(std::memory_order_acquire) & bit)) {
+        SHV_HIP_CHECK(hipFuncSetAttribute(reinterpret_cast<const void *>(&dn_tree_kernel<CT>), hipFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(sizeof(TreeLds<CT>))));
+        raised.fetch_or(bit, std::memory_order_release);
+    }
+    SHV_LAUNCH(ctx, dn_tree_kernel<CT>, dim3(8 / CT, a.n_head_v, a.n_seq), dim3(64 * kWaves), sizeof(TreeLds<CT>), a);
+    return SHV_OK;
 }
 
 // grid: (8 slabs of 16 state rows, n_head_v, n_seq): a thread holds eight values of one row.  HBM-bound: the state is read once
@@ -239,13 +501,13 @@ int shv_launch_dn_tree(shv_ctx *ctx, const shv_dn_tree_args *pa) {
     SHV_REQUIRE(shv_aligned16(a.x) && shv_aligned16(a.state) && shv_aligned16(a.conv1d) && shv_aligned16(a.ring) && shv_aligned16(a.out) &&
                     shv_aligned16(a.kn) && shv_aligned16(a.delta),
                 "dn_tree: x, ring, conv1d, state, out, kn and delta must be 16-byte aligned");
-    static std::atomic<bool> raised{false};
-    if (!raised.load(std::memory_order_acquire)) {
-        SHV_HIP_CHECK(hipFuncSetAttribute(reinterpret_cast<const void *>(&dn_tree_kernel), hipFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(sizeof(TreeLds))));
-        raised.store(true, std::memory_order_release);
-    }
-    SHV_LAUNCH(ctx, dn_tree_kernel, dim3(kD / kCols, a.n_head_v, a.n_seq), dim3(kBlock), sizeof(TreeLds), a);
-    return SHV_OK;
+    // Columns cut in four, two or not at all: as far as every block still finds a compute unit of its own (a block's rows are prepared anew
+    // whatever its columns).  us of 5 / 64 rows of one sequence of 32 value heads cut in four 7.3 / 19.5, in two 8.2 / 19.4, whole
+    // 10.1 / 21.7; of four sequences 13.7 / 41, 8.5 / 22, 10.3 / 24.
+    const int heads = a.n_seq * a.n_head_v, units = ctx->prop.multiProcessorCount;
+    if (4 * heads <= units) return launch_tree<2>(ctx, a);
+    if (2 * heads <= units) return launch_tree<4>(ctx, a);
+    return launch_tree<8>(ctx, a);
 }
 
 int shv_launch_dn_keep(shv_ctx *ctx, const shv_dn_keep_args *pa) {

@@ -85,8 +85,8 @@ int shv_init(int device, shv_ctx **out) {
     if (e == hipSuccess) e = hipMalloc(reinterpret_cast<void **>(&ctx->argmax_idx), shv_ctx::kArgmaxBlocks * sizeof(int32_t));
     if (e == hipSuccess) e = hipMalloc(reinterpret_cast<void **>(&ctx->tree_val), shv_ctx::kTreePairs * sizeof(float));
     if (e == hipSuccess) e = hipMalloc(reinterpret_cast<void **>(&ctx->tree_idx), shv_ctx::kTreePairs * sizeof(int32_t));
-    if (e == hipSuccess) e = hipMalloc(reinterpret_cast<void **>(&ctx->tree_counters), shv_ctx::kTreeSeqs * shv_ctx::kTreeCounterStep * sizeof(int32_t));
-    if (e == hipSuccess) e = hipMemset(ctx->tree_counters, 0, shv_ctx::kTreeSeqs * shv_ctx::kTreeCounterStep * sizeof(int32_t));
+    if (e == hipSuccess) e = hipMalloc(reinterpret_cast<void **>(&ctx->tree_counters), shv_ctx::kTreeCounters * sizeof(int32_t));
+    if (e == hipSuccess) e = hipMemset(ctx->tree_counters, 0, shv_ctx::kTreeCounters * sizeof(int32_t));
     if (e == hipSuccess) e = hipMalloc(reinterpret_cast<void **>(&ctx->gemv_amax_val), shv_ctx::kGemvAmaxBlocks * sizeof(float));
     if (e == hipSuccess) e = hipMalloc(reinterpret_cast<void **>(&ctx->gemv_amax_idx), shv_ctx::kGemvAmaxBlocks * sizeof(int32_t));
     if (e != hipSuccess) {

@@ -79,11 +79,11 @@ struct shv_ctx {
     float *gemv_amax_val = nullptr;
     int32_t *gemv_amax_idx = nullptr;
     enum { kGemvAmaxBlocks = 2048 };
-    // per-block (value, index) pairs of a tree's rows, and the arrival counters of its sequences, a line apart (tree_accept)
+    // per-block (value, index) pairs of a tree's rows, and the arrival counters of its sequences and rows, a line apart (tree_accept)
     float *tree_val = nullptr;
     int32_t *tree_idx = nullptr;
     int32_t *tree_counters = nullptr;
-    enum { kTreePairs = SHV_TREE_ACCEPT_MAX_ROWS, kTreeSeqs = 1024, kTreeCounterStep = 32 };
+    enum { kTreePairs = SHV_TREE_ACCEPT_MAX_ROWS, kTreeSeqs = 1024, kTreeCounterStep = 32, kTreeCounters = (kTreeSeqs + SHV_TREE_ACCEPT_MAX_ROWS) * kTreeCounterStep };
     // device address of this GPU's copy of the library's static scratch array (misc.hip), for the
     // entry point that allocates nothing
     void *static_scratch = nullptr;

@@ -1,7 +1,8 @@
 // The branch of a drafted tree that the model agrees with: the arg-max of every row's logits and the walk over them, one launch.
 //
 // HBM-bound on the logits, which are read once: a row is cut into as many pieces as fill the chip, each block leaves its
-// piece's best, and the block of a sequence that finishes last joins the pieces of all its rows and walks the tree.  The walk
+// piece's best, the block of a row that finishes last joins the row's pieces, and the row of a sequence that does walks the tree.
+// (Counted by sequence alone, 64 rows of 64 pieces wait 15 ns each for one counter: 60 us, now 9.6.)  The walk
 // is one wave: lane i holds row i, a step asks all lanes at once which of them follow the row it stands on with the token that row
 // wants, and takes the lowest.
 #include "shv_device.hpp"
@@ -13,8 +14,10 @@ namespace {
 using namespace shv;
 
 constexpr int kBlock = 256;
+// us of 5 / 64 / 192 rows of 151936: pieces of 1024 floats at least 6.4 / 9.7 / 21, of 2048 5.6 / 9.6 / 21 (5.6 TB/s), of 8192 6.3 / 9.7 / 21; cut for
+// 4096 blocks 5.6 / 12.4 / 22.4, for 1024 5.6 / 9.6 / 20.9
 constexpr int kPiece = 2048;       // floats of a row a block takes at least
-constexpr int kBlocksWanted = 4096;
+constexpr int kBlocksWanted = 2048;
 
 // By one whole wave: best_of is the lane's row's best.
 __device__ __forceinline__ void walk(const shv_tree_accept_args &a, int seq, int best_of, int lane) {
@@ -47,7 +50,6 @@ __device__ __forceinline__ void walk(const shv_tree_accept_args &a, int seq, int
 __global__ __launch_bounds__(kBlock) void tree_accept_kernel(shv_tree_accept_args a, float *pval, int32_t *pidx, int32_t *counters) {
     __shared__ float sv[4];
     __shared__ int si[4];
-    __shared__ int best[SHV_TREE_MAX_ROWS];
     __shared__ int is_last;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int piece = blockIdx.x, nb = gridDim.x, r = blockIdx.y, seq = blockIdx.z;
@@ -83,22 +85,20 @@ __global__ __launch_bounds__(kBlock) void tree_accept_kernel(shv_tree_accept_arg
         store_agent(pval + row * nb + piece, bv);
         store_agent(pidx + row * nb + piece, bi);
     }
-    if (!arrive_last(counters + static_cast<size_t>(seq) * shv_ctx::kTreeCounterStep, n * nb, &is_last)) return;
-    // a wave joins every fourth row's pieces
-    for (int q = wave; q < n; q += 4) {
-        const size_t at = (static_cast<size_t>(seq) * a.rows + q) * nb;
-        bv = -INFINITY;
-        bi = a.n;
-        for (int b = lane; b < nb; b += 64) take(load_agent(pval + at + b), load_agent(pidx + at + b));
-        amax_wave(bv, bi);
-        if (bi >= a.n) bi = 0;  // nothing but NaN
-        if (lane == 0) {
-            best[q] = bi;
-            a.best[static_cast<size_t>(seq) * a.rows + q] = bi;
-        }
-    }
+    if (!arrive_last(counters + (shv_ctx::kTreeSeqs + row) * shv_ctx::kTreeCounterStep, nb, &is_last)) return;
+    bv = -INFINITY;
+    bi = a.n;
+    for (int b = tid; b < nb; b += kBlock) take(load_agent(pval + row * nb + b), load_agent(pidx + row * nb + b));
+    amax_wave(bv, bi);
+    if (lane == 0) { sv[wave] = bv; si[wave] = bi; }
     __syncthreads();
-    if (wave == 0) walk(a, seq, lane < n ? best[lane] : -1, lane);
+    if (tid == 0) {
+        for (int w = 1; w < 4; w++)
+            if (amax_better(sv[w], si[w], bv, bi)) { bv = sv[w]; bi = si[w]; }
+        store_agent(a.best + row, bi < a.n ? bi : 0);  // nothing but NaN: 0
+    }
+    if (!arrive_last(counters + static_cast<size_t>(seq) * shv_ctx::kTreeCounterStep, n, &is_last)) return;
+    if (wave == 0) walk(a, seq, lane < n ? load_agent(a.best + static_cast<size_t>(seq) * a.rows + lane) : -1, lane);
 }
 
 // grid: n_seq, one wave: the rows' tokens are in best already

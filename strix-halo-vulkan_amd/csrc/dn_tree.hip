@@ -91,7 +91,8 @@ struct TreeLds {
     _Float16 th[4][16][kTS], tl[4][16][kTS];                                  // the inverses of the diagonal blocks of I + A
     float adiag[4][16][17];
     float v[kRows][16 * CT + 4];
-    float G[kRows], beta[kRows];
+    double G[kRows];  // (differences of two of them are what counts: in float32 a row that forgets, log g = -100, would cost those behind it 2^-18)
+    float beta[kRows];
     uint64_t anc[kRows];
     int lost[kRows];  // bit 0: A's row holds what is no number, bit 1: M's
 };
@@ -182,13 +183,13 @@ __global__ __launch_bounds__(64 * kWaves, 2) void dn_tree_kernel(shv_dn_tree_arg
     Taps now;
     if (wave < rows) load(now, wave);
     {
-        const float G = tree_sum(t, lane < rows ? softplus_ref(alpha + dt_bias) * decay : 0.f, a.rows, lane);
+        const double G = tree_sum(t, lane < rows ? softplus_ref(alpha + dt_bias) * decay : 0.f, a.rows, lane);
         if (wave == 0) {
             L.G[lane] = G;
             L.beta[lane] = lane < rows ? sigmoid_exact(write) : 0.f;
             L.anc[lane] = t.ancestors;
             L.lost[lane] = 0;
-            if (slab == 0 && lane < rows) a.decay[(static_cast<size_t>(seq) * a.rows + lane) * a.n_head_v + h] = G;
+            if (slab == 0 && lane < rows) a.decay[(static_cast<size_t>(seq) * a.rows + lane) * a.n_head_v + h] = static_cast<float>(G);
         }
     }
     const auto silu = [](float c) { return c * __builtin_amdgcn_rcpf(1.f + __expf(-c)); };
@@ -252,12 +253,12 @@ __global__ __launch_bounds__(64 * kWaves, 2) void dn_tree_kernel(shv_dn_tree_arg
             mma32(*reinterpret_cast<const half8_t *>(&L.qh[16 * tt + n][c]), *reinterpret_cast<const half8_t *>(&L.ql[16 * tt + n][c]), bh, bl, rm, rl);
         }
         const int s = 16 * st + n;
-        const float Gs = L.G[s];
+        const double Gs = L.G[s];
 #pragma unroll
         for (int r = 0; r < 4; r++) {
             const int row = 16 * tt + 4 * g + r;
             const bool above = (L.anc[row] >> s & 1) != 0;
-            const float dec = __expf(L.G[row] - Gs);
+            const float dec = __expf(static_cast<float>(L.G[row] - Gs));
             float av = above && s != row ? L.beta[row] * dec * fmaf(pl[r], kLoInv, pm[r]) : 0.f;
             float mv = above ? dec * fmaf(rl[r], kLoInv, rm[r]) : 0.f;
             if (!(fabsf(av) < INFINITY)) {
@@ -338,7 +339,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void dn_tree_kernel(shv_dn_tree_arg
 #pragma unroll
             for (int r = 0; r < 4; r++) {
                 const int row = 16 * tt + 4 * g + r;
-                const float fall = __expf(L.G[row]) * scale.up;
+                const float fall = __expf(static_cast<float>(L.G[row])) * scale.up;
                 float b = L.beta[row] * (L.v[row][16 * wave + n] - fall * fmaf(kl[r], kLoInv, km[r]));
                 if (!(fabsf(b) < INFINITY)) {
                     if (row < 32) bad_lo |= 1u << row;

@@ -59,11 +59,11 @@ __device__ __forceinline__ TreeRow tree_row(int n, int parent, int rows, int lan
 }
 
 // Sum of v over a lane's row and the rows on its way to the root.
-__device__ __forceinline__ float tree_sum(const TreeRow &t, float v, int rows, int lane) {
+__device__ __forceinline__ double tree_sum(const TreeRow &t, double v, int rows, int lane) {
     int up = t.parent;
     for (int far = 1; far < rows; far *= 2) {
         const int from = up < 0 ? lane : up;
-        const float more = __shfl(v, from, 64);
+        const double more = __shfl(v, from, 64);
         const int next = __shfl(up, from, 64);
         v = up < 0 ? v : v + more;
         up = up < 0 ? -1 : next;

@@ -87,36 +87,73 @@ struct Plan {
 };
 __device__ __forceinline__ int over_rep(const Plan &plan, int r) { return static_cast<int>(static_cast<uint32_t>(r) * plan.rep_magic >> 20); }
 
+// Tiles that sequence s looks at; -1: it is left alone, as any behind the last is.
+__device__ __forceinline__ int tiles_of(const shv_attn_tree_args &a, int s) {
+    if (s >= a.n_seq) return -1;
+    const int pos = a.pos ? a.pos[s] : 0;
+    return fits(pos, tree_rows(a.count, s, a.rows), a.max_cells) ? Tiles(a, pos).all : -1;
+}
+
+// Tiles that all sequences look at.
+__device__ __forceinline__ uint32_t all_tiles(const shv_attn_tree_args &a, int lane) {
+    uint32_t total = 0;
+    for (int s0 = 0; s0 < a.n_seq; s0 += 64) {
+        uint32_t sum = max(tiles_of(a, s0 + lane), 0);
+#pragma unroll
+        for (int off = 32; off >= 1; off >>= 1) sum += __shfl_xor(sum, off, 64);
+        total = min(total + sum, 1u << 30);  // (64 sequences have at most 2^32 / 2^6 tiles)
+    }
+    return __builtin_amdgcn_readfirstlane(total);
+}
+
 // How a call's sequences are cut: slices of `len` tiles as many as the call has blocks for, and behind them one for the rows
 // themselves; where a call has one slice, it holds both.
 struct Cut {
     int len, cache, all;  // tiles of a slice, slices of the cache, slices
-    __device__ __forceinline__ Cut(const shv_attn_tree_args &a, int tiles, const Plan &plan, int lane) {
+    __device__ __forceinline__ Cut(const shv_attn_tree_args &a, int tiles, uint32_t total, const Plan &plan) {
         if (a.n_splits == 1) {
             len = tiles;
             cache = 0;
             all = 1;
             return;
         }
-        uint32_t total = tiles;
-        if (a.n_seq > 1) {
-            total = 0;
-            for (int s0 = 0; s0 < a.n_seq; s0 += 64) {
-                const int s = min(s0 + lane, a.n_seq - 1);
-                const int pos = a.pos ? a.pos[s] : 0;
-                uint32_t sum = s0 + lane < a.n_seq && fits(pos, tree_rows(a.count, s, a.rows), a.max_cells) ? Tiles(a, pos).all : 0;
-#pragma unroll
-                for (int off = 32; off >= 1; off >>= 1) sum += __shfl_xor(sum, off, 64);
-                total = min(total + sum, 1u << 30);  // (64 sequences have at most 2^32 / 2^6 tiles)
-            }
-        }
-        total = __builtin_amdgcn_readfirstlane(total);
         const uint32_t slots = plan.slots, least = plan.least, share = (total + slots - 1) / slots, room = a.n_splits - 1;
         uint32_t l = share > least ? share : least;
         if (l * static_cast<uint64_t>(room) < static_cast<uint32_t>(tiles)) l = (tiles + room - 1) / room;
         len = l;
         cache = (tiles + l - 1) / l;
         all = cache + 1;
+    }
+};
+
+// The `work`-th slice of all the call's: whose it is and which of its own; seq -1: there are fewer.  The slices stand in a row, without gaps for
+// sequences that have fewer of them: blocks that find nothing to do and end, one in seven between those that work, leave the latter on
+// few compute units (six windows of 9 slices in a grid of 64 a sequence 66 us, of 72 40, in a row 24).
+struct Slice {
+    int seq, split;
+    __device__ __forceinline__ Slice(const shv_attn_tree_args &a, int work, uint32_t total, const Plan &plan, int lane) {
+        seq = a.n_seq == 1 ? 0 : -1;
+        split = work;
+        if (a.n_seq == 1) return;
+        int before = 0;
+        for (int s0 = 0; s0 < a.n_seq; s0 += 64) {
+            const int tiles = tiles_of(a, s0 + lane);
+            const int mine = tiles < 0 ? 0 : Cut(a, tiles, total, plan).all;
+            int upto = mine;
+#pragma unroll
+            for (int off = 1; off < 64; off <<= 1) {
+                const int less = __shfl_up(upto, off, 64);
+                if (lane >= off) upto += less;
+            }
+            const uint64_t past = __ballot(before + upto > work);
+            if (past != 0) {
+                const int l = __ffsll(static_cast<unsigned long long>(past)) - 1;
+                seq = s0 + l;
+                split = work - before - __builtin_amdgcn_readlane(upto - mine, l);
+                return;
+            }
+            before += __builtin_amdgcn_readlane(upto, 63);
+        }
     }
 };
 
@@ -284,10 +321,10 @@ __global__ __launch_bounds__(256) void tree_prep_kernel(shv_attn_tree_args a, Pl
 template <int D, int W>
 struct TreeSmem {
     char ring[kStages][D / 8 * kChunk];
-    float p[W][16 * kTile];  // a wave's weights of a tile, where its values are not all finite
+    float p[W][16 * kTile / 2];  // a wave's weights of half a tile, where its values are not all finite (a whole one's would leave a unit one block of D 128)
 };
 
-// grid: (slices rounded up to 8, times query blocks; n_head_kv; n_seq), four waves.  A wave holds GW groups of 16 query rows: query row r of a KV
+// grid: (slices rounded up to 8, times query blocks; n_head_kv), W waves.  A wave holds GW groups of 16 query rows: query row r of a KV
 // head is head r % rep of tree row r / rep.  GW 1: calls of up to 64 query rows a KV head, whose rows are normed and turned here, by every
 // block; GW 2: wider ones, whose rows a launch before (tree_prep_kernel) has left as operands: there every block has 128 rows to prepare,
 // 5 us before its first product, and the launch costs 4.
@@ -304,8 +341,12 @@ __global__ __launch_bounds__(64 * W, W == 4 || D == 256 ? 2 : 4) void tree_attn_
     const int n = lane & 15, q = lane >> 4;
     // blocks of one slice lie on one die (workgroups go to the dies in turn) and find its tiles in the die's L2
     const int eight = blockIdx.x >> 3, of_eight = static_cast<int>(static_cast<uint32_t>(eight) / static_cast<uint32_t>(plan.q_blocks));
-    const int split = of_eight * 8 + (blockIdx.x & 7), qb = eight - of_eight * plan.q_blocks;
-    const int kvh = blockIdx.y, seq = blockIdx.z;
+    const int work = of_eight * 8 + (blockIdx.x & 7), qb = eight - of_eight * plan.q_blocks;
+    const int kvh = blockIdx.y;
+    const uint32_t total = a.n_seq > 1 ? all_tiles(a, lane) : 0;
+    const Slice slice(a, work, total, plan, lane);
+    if (slice.seq < 0) return;
+    const int seq = __builtin_amdgcn_readfirstlane(slice.seq), split = __builtin_amdgcn_readfirstlane(slice.split);
     const int rep = a.n_head / a.n_head_kv;
     const TreeWords words(a.count, a.pos, a.slot, a.parent, a.q_norm, seq, a.rows, lane);
     const float *qkv = a.qkv + static_cast<size_t>(seq) * a.rows * a.qkv_stride;
@@ -329,7 +370,7 @@ __global__ __launch_bounds__(64 * W, W == 4 || D == 256 ? 2 : 4) void tree_attn_
     const int r_end = rows * rep;
     if (!fits(pos, rows, a.max_cells) || qb * W * 16 >= r_end) return;
     const Tiles tiles(a, pos);
-    const Cut cut(a, tiles.all, plan, lane);
+    const Cut cut(a, tiles.all, a.n_seq > 1 ? total : tiles.all, plan);
     if (split >= cut.all) return;
     const bool with_rows = split == cut.all - 1;
     const int t0 = with_rows && cut.all > 1 ? 0 : split * cut.len;
@@ -604,21 +645,28 @@ __global__ __launch_bounds__(64 * W, W == 4 || D == 256 ? 2 : 4) void tree_attn_
             }
             if (__ballot(odd != 0) != 0ull) {
                 float *p = sm.p[wave];
+#pragma unroll 1
+                for (int h = 0; h < 2; h++) {
+                    if ((q >> 1) == h) {
 #pragma unroll
-                for (int e = 0; e < 8; e++) p[n * kTile + 8 * q + e] = seen >> e & 1 ? pv[e] : -1.f;
-                __builtin_amdgcn_wave_barrier();
-                for (int c = 0; c < kTile; c++) {
-                    float w[4];
-#pragma unroll
-                    for (int e = 0; e < 4; e++) w[e] = p[(4 * q + e) * kTile + c];
-#pragma unroll
-                    for (int db = 0; db < DB; db++) {
-                        const float v = static_cast<float>(*reinterpret_cast<const _Float16 *>(vt + db * kChunk + (16 * (c >> 3) + n) * 16 + (c & 7) * 2));
-#pragma unroll
-                        for (int e = 0; e < 4; e++) o[db][e] = w[e] < 0.f ? o[db][e] : fmaf(w[e], v, o[db][e]);
+                        for (int e = 0; e < 8; e++) p[n * (kTile / 2) + 8 * (q & 1) + e] = seen >> e & 1 ? pv[e] : -1.f;
                     }
+                    __builtin_amdgcn_wave_barrier();
+#pragma unroll 1
+                    for (int i = 0; i < kTile / 2; i++) {
+                        const int c = kTile / 2 * h + i;
+                        float w[4];
+#pragma unroll
+                        for (int e = 0; e < 4; e++) w[e] = p[(4 * q + e) * (kTile / 2) + i];
+#pragma unroll
+                        for (int db = 0; db < DB; db++) {
+                            const float v = static_cast<float>(*reinterpret_cast<const _Float16 *>(vt + db * kChunk + (16 * (c >> 3) + n) * 16 + (c & 7) * 2));
+#pragma unroll
+                            for (int e = 0; e < 4; e++) o[db][e] = w[e] < 0.f ? o[db][e] : fmaf(w[e], v, o[db][e]);
+                        }
+                    }
+                    __builtin_amdgcn_wave_barrier();
                 }
-                __builtin_amdgcn_wave_barrier();
                 continue;
             }
         }
@@ -686,7 +734,8 @@ __global__ __launch_bounds__(64 * NW) void tree_merge_kernel(shv_attn_tree_args 
     const int rep = a.n_head / a.n_head_kv, kvh = head / rep;
     const int pos = a.pos ? a.pos[seq] : 0, rows = tree_rows(a.count, seq, a.rows);
     if (row >= rows || !fits(pos, rows, a.max_cells)) return;
-    const Cut cut(a, Tiles(a, pos).all, plan, lane);
+    const int tiles = Tiles(a, pos).all;
+    const Cut cut(a, tiles, a.n_seq > 1 ? all_tiles(a, lane) : tiles, plan);
     if (cut.all == 1) return;  // put straight out
     const float c2 = 1.44269504088896f / sqrtf(static_cast<float>(D));
     const size_t step = static_cast<size_t>(a.rows) * rep * (D + 2);
@@ -745,7 +794,8 @@ int launch_tree(shv_ctx *ctx, const shv_attn_tree_args &a) {
     constexpr int kBlocksPerUnit = D == 256 ? 1 : 2;
     Plan plan;
     plan.q_blocks = (a.rows * rep + 16 * W - 1) / (16 * W);
-    plan.slots = ctx->prop.multiProcessorCount * kBlocksPerUnit / (a.n_head_kv * plan.q_blocks) - a.n_seq;
+    // beside them every sequence has a slice for its rows and, of several, one that is not full
+    plan.slots = ctx->prop.multiProcessorCount * kBlocksPerUnit / (a.n_head_kv * plan.q_blocks) - (a.n_seq > 1 ? 2 : 1) * a.n_seq;
     if (plan.slots < 1) plan.slots = 1;
     // A tile more to a slice costs a narrow call 1.2 us and a wide one 1.4; of a slice more the merge reads a record more of every row.
     plan.least = W == 4 ? kLeastNarrow : kLeastWide;
@@ -767,9 +817,10 @@ int launch_tree(shv_ctx *ctx, const shv_attn_tree_args &a) {
         const int items = a.rows * (a.n_head + a.n_head_kv);
         SHV_LAUNCH(ctx, tree_prep_kernel<D>, dim3((items + 3) / 4, a.n_seq), dim3(256), 0, a, plan, stage);
     }
-    const int most = plan.slots + 1 + a.n_seq;
-    if (b.n_splits > most) b.n_splits = most;
-    SHV_LAUNCH(ctx, (tree_attn_kernel<D, W>), dim3((b.n_splits + 7) / 8 * 8 * plan.q_blocks, a.n_head_kv, a.n_seq), dim3(64 * W), sizeof(TreeSmem<D, W>), b, plan, stage);
+    if (b.n_splits > plan.slots + 2) b.n_splits = plan.slots + 2;  // no sequence is cut into more
+    // slices of len tiles: all / len <= slots of them are full, every sequence may have one that is not, and has one of its rows
+    const long long slices = b.n_splits == 1 ? a.n_seq : plan.slots + 2ll * a.n_seq;
+    SHV_LAUNCH(ctx, (tree_attn_kernel<D, W>), dim3(static_cast<unsigned>((slices + 7) / 8 * 8 * plan.q_blocks), a.n_head_kv), dim3(64 * W), sizeof(TreeSmem<D, W>), b, plan, stage);
     if (b.n_splits > 1) {
         const dim3 grid(a.n_head * (D / 64), a.rows, a.n_seq);
         if (a.n_head * (D / 64) * a.rows * a.n_seq < kMergeMany) SHV_LAUNCH(ctx, (tree_merge_kernel<D, 8>), grid, dim3(512), 0, b, plan);

@@ -61,7 +61,10 @@ constexpr int kStages = 4, kAhead = kStages - 1;
 // 2^-31 of the largest with the smaller half's last place (at a lift of 0 2^-24, 6e-6 of a weight of a hundredth).
 constexpr float kLift = 7.f, kSlack = 8.f;
 constexpr int kLeastNarrow = 2, kLeastWide = 3;
-constexpr int kMergeMany = 1024;  // 64-dim pieces of rows and heads from which one wave joins the slices of each
+// Waves that join the slices of 256 dims' rows: one where there are many such pieces, eight where there are some, four where there are few.  us
+// by one / four / eight waves: 32 pieces of 13 slices 3.9 / 4.2 / 5.4 (of 130 slices one wave would go to memory nine times in a row), 192 of
+// 95 14.5 / 8.6 / 7.6, 1024 of 32 10.8 / 11.9 / 19, 2016 of 11 6.0 / 10.7 / 21.
+constexpr int kMergeMany = 512, kMergeSome = 64;
 
 // Which tiles of 32 cells a sequence's rows look at: the sinks', then those the window of the first row reaches.
 struct Tiles {
@@ -317,6 +320,9 @@ __global__ __launch_bounds__(256) void tree_prep_kernel(shv_attn_tree_args a, Pl
     put_bytes<2 * VEC>(dst + 4 * here * 16, lo);
     static_assert(KI * 32 == D, "whole steps");
 }
+
+// Floats of all records' sums.
+__device__ __forceinline__ size_t record_floats(const shv_attn_tree_args &a, int D) { return static_cast<size_t>(a.n_seq) * a.rows * a.n_head * a.n_splits * D; }
 
 template <int D, int W>
 struct TreeSmem {
@@ -711,81 +717,82 @@ __global__ __launch_bounds__(64 * W, W == 4 || D == 256 ? 2 : 4) void tree_attn_
         }
         return;
     }
-    // the slice's record of each query row: unnormalised sums, then (max, sum)
-    float *rec = a.partial + ((static_cast<size_t>(seq) * a.n_head_kv + kvh) * a.n_splits + split) * (a.rows * rep) * (D + 2);
+    // the slice's record of each query row: unnormalised sums, and behind all records' the (max, sum)
+    const size_t base = ((static_cast<size_t>(seq) * a.n_head_kv + kvh) * a.n_splits + split) * (static_cast<size_t>(a.rows) * rep);
 #pragma unroll
     for (int i = 0; i < 4; i++) {
         const int r = r0 + 4 * q + i;
         if (r >= r_end) continue;
+        float *rec = a.partial + (base + r) * D;
 #pragma unroll
-        for (int db = 0; db < DB; db++) rec[static_cast<size_t>(r) * (D + 2) + 16 * db + n] = o[db][i];
+        for (int db = 0; db < DB; db++) rec[16 * db + n] = o[db][i];
     }
-    if (q == 0 && r0 + n < r_end) *reinterpret_cast<float2 *>(rec + static_cast<size_t>(r0 + n) * (D + 2) + D) = make_float2(m_run, sum);
+    if (q == 0 && r0 + n < r_end) reinterpret_cast<float2 *>(a.partial + record_floats(a, D))[base + r0 + n] = make_float2(m_run, sum);
 }
 
-// The slices' records of a row and head joined, a thread a dim.  NW waves share the records of 64 dims, each folds its share with all of a
-// batch's loads on their way together, and the first wave folds their results: eight waves where a call has few rows and heads, one
-// otherwise.  grid: (n_head * D / 64, rows, n_seq).
+// The slices' records of a row and head joined, a lane four dims.  NW waves share the records of 256 / D rows' heads, each folds its share with
+// all of a batch's loads on their way together, and the first wave folds their results.  grid: (ceil(rows * n_head * D / 256), n_seq).
 template <int D, int NW>
 __global__ __launch_bounds__(64 * NW) void tree_merge_kernel(shv_attn_tree_args a, Plan plan) {
-    __shared__ float red[3][NW][64];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int head = blockIdx.x / (D / 64), d = blockIdx.x % (D / 64) * 64 + lane, row = blockIdx.y, seq = blockIdx.z;
-    const int rep = a.n_head / a.n_head_kv, kvh = head / rep;
+    __shared__ float4_t sums[NW][64];
+    __shared__ float2 of[NW][64];
+    constexpr int kLanes = D / 4;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, seq = blockIdx.y;
+    const int rep = a.n_head / a.n_head_kv;
     const int pos = a.pos ? a.pos[seq] : 0, rows = tree_rows(a.count, seq, a.rows);
-    if (row >= rows || !fits(pos, rows, a.max_cells)) return;
+    const uint32_t unit = blockIdx.x * (64 / kLanes) + lane / kLanes;
+    const int row = static_cast<int>(unit / static_cast<uint32_t>(a.n_head)), head = static_cast<int>(unit) - row * a.n_head;
+    const bool there = row < rows;
+    if (!fits(pos, rows, a.max_cells) || __ballot(there) == 0ull) return;
     const int tiles = Tiles(a, pos).all;
     const Cut cut(a, tiles, a.n_seq > 1 ? all_tiles(a, lane) : tiles, plan);
     if (cut.all == 1) return;  // put straight out
     const float c2 = 1.44269504088896f / sqrtf(static_cast<float>(D));
-    const size_t step = static_cast<size_t>(a.rows) * rep * (D + 2);
-    const float *from = a.partial + (static_cast<size_t>(seq) * a.n_head_kv + kvh) * a.n_splits * step + static_cast<size_t>(row * rep + head % rep) * (D + 2);
+    const int kvh = over_rep(plan, head), r = there ? row * rep + head - kvh * rep : 0;
+    const size_t per = static_cast<size_t>(a.rows) * rep, base = (static_cast<size_t>(seq) * a.n_head_kv + kvh) * a.n_splits * per + r;
+    const float4_t *from = reinterpret_cast<const float4_t *>(a.partial + base * D) + lane % kLanes;
+    const float2 *from_of = reinterpret_cast<const float2 *>(a.partial + record_floats(a, D)) + base;
     constexpr int MB = 16;
-    float num = 0.f, den = 0.f, M = -INFINITY;
+    float4_t num = {0.f, 0.f, 0.f, 0.f};
+    float den = 0.f, M = -INFINITY;
+    const auto fold = [&](const float4_t &v, float2 ml) {
+        if (ml.x == -INFINITY && ml.y == 0.f) return;  // (sees nothing; a sum of NaN stays)
+        const float Mn = fmaxf(M, ml.x);
+        const float shrink = __builtin_amdgcn_exp2f((M - Mn) * c2), w = __builtin_amdgcn_exp2f((ml.x - Mn) * c2);
+        den = fmaf(den, shrink, w * ml.y);
+#pragma unroll
+        for (int e = 0; e < 4; e++) num[e] = fmaf(num[e], shrink, w * v[e]);
+        M = Mn;
+    };
     for (int s0 = wave; s0 < cut.all; s0 += NW * MB) {
-        float v[MB];
+        float4_t v[MB];
         float2 ml[MB];
 #pragma unroll
         for (int u = 0; u < MB; u++) {
-            const int s = s0 + NW * u < cut.all ? s0 + NW * u : s0;
-            v[u] = from[s * step + d];
-            ml[u] = *reinterpret_cast<const float2 *>(from + s * step + D);
+            const size_t s = s0 + NW * u < cut.all ? s0 + NW * u : s0;
+            v[u] = from[s * per * kLanes];
+            ml[u] = from_of[s * per];
         }
 #pragma unroll
         for (int u = 0; u < MB; u++) asm volatile("" : "+v"(v[u]));  // asked for together, not each behind the one before's test
 #pragma unroll
-        for (int u = 0; u < MB; u++) {
-            if (s0 + NW * u >= cut.all || (ml[u].x == -INFINITY && ml[u].y == 0.f)) continue;  // (sees nothing; a sum of NaN stays)
-            const float Mn = fmaxf(M, ml[u].x);
-            const float shrink = __builtin_amdgcn_exp2f((M - Mn) * c2), w = __builtin_amdgcn_exp2f((ml[u].x - Mn) * c2);
-            den = fmaf(den, shrink, w * ml[u].y);
-            num = fmaf(num, shrink, w * v[u]);
-            M = Mn;
-        }
+        for (int u = 0; u < MB; u++)
+            if (s0 + NW * u < cut.all) fold(v[u], ml[u]);
     }
-    float *out = a.out + ((static_cast<size_t>(seq) * a.rows + row) * a.n_head + head) * D + d;
-    if constexpr (NW == 1) {
-        *out = num / den;
-        return;
-    }
-    red[0][wave][lane] = M;
-    red[1][wave][lane] = den;
-    red[2][wave][lane] = num;
-    __syncthreads();
-    if (wave != 0) return;
-    float Mt = red[0][0][lane];
+    if constexpr (NW > 1) {
+        sums[wave][lane] = num;
+        of[wave][lane] = make_float2(M, den);
+        __syncthreads();
+        if (wave != 0) return;
 #pragma unroll
-    for (int k = 1; k < NW; k++) Mt = fmaxf(Mt, red[0][k][lane]);
-    float nt = 0.f, dt = 0.f;
-#pragma unroll
-    for (int k = 0; k < NW; k++) {
-        const float mk = red[0][k][lane];
-        if (mk == -INFINITY && red[1][k][lane] == 0.f) continue;
-        const float w = __builtin_amdgcn_exp2f((mk - Mt) * c2);
-        dt = fmaf(w, red[1][k][lane], dt);
-        nt = fmaf(w, red[2][k][lane], nt);
+        for (int k = 1; k < NW; k++) fold(sums[k][lane], of[k][lane]);
     }
-    *out = nt / dt;
+    if (there) {
+        float4_t y;
+#pragma unroll
+        for (int e = 0; e < 4; e++) y[e] = num[e] / den;
+        *(reinterpret_cast<float4_t *>(a.out + ((static_cast<size_t>(seq) * a.rows + row) * a.n_head + head) * D) + lane % kLanes) = y;
+    }
 }
 
 template <int D, int W>
@@ -822,9 +829,11 @@ int launch_tree(shv_ctx *ctx, const shv_attn_tree_args &a) {
     const long long slices = b.n_splits == 1 ? a.n_seq : plan.slots + 2ll * a.n_seq;
     SHV_LAUNCH(ctx, (tree_attn_kernel<D, W>), dim3(static_cast<unsigned>((slices + 7) / 8 * 8 * plan.q_blocks), a.n_head_kv), dim3(64 * W), sizeof(TreeSmem<D, W>), b, plan, stage);
     if (b.n_splits > 1) {
-        const dim3 grid(a.n_head * (D / 64), a.rows, a.n_seq);
-        if (a.n_head * (D / 64) * a.rows * a.n_seq < kMergeMany) SHV_LAUNCH(ctx, (tree_merge_kernel<D, 8>), grid, dim3(512), 0, b, plan);
-        else SHV_LAUNCH(ctx, (tree_merge_kernel<D, 1>), grid, dim3(64), 0, b, plan);
+        const int units = (a.rows * a.n_head * D + 255) / 256;
+        const dim3 grid(units, a.n_seq);
+        if (units * a.n_seq >= kMergeMany) SHV_LAUNCH(ctx, (tree_merge_kernel<D, 1>), grid, dim3(64), 0, b, plan);
+        else if (units * a.n_seq >= kMergeSome) SHV_LAUNCH(ctx, (tree_merge_kernel<D, 8>), grid, dim3(512), 0, b, plan);
+        else SHV_LAUNCH(ctx, (tree_merge_kernel<D, 4>), grid, dim3(256), 0, b, plan);
     }
     return SHV_OK;
 }

@@ -46,13 +46,13 @@ __device__ __forceinline__ void walk(const shv_tree_accept_args &a, int seq, int
     }
 }
 
-// grid: (pieces, rows, n_seq)
+// grid: (pieces, n_seq, rows): rows that are not in use come last
 __global__ __launch_bounds__(kBlock) void tree_accept_kernel(shv_tree_accept_args a, float *pval, int32_t *pidx, int32_t *counters) {
     __shared__ float sv[4];
     __shared__ int si[4];
     __shared__ int is_last;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const int piece = blockIdx.x, nb = gridDim.x, r = blockIdx.y, seq = blockIdx.z;
+    const int piece = blockIdx.x, nb = gridDim.x, r = blockIdx.z, seq = blockIdx.y;
     const int n = tree_rows(a.count, seq, a.rows);
     if (r >= n) {
         if (n == 0 && r == 0 && piece == 0 && wave == 0) walk(a, seq, -1, lane);
@@ -127,6 +127,6 @@ int shv_launch_tree_accept(shv_ctx *ctx, const shv_tree_accept_args *pa) {
     int nb = (a.n + kPiece - 1) / kPiece;
     const int fill = kBlocksWanted / all > 1 ? kBlocksWanted / all : 1;
     if (nb > fill) nb = fill;
-    SHV_LAUNCH(ctx, tree_accept_kernel, dim3(nb, a.rows, a.n_seq), dim3(kBlock), 0, a, ctx->tree_val, ctx->tree_idx, ctx->tree_counters);
+    SHV_LAUNCH(ctx, tree_accept_kernel, dim3(nb, a.n_seq, a.rows), dim3(kBlock), 0, a, ctx->tree_val, ctx->tree_idx, ctx->tree_counters);
     return SHV_OK;
 }

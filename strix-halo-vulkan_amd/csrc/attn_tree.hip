@@ -413,7 +413,9 @@ __global__ __launch_bounds__(64 * W, W == 4 || D == 256 ? 2 : 4) void tree_attn_
             ql[i] = *reinterpret_cast<const half8_t *>(mine + (i * 8 + 4) * here * 16);
         }
     }
-    const TreeRow t = tree_row(rows, words.parent, a.rows, lane);
+    // (a wide call's slice of the cache has no use for the tree but for a window's edge: 2 of its 24 thousand cycles)
+    TreeRow t{rows, -1, 0, 0};
+    if (!kWide || with_rows || a.window > 0) t = tree_row(rows, words.parent, a.rows, lane);
     const Turn<D> shape(a.rope_dims, lane);
     const auto load_turn = [&](Turn<D> &turn, int row) { turn.load(a.rope + static_cast<size_t>(pos + __builtin_amdgcn_readlane(t.depth, row)) * a.rope_dims, a.rope_dims); };
     const auto turn_four = [&](Turn<D>(&turn)[4], int f) {

@@ -576,8 +576,8 @@ typedef struct {
  * rows of a sequence form a tree, row 0 the token the sequence goes on with and every other row one that may follow its parent.
  *   parent [n_seq][rows]: the row each row follows, a lower one.  A parent that is not (-1 by custom) makes the row follow the
  *     sequence's last kept token, as row 0 does; such a row is computed but never accepted.  NULL: a chain, parent[i] = i - 1.
- *   count [n_seq]: rows in use, 0 .. rows; a larger number means rows, a negative one 0.  NULL: all.  Of rows past it nothing
- *     is read and nothing is written.
+ *   count [n_seq]: rows in use, 0 .. rows; a larger number means rows, a negative one 0.  NULL: all.  Rows past it may hold
+ *     anything, and what would be theirs in an output stays as it was.
  *   pos, slot as in the other ops: sequence s has kept pos[s] tokens (NULL: none) and owns cache or state slot slot[s] (NULL: s).
  * A row sits at position pos + its depth.  The pass itself changes neither cache, ring nor state: shv_attn_tree and shv_dn_tree
  * leave beside their outputs what is needed to keep a branch, shv_tree_accept finds the branch, shv_attn_keep and

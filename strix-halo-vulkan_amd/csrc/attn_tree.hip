@@ -1,4 +1,19 @@
 // Full attention over a tree of drafted tokens, and the kept branch's cells into the cache.
+//
+// Row i of a tree, at position p_i = pos + depth_i, sees the cells c < pos, the rows on its way to the root and itself; with a window those of
+// them alone whose position is below `sinks` or above p_i - window:
+//     out_i = sum over them of softmax(q_i . k_j / sqrt(d)) v_j
+// q and k normed over a head and rotated at their positions.  A block takes one KV head, a slice of the cache in tiles of 32 cells and up to
+// 64 or 128 query rows (query row r is head r % rep of tree row r / rep), 16 a wave, on v_mfma_f32_16x16x32_f16:
+//     S^T = K Q^T   the cache's binary16 keys against the queries as two halves; a lane then holds eight cells of one query row, the operand
+//                   of the second product
+//     O  += P V     weights as two halves against values, which the cache holds by dim
+// with a running maximum and sum.  Tiles go from memory to LDS past the registers, three ahead.  The rows' own keys and values never enter the
+// cache here: one more block of a KV head forms their cells, attends over them by the ancestors' bits, and leaves them for attn_keep.  A second
+// launch joins the slices.
+// What bounds it: one or two rows behind a long cache the cache's bytes (131000 cells 54 us, 5.0 TB/s of K and V); 64 rows the matrix cores (64
+// rows of 16 heads behind 131000 cells 262 us, 1.05 PFLOP/s of binary16 products, where a large library product reaches 1.18); short
+// caches the chain of trips to memory before the first product (2 rows behind 700 cells 9 us and 4 for the join).
 #include <atomic>
 
 #include "shv_device.hpp"
@@ -60,7 +75,7 @@ constexpr int kStages = 4, kAhead = kStages - 1;
 // Weights are e^(s - m) 2^kLift, and m stands until a score is more than 2^kSlack above it: up to 2^15, which the larger half holds, and down to
 // 2^-31 of the largest with the smaller half's last place (at a lift of 0 2^-24, 6e-6 of a weight of a hundredth).
 constexpr float kLift = 7.f, kSlack = 8.f;
-constexpr int kLeastNarrow = 2, kLeastWide = 3;
+constexpr int kLeastNarrow = 2, kLeastWide = 3;  // tiles a slice gets at least: launch_tree has the figures
 // Waves that join the slices of 256 dims' rows: one where there are many such pieces, eight where there are some, four where there are few.  us
 // by one / four / eight waves: 32 pieces of 13 slices 3.9 / 4.2 / 5.4 (of 130 slices one wave would go to memory nine times in a row), 192 of
 // 95 14.5 / 8.6 / 7.6, 1024 of 32 10.8 / 11.9 / 19, 2016 of 11 6.0 / 10.7 / 21.
@@ -268,7 +283,8 @@ __device__ __forceinline__ char *staged(char *stage, const shv_attn_tree_args &a
     return stage + (static_cast<size_t>(seq) * a.rows * a.n_head + static_cast<size_t>(kvh) * rows * rep + 16 * g) * D * 4;
 }
 
-// grid: (ceil((rows * n_head + rows * n_head_kv) / 4), n_seq), a wave a query row or a row's cell of a KV head.
+// A wide call's query rows as operands, and its rows' cells.  grid: (ceil((rows * n_head + rows * n_head_kv) / 4), n_seq), a wave a query row or a
+// row's cell of a KV head.  Bound by its chain of trips to memory (parents, then the position's rotation): 4 us whatever its size.
 template <int D>
 __global__ __launch_bounds__(256) void tree_prep_kernel(shv_attn_tree_args a, Plan plan, char *stage) {
     constexpr int VEC = D / 64, KI = D / 32;
@@ -330,12 +346,12 @@ struct TreeSmem {
     float p[W][16 * kTile / 2];  // a wave's weights of half a tile, where its values are not all finite (a whole one's would leave a unit one block of D 128)
 };
 
-// grid: (slices rounded up to 8, times query blocks; n_head_kv), W waves.  A wave holds GW groups of 16 query rows: query row r of a KV
-// head is head r % rep of tree row r / rep.  GW 1: calls of up to 64 query rows a KV head, whose rows are normed and turned here, by every
-// block; GW 2: wider ones, whose rows a launch before (tree_prep_kernel) has left as operands: there every block has 128 rows to prepare,
-// 5 us before its first product, and the launch costs 4.
-// What bounds a wide call is the matrix cores and the LDS reads that feed them: a key's and a value's operand read once serves both
-// groups, and one group's exponentials run under the other's products.
+// grid: (slices rounded up to 8, times query blocks; n_head_kv), W waves of 16 query rows.  Four waves: calls of up to 64 query rows a KV head, whose
+// rows every block norms and turns itself, the waves sharing the rows of however few groups there are.  Eight: wider ones, whose rows a
+// launch before (tree_prep_kernel) has left as operands.  There every block would have 128 rows to prepare, 5 us before its first product,
+// and the launch costs 4 (us of 12 rows behind 9000 cells so / with the launch 31.7 / 30.1, a batch of six windows 68 / 54).
+// Tried beside it: two groups a wave, so that an operand read serves both (512 registers a lane do not hold them: 1130 us where this takes
+// 260); a tile's keys multiplied under the weights of the one before (275 for 260: the matrix cores are near their rate already).
 template <int D, int W>
 __global__ __launch_bounds__(64 * W, W == 4 || D == 256 ? 2 : 4) void tree_attn_kernel(shv_attn_tree_args a, Plan plan, char *stage) {
     constexpr bool kWide = W == 8;
@@ -806,7 +822,8 @@ int launch_tree(shv_ctx *ctx, const shv_attn_tree_args &a) {
     // beside them every sequence has a slice for its rows and, of several, one that is not full
     plan.slots = ctx->prop.multiProcessorCount * kBlocksPerUnit / (a.n_head_kv * plan.q_blocks) - (a.n_seq > 1 ? 2 : 1) * a.n_seq;
     if (plan.slots < 1) plan.slots = 1;
-    // A tile more to a slice costs a narrow call 1.2 us and a wide one 1.4; of a slice more the merge reads a record more of every row.
+    // us with slices of 1 / 2 / 3 / 4 / 6 tiles at least: 2 rows behind 700 cells 12.4 / 12.6 / 13.2 / 14.0 / 16.2, 8 behind 3000 25.4 / 22.2 / 22.1 /
+    // 22.9 / 24.0 (a slice more is a record more of every row to join); 32 behind 4000 (wide) - / 36.0 / 33.5 / 33.3 / 33.6
     plan.least = W == 4 ? kLeastNarrow : kLeastWide;
     plan.rep_magic = ((1u << 20) + rep - 1) / rep;
     static std::atomic<uint64_t> raised{0};  // by device

@@ -70,12 +70,12 @@ __device__ __forceinline__ float sum32(float v) {
     const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
     return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
-// The power of two that brings values of up to m to 1 and below (of 0 and of what is no number, 1), and its inverse.
+// The power of two that brings values of up to m to about 1 (of 0 and of what is no number, 1), and its inverse.
 struct Scale {
     float down, up;
     __device__ __forceinline__ explicit Scale(float m) {
         int e = static_cast<int>(__float_as_uint(m) >> 23) - 126;  // m < 2^e
-        e = m > 0.f && m < INFINITY ? max(e, -120) : 0;
+        e = m > 0.f && m < INFINITY ? min(max(e, -120), 126) : 0;  // (what is left over, a factor of four at most, the halves hold)
         down = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
         up = __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
     }

@@ -11,7 +11,7 @@ pytestmark = pytest.mark.gpu
 A = shv.api
 EPS = 1e-6
 LAYOUTS = {"16/2x256": (16, 2, 256, 64), "32/8x128": (32, 8, 128, 128), "12/2x128": (12, 2, 128, 0), "8/8x64": (8, 8, 64, 32), "5/1x64": (5, 1, 64, 6),
-           "32/2x256": (32, 2, 256, 256)}
+           "32/2x256": (32, 2, 256, 256), "64/1x64": (64, 1, 64, 10), "6/2x256": (6, 2, 256, 24), "9/3x128": (9, 3, 128, 12)}
 # Outputs: a score is a sum of d products q k / sqrt(d) of normed vectors, in absolute values at most about sqrt(d) <= 16.  Queries and
 # weights enter the products to 22 bits and sums are float32: an error of a score is within 16 * (2^-22 + a few 2^-24) = 1e-5, of a
 # weight as much again relative to it, of a weighted mean of the values no more than that.
@@ -105,6 +105,89 @@ def test_tree_attention(ctx, layout, rows, pos, n_splits, kind):
     t.upload(ctx)
     ctx.enqueue(A.OP_ATTN_TREE, t.args(ctx, n_splits))
     t.check()
+
+
+@pytest.mark.parametrize("layout,rows,pos,n_splits", [
+    # every query row of a KV head at most: 64 heads of 64 rows; 64 and 65 query rows, on both sides of the line between the two kernels
+    ("64/1x64", 64, [700], 9), ("64/1x64", 1, [95, 3], 4), ("16/2x256", 8, [400], 7), ("6/2x256", 22, [64, 200], 6), ("9/3x128", 21, [1000], 12), ("9/3x128", 22, [31], 3),
+    # one slice, and the two of which a wide call keeps one for its rows
+    ("16/2x256", 64, [1000], 1), ("16/2x256", 40, [70, 0], 2), ("16/2x256", 3, [1000, 40], 1), ("16/2x256", 3, [333], 2), ("32/8x128", 33, [500], 1), ("5/1x64", 64, [129], 2)])
+def test_query_rows_and_slices_at_their_lines(ctx, layout, rows, pos, n_splits):
+    t = AttnTree(300 + rows + n_splits, layout, rows, pos)
+    t.upload(ctx)
+    ctx.enqueue(A.OP_ATTN_TREE, t.args(ctx, n_splits))
+    t.check()
+
+
+@pytest.mark.parametrize("rows,n_splits,window", [(2, 16, 0), (9, 5, 0), (12, 16, 40)])
+def test_many_sequences_of_which_some_do_not_fit(ctx, rows, n_splits, window):
+    """More sequences than a wave has lanes, of lengths from nothing to hundreds of cells, some without rows and some that do not fit the cache."""
+    n_seq = 75
+    rng = np.random.default_rng(9)
+    t = AttnTree(310, "16/2x256", rows, [int(p) for p in rng.choice([0, 1, 31, 32, 33, 64, 150, 700], n_seq)], count=rng.integers(0, rows + 2, n_seq))
+    odd = np.arange(5, n_seq, 9)
+    t.pos[odd] = np.where(odd % 2, -1 - odd, t.max_cells + odd).astype(np.int32)
+    t.upload(ctx)
+    ctx.enqueue(A.OP_ATTN_TREE, t.args(ctx, n_splits, window, 3))
+    t.pos[odd] = 0
+    t.count[odd] = 0  # nothing of these is written
+    t.check(window, 3)
+
+
+def test_absent_arrays(ctx):
+    """pos, slot, parent and count NULL: sequences without a past, slot s, chains, all rows."""
+    t = AttnTree(311, "16/2x256", 7, [0, 0, 0], kind="chain")
+    t.slot = np.arange(3, dtype=np.int32)
+    t.upload(ctx)
+    a = t.args(ctx, parent=False)
+    a.pos = a.slot = None
+    ctx.enqueue(A.OP_ATTN_TREE, a)
+    t.check()
+    d = DnTree(312, 7, [0, 0, 0], 2, 4, kind="chain", planes=0)
+    d.slot = np.arange(3, dtype=np.int32)
+    d.upload(ctx)
+    a = d.args(parent=False)
+    a.pos = a.slot = None
+    ctx.enqueue(A.OP_DN_TREE, a)
+    states = d.check()
+    path = np.tile(np.array([0, 1, 2, 3, -1, -1, -1], np.int32), (3, 1))
+    k = d.keep_args(ctx.upload(path), ctx.upload(np.full(3, 4, np.int32)))
+    k.pos = k.slot = None
+    ctx.enqueue(A.OP_DN_KEEP, k)
+    got = d.d_state.read(np.float32, d.state.size).reshape(d.state.shape)
+    for s in range(3):
+        assert O.rel_l2(got[s, 0], states[s][3]) <= DN_TOL
+    p = ctx.upload(path)
+    a = A.AttnKeepArgs(t.d_kx.ptr, t.d_vx.ptr, t.d_kc.ptr, t.d_vc.ptr, p.ptr, ctx.upload(np.full(3, 4, np.int32)).ptr, None, None, 3, 7, t.nkv, t.d, t.max_cells)
+    ctx.enqueue(A.OP_ATTN_KEEP, a)
+    kx = t.results()[1]
+    kc = t.d_kc.read(np.float16, t.kc.size).reshape(t.kc.shape)
+    assert np.array_equal(kc[:, :4], kx[:, :4]) and np.array_equal(kc[:, 4:], t.kc[:, 4:])
+
+
+def test_two_contexts_at_once(ctx):
+    """The same calls on two streams, nothing waited for between them: a context's scratch is its own."""
+    other = shv.pkg.Context(0)
+    sets = []
+    for c, seed in ((ctx, 320), (other, 321)):
+        at, dn, ac = AttnTree(seed, "16/2x256", 17, [300, 700]), DnTree(seed, 17, [300, 700], 4, 8), Accept(seed, 2, 17, 30000)
+        at.upload(c)
+        dn.upload(c)
+        bufs = [c.upload(np.full(34, -7, np.int32)) for _ in range(4)]
+        up = [c.upload(x) for x in (ac.logits, ac.ids, ac.parent)]
+        acc = A.TreeAcceptArgs(up[0].ptr, up[1].ptr, up[2].ptr, None, bufs[0].ptr, bufs[1].ptr, bufs[2].ptr, bufs[3].ptr, None, None, 2, 17, 30000, 30000)
+        sets.append((c, at, dn, ac, at.args(c), dn.args(), acc, bufs, up))
+    for _ in range(20):
+        for c, _, _, _, a, d, acc, *_ in sets:
+            c.enqueue(A.OP_ATTN_TREE, a)
+            c.enqueue(A.OP_TREE_ACCEPT, acc)
+            c.enqueue(A.OP_DN_TREE, d)
+    for c, at, dn, ac, _, _, _, bufs, _ in sets:
+        c.sync()
+        at.check()
+        dn.check()
+        ac.check([bufs[0].read(np.int32, 34).reshape(2, -1), bufs[1].read(np.int32, 34).reshape(2, -1), bufs[2].read(np.int32, 2), bufs[3].read(np.int32, 2)])
+    other.destroy()
 
 
 @pytest.mark.parametrize("window,sinks", [(1, 0), (2, 1), (7, 4), (32, 0), (33, 40), (100, 3), (700, 700), (2**31 - 1, 2**31 - 1)])
@@ -366,6 +449,27 @@ def test_rows_with_nan_reach_their_descendants_alone(ctx):
     for r in set(range(20)) - below:
         assert O.rel_l2(out[r], want[r]) <= DN_TOL, r
     assert all(np.isnan(out[r]).any() for r in below)
+
+
+@pytest.mark.parametrize("rows", [3, 40])
+def test_values_and_states_of_any_size(ctx, rows):
+    """Value columns and states from 2^-100 to 2^100, far outside binary16: each column by its own scale."""
+    t = DnTree(13, rows, [10], 2, 4)
+    size = np.exp2(t.rng.integers(-100, 100, 4 * D)).astype(np.float32)
+    v0 = 4 * D
+    # (conv and SiLU come before the size does: a value is its channel's size times an ordinary number for large sizes, its square for small)
+    t.x[0, :, v0:v0 + 4 * D] *= size
+    t.ring[:, :, v0:v0 + 4 * D] *= size
+    t.state *= size.reshape(4, D, 1)
+    t.upload(ctx)
+    ctx.enqueue(A.OP_DN_TREE, t.args())
+    got = t.results()
+    want = t.want(0)
+    for name, g, w in (("out", got[0][0], want[0]), ("delta", got[2][0], want[2])):
+        for h in range(4):
+            for c in range(0, D, 7):
+                # a column of `rows` numbers alone: the tolerance of the whole, with room for a sum of 128 products that cancel in one column
+                assert O.rel_l2(g[:, h, c], w[:, h, c]) <= 4 * DN_TOL, (name, h, c)
 
 
 def test_strong_and_weak_decays(ctx):

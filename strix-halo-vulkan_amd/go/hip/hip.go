@@ -354,6 +354,102 @@ func AttnDecode(d AttnArgs) Op {
 	return mk(C.SHV_OP_ATTN_DECODE, unsafe.Pointer(&a), C.sizeof_shv_attn_decode_args)
 }
 
+// Tree names the trees of drafted tokens a pass verifies: NSeq sequences of up to Rows rows (64 at most); Parent nil makes
+// them chains, Count nil uses all rows, Pos and Slot are as in PassRows.
+type Tree struct {
+	NSeq, Rows               int
+	Pos, Slot, Parent, Count *Buffer // device int32
+}
+
+// AttnTreeArgs are the fields of shv_attn_tree_args a caller sets.
+type AttnTreeArgs struct {
+	QKV, QNorm, KNorm, Rope *Buffer
+	KCache, VCache          *Buffer
+	KCells, VCells          *Buffer // each row's key and value, for AttnKeep
+	Partial, Out            *Buffer
+	Tree                    Tree
+	NHead, NHeadKV, HeadDim int
+	RopeDims, MaxCells      int
+	QKVStride, Splits       int
+	Window, Sinks           int // Window 0: every cell
+	Eps                     float32
+}
+
+// AttnTree attends from every row of each tree over its sequence's cells and its own ancestors; the cache stays as it is.
+func AttnTree(d AttnTreeArgs) Op {
+	var a C.shv_attn_tree_args
+	a.qkv, a.q_norm, a.k_norm, a.rope = fp(d.QKV), fp(d.QNorm), fp(d.KNorm), fp(d.Rope)
+	a.kcache, a.vcache, a.kcells, a.vcells = vp(d.KCache), vp(d.VCache), vp(d.KCells), vp(d.VCells)
+	a.partial, a.out = fp(d.Partial), fp(d.Out)
+	a.pos, a.slot, a.parent, a.count = ip(d.Tree.Pos), ip(d.Tree.Slot), ip(d.Tree.Parent), ip(d.Tree.Count)
+	a.n_seq, a.rows = C.int32_t(d.Tree.NSeq), C.int32_t(d.Tree.Rows)
+	a.n_head, a.n_head_kv, a.head_dim = C.int32_t(d.NHead), C.int32_t(d.NHeadKV), C.int32_t(d.HeadDim)
+	a.rope_dims, a.max_cells = C.int32_t(d.RopeDims), C.int32_t(d.MaxCells)
+	a.qkv_stride, a.n_splits, a.eps = C.int32_t(d.QKVStride), C.int32_t(d.Splits), C.float(d.Eps)
+	a.window, a.sinks = C.int32_t(d.Window), C.int32_t(d.Sinks)
+	return mk(C.SHV_OP_ATTN_TREE, unsafe.Pointer(&a), C.sizeof_shv_attn_tree_args)
+}
+
+// AttnKeep moves the kept branch's cells (path and nKeep from TreeAccept) into a layer's cache.  t.Pos: the positions
+// before acceptance.
+func AttnKeep(kcells, vcells, kcache, vcache, path, nKeep *Buffer, t Tree, nHeadKV, headDim, maxCells int) Op {
+	var a C.shv_attn_keep_args
+	a.kcells, a.vcells, a.kcache, a.vcache = vp(kcells), vp(vcells), vp(kcache), vp(vcache)
+	a.path, a.n_keep, a.pos, a.slot = ip(path), ip(nKeep), ip(t.Pos), ip(t.Slot)
+	a.n_seq, a.rows = C.int32_t(t.NSeq), C.int32_t(t.Rows)
+	a.n_head_kv, a.head_dim, a.max_cells = C.int32_t(nHeadKV), C.int32_t(headDim), C.int32_t(maxCells)
+	return mk(C.SHV_OP_ATTN_KEEP, unsafe.Pointer(&a), C.sizeof_shv_attn_keep_args)
+}
+
+// DNTreeArgs are the fields of shv_dn_tree_args and shv_dn_keep_args a caller sets.
+type DNTreeArgs struct {
+	X, Ring, Conv1D, A, DtBias, State, Out *Buffer
+	Kn, Delta, Decay                       *Buffer // what DNKeep needs of the rows
+	Tree                                   Tree
+	HeadK, HeadV, HeadDim, Conv            int
+	XStride, RingSlots, RingStride         int
+	Plane                                  *Buffer
+	Planes                                 int
+	Eps                                    float32
+}
+
+// DNTree is the gated delta rule over the rows of each tree; ring and state stay as they are.
+func DNTree(d DNTreeArgs) Op {
+	var a C.shv_dn_tree_args
+	a.x, a.ring, a.conv1d, a.a, a.dt_bias = fp(d.X), fp(d.Ring), fp(d.Conv1D), fp(d.A), fp(d.DtBias)
+	a.state, a.out, a.kn, a.delta, a.decay = fp(d.State), fp(d.Out), fp(d.Kn), fp(d.Delta), fp(d.Decay)
+	a.pos, a.slot, a.plane, a.parent, a.count = ip(d.Tree.Pos), ip(d.Tree.Slot), ip(d.Plane), ip(d.Tree.Parent), ip(d.Tree.Count)
+	a.n_seq, a.rows = C.int32_t(d.Tree.NSeq), C.int32_t(d.Tree.Rows)
+	a.n_head_k, a.n_head_v, a.head_dim, a.conv = C.int32_t(d.HeadK), C.int32_t(d.HeadV), C.int32_t(d.HeadDim), C.int32_t(d.Conv)
+	a.x_stride, a.ring_slots, a.ring_stride = C.int32_t(d.XStride), C.int32_t(d.RingSlots), C.int32_t(d.RingStride)
+	a.n_planes, a.eps = C.int32_t(d.Planes), C.float(d.Eps)
+	return mk(C.SHV_OP_DN_TREE, unsafe.Pointer(&a), C.sizeof_shv_dn_tree_args)
+}
+
+// DNKeep forms the state behind the kept branch in the next plane and leaves its last rows in the ring.  d.Tree.Pos: the
+// positions before acceptance.
+func DNKeep(d DNTreeArgs, path, nKeep *Buffer) Op {
+	var a C.shv_dn_keep_args
+	a.x, a.kn, a.delta, a.decay = fp(d.X), fp(d.Kn), fp(d.Delta), fp(d.Decay)
+	a.state, a.ring, a.path, a.n_keep = fp(d.State), fp(d.Ring), ip(path), ip(nKeep)
+	a.pos, a.slot, a.plane = ip(d.Tree.Pos), ip(d.Tree.Slot), ip(d.Plane)
+	a.n_seq, a.rows = C.int32_t(d.Tree.NSeq), C.int32_t(d.Tree.Rows)
+	a.n_head_k, a.n_head_v, a.head_dim, a.conv = C.int32_t(d.HeadK), C.int32_t(d.HeadV), C.int32_t(d.HeadDim), C.int32_t(d.Conv)
+	a.x_stride, a.ring_slots, a.ring_stride = C.int32_t(d.XStride), C.int32_t(d.RingSlots), C.int32_t(d.RingStride)
+	a.n_planes = C.int32_t(d.Planes)
+	return mk(C.SHV_OP_DN_KEEP, unsafe.Pointer(&a), C.sizeof_shv_dn_keep_args)
+}
+
+// TreeAccept finds the branch of each tree the logits agree with; logits nil: best holds a token drawn for every row.  pos and
+// base (both or neither): base takes the positions, pos moves on by what was kept.
+func TreeAccept(logits, ids, best, path, nKeep, next, pos, base *Buffer, t Tree, n, stride int) Op {
+	var a C.shv_tree_accept_args
+	a.logits, a.ids, a.parent, a.count = fp(logits), ip(ids), ip(t.Parent), ip(t.Count)
+	a.best, a.path, a.n_keep, a.next, a.pos, a.base = ip(best), ip(path), ip(nKeep), ip(next), ip(pos), ip(base)
+	a.n_seq, a.rows, a.n, a.logits_stride = C.int32_t(t.NSeq), C.int32_t(t.Rows), C.int32_t(n), C.int32_t(stride)
+	return mk(C.SHV_OP_TREE_ACCEPT, unsafe.Pointer(&a), C.sizeof_shv_tree_accept_args)
+}
+
 // QSAArgs are the fields of shv_qsa_index_args (indexerAt / selected / topK, llm/attn.go:247-443).
 type QSAArgs struct {
 	X, Gamma, W, QNorm, KNorm, Rope *Buffer

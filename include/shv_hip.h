@@ -587,7 +587,8 @@ typedef struct {
 
 /* Gated full attention of a tree's rows over a sequence's cells and their own ancestors.  qkv rows, norms, rotary table and
  * caches as shv_attn_decode has them, for head_dim 64, 128 or 256, any number of query heads per KV head up to 64, and rope_dims
- * any multiple of head_dim / 32 up to head_dim.  Row i sees cell c < pos and each row on its way to the root, itself included, and with window > 0
+ * any multiple of head_dim / 32 up to head_dim; norms and rotary table 16-byte aligned.  A query's values, normed and rotated, lie within
+ * binary16's range (norm weights up to 2000 keep them there; a larger value makes its row's result no number).  Row i sees cell c < pos and each row on its way to the root, itself included, and with window > 0
  * only those of them whose position p is below sinks (the first tokens, which stay visible) or within the last `window`
  * positions up to the row's own, position(i) - p < window.  Cells at pos and behind it are not looked at.
  * kcells / vcells [n_seq][rows][n_head_kv][head_dim] binary16 receive each row's key (normed and rotated; formed in
@@ -641,7 +642,7 @@ typedef struct {
  * rows are solved together, (I + A) delta = B with A[i][j] = beta_i e^(G_i - G_j) (k_j . k_i) where j is an ancestor of i, G_i
  * the sum of log g from the root to row i.
  * Beside out [n_seq][rows][hv*d] the call leaves kn [n_seq][rows][hk*d] (the normed keys), delta [n_seq][rows][hv*d] and
- * decay [n_seq][rows][hv] (G) for shv_dn_keep.  head_dim 128, conv 4, n_head_v a multiple of n_head_k, ring_slots >= 3. */
+ * decay [n_seq][rows][hv] (G, whose rounding to float32 moves a weight of shv_dn_keep's sum by up to |G| 2^-23) for shv_dn_keep.  head_dim 128, conv 4, n_head_v a multiple of n_head_k, ring_slots >= 3. */
 typedef struct {
     const float *x;
     const float *ring;

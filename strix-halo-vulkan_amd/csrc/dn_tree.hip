@@ -6,6 +6,9 @@
 //     out_i   = (e^(G_i) S0^T q_i + sum over ancestors j and i itself of e^(G_i - G_j) (k_j . q_i) delta_j) / sqrt(d)
 // so no row needs a state of its own: S0 is read once, whatever the tree's shape, and the deltas are a triangular solve whose
 // matrix is masked by ancestry.
+// What bounds it, of 16 key and 32 value heads: a small tree its chain of steps, each waiting for the one before (parents, rows, products of
+// rows, inverse, solve: 5 rows 7.6 us, whose 2.5 MB would take 0.5); wide ones the preparing of rows, which every value head's block does for
+// itself on the vector units, and then the same chain (eight sequences of up to 64 rows 24.5 us, whose 36 MB would take 8).
 #include <atomic>
 
 #include "shv_device.hpp"
@@ -421,7 +424,7 @@ int launch_tree(shv_ctx *ctx, const shv_dn_tree_args &a) {
 }
 
 // grid: (8 slabs of 16 state rows, n_head_v, n_seq): a thread holds eight values of one row.  HBM-bound: the state is read once
-// and written once.
+// and written once (twelve sequences of 32 heads 12.9 us, 54 MB at 4.2 TB/s; one 4.1 us, the launch and two trips to memory).
 constexpr int kKeepRows = 16;
 __global__ __launch_bounds__(kBlock) void dn_keep_kernel(shv_dn_keep_args a) {
     __shared__ float fall[kRows];

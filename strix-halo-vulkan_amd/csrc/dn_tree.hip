@@ -7,8 +7,8 @@
 // so no row needs a state of its own: S0 is read once, whatever the tree's shape, and the deltas are a triangular solve whose
 // matrix is masked by ancestry.
 // What bounds it, of 16 key and 32 value heads: a small tree its chain of steps, each waiting for the one before (parents, rows, products of
-// rows, inverse, solve: 5 rows 7.6 us, whose 2.5 MB would take 0.5); wide ones the preparing of rows, which every value head's block does for
-// itself on the vector units, and then the same chain (eight sequences of up to 64 rows 24.5 us, whose 36 MB would take 8).
+// rows, inverse, solve: 5 rows 7.4 us, whose 2.5 MB would take 0.5); wide ones the preparing of rows, which every value head's block does for
+// itself on the vector units, and then the same chain (eight sequences of up to 64 rows 22.6 us, whose 36 MB would take 8).
 #include <atomic>
 
 #include "shv_device.hpp"
@@ -27,8 +27,6 @@ constexpr int kWaves = 8;
 typedef _Float16 half4_t __attribute__((ext_vector_type(4)));
 typedef _Float16 half8_t __attribute__((ext_vector_type(8)));
 typedef float float4_t __attribute__((ext_vector_type(4)));
-typedef float float4_u __attribute__((ext_vector_type(4), aligned(4)));  // rows may lie any number of floats apart
-typedef float float2_u __attribute__((ext_vector_type(2), aligned(4)));
 
 __device__ __forceinline__ float softplus_ref(float x) {
     // the add inside the log is float32 on purpose, as in the step's kernels: below about -16.6 it returns exactly 0
@@ -40,7 +38,7 @@ __device__ __forceinline__ float softplus_ref(float x) {
 constexpr float kLoScale = 2048.f, kLoInv = 1.f / 2048.f;
 __device__ __forceinline__ void split(float x, _Float16 &hi, _Float16 &lo) {
     hi = static_cast<_Float16>(x);
-    lo = static_cast<_Float16>((x - static_cast<float>(hi)) * kLoScale);
+    lo = static_cast<_Float16>(fmaf(static_cast<float>(hi), -1.f, x) * kLoScale);
 }
 __device__ __forceinline__ void mma32(half8_t xh, half8_t xl, half8_t yh, half8_t yl, float4_t &main, float4_t &low) {
     main = __builtin_amdgcn_mfma_f32_16x16x32_f16(xh, yh, main, 0, 0, 0);
@@ -153,38 +151,49 @@ __global__ __launch_bounds__(64 * kWaves, 2) void dn_tree_kernel(shv_dn_tree_arg
         float4_t qk[4];
         float v[4][VC];
     };
-    // the row, its parent, grandparent and the one above it; behind the root the ring's rows, zeros before the start
+    // Where a lane's row's taps are: the row, its parent, grandparent and the one above it; behind the root the ring's rows.  Each is read as a buffer
+    // of the conv's channels, and of none before the sequence's start, where loads give zeros: nothing waits to put them there, and a
+    // row's loads stay on their way under the row before (64 rows of one sequence 17.5 us, of eight 25.4; where a select put the zeros 19.5 and 27.3).
+    const uint32_t width = static_cast<uint32_t>(2 * qk + vw) * 4;
+    const float *from[3];
+    uint64_t there[3];
+    {
+        int up = t.parent, back = 0;
+#pragma unroll
+        for (int k = 0; k < 3; k++) {
+            const int next = __shfl(t.parent, up < 0 ? 0 : up, 64);
+            back += up < 0;
+            const int p = pos - back;
+            const uint32_t behind = p < 0 ? 0 : static_cast<uint32_t>(p) % static_cast<uint32_t>(a.ring_slots);
+            from[k] = up < 0 ? ring + static_cast<size_t>(behind) * a.ring_stride : x + static_cast<size_t>(up) * a.x_stride;
+            there[k] = __ballot(up >= 0 || p >= 0);
+            up = up < 0 ? -1 : next;
+        }
+    }
     const auto load = [&](Taps &f, int r) {
-        int up = r, back = 0;
 #pragma unroll
         for (int k = 0; k < 4; k++) {
-            const float *row;
-            bool there = true;
-            if (up >= 0) {
-                row = x + static_cast<size_t>(up) * a.x_stride;
-                up = __builtin_amdgcn_readlane(t.parent, up);
-            } else {
-                const int p = pos - ++back;
-                there = p >= 0;
-                row = ring + static_cast<size_t>(there ? static_cast<uint32_t>(p) % static_cast<uint32_t>(a.ring_slots) : 0) * a.ring_stride;
+            const float *row = x + static_cast<size_t>(r) * a.x_stride;
+            uint32_t bytes = width;
+            if (k > 0) {
+                const uint64_t at = reinterpret_cast<uint64_t>(from[k - 1]);
+                const uint32_t lo = __builtin_amdgcn_readlane(static_cast<int>(at), r), hi = __builtin_amdgcn_readlane(static_cast<int>(at >> 32), r);
+                row = reinterpret_cast<const float *>(static_cast<uint64_t>(hi) << 32 | lo);
+                bytes = there[k - 1] >> r & 1 ? width : 0;
             }
-            f.qk[k] = *reinterpret_cast<const float4_u *>(row + ch);
+            const __amdgpu_buffer_rsrc_t buf = __builtin_amdgcn_make_buffer_rsrc(const_cast<float *>(row), 0, bytes, 0x00027000);
+            f.qk[k] = __builtin_bit_cast(float4_t, __builtin_amdgcn_raw_buffer_load_b128(buf, ch * 4, 0, 0));
             if constexpr (VC == 2) {
-                const float2_u v = *reinterpret_cast<const float2_u *>(row + vch);
-                f.v[k][0] = v.x;
-                f.v[k][1] = v.y;
+                const auto v = __builtin_amdgcn_raw_buffer_load_b64(buf, vch * 4, 0, 0);
+                f.v[k][0] = __uint_as_float(v[0]);
+                f.v[k][1] = __uint_as_float(v[1]);
             } else {
-                f.v[k][0] = row[vch];
-            }
-            if (!there) {
-                f.qk[k] = float4_t{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                for (int c = 0; c < VC; c++) f.v[k][c] = 0.f;
+                f.v[k][0] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(buf, vch * 4, 0, 0));
             }
         }
     };
-    Taps now;
-    if (wave < rows) load(now, wave);
+    Taps even, odd;
+    if (wave < rows) load(even, wave);
     {
         const double G = tree_sum(t, lane < rows ? softplus_ref(alpha + dt_bias) * decay : 0.f, a.rows, lane);
         if (wave == 0) {
@@ -196,9 +205,11 @@ __global__ __launch_bounds__(64 * kWaves, 2) void dn_tree_kernel(shv_dn_tree_arg
         }
     }
     const auto silu = [](float c) { return c * __builtin_amdgcn_rcpf(1.f + __expf(-c)); };
-    for (int r = wave; r < 16 * tiles; r += kWaves) {
+    // a row of a wave's, and the loads of its next one under it
+    const auto prepare = [&](Taps &now, Taps &next, int r) {
         float y[4], v[VC];
         if (r < rows) {
+            if (r + kWaves < rows) load(next, r + kWaves);
             float ss = 0.f;
 #pragma unroll
             for (int c = 0; c < 4; c++) {
@@ -215,7 +226,6 @@ __global__ __launch_bounds__(64 * kWaves, 2) void dn_tree_kernel(shv_dn_tree_arg
                 s = fmaf(now.v[1][c], vtap[c].z, s);
                 v[c] = silu(fmaf(now.v[0][c], vtap[c].w, s));
             }
-            if (r + kWaves < rows) load(now, r + kWaves);  // under the rest of this one
             ss = sum32(ss);
             const float nrm = a.qk_norm_max ? 1.f / fmaxf(sqrtf(ss), a.eps) : __builtin_amdgcn_rsqf(ss + a.eps);
 #pragma unroll
@@ -242,6 +252,10 @@ __global__ __launch_bounds__(64 * kWaves, 2) void dn_tree_kernel(shv_dn_tree_arg
 #pragma unroll
             for (int c = 0; c < VC; c++) L.v[r][vcol + c] = v[c];
         }
+    };
+    for (int r = wave; r < 16 * tiles; r += 2 * kWaves) {
+        prepare(even, odd, r);
+        prepare(odd, even, r + kWaves);
     }
     __syncthreads();
 
@@ -506,8 +520,8 @@ int shv_launch_dn_tree(shv_ctx *ctx, const shv_dn_tree_args *pa) {
                     shv_aligned16(a.kn) && shv_aligned16(a.delta),
                 "dn_tree: x, ring, conv1d, state, out, kn and delta must be 16-byte aligned");
     // Columns cut in four, two or not at all: as far as every block still finds a compute unit of its own (a block's rows are prepared anew
-    // whatever its columns).  us of 5 / 64 rows of one sequence of 32 value heads cut in four 7.3 / 19.5, in two 8.2 / 19.4, whole
-    // 10.1 / 21.7; of four sequences 13.7 / 41, 8.5 / 22, 10.3 / 24.
+    // whatever its columns).  us of 5 / 64 rows of one sequence of 32 value heads cut in four 7.3 / 17.8, in two 7.9 / 17.7, whole
+    // 9.8 / 20.6; of four sequences 13.6 / 38, 8.3 / 20.8, 10.2 / 23.5.
     const int heads = a.n_seq * a.n_head_v, units = ctx->prop.multiProcessorCount;
     if (4 * heads <= units) return launch_tree<2>(ctx, a);
     if (2 * heads <= units) return launch_tree<4>(ctx, a);

@@ -11,8 +11,9 @@
 // with a running maximum and sum.  Tiles go from memory to LDS past the registers, three ahead.  The rows' own keys and values never enter the
 // cache here: one more block of a KV head forms their cells, attends over them by the ancestors' bits, and leaves them for attn_keep.  A second
 // launch joins the slices.
-// What bounds it: one or two rows behind a long cache the cache's bytes (131000 cells 54 us, 5.0 TB/s of K and V); 64 rows the matrix cores (64
-// rows of 16 heads behind 131000 cells 262 us, 1.05 PFLOP/s of binary16 products, where a large library product reaches 1.18); short
+// What bounds it: one or two rows behind a long cache the cache's bytes (131000 cells 54 us, 5.0 TB/s of K and V); 64 rows products and their
+// operands' reads from LDS, each half of the cycles at its rate, with the softmax on the vector units between them (64 rows of 16 heads behind 131000
+// cells 259 us, 1.06 PFLOP/s of binary16 products, where a large library product reaches 1.18); short
 // caches the chain of trips to memory before the first product (2 rows behind 700 cells 9 us and 4 for the join).
 #include <atomic>
 
@@ -351,7 +352,8 @@ struct TreeSmem {
 // launch before (tree_prep_kernel) has left as operands.  There every block would have 128 rows to prepare, 5 us before its first product,
 // and the launch costs 4 (us of 12 rows behind 9000 cells so / with the launch 31.7 / 30.1, a batch of six windows 68 / 54).
 // Tried beside it: two groups a wave, so that an operand read serves both (512 registers a lane do not hold them: 1130 us where this takes
-// 260); a tile's keys multiplied under the weights of the one before (275 for 260: the matrix cores are near their rate already).
+// 260); a tile's keys multiplied under the weights of the one before (275 for 260); half of the waves half a tile behind the others (263, and a
+// batch of six windows 43 for 37).
 template <int D, int W>
 __global__ __launch_bounds__(64 * W, W == 4 || D == 256 ? 2 : 4) void tree_attn_kernel(shv_attn_tree_args a, Plan plan, char *stage) {
     constexpr bool kWide = W == 8;

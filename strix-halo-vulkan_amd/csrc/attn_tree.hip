@@ -101,7 +101,8 @@ struct Tiles {
 struct Plan {
     int q_blocks;        // blocks that share a slice, 16 query rows a wave
     int least;           // tiles a slice gets at least
-    int slots;           // slices of the cache that all sequences have together: as many blocks as the chip holds at once
+    int slots;           // full slices of the cache that all sequences may have together: with the others as many blocks as the chip holds at once
+    int32_t *len;        // of several sequences, where the slices' length is left for the join
     uint32_t rep_magic;  // r / rep = r * rep_magic >> 20 for r < 4096 and rep <= 64: off by less than r / 2^20 <= 1 / 256 before it is cut
 };
 __device__ __forceinline__ int over_rep(const Plan &plan, int r) { return static_cast<int>(static_cast<uint32_t>(r) * plan.rep_magic >> 20); }
@@ -125,22 +126,42 @@ __device__ __forceinline__ uint32_t all_tiles(const shv_attn_tree_args &a, int l
     return __builtin_amdgcn_readfirstlane(total);
 }
 
-// How a call's sequences are cut: slices of `len` tiles as many as the call has blocks for, and behind them one for the rows
-// themselves; where a call has one slice, it holds both.
+// Of several sequences, tiles a slice may have: the least for which all slices of the cache find a block.  Slices as long as the full ones
+// alone call for, 1 / slots of all tiles, are enough whatever the sequences' remainders; 1 / (slots + n_seq) is the least that could be.  A lane tries a
+// length between (longest 62 steps apart), by float32 quotients that are exact below 2^21.  Not tried
+// where it could take off an eighth or less (us of eight sequences of up to 54 rows of 32 heads behind up to 1872 cells 70, so 62; of 20 rows behind up
+// to 16000 116, so 104; six windows that it does not change 38.0 either way, 38.6 with the trial).
+__device__ __forceinline__ int call_len(const shv_attn_tree_args &a, const Plan &plan, int lane) {
+    const uint32_t total = all_tiles(a, lane), most = plan.slots + a.n_seq;
+    const int hi = max(static_cast<int>((total + plan.slots - 1) / plan.slots), plan.least), lo = max(static_cast<int>((total + most - 1) / most), plan.least);
+    if (hi - lo <= hi / 8 || total >= 1u << 20) return hi;
+    const int mine = lane == 63 ? hi : min(hi, lo + lane * ((hi - lo + 62) / 63));
+    const float inv = 1.f / static_cast<float>(mine), up = static_cast<float>(mine) - 0.5f;
+    uint32_t slices = 0;
+    for (int s0 = 0; s0 < a.n_seq; s0 += 64) {
+        const float tiles = static_cast<float>(max(tiles_of(a, s0 + lane), 0));
+        for (int s = 0; s < min(64, a.n_seq - s0); s++) slices += static_cast<uint32_t>((__uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(tiles), s)) + up) * inv);
+    }
+    return __builtin_amdgcn_readlane(mine, __ffsll(static_cast<unsigned long long>(__ballot(slices <= most || lane == 63))) - 1);
+}
+
+// How a call's sequences are cut: slices, of several sequences of equal length, as many as the call has blocks for, and behind them one for the rows
+// themselves; where a call has one slice, it holds both.  most: call_len of several sequences.
+template <bool MANY>
 struct Cut {
     int len, cache, all;  // tiles of a slice, slices of the cache, slices
-    __device__ __forceinline__ Cut(const shv_attn_tree_args &a, int tiles, uint32_t total, const Plan &plan) {
+    __device__ __forceinline__ Cut(const shv_attn_tree_args &a, int tiles, int most, const Plan &plan) {
         if (a.n_splits == 1) {
             len = tiles;
             cache = 0;
             all = 1;
             return;
         }
-        const uint32_t slots = plan.slots, least = plan.least, share = (total + slots - 1) / slots, room = a.n_splits - 1;
-        uint32_t l = share > least ? share : least;
+        const uint32_t slots = plan.slots, least = plan.least, share = (tiles + slots - 1) / slots, room = a.n_splits - 1;
+        uint32_t l = MANY ? most : share > least ? share : least;
         if (l * static_cast<uint64_t>(room) < static_cast<uint32_t>(tiles)) l = (tiles + room - 1) / room;
-        len = l;
         cache = (tiles + l - 1) / l;
+        len = MANY && cache > 1 ? (tiles + cache - 1) / cache : l;  // (one sequence's last slice may be short: a division less)
         all = cache + 1;
     }
 };
@@ -148,16 +169,17 @@ struct Cut {
 // The `work`-th slice of all the call's: whose it is and which of its own; seq -1: there are fewer.  The slices stand in a row, without gaps for
 // sequences that have fewer of them: blocks that find nothing to do and end, one in seven between those that work, leave the latter on
 // few compute units (six windows of 9 slices in a grid of 64 a sequence 66 us, of 72 40, in a row 24).
+template <bool MANY>
 struct Slice {
     int seq, split;
-    __device__ __forceinline__ Slice(const shv_attn_tree_args &a, int work, uint32_t total, const Plan &plan, int lane) {
-        seq = a.n_seq == 1 ? 0 : -1;
+    __device__ __forceinline__ Slice(const shv_attn_tree_args &a, int work, int most, const Plan &plan, int lane) {
+        seq = MANY ? -1 : 0;
         split = work;
-        if (a.n_seq == 1) return;
+        if (!MANY) return;
         int before = 0;
         for (int s0 = 0; s0 < a.n_seq; s0 += 64) {
             const int tiles = tiles_of(a, s0 + lane);
-            const int mine = tiles < 0 ? 0 : Cut(a, tiles, total, plan).all;
+            const int mine = tiles < 0 ? 0 : Cut<true>(a, tiles, most, plan).all;
             int upto = mine;
 #pragma unroll
             for (int off = 1; off < 64; off <<= 1) {
@@ -347,14 +369,15 @@ struct TreeSmem {
     float p[W][16 * kTile / 2];  // a wave's weights of half a tile, where its values are not all finite (a whole one's would leave a unit one block of D 128)
 };
 
-// grid: (slices rounded up to 8, times query blocks; n_head_kv), W waves of 16 query rows.  Four waves: calls of up to 64 query rows a KV head, whose
+// grid: (slices rounded up to 8, times query blocks; n_head_kv), W waves of 16 query rows.  MANY: several sequences; of one the slices are known
+// without counting (one kernel for both costs a call of one 0.2 to 0.5 us).  Four waves: calls of up to 64 query rows a KV head, whose
 // rows every block norms and turns itself, the waves sharing the rows of however few groups there are.  Eight: wider ones, whose rows a
 // launch before (tree_prep_kernel) has left as operands.  There every block would have 128 rows to prepare, 5 us before its first product,
 // and the launch costs 4 (us of 12 rows behind 9000 cells so / with the launch 31.7 / 30.1, a batch of six windows 68 / 54).
 // Tried beside it: two groups a wave, so that an operand read serves both (512 registers a lane do not hold them: 1130 us where this takes
 // 260); a tile's keys multiplied under the weights of the one before (275 for 260); half of the waves half a tile behind the others (263, and a
 // batch of six windows 43 for 37).
-template <int D, int W>
+template <int D, int W, bool MANY>
 __global__ __launch_bounds__(64 * W, W == 4 || D == 256 ? 2 : 4) void tree_attn_kernel(shv_attn_tree_args a, Plan plan, char *stage) {
     constexpr bool kWide = W == 8;
     constexpr int VEC = D / 64, KI = D / 32, DB = D / 16;
@@ -367,8 +390,9 @@ __global__ __launch_bounds__(64 * W, W == 4 || D == 256 ? 2 : 4) void tree_attn_
     const int eight = blockIdx.x >> 3, of_eight = static_cast<int>(static_cast<uint32_t>(eight) / static_cast<uint32_t>(plan.q_blocks));
     const int work = of_eight * 8 + (blockIdx.x & 7), qb = eight - of_eight * plan.q_blocks;
     const int kvh = blockIdx.y;
-    const uint32_t total = a.n_seq > 1 ? all_tiles(a, lane) : 0;
-    const Slice slice(a, work, total, plan, lane);
+    const int most = MANY && a.n_splits > 1 ? call_len(a, plan, lane) : 0;
+    if (MANY && blockIdx.x == 0 && blockIdx.y == 0 && tid == 0) *plan.len = most;
+    const Slice<MANY> slice(a, work, most, plan, lane);
     if (slice.seq < 0) return;
     const int seq = __builtin_amdgcn_readfirstlane(slice.seq), split = __builtin_amdgcn_readfirstlane(slice.split);
     const int rep = a.n_head / a.n_head_kv;
@@ -394,7 +418,7 @@ __global__ __launch_bounds__(64 * W, W == 4 || D == 256 ? 2 : 4) void tree_attn_
     const int r_end = rows * rep;
     if (!fits(pos, rows, a.max_cells) || qb * W * 16 >= r_end) return;
     const Tiles tiles(a, pos);
-    const Cut cut(a, tiles.all, a.n_seq > 1 ? total : tiles.all, plan);
+    const Cut<MANY> cut(a, tiles.all, most, plan);
     if (split >= cut.all) return;
     const bool with_rows = split == cut.all - 1;
     const int t0 = with_rows && cut.all > 1 ? 0 : split * cut.len;
@@ -752,20 +776,20 @@ __global__ __launch_bounds__(64 * W, W == 4 || D == 256 ? 2 : 4) void tree_attn_
 
 // The slices' records of a row and head joined, a lane four dims.  NW waves share the records of 256 / D rows' heads, each folds its share with
 // all of a batch's loads on their way together, and the first wave folds their results.  grid: (ceil(rows * n_head * D / 256), n_seq).
-template <int D, int NW>
+template <int D, int NW, bool MANY>
 __global__ __launch_bounds__(64 * NW) void tree_merge_kernel(shv_attn_tree_args a, Plan plan) {
     __shared__ float4_t sums[NW][64];
     __shared__ float2 of[NW][64];
     constexpr int kLanes = D / 4;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, seq = blockIdx.y;
     const int rep = a.n_head / a.n_head_kv;
-    const int pos = a.pos ? a.pos[seq] : 0, rows = tree_rows(a.count, seq, a.rows);
+    const int most = MANY ? *plan.len : 0, pos = a.pos ? a.pos[seq] : 0, rows = tree_rows(a.count, seq, a.rows);
     const uint32_t unit = blockIdx.x * (64 / kLanes) + lane / kLanes;
     const int row = static_cast<int>(unit / static_cast<uint32_t>(a.n_head)), head = static_cast<int>(unit) - row * a.n_head;
     const bool there = row < rows;
     if (!fits(pos, rows, a.max_cells) || __ballot(there) == 0ull) return;
     const int tiles = Tiles(a, pos).all;
-    const Cut cut(a, tiles, a.n_seq > 1 ? all_tiles(a, lane) : tiles, plan);
+    const Cut<MANY> cut(a, tiles, most, plan);
     if (cut.all == 1) return;  // put straight out
     const float c2 = 1.44269504088896f / sqrtf(static_cast<float>(D));
     const int kvh = over_rep(plan, head), r = there ? row * rep + head - kvh * rep : 0;
@@ -815,15 +839,16 @@ __global__ __launch_bounds__(64 * NW) void tree_merge_kernel(shv_attn_tree_args 
     }
 }
 
-template <int D, int W>
+template <int D, int W, bool MANY>
 int launch_tree(shv_ctx *ctx, const shv_attn_tree_args &a) {
     const int rep = a.n_head / a.n_head_kv;
     constexpr int kBlocksPerUnit = D == 256 ? 1 : 2;
     Plan plan;
     plan.q_blocks = (a.rows * rep + 16 * W - 1) / (16 * W);
     // beside them every sequence has a slice for its rows and, of several, one that is not full
-    plan.slots = ctx->prop.multiProcessorCount * kBlocksPerUnit / (a.n_head_kv * plan.q_blocks) - (a.n_seq > 1 ? 2 : 1) * a.n_seq;
+    plan.slots = ctx->prop.multiProcessorCount * kBlocksPerUnit / (a.n_head_kv * plan.q_blocks) - (MANY ? 2 : 1) * a.n_seq;
     if (plan.slots < 1) plan.slots = 1;
+    plan.len = ctx->tree_len;
     // us with slices of 1 / 2 / 3 / 4 / 6 tiles at least: 2 rows behind 700 cells 12.4 / 12.6 / 13.2 / 14.0 / 16.2, 8 behind 3000 25.4 / 22.2 / 22.1 /
     // 22.9 / 24.0 (a slice more is a record more of every row to join); 32 behind 4000 (wide) - / 36.0 / 33.5 / 33.3 / 33.6
     plan.least = W == 4 ? kLeastNarrow : kLeastWide;
@@ -831,7 +856,7 @@ int launch_tree(shv_ctx *ctx, const shv_attn_tree_args &a) {
     static std::atomic<uint64_t> raised{0};  // by device
     const uint64_t bit = 1ull << (ctx->device & 63);
     if (!(raised.load(std::memory_order_acquire) & bit)) {
-        SHV_HIP_CHECK(hipFuncSetAttribute(reinterpret_cast<const void *>(&tree_attn_kernel<D, W>), hipFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(sizeof(TreeSmem<D, W>))));
+        SHV_HIP_CHECK(hipFuncSetAttribute(reinterpret_cast<const void *>(&tree_attn_kernel<D, W, MANY>), hipFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(sizeof(TreeSmem<D, W>))));
         raised.fetch_or(bit, std::memory_order_release);
     }
     // A sequence may have all the slices of the cache to itself, and those its share leaves over.  Of a wide call the last slice's records
@@ -845,23 +870,25 @@ int launch_tree(shv_ctx *ctx, const shv_attn_tree_args &a) {
         const int items = a.rows * (a.n_head + a.n_head_kv);
         SHV_LAUNCH(ctx, tree_prep_kernel<D>, dim3((items + 3) / 4, a.n_seq), dim3(256), 0, a, plan, stage);
     }
-    if (b.n_splits > plan.slots + 2) b.n_splits = plan.slots + 2;  // no sequence is cut into more
-    // slices of len tiles: all / len <= slots of them are full, every sequence may have one that is not, and has one of its rows
+    if (b.n_splits > plan.slots + a.n_seq + 1) b.n_splits = plan.slots + a.n_seq + 1;  // no sequence is cut into more
+    // slots + n_seq slices of the cache at most (call_len), and each sequence's of its rows
     const long long slices = b.n_splits == 1 ? a.n_seq : plan.slots + 2ll * a.n_seq;
-    SHV_LAUNCH(ctx, (tree_attn_kernel<D, W>), dim3(static_cast<unsigned>((slices + 7) / 8 * 8 * plan.q_blocks), a.n_head_kv), dim3(64 * W), sizeof(TreeSmem<D, W>), b, plan, stage);
+    SHV_LAUNCH(ctx, (tree_attn_kernel<D, W, MANY>), dim3(static_cast<unsigned>((slices + 7) / 8 * 8 * plan.q_blocks), a.n_head_kv), dim3(64 * W), sizeof(TreeSmem<D, W>), b, plan, stage);
     if (b.n_splits > 1) {
         const int units = (a.rows * a.n_head * D + 255) / 256;
         const dim3 grid(units, a.n_seq);
-        if (units * a.n_seq >= kMergeMany) SHV_LAUNCH(ctx, (tree_merge_kernel<D, 1>), grid, dim3(64), 0, b, plan);
-        else if (units * a.n_seq >= kMergeSome) SHV_LAUNCH(ctx, (tree_merge_kernel<D, 8>), grid, dim3(512), 0, b, plan);
-        else SHV_LAUNCH(ctx, (tree_merge_kernel<D, 4>), grid, dim3(256), 0, b, plan);
+        if (units * a.n_seq >= kMergeMany) SHV_LAUNCH(ctx, (tree_merge_kernel<D, 1, MANY>), grid, dim3(64), 0, b, plan);
+        else if (units * a.n_seq >= kMergeSome) SHV_LAUNCH(ctx, (tree_merge_kernel<D, 8, MANY>), grid, dim3(512), 0, b, plan);
+        else SHV_LAUNCH(ctx, (tree_merge_kernel<D, 4, MANY>), grid, dim3(256), 0, b, plan);
     }
     return SHV_OK;
 }
 
 template <int D>
 int launch_tree(shv_ctx *ctx, const shv_attn_tree_args &a) {
-    return a.rows * (a.n_head / a.n_head_kv) <= 64 ? launch_tree<D, 4>(ctx, a) : launch_tree<D, 8>(ctx, a);
+    const bool narrow = a.rows * (a.n_head / a.n_head_kv) <= 64;
+    if (a.n_seq == 1) return narrow ? launch_tree<D, 4, false>(ctx, a) : launch_tree<D, 8, false>(ctx, a);
+    return narrow ? launch_tree<D, 4, true>(ctx, a) : launch_tree<D, 8, true>(ctx, a);
 }
 
 // grid: (rows, n_seq): one kept row; the cells' keys lie as they will, their values go to their places in a tile of 32 cells.  Bound by the

@@ -86,6 +86,7 @@ int shv_init(int device, shv_ctx **out) {
     if (e == hipSuccess) e = hipMalloc(reinterpret_cast<void **>(&ctx->tree_val), shv_ctx::kTreePairs * sizeof(float));
     if (e == hipSuccess) e = hipMalloc(reinterpret_cast<void **>(&ctx->tree_idx), shv_ctx::kTreePairs * sizeof(int32_t));
     if (e == hipSuccess) e = hipMalloc(reinterpret_cast<void **>(&ctx->tree_counters), shv_ctx::kTreeCounters * sizeof(int32_t));
+    if (e == hipSuccess) e = hipMalloc(reinterpret_cast<void **>(&ctx->tree_len), sizeof(int32_t));
     if (e == hipSuccess) e = hipMemset(ctx->tree_counters, 0, shv_ctx::kTreeCounters * sizeof(int32_t));
     if (e == hipSuccess) e = hipMalloc(reinterpret_cast<void **>(&ctx->gemv_amax_val), shv_ctx::kGemvAmaxBlocks * sizeof(float));
     if (e == hipSuccess) e = hipMalloc(reinterpret_cast<void **>(&ctx->gemv_amax_idx), shv_ctx::kGemvAmaxBlocks * sizeof(int32_t));
@@ -122,6 +123,7 @@ void shv_destroy(shv_ctx *ctx) {
     if (ctx->tree_val) (void)hipFree(ctx->tree_val);
     if (ctx->tree_idx) (void)hipFree(ctx->tree_idx);
     if (ctx->tree_counters) (void)hipFree(ctx->tree_counters);
+    if (ctx->tree_len) (void)hipFree(ctx->tree_len);
     if (ctx->gemv_amax_val) (void)hipFree(ctx->gemv_amax_val);
     if (ctx->gemv_amax_idx) (void)hipFree(ctx->gemv_amax_idx);
     if (ctx->up_ring) (void)hipHostFree(ctx->up_ring);

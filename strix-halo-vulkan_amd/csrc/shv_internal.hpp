@@ -83,6 +83,7 @@ struct shv_ctx {
     float *tree_val = nullptr;
     int32_t *tree_idx = nullptr;
     int32_t *tree_counters = nullptr;
+    int32_t *tree_len = nullptr;  // tiles of an attn_tree's slices, for its join
     enum { kTreePairs = SHV_TREE_ACCEPT_MAX_ROWS, kTreeSeqs = 1024, kTreeCounterStep = 32, kTreeCounters = (kTreeSeqs + SHV_TREE_ACCEPT_MAX_ROWS) * kTreeCounterStep };
     // device address of this GPU's copy of the library's static scratch array (misc.hip), for the
     // entry point that allocates nothing

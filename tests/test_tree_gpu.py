@@ -11,7 +11,8 @@ pytestmark = pytest.mark.gpu
 A = shv.api
 EPS = 1e-6
 LAYOUTS = {"16/2x256": (16, 2, 256, 64), "32/8x128": (32, 8, 128, 128), "12/2x128": (12, 2, 128, 0), "8/8x64": (8, 8, 64, 32), "5/1x64": (5, 1, 64, 6),
-           "32/2x256": (32, 2, 256, 256), "64/1x64": (64, 1, 64, 10), "6/2x256": (6, 2, 256, 24), "9/3x128": (9, 3, 128, 12)}
+           "32/2x256": (32, 2, 256, 256), "64/1x64": (64, 1, 64, 10), "6/2x256": (6, 2, 256, 24), "9/3x128": (9, 3, 128, 12),
+           "32/16x128": (32, 16, 128, 64)}
 # Outputs: a score is a sum of d products q k / sqrt(d) of normed vectors, in absolute values at most about sqrt(d) <= 16.  Queries and
 # weights enter the products to 22 bits and sums are float32: an error of a score is within 16 * (2^-22 + a few 2^-24) = 1e-5, of a
 # weight as much again relative to it, of a weighted mean of the values no more than that.
@@ -132,6 +133,17 @@ def test_many_sequences_of_which_some_do_not_fit(ctx, rows, n_splits, window):
     t.pos[odd] = 0
     t.count[odd] = 0  # nothing of these is written
     t.check(window, 3)
+
+
+@pytest.mark.parametrize("layout,rows,pos,n_splits,window", [
+    ("32/16x128", 40, [1500, 3, 700, 1100, 0, 31, 64, 900], 32, 0), ("32/16x128", 3, [2000, 40, 1990, 5, 1, 800], 32, 0), ("8/8x64", 9, [33 * i for i in range(40)], 64, 0),
+    ("8/8x64", 9, [0] * 39 + [5000], 512, 0), ("16/2x256", 12, [4000, 4031, 4033, 96], 8, 0), ("32/8x128", 17, [3000, 2999, 17, 1600, 0], 64, 700)])
+def test_sequences_of_uneven_lengths_share_the_blocks(ctx, layout, rows, pos, n_splits, window):
+    """Lengths for which the slices' common length is looked for among many, with few and many slices a sequence."""
+    t = AttnTree(320 + rows, layout, rows, pos)
+    t.upload(ctx)
+    ctx.enqueue(A.OP_ATTN_TREE, t.args(ctx, n_splits, window, 2 if window else 0))
+    t.check(window, 2 if window else 0)
 
 
 def test_absent_arrays(ctx):

@@ -651,13 +651,20 @@ int launch(shv_ctx *ctx, const shv_gemv_q4k_args &a, int tiles) {
     return SHV_OK;
 }
 
+// Column parts of a row of sbs super-blocks, whose blocks each sum the whole row for its norm: until they fill the chip, and no more than
+// super-blocks, since a block asks for its first one before it knows anything else.
+constexpr int norm_parts(int sbs, int tiles) {
+    int parts = 1;
+    while (parts < sbs && parts * 4 * tiles < 512) parts *= 2;
+    return parts < sbs ? parts : sbs;
+}
+static_assert(norm_parts(8, 1) == 8 && norm_parts(8, 64) == 2, "2048 columns");
+static_assert(norm_parts(9, 10) == 9 && norm_parts(5, 8) == 5 && norm_parts(3, 8) == 3 && norm_parts(1, 8) == 1, "a count that is no power of two is not passed");
+
 int launch_stage(shv_ctx *ctx, const shv_gemv_q4k_args &a, int tiles, float *x_out) {
     const int sbs = a.k / 256;
-    // Only the RMSNorm prologue needs the whole row before a column of it: its blocks take column parts until they fill the
-    // chip, every one of them summing the whole row
-    int parts = sbs;
-    if (a.prologue == SHV_PRO_RMSNORM)
-        for (parts = 1; parts < sbs && parts * 4 * tiles < 512;) parts *= 2;
+    // Only the RMSNorm prologue needs the whole row before a column of it
+    const int parts = a.prologue == SHV_PRO_RMSNORM ? norm_parts(sbs, tiles) : sbs;
     const dim3 grid(parts, 4, tiles), block(256);
     switch (a.prologue) {
         case SHV_PRO_NONE: SHV_LAUNCH(ctx, (gemm_mid_stage_kernel<SHV_PRO_NONE, 0>), grid, block, 0, a, ctx->gemm_stage, tiles, x_out); break;

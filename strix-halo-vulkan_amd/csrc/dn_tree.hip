@@ -45,10 +45,11 @@ __device__ __forceinline__ void mma32(half8_t xh, half8_t xl, half8_t yh, half8_
     low = __builtin_amdgcn_mfma_f32_16x16x32_f16(xh, yl, low, 0, 0, 0);
     low = __builtin_amdgcn_mfma_f32_16x16x32_f16(xl, yh, low, 0, 0, 0);
 }
-__device__ __forceinline__ void mma16(half4_t xh, half4_t xl, half4_t yh, half4_t yl, float4_t &main, float4_t &low) {
-    main = __builtin_amdgcn_mfma_f32_16x16x16f16(xh, yh, main, 0, 0, 0);
-    low = __builtin_amdgcn_mfma_f32_16x16x16f16(xh, yl, low, 0, 0, 0);
-    low = __builtin_amdgcn_mfma_f32_16x16x16f16(xl, yh, low, 0, 0, 0);
+// acc + X Y for 16 x 16 tiles in float32: lane (n, g) holds X[n][4g ..] and Y[4g ..][n], the sum's own layout.
+__device__ __forceinline__ float4_t mma16(float4_t x, float4_t y, float4_t acc) {
+#pragma unroll
+    for (int e = 0; e < 4; e++) acc = __builtin_amdgcn_mfma_f32_16x16x4f32(x[e], y[e], acc, 0, 0, 0);
+    return acc;
 }
 __device__ __forceinline__ float max_over_g(float v) {
     auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
@@ -83,13 +84,13 @@ struct Scale {
 };
 
 constexpr int kKS = kD + 8;      // halves between rows of the [64][128] operands (272 B: 16 rows cover all banks)
-constexpr int kAS = kRows + 8;   // halves between rows of the [64][64] ones
-constexpr int kTS = 24;          // halves between rows of a 16 x 16 inverse
+constexpr int kAS = kRows + 4;   // floats between rows of the [64][64] ones (272 B as well)
+constexpr int kTS = 20;          // floats between rows of a 16 x 16 inverse
 template <int CT>
 struct TreeLds {
     _Float16 kh[kRows][kKS], kl[kRows][kKS], qh[kRows][kKS], ql[kRows][kKS];
-    _Float16 ah[kRows][kAS], al[kRows][kAS], mh[kRows][kAS], ml[kRows][kAS];  // -A, strictly below the diagonal blocks' diagonals, and M
-    _Float16 th[4][16][kTS], tl[4][16][kTS];                                  // the inverses of the diagonal blocks of I + A
+    float a[kRows][kAS], m[kRows][kAS];  // -A below the diagonal blocks, and M
+    float t[4][16][kTS];                 // the inverses of the diagonal blocks of I + A
     float adiag[4][16][17];
     float v[kRows][16 * CT + 4];
     double G[kRows];  // (differences of two of them are what counts: in float32 a row that forgets, log g = -100, would cost those behind it 2^-18)
@@ -105,9 +106,12 @@ struct TreeLds {
 //      K and Q against the state, which goes from memory to registers once
 //   3  a column tile a wave: the block rows' solve, the outputs.  A product's result is laid out as the next one's second operand,
 //      so a column tile never leaves its wave
-// A row whose delta is no number must reach its descendants alone, and the products are of whole tiles: A, M and B are cleaned of such values
-// first, and the outputs of rows that stand on one are made NaN at the end.  v, the state and B enter the products scaled by a power of two a column: any
-// float32.
+// The state enters the products scaled by a power of two a column, any float32: what binary16 cannot hold of it beside the column's largest, 2^-35 of that, is
+// below the rounding of a sum of 128 products with them.  The deltas of one column are of different branches, of which one may be of any size beside another, so the solve's
+// products are float32's own: where a row is no ancestor the weight is 0, and what it would add is exactly 0.  (With deltas as two binary16 values under a
+// common scale the rows beside a branch 2^40 times theirs were off by 0.2.)
+// A row whose delta is no number must reach its descendants alone, and the products are of whole tiles: A, M, B and the deltas are cleaned of such values
+// first, and the outputs of rows that stand on one are made NaN at the end.
 template <int CT>
 __global__ __launch_bounds__(64 * kWaves, 2) void dn_tree_kernel(shv_dn_tree_args a) {
     extern __shared__ __align__(16) char raw[];
@@ -286,14 +290,9 @@ __global__ __launch_bounds__(64 * kWaves, 2) void dn_tree_kernel(shv_dn_tree_arg
                 atomicOr(&L.lost[row], 2);
                 mv = 0.f;
             }
-            _Float16 hi, lo;
-            split(-av, hi, lo);
-            L.ah[row][s] = hi;
-            L.al[row][s] = lo;
-            split(mv, hi, lo);
-            L.mh[row][s] = hi;
-            L.ml[row][s] = lo;
             if (st == tt) L.adiag[tt][4 * g + r][n] = av;
+            else L.a[row][s] = -av;
+            L.m[row][s] = mv;
         }
     };
     if (wave < tiles) tile(wave, wave);
@@ -312,10 +311,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void dn_tree_kernel(shv_dn_tree_arg
                     else s0 = fmaf(-av, T[j], s0);
                 }
                 T[i] = s0 + s1;
-                _Float16 hi, lo;
-                split(T[i], hi, lo);
-                L.th[g][i][n] = hi;
-                L.tl[g][i][n] = lo;
+                L.t[g][i][n] = T[i];
             }
         }
     } else {
@@ -373,54 +369,40 @@ __global__ __launch_bounds__(64 * kWaves, 2) void dn_tree_kernel(shv_dn_tree_arg
 
     // ---- 3 ----
     const int lost_here = L.lost[lane];
-    const uint64_t bad = (static_cast<uint64_t>(or_over_g(bad_hi)) << 32 | or_over_g(bad_lo)) | __ballot((lost_here & 1) != 0), bad_out = __ballot((lost_here & 2) != 0);
-    float m = 0.f;
+    uint64_t bad = (static_cast<uint64_t>(or_over_g(bad_hi)) << 32 | or_over_g(bad_lo)) | __ballot((lost_here & 1) != 0);
+    const uint64_t bad_out = __ballot((lost_here & 2) != 0);
+    const auto clean = [&](float4_t &of, int tt) {  // of sums past float32's range
+        uint32_t over = 0;
 #pragma unroll
-    for (int tt = 0; tt < 4; tt++)
+        for (int r = 0; r < 4; r++) over |= fabsf(of[r]) < INFINITY ? 0u : 1u << (4 * g + r);
+        if (__ballot(over != 0) == 0ull) return;
+        bad |= static_cast<uint64_t>(or_over_g(over)) << (16 * tt);
 #pragma unroll
-        for (int r = 0; r < 4; r++) m = fmaxf(m, fabsf(B[tt][r]));
-    const Scale scale(max_over_g(m));
-    half4_t uh[4], ul[4];
+        for (int r = 0; r < 4; r++) of[r] = over >> (4 * g + r) & 1 ? 0.f : of[r];
+    };
+    float4_t u[4];
     const float root = 1.f / sqrtf(static_cast<float>(kD));
 #pragma unroll
     for (int tt = 0; tt < 4; tt++) {
         if (tt >= tiles) continue;
         // U_t = T_tt (B_t - sum over s < t of A_ts U_s)
-        float4_t am = {0.f, 0.f, 0.f, 0.f}, alo = am;
+        float4_t rest = B[tt];
 #pragma unroll
-        for (int st = 0; st < tt; st++)
-            mma16(*reinterpret_cast<const half4_t *>(&L.ah[16 * tt + n][16 * st + 4 * g]), *reinterpret_cast<const half4_t *>(&L.al[16 * tt + n][16 * st + 4 * g]), uh[st], ul[st], am, alo);
-        half4_t bh, bl;
+        for (int st = 0; st < tt; st++) rest = mma16(*reinterpret_cast<const float4_t *>(&L.a[16 * tt + n][16 * st + 4 * g]), u[st], rest);
+        clean(rest, tt);
+        u[tt] = mma16(*reinterpret_cast<const float4_t *>(&L.t[tt][n][4 * g]), rest, float4_t{0.f, 0.f, 0.f, 0.f});
+        clean(u[tt], tt);
+        float4_t om = O[tt];
 #pragma unroll
-        for (int r = 0; r < 4; r++) {
-            _Float16 hi, lo;
-            split(fmaf(B[tt][r], scale.down, fmaf(alo[r], kLoInv, am[r])), hi, lo);
-            bh[r] = hi;
-            bl[r] = lo;
-        }
-        float4_t um = {0.f, 0.f, 0.f, 0.f}, ulo = um;
-        mma16(*reinterpret_cast<const half4_t *>(&L.th[tt][n][4 * g]), *reinterpret_cast<const half4_t *>(&L.tl[tt][n][4 * g]), bh, bl, um, ulo);
-        float4_t u;
-#pragma unroll
-        for (int r = 0; r < 4; r++) {
-            u[r] = fmaf(ulo[r], kLoInv, um[r]);
-            _Float16 hi, lo;
-            split(u[r], hi, lo);
-            uh[tt][r] = hi;
-            ul[tt][r] = lo;
-        }
-        float4_t om = {0.f, 0.f, 0.f, 0.f}, olo = om;
-#pragma unroll
-        for (int st = 0; st <= tt; st++)
-            mma16(*reinterpret_cast<const half4_t *>(&L.mh[16 * tt + n][16 * st + 4 * g]), *reinterpret_cast<const half4_t *>(&L.ml[16 * tt + n][16 * st + 4 * g]), uh[st], ul[st], om, olo);
+        for (int st = 0; st <= tt; st++) om = mma16(*reinterpret_cast<const float4_t *>(&L.m[16 * tt + n][16 * st + 4 * g]), u[st], om);
 #pragma unroll
         for (int r = 0; r < 4; r++) {
             const int row = 16 * tt + 4 * g + r;
             if (row >= rows) continue;
             const bool lost = (L.anc[row] & bad) != 0, lost_out = lost || (bad_out >> row & 1) != 0;
             const size_t at = (static_cast<size_t>(seq) * a.rows + row) * vw + static_cast<size_t>(h) * kD + (slab * CT + wave) * 16 + n;
-            a.out[at] = lost_out ? __int_as_float(0x7fc00000) : fmaf(fmaf(olo[r], kLoInv, om[r]), scale.up, O[tt][r]) * root;
-            a.delta[at] = lost ? __int_as_float(0x7fc00000) : u[r] * scale.up;
+            a.out[at] = lost_out ? __int_as_float(0x7fc00000) : om[r] * root;
+            a.delta[at] = lost ? __int_as_float(0x7fc00000) : u[tt][r];
         }
     }
 }

@@ -484,6 +484,20 @@ def test_values_and_states_of_any_size(ctx, rows):
                 assert O.rel_l2(g[:, h, c], w[:, h, c]) <= 4 * DN_TOL, (name, h, c)
 
 
+@pytest.mark.parametrize("rows,far,columns", [(3, 20, None), (20, 40, None), (20, 40, 3), (64, 60, None), (64, 60, 77), (40, 24, 5), (33, -60, None)])
+def test_rows_of_one_branch_do_not_cost_the_others_their_places(ctx, rows, far, columns):
+    """Two branches behind one root, the values of one (all channels of them, or a single one a head) 2^far times the other's: every row of either is as near
+    to its own formula as if it were alone."""
+    t = DnTree(14, rows, [10], 2, 4)
+    t.parent[0] = np.maximum(np.arange(rows) - 2, 0)  # row 0, then odd rows on odd ones and even rows on even ones
+    t.parent[0, 0] = -1
+    v = np.arange(4 * D, 8 * D) if columns is None else 4 * D + columns + D * np.arange(4)
+    t.x[0, 1::2, v] *= np.float32(2.0 ** far)
+    t.upload(ctx)
+    ctx.enqueue(A.OP_DN_TREE, t.args())
+    t.check()
+
+
 def test_strong_and_weak_decays(ctx):
     """Gates far out: states that vanish in one row (a sum of logs of -1000 and below) and states that do not decay at all."""
     t = DnTree(9, 40, [10], 2, 4)

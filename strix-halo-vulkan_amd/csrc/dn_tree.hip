@@ -63,6 +63,8 @@ __device__ __forceinline__ uint32_t or_over_g(uint32_t v) {
     r = __builtin_amdgcn_permlane32_swap(v, v, false, false);
     return r[0] | r[1];
 }
+// e to this is 0 in float32 beside anything it may be a factor of, the growth of other rows by up to e^800 included.
+constexpr float kForgets = -1000.f;
 // Sum over each half of the wave, in every lane of it.
 __device__ __forceinline__ float sum32(float v) {
     v += dpp_f32<kDppXor1>(v);
@@ -199,13 +201,20 @@ __global__ __launch_bounds__(64 * kWaves, 2) void dn_tree_kernel(shv_dn_tree_arg
     Taps even, odd;
     if (wave < rows) load(even, wave);
     {
-        const double G = tree_sum(t, lane < rows ? softplus_ref(alpha + dt_bias) * decay : 0.f, a.rows, lane);
+        const float log_g = lane < rows ? softplus_ref(alpha + dt_bias) * decay : 0.f;
+        // A row of log g below kForgets, infinite perhaps, counts as kForgets: the rows' sums stay numbers whose differences say what lies between them.  What
+        // leaves the kernel is the sum as it is.
+        const bool forgets = log_g < kForgets;
+        const double G = tree_sum(t, forgets ? kForgets : log_g, a.rows, lane);
         if (wave == 0) {
             L.G[lane] = G;
             L.beta[lane] = lane < rows ? sigmoid_exact(write) : 0.f;
             L.anc[lane] = t.ancestors;
             L.lost[lane] = 0;
-            if (slab == 0 && lane < rows) a.decay[(static_cast<size_t>(seq) * a.rows + lane) * a.n_head_v + h] = static_cast<float>(G);
+        }
+        if (wave == kWaves - 1 && slab == 0) {
+            const double sum = __ballot(forgets) == 0ull ? G : tree_sum(t, log_g, a.rows, lane);
+            if (lane < rows) a.decay[(static_cast<size_t>(seq) * a.rows + lane) * a.n_head_v + h] = static_cast<float>(sum);
         }
     }
     const auto silu = [](float c) { return c * __builtin_amdgcn_rcpf(1.f + __expf(-c)); };

@@ -498,6 +498,28 @@ def test_rows_of_one_branch_do_not_cost_the_others_their_places(ctx, rows, far, 
     t.check()
 
 
+def test_a_row_that_forgets_everything(ctx):
+    """A log decay beyond float32's range (a of -3e38): the state before the row counts nothing, the row itself and those behind it are as ever."""
+    t = DnTree(15, 20, [10], 2, 4)
+    gates = t.x[0, :, t.cw + 4 * D:t.cw + 4 * D + 4]
+    gates[:, 1] = -40  # does not decay at all (log(1 + e^-40) is 0 in float32),
+    gates[[3, 8, 9], 1] = 12  # but for three rows
+    t.dt_bias[1] = 0
+    t.a[1] = -3e38
+    t.upload(ctx)
+    ctx.enqueue(A.OP_DN_TREE, t.args())
+    got = t.results()
+    with np.errstate(all="ignore"):
+        t.a = t.a.astype(np.float64)
+        t.x = t.x.astype(np.float64)
+        t.x[0, [r for r in range(20) if r not in (3, 8, 9)], t.cw + 4 * D + 1] = -2000  # (in 64 bits a gate that is 0 all the same)
+        want = t.want(0)
+    for name, g, w in (("out", got[0][0], want[0]), ("delta", got[2][0], want[2])):
+        for r in range(20):
+            for h in range(4):
+                assert O.rel_l2(g[r, h], w[r, h]) <= 2 * DN_TOL, (name, r, h)
+
+
 def test_strong_and_weak_decays(ctx):
     """Gates far out: states that vanish in one row (a sum of logs of -1000 and below) and states that do not decay at all."""
     t = DnTree(9, 40, [10], 2, 4)

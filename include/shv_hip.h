@@ -642,7 +642,8 @@ typedef struct {
  * rows are solved together, (I + A) delta = B with A[i][j] = beta_i e^(G_i - G_j) (k_j . k_i) where j is an ancestor of i, G_i
  * the sum of log g from the root to row i.
  * Beside out [n_seq][rows][hv*d] the call leaves kn [n_seq][rows][hk*d] (the normed keys), delta [n_seq][rows][hv*d] and
- * decay [n_seq][rows][hv] (G, whose rounding to float32 moves a weight of shv_dn_keep's sum by up to |G| 2^-23) for shv_dn_keep.  head_dim 128, conv 4, n_head_v a multiple of n_head_k, ring_slots >= 3. */
+ * decay [n_seq][rows][hv] (G) for shv_dn_keep, and, if log_g is not NULL, log_g [n_seq][rows][hv], each row's own log g.  head_dim 128, conv 4,
+ * n_head_v a multiple of n_head_k, ring_slots >= 3. */
 typedef struct {
     const float *x;
     const float *ring;
@@ -664,13 +665,16 @@ typedef struct {
     int32_t x_stride, ring_slots, ring_stride;
     int32_t n_planes, qk_norm_max;
     float eps;
+    float *log_g;            /* or NULL */
 } shv_dn_tree_args;
 
 /* The state behind the kept branch, S' = e^(G_last) S + sum_j e^(G_last - G_j) k_j delta_j^T over the rows path[s][0 .. n_keep[s]), from what
  * shv_dn_tree left, into plane (plane[slot] + 1) % n_planes (in place with n_planes 0 or 1; with n_keep 0 the state as it is), and the conv
  * channels (2*hk*d + hv*d floats) of its last three rows from x into the ring's rows at their positions.  With planes the
  * caller makes the new one the committed one, plane[slot] = (plane[slot] + 1) % n_planes.  n_keep counts at most rows; path entries that
- * are no row are passed over. */
+ * are no row are passed over.  With log_g, what lies between a row and the last is the sum of log g over the rows between and decay is not read (it may then be
+ * NULL): the state is as shv_dn_step leaves it row after row, however far a row forgets.  Without it the difference of two sums G in float32 moves a
+ * weight by up to |G| 2^-23: 2^-13 behind a row of log g = -1200. */
 typedef struct {
     const float *x;
     const float *kn;
@@ -687,6 +691,7 @@ typedef struct {
     int32_t n_head_k, n_head_v, head_dim, conv;
     int32_t x_stride, ring_slots, ring_stride;
     int32_t n_planes;
+    const float *log_g;      /* what shv_dn_tree left there, or NULL */
 } shv_dn_keep_args;
 
 /* The branch the model agrees with: best [n_seq][rows] receives each row's arg-max over logits [n_seq*rows][n] (logits_stride

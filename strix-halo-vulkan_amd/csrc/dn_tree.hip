@@ -214,7 +214,9 @@ __global__ __launch_bounds__(64 * kWaves, 2) void dn_tree_kernel(shv_dn_tree_arg
         }
         if (wave == kWaves - 1 && slab == 0) {
             const double sum = __ballot(forgets) == 0ull ? G : tree_sum(t, log_g, a.rows, lane);
-            if (lane < rows) a.decay[(static_cast<size_t>(seq) * a.rows + lane) * a.n_head_v + h] = static_cast<float>(sum);
+            const size_t at = (static_cast<size_t>(seq) * a.rows + lane) * a.n_head_v + h;
+            if (lane < rows) a.decay[at] = static_cast<float>(sum);
+            if (lane < rows && a.log_g) a.log_g[at] = log_g;
         }
     }
     const auto silu = [](float c) { return c * __builtin_amdgcn_rcpf(1.f + __expf(-c)); };
@@ -431,6 +433,8 @@ int launch_tree(shv_ctx *ctx, const shv_dn_tree_args &a) {
 // grid: (8 slabs of 16 state rows, n_head_v, n_seq): a thread holds eight values of one row.  HBM-bound: the state is read once
 // and written once (twelve sequences of 32 heads 12.9 us, 54 MB at 4.2 TB/s; one 4.1 us, the launch and two trips to memory).
 constexpr int kKeepRows = 16;
+// OWN: the rows' own log decays are there.
+template <bool OWN>
 __global__ __launch_bounds__(kBlock) void dn_keep_kernel(shv_dn_keep_args a) {
     __shared__ float fall[kRows];
     __shared__ int row[kRows];
@@ -451,17 +455,31 @@ __global__ __launch_bounds__(kBlock) void dn_keep_kernel(shv_dn_keep_args a) {
     if (tid < 64) {
         const int r = lane < keep ? a.path[base + lane] : -1;
         const bool on = r >= 0 && r < a.rows;
-        const float G = on ? a.decay[(base + r) * a.n_head_v + h] : 0.f;
+        const float G = on ? (OWN ? a.log_g : a.decay)[(base + r) * a.n_head_v + h] : 0.f;
         const uint64_t there = __ballot(on);
         const int n = __popcll(there);
-        const float last = n ? __shfl(G, 63 - __clzll(there), 64) : 0.f;
+        float behind, whole;  // log of the decay by the rows behind the lane's, and by all
+        if constexpr (OWN) {
+            double sum = G;  // from the lane's row to the last: each sum by itself, since of two long ones the difference loses what is short
+#pragma unroll
+            for (int far = 1; far < 64; far *= 2) {
+                const double more = __shfl_down(sum, far, 64);
+                sum += lane + far < 64 ? more : 0.0;
+            }
+            whole = static_cast<float>(__shfl(sum, 0, 64));
+            const float next = static_cast<float>(__shfl_down(sum, 1, 64));
+            behind = lane < 63 ? next : 0.f;
+        } else {
+            whole = n ? __shfl(G, 63 - __clzll(there), 64) : 0.f;
+            behind = whole - G;
+        }
         if (on) {
             const int k = __popcll(there & ((1ull << lane) - 1));
-            fall[k] = expf(last - G);
+            fall[k] = expf(behind);
             row[k] = r;
         }
         if (lane == 0) {
-            all = expf(last);
+            all = expf(whole);
             used = n;
         }
     }
@@ -521,7 +539,7 @@ int shv_launch_dn_tree(shv_ctx *ctx, const shv_dn_tree_args *pa) {
 
 int shv_launch_dn_keep(shv_ctx *ctx, const shv_dn_keep_args *pa) {
     const shv_dn_keep_args &a = *pa;
-    SHV_REQUIRE(a.x && a.kn && a.delta && a.decay && a.state && a.ring && a.path && a.n_keep, "dn_keep: NULL argument");
+    SHV_REQUIRE(a.x && a.kn && a.delta && (a.decay || a.log_g) && a.state && a.ring && a.path && a.n_keep, "dn_keep: NULL argument");
     SHV_REQUIRE(a.rows >= 1 && a.rows <= kRows, "dn_keep: %d rows; 1..%d", a.rows, kRows);
     SHV_REQUIRE(a.n_seq >= 1 && a.n_seq <= 65535, "dn_keep: %d sequences", a.n_seq);
     SHV_REQUIRE(a.head_dim == kD, "dn_keep: head_dim %d; built for %d", a.head_dim, kD);
@@ -532,6 +550,8 @@ int shv_launch_dn_keep(shv_ctx *ctx, const shv_dn_keep_args *pa) {
     SHV_REQUIRE(a.ring_stride >= cw && a.ring_slots >= a.conv - 1, "dn_keep: a ring of %d rows %d floats apart", a.ring_slots, a.ring_stride);
     SHV_REQUIRE(a.n_planes >= 0 && a.n_planes <= 64, "dn_keep: %d state planes", a.n_planes);
     SHV_REQUIRE(shv_aligned16(a.state) && shv_aligned16(a.kn), "dn_keep: state and kn must be 16-byte aligned");
-    SHV_LAUNCH(ctx, dn_keep_kernel, dim3(kD / kKeepRows, a.n_head_v, a.n_seq), dim3(kBlock), 0, a);
+    const dim3 grid(kD / kKeepRows, a.n_head_v, a.n_seq);
+    if (a.log_g) SHV_LAUNCH(ctx, dn_keep_kernel<true>, grid, dim3(kBlock), 0, a);
+    else SHV_LAUNCH(ctx, dn_keep_kernel<false>, grid, dim3(kBlock), 0, a);
     return SHV_OK;
 }

@@ -405,6 +405,7 @@ func AttnKeep(kcells, vcells, kcache, vcache, path, nKeep *Buffer, t Tree, nHead
 type DNTreeArgs struct {
 	X, Ring, Conv1D, A, DtBias, State, Out *Buffer
 	Kn, Delta, Decay                       *Buffer // what DNKeep needs of the rows
+	LogG                                   *Buffer // or nil: each row's log g, by which DNKeep's state is exact behind rows that forget
 	Tree                                   Tree
 	HeadK, HeadV, HeadDim, Conv            int
 	XStride, RingSlots, RingStride         int
@@ -422,7 +423,7 @@ func DNTree(d DNTreeArgs) Op {
 	a.n_seq, a.rows = C.int32_t(d.Tree.NSeq), C.int32_t(d.Tree.Rows)
 	a.n_head_k, a.n_head_v, a.head_dim, a.conv = C.int32_t(d.HeadK), C.int32_t(d.HeadV), C.int32_t(d.HeadDim), C.int32_t(d.Conv)
 	a.x_stride, a.ring_slots, a.ring_stride = C.int32_t(d.XStride), C.int32_t(d.RingSlots), C.int32_t(d.RingStride)
-	a.n_planes, a.eps = C.int32_t(d.Planes), C.float(d.Eps)
+	a.n_planes, a.eps, a.log_g = C.int32_t(d.Planes), C.float(d.Eps), fp(d.LogG)
 	return mk(C.SHV_OP_DN_TREE, unsafe.Pointer(&a), C.sizeof_shv_dn_tree_args)
 }
 
@@ -436,7 +437,7 @@ func DNKeep(d DNTreeArgs, path, nKeep *Buffer) Op {
 	a.n_seq, a.rows = C.int32_t(d.Tree.NSeq), C.int32_t(d.Tree.Rows)
 	a.n_head_k, a.n_head_v, a.head_dim, a.conv = C.int32_t(d.HeadK), C.int32_t(d.HeadV), C.int32_t(d.HeadDim), C.int32_t(d.Conv)
 	a.x_stride, a.ring_slots, a.ring_stride = C.int32_t(d.XStride), C.int32_t(d.RingSlots), C.int32_t(d.RingStride)
-	a.n_planes = C.int32_t(d.Planes)
+	a.n_planes, a.log_g = C.int32_t(d.Planes), fp(d.LogG)
 	return mk(C.SHV_OP_DN_KEEP, unsafe.Pointer(&a), C.sizeof_shv_dn_keep_args)
 }
 

@@ -155,7 +155,7 @@ class DnTreeArgs(C.Structure):
                 ("pos", C.c_void_p), ("slot", C.c_void_p), ("plane", C.c_void_p), ("parent", C.c_void_p), ("count", C.c_void_p),
                 ("n_seq", C.c_int32), ("rows", C.c_int32), ("n_head_k", C.c_int32), ("n_head_v", C.c_int32), ("head_dim", C.c_int32),
                 ("conv", C.c_int32), ("x_stride", C.c_int32), ("ring_slots", C.c_int32), ("ring_stride", C.c_int32), ("n_planes", C.c_int32),
-                ("qk_norm_max", C.c_int32), ("eps", C.c_float)]
+                ("qk_norm_max", C.c_int32), ("eps", C.c_float), ("log_g", C.c_void_p)]
 
 
 class DnKeepArgs(C.Structure):
@@ -163,7 +163,7 @@ class DnKeepArgs(C.Structure):
                 ("ring", C.c_void_p), ("path", C.c_void_p), ("n_keep", C.c_void_p), ("pos", C.c_void_p), ("slot", C.c_void_p),
                 ("plane", C.c_void_p), ("n_seq", C.c_int32), ("rows", C.c_int32), ("n_head_k", C.c_int32), ("n_head_v", C.c_int32),
                 ("head_dim", C.c_int32), ("conv", C.c_int32), ("x_stride", C.c_int32), ("ring_slots", C.c_int32), ("ring_stride", C.c_int32),
-                ("n_planes", C.c_int32)]
+                ("n_planes", C.c_int32), ("log_g", C.c_void_p)]
 
 
 class TreeAcceptArgs(C.Structure):

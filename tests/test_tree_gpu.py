@@ -564,6 +564,78 @@ def test_kept_state(ctx, rows, pos, heads, kind, planes):
     assert np.array_equal(ring, want_ring)
 
 
+@pytest.mark.parametrize("kind", ["one row", "twenty rows", "beyond float32", "none"])
+def test_kept_state_behind_rows_that_forget(ctx, kind):
+    """With log_g the state behind a branch is the rule's, row after row, where a row of it forgets all that was: log g of -1200 and then ordinary rows, twenty
+    rows of about -37, one of -3e38 times 12.  A weight is e to a sum of at most 30 ordinary log g of 1 or so, each within 2^-22 of itself: 30 * 2^-22 = 7e-6."""
+    rows, hv = 32, 4
+    t = DnTree(34, rows, [10, 3], 2, hv, kind="chain")
+    gates = t.x[:, :, t.cw + hv * D:t.cw + hv * D + hv]
+    t.a[:], t.dt_bias[:] = np.array([-1, -0.3, -1, -2], np.float32), 0
+    if kind == "one row":
+        gates[:, 4] = 1200
+    elif kind == "twenty rows":
+        gates[:, :20] = 37
+    elif kind == "beyond float32":
+        gates[:, :, 0] = -40  # a log g of 0 but for three rows
+        gates[:, [2, 3, 9], 0] = 12
+        t.a[0] = -3e38
+    t.upload(ctx)
+    d_log = ctx.upload(np.full(2 * rows * hv, 77.0, np.float32))
+    a = t.args()
+    a.log_g = d_log.ptr
+    ctx.enqueue(A.OP_DN_TREE, a)
+    if kind == "beyond float32":
+        t.a, t.x = t.a.astype(np.float64), t.x.astype(np.float64)
+        t.x[:, [r for r in range(rows) if r not in (2, 3, 9)], t.cw + hv * D] = -2000  # (in 64 bits a log g of 0 all the same)
+    path = np.tile(np.arange(rows, dtype=np.int32), (2, 1))
+    path[1, [3, 30]] = -1, rows  # passed over; the rule without these rows' products and decays is not the chain's: looked at below
+    lens = np.array([rows, 0], np.int32)
+    k = t.keep_args(ctx.upload(path), ctx.upload(lens))
+    k.log_g, k.decay = d_log.ptr, None
+    ctx.enqueue(A.OP_DN_KEEP, k)
+    got = t.d_state.read(np.float32, t.state.size).reshape(t.state.shape)
+    with np.errstate(all="ignore"):
+        want = t.want(0)[-1][-1]
+    slot = t.slot[0]
+    for h in range(hv):
+        assert O.rel_l2(got[slot, 1 - t.plane[slot], h], want[h]) <= DN_TOL, h
+    slot = t.slot[1]
+    assert np.array_equal(got[slot, 1 - t.plane[slot]], t.state[slot, t.plane[slot]])
+    # entries that are no row: as the same path without them
+    out = []
+    for p, n in ((path[1], rows), (np.delete(path[1], [3, 30]), rows - 2)):
+        state = ctx.upload(t.state)
+        k = t.keep_args(ctx.upload(np.stack([np.resize(p, rows)] * 2)), ctx.upload(np.array([0, n], np.int32)))
+        k.log_g, k.state, k.ring = d_log.ptr, state.ptr, ctx.upload(t.ring).ptr
+        ctx.enqueue(A.OP_DN_KEEP, k)
+        out.append(state.read(np.float32, t.state.size))
+    assert np.array_equal(out[0], out[1])
+
+
+@pytest.mark.parametrize("heads,count", [((16, 32), [7, 5]), ((2, 6), [0, 3])])
+def test_log_decays_of_the_rows(ctx, heads, count):
+    """log_g is each row's own, of rows in use alone, and leaves everything else as it is without it."""
+    t = DnTree(35, 7, [10, 2], *heads, count=count)
+    t.upload(ctx)
+    hv = heads[1]
+    ctx.enqueue(A.OP_DN_TREE, t.args())
+    plain = t.results()
+    d_log = ctx.upload(np.full(2 * 7 * hv, 77.0, np.float32))
+    a = t.args()
+    a.log_g = d_log.ptr
+    ctx.enqueue(A.OP_DN_TREE, a)
+    t.check()
+    assert all(np.array_equal(x, y) for x, y in zip(plain, t.results()))
+    got = d_log.read(np.float32, 2 * 7 * hv).reshape(2, 7, hv)
+    for s in range(2):
+        n, decay = t.n(s), t.want(s)[3]
+        for r in range(n):
+            way = T.chain(t.parent[s], r)
+            assert O.rel_l2(got[s, r], decay[r] - (decay[way[1]] if len(way) > 1 else 0)) <= DN_TOL, (s, r)
+        assert (got[s, n:] == 77.0).all()
+
+
 def test_keeping_passes_over_what_is_no_row(ctx):
     t = DnTree(33, 8, [4, 9], 2, 2)
     t.upload(ctx)

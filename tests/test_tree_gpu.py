@@ -120,6 +120,22 @@ def test_query_rows_and_slices_at_their_lines(ctx, layout, rows, pos, n_splits):
     t.check()
 
 
+@pytest.mark.parametrize("rows", [3, 8, 9, 40])
+def test_values_left_for_keeping_are_rounded_bit_by_bit(ctx, rows):
+    """vcells against the nearest binary16, signs and zeros too: values of either sign, zeros of either, denormals, ties, and what becomes infinite."""
+    t = AttnTree(330 + rows, "16/2x256", rows, [70, 5])
+    v0 = 2 * t.nh * t.d + t.nkv * t.d
+    v = t.qkv[:, :, v0:v0 + t.nkv * t.d]
+    odd = np.array([0.0, -0.0, 2.0 ** -24, -2.0 ** -25, 3 * 2.0 ** -25, -6e-8, 1 + 2.0 ** -11, -(1 + 3 * 2.0 ** -11), 65504, -65504, 65519.99, -65520, 7e4], np.float32)
+    v[:, :, :40] = t.rng.choice(odd, v[:, :, :40].shape)
+    t.upload(ctx)
+    ctx.enqueue(A.OP_ATTN_TREE, t.args(ctx))
+    with np.errstate(over="ignore"):
+        want = v.astype(np.float16).reshape(2, rows, t.nkv, t.d)
+    assert (np.signbit(want) & (want == 0)).any() and np.isinf(want).any()
+    assert np.array_equal(t.results()[2].view(np.uint16), want.view(np.uint16))
+
+
 @pytest.mark.parametrize("rows,n_splits,window", [(2, 16, 0), (9, 5, 0), (12, 16, 40)])
 def test_many_sequences_of_which_some_do_not_fit(ctx, rows, n_splits, window):
     """More sequences than a wave has lanes, of lengths from nothing to hundreds of cells, some without rows and some that do not fit the cache."""

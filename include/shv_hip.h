@@ -595,7 +595,9 @@ typedef struct {
  * float64 and rounded through float32, so that it does not depend on the order of a sum) and value; a value beyond
  * binary16's range becomes infinite there as in the cache, and reaches those rows that see its row and no others.  NaN and infinities in cells a row
  * does not see never reach it.  out [n_seq][rows][n_head*head_dim], before the sigmoid gate.
- * A sequence with pos < 0 or pos + rows in use > max_cells is left alone: nothing of it is written.
+ * A sequence with pos < 0 or pos + rows in use > max_cells is left alone: nothing of it is written, and out and cells hold what they held (shv_tree_accept with
+ * the same max_cells keeps nothing of it).  Its rows in use count and not their depths, so that room for the pass does not hang on the tree's shape: a
+ * caller that wants the last cells too drafts fewer rows there.
  * partial: n_seq*rows*n_head*n_splits*(head_dim+2) floats of scratch; n_splits 1..512 is how many ways the cells may be split. */
 typedef struct {
     const float *qkv;
@@ -700,7 +702,10 @@ typedef struct {
  * behind them, n_keep [n_seq] their number, next [n_seq] the best of the last: the token after the branch.  logits NULL: best is read
  * instead (tokens the caller drew for each row).  With count 0 n_keep is 0 and next -1.  ids [n_seq][rows] are the rows' tokens.
  * pos and base (both or neither; [n_seq]): base receives pos and pos moves on by n_keep, so that what keeps the branch takes base for its
- * pos and the next pass finds pos where it belongs.  At most SHV_TREE_ACCEPT_MAX_ROWS rows and 1024 sequences a call. */
+ * pos and the next pass finds pos where it belongs.  max_cells > 0 (with pos and base): a sequence that shv_attn_tree leaves alone with as many cells
+ * (pos < 0 or pos + rows in use > max_cells), whose logits are therefore of no pass, keeps nothing: path -1, n_keep 0, next -1, pos where it was; shv_attn_keep and
+ * shv_dn_keep then leave its cells, state and ring as they are, and the other sequences of a recorded round go on.  0: the caller sees to the room itself.
+ * At most SHV_TREE_ACCEPT_MAX_ROWS rows and 1024 sequences a call. */
 #define SHV_TREE_ACCEPT_MAX_ROWS 16384
 typedef struct {
     const float *logits;
@@ -715,6 +720,7 @@ typedef struct {
     int32_t *base;
     int32_t n_seq, rows;
     int32_t n, logits_stride;
+    int32_t max_cells, reserved;
 } shv_tree_accept_args;
 
 typedef struct {

@@ -29,9 +29,6 @@ constexpr int kBlock = 256;
 constexpr int kTile = 32;  // cells of a tile of V
 constexpr int kMaxSplits = 512;
 
-// Whether a sequence's rows fit behind what it has kept; the others are left alone.
-__device__ __forceinline__ bool fits(int pos, int n, int max_cells) { return n > 0 && pos >= 0 && pos <= max_cells - n; }
-
 // Sum over a wave, in every lane.
 template <int CTRL, int ROW_MASK = 0xF>
 __device__ __forceinline__ double dpp_f64(double v) {
@@ -111,7 +108,7 @@ __device__ __forceinline__ int over_rep(const Plan &plan, int r) { return static
 __device__ __forceinline__ int tiles_of(const shv_attn_tree_args &a, int s) {
     if (s >= a.n_seq) return -1;
     const int pos = a.pos ? a.pos[s] : 0;
-    return fits(pos, tree_rows(a.count, s, a.rows), a.max_cells) ? Tiles(a, pos).all : -1;
+    return tree_fits(pos, tree_rows(a.count, s, a.rows), a.max_cells) ? Tiles(a, pos).all : -1;
 }
 
 // Tiles that all sequences look at.
@@ -325,7 +322,7 @@ __global__ __launch_bounds__(256) void tree_prep_kernel(shv_attn_tree_args a, Pl
     val.load(query ? src : src + static_cast<size_t>(a.n_head_kv) * D, lane);
     gamma.load(query ? a.q_norm : a.k_norm, lane);
     const int pos = __builtin_amdgcn_readfirstlane(words.pos), rows = __builtin_amdgcn_readfirstlane(words.count);
-    if (row >= rows || !fits(pos, rows, a.max_cells)) return;
+    if (row >= rows || !tree_fits(pos, rows, a.max_cells)) return;
     const TreeRow t = tree_row(rows, words.parent, a.rows, lane);
     Turn<D> turn(a.rope_dims, lane);
     if (a.rope_dims > 0) {
@@ -416,7 +413,7 @@ __global__ __launch_bounds__(64 * W, W == 4 || D == 256 ? 2 : 4) void tree_attn_
     }
     const int slot = words.slot, pos = __builtin_amdgcn_readfirstlane(words.pos), rows = __builtin_amdgcn_readfirstlane(words.count);
     const int r_end = rows * rep;
-    if (!fits(pos, rows, a.max_cells) || qb * W * 16 >= r_end) return;
+    if (!tree_fits(pos, rows, a.max_cells) || qb * W * 16 >= r_end) return;
     const Tiles tiles(a, pos);
     const Cut<MANY> cut(a, tiles.all, most, plan);
     if (split >= cut.all) return;
@@ -787,7 +784,7 @@ __global__ __launch_bounds__(64 * NW) void tree_merge_kernel(shv_attn_tree_args 
     const uint32_t unit = blockIdx.x * (64 / kLanes) + lane / kLanes;
     const int row = static_cast<int>(unit / static_cast<uint32_t>(a.n_head)), head = static_cast<int>(unit) - row * a.n_head;
     const bool there = row < rows;
-    if (!fits(pos, rows, a.max_cells) || __ballot(there) == 0ull) return;
+    if (!tree_fits(pos, rows, a.max_cells) || __ballot(there) == 0ull) return;
     const int tiles = Tiles(a, pos).all;
     const Cut<MANY> cut(a, tiles, most, plan);
     if (cut.all == 1) return;  // put straight out

@@ -19,6 +19,9 @@ __device__ __forceinline__ int tree_rows(const int32_t *count, int seq, int rows
     return n < 0 ? 0 : n > rows ? rows : n;
 }
 
+// Whether a sequence has rows and they fit behind what it has kept; the others are left alone.
+__device__ __forceinline__ bool tree_fits(int pos, int n, int max_cells) { return n > 0 && pos >= 0 && pos <= max_cells - n; }
+
 // What memory says of a sequence and its tree, as words that are asked for together and branch nowhere: an absent array's word is
 // read from `any`, which is readable, and not used.
 struct TreeWords {

@@ -22,7 +22,8 @@ constexpr int kBlocksWanted = 2048;
 // By one whole wave: best_of is the lane's row's best.
 __device__ __forceinline__ void walk(const shv_tree_accept_args &a, int seq, int best_of, int lane) {
     const size_t base = static_cast<size_t>(seq) * a.rows;
-    const int n = tree_rows(a.count, seq, a.rows);
+    int n = tree_rows(a.count, seq, a.rows);
+    if (a.max_cells > 0 && !tree_fits(a.pos[seq], n, a.max_cells)) n = 0;  // no pass has looked at its rows
     const int parent = lane >= n ? -1 : a.parent ? a.parent[base + lane] : lane - 1;
     const int id = lane < n ? a.ids[base + lane] : 0;
     int kept = 0, at = 0, row_here = -1, next = -1;
@@ -117,6 +118,7 @@ int shv_launch_tree_accept(shv_ctx *ctx, const shv_tree_accept_args *pa) {
     SHV_REQUIRE(a.n_seq >= 1 && a.n_seq <= shv_ctx::kTreeSeqs, "tree_accept: %d sequences; 1..%d", a.n_seq, static_cast<int>(shv_ctx::kTreeSeqs));
     SHV_REQUIRE((a.pos == nullptr) == (a.base == nullptr), "tree_accept: pos and base go together");
     SHV_REQUIRE(!a.pos || a.pos != a.base, "tree_accept: pos and base are one array");
+    SHV_REQUIRE(a.max_cells == 0 || (a.max_cells > 0 && a.pos), "tree_accept: max_cells %d; 0, or the cache's with pos and base", a.max_cells);
     if (!a.logits) {
         SHV_LAUNCH(ctx, tree_walk_kernel, dim3(a.n_seq), dim3(64), 0, a);
         return SHV_OK;

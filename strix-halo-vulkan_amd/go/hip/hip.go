@@ -359,6 +359,7 @@ func AttnDecode(d AttnArgs) Op {
 type Tree struct {
 	NSeq, Rows               int
 	Pos, Slot, Parent, Count *Buffer // device int32
+	MaxCells                 int     // of the caches, for TreeAccept (with its pos and base): a sequence without room keeps nothing; 0: not looked at
 }
 
 // AttnTreeArgs are the fields of shv_attn_tree_args a caller sets.
@@ -448,6 +449,7 @@ func TreeAccept(logits, ids, best, path, nKeep, next, pos, base *Buffer, t Tree,
 	a.logits, a.ids, a.parent, a.count = fp(logits), ip(ids), ip(t.Parent), ip(t.Count)
 	a.best, a.path, a.n_keep, a.next, a.pos, a.base = ip(best), ip(path), ip(nKeep), ip(next), ip(pos), ip(base)
 	a.n_seq, a.rows, a.n, a.logits_stride = C.int32_t(t.NSeq), C.int32_t(t.Rows), C.int32_t(n), C.int32_t(stride)
+	a.max_cells = C.int32_t(t.MaxCells)
 	return mk(C.SHV_OP_TREE_ACCEPT, unsafe.Pointer(&a), C.sizeof_shv_tree_accept_args)
 }
 

@@ -169,7 +169,8 @@ class DnKeepArgs(C.Structure):
 class TreeAcceptArgs(C.Structure):
     _fields_ = [("logits", C.c_void_p), ("ids", C.c_void_p), ("parent", C.c_void_p), ("count", C.c_void_p), ("best", C.c_void_p),
                 ("path", C.c_void_p), ("n_keep", C.c_void_p), ("next", C.c_void_p), ("pos", C.c_void_p), ("base", C.c_void_p),
-                ("n_seq", C.c_int32), ("rows", C.c_int32), ("n", C.c_int32), ("logits_stride", C.c_int32)]
+                ("n_seq", C.c_int32), ("rows", C.c_int32), ("n", C.c_int32), ("logits_stride", C.c_int32), ("max_cells", C.c_int32),
+                ("reserved", C.c_int32)]
 
 
 class EmbedArgs(C.Structure):

@@ -98,3 +98,8 @@ def test_argument_blocks_fit_the_op_record():
         L = shv.pkg.load()
         assert L.shv_enqueue(_ctx(), kind, C.byref(args), C.sizeof(args) - 1) == -1
         assert b"argument block" in L.shv_last_error()
+
+
+@pytest.mark.parametrize("bad", [{"max_cells": -1}, {"max_cells": 64}, {"max_cells": -64, "pos": P, "base": P + 64}])
+def test_tree_accept_refuses_room_it_cannot_look_at(bad):
+    _refused("shv_tree_accept", acc(**bad), "max_cells")

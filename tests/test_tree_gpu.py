@@ -777,6 +777,31 @@ def test_of_equal_children_the_lowest_goes_on_and_positions_move(ctx):
     assert got[4].tolist() == [13, 205] and got[5].tolist() == [10, 200] and np.array_equal(got[0], picks)
 
 
+@pytest.mark.parametrize("given", [False, True])
+def test_a_sequence_without_room_keeps_nothing(ctx, given):
+    """max_cells: by rows in use, on both sides of the line; without it the walk is the tree's."""
+    t = Accept(63, 7, 6, 400, count=[6, 6, 5, 6, 1, 0, 6])
+    pos = np.array([58, 59, 59, -1, 63, 64, 2**31 - 3], np.int32)
+    left = [1, 3, 5, 6]
+    for cells in (64, 0):
+        up = ctx.upload
+        bufs = [up(t.best if given else np.full((7, 6), -7, np.int32)), up(np.full((7, 6), -8, np.int32)), up(np.full(7, -9, np.int32)), up(np.full(7, -9, np.int32)), up(pos),
+                up(np.full(7, -9, np.int32))]
+        a = A.TreeAcceptArgs(None if given else up(t.logits).ptr, up(t.ids).ptr, up(t.parent).ptr, up(t.count).ptr, *[b.ptr for b in bufs], 7, 6, t.n, t.stride, cells)
+        if not cells:
+            a.pos = a.base = None
+        ctx.enqueue(A.OP_TREE_ACCEPT, a)
+        best, path, n_keep, nxt, after, base = [b.read(np.int32, 42 if i < 2 else 7) for i, b in enumerate(bufs)]
+        best, path = best.reshape(7, 6), path.reshape(7, 6)
+        if not cells:
+            t.check([best, path, n_keep, nxt], best=t.best if given else None)
+            continue
+        assert np.array_equal(base, pos)
+        for s in range(7):
+            way, want_next = T.accept(t.best[s], t.ids[s], t.parent[s], 0 if s in left else t.n_of(s))
+            assert path[s].tolist() == way + [-1] * (6 - len(way)) and n_keep[s] == len(way) and nxt[s] == want_next and after[s] == pos[s] + len(way), s
+
+
 # ---- as they are used together -----------------------------------------------------------------
 
 
@@ -841,6 +866,76 @@ def test_rounds_of_a_hybrid_pair_of_layers_recorded_and_replayed(ctx):
         assert np.array_equal(dn.d_ring.read(np.float32, dn.ring.size).reshape(dn.ring.shape), dn.ring)
         pos, plane = pos + n_keep, plane + 1
         assert np.array_equal(at.d_pos.read(np.int32, 2), pos)
+    rec.destroy()
+
+
+def test_a_recorded_round_at_the_caches_end(ctx):
+    """Rounds of four sequences of which two run out of cells, one at once and one after a round: these stay as they are, round after round, while the others go on."""
+    rounds, rows, n_seq, vocab, cells = 4, 8, 4, 300, 96
+    c = ctx
+    at = AttnTree(90, "16/2x256", rows, [40, 89, 80, 3])
+    at.max_cells = cells
+    at.table = T.rope_table(cells, at.dims)
+    at.kc, at.vc = (at.rng.standard_normal((n_seq, cells, at.nkv, at.d), dtype=np.float32).astype(np.float16) for _ in range(2))
+    dn = DnTree(91, rows, [40, 89, 80, 3], 2, 4, slots=5)
+    dn.slot = at.slot
+    ac = Accept(92, n_seq, rows, vocab)
+    at.upload(c)
+    dn.upload(c)
+    d_ids, d_logits = c.upload(ac.ids), c.upload(ac.logits)
+    d_best, d_path, d_n, d_next, d_base = (c.alloc(4 * k) for k in (32, 32, 4, 4, 4))
+    dargs, kargs = dn.args(), dn.keep_args(d_path, d_n)
+    d_log = c.alloc(n_seq * rows * dn.hv * 4)
+    dargs.pos, dargs.parent, kargs.pos, kargs.plane, dargs.log_g, kargs.log_g = at.d_pos.ptr, at.d_parent.ptr, d_base.ptr, dn.d_plane.ptr, d_log.ptr, d_log.ptr
+    rec = c.prerecord([
+        A.make_op(A.OP_ATTN_TREE, at.args(c, 8)), A.make_op(A.OP_DN_TREE, dargs),
+        A.make_op(A.OP_TREE_ACCEPT, A.TreeAcceptArgs(d_logits.ptr, d_ids.ptr, at.d_parent.ptr, None, d_best.ptr, d_path.ptr, d_n.ptr, d_next.ptr, at.d_pos.ptr, d_base.ptr,
+                                                     n_seq, rows, vocab, vocab, cells)),
+        A.make_op(A.OP_ATTN_KEEP, A.AttnKeepArgs(at.d_kx.ptr, at.d_vx.ptr, at.d_kc.ptr, at.d_vc.ptr, d_path.ptr, d_n.ptr, d_base.ptr, at.d_slot.ptr, n_seq, rows, at.nkv,
+                                                 at.d, cells)),
+        A.make_op(A.OP_DN_KEEP, kargs), A.make_op(A.OP_ADVANCE, A.AdvanceArgs(dn.d_plane.ptr, n_seq, 1))])
+    pos, plane = at.pos.copy(), dn.plane.copy()
+    full = 0
+    for k in range(rounds):
+        at.qkv = at.rng.standard_normal(at.qkv.shape).astype(np.float32)
+        dn.x = at.rng.standard_normal(dn.x.shape).astype(np.float32)
+        at.parent = dn.parent = ac.parent = np.stack([T.tree(at.rng, rows) for _ in range(n_seq)])
+        ac.logits = at.rng.standard_normal(ac.logits.shape).astype(np.float32)
+        ac.settle(1.0)
+        kx_was, vx_was, out_was = at.results()[1:] + (at.results()[0],)
+        for b, v in ((at.d_qkv, at.qkv), (dn.d_x, dn.x), (at.d_parent, at.parent), (d_ids, ac.ids), (d_logits, ac.logits)):
+            b.write(v)
+        dn.plane = plane % 2
+        rec.launch()
+        out, kx, vx = at.results()
+        state = dn.d_state.read(np.float32, dn.state.size).reshape(dn.state.shape)
+        path, n_keep, nxt = d_path.read(np.int32, 32).reshape(4, 8), d_n.read(np.int32, 4), d_next.read(np.int32, 4)
+        for s in range(n_seq):
+            slot, cur = at.slot[s], plane[at.slot[s]] % 2
+            if pos[s] + rows > cells:
+                full += 1
+                assert n_keep[s] == 0 and nxt[s] == -1 and (path[s] == -1).all()
+                assert np.array_equal(out[s], out_was[s]) and np.array_equal(kx[s], kx_was[s]) and np.array_equal(vx[s], vx_was[s])
+                assert np.array_equal(state[slot, 1 - cur], dn.state[slot, cur])
+                continue
+            way, after = T.accept(ac.best[s], ac.ids[s], ac.parent[s], rows)
+            n = len(way)
+            assert path[s, :n].tolist() == way and n_keep[s] == n and nxt[s] == after
+            want = T.attn_tree(at.qkv[s], at.q_norm, at.k_norm, at.table, at.kc[slot], at.vc[slot], int(pos[s]), at.parent[s], rows, at.nh, at.nkv, at.d, at.dims, EPS)[0]
+            assert O.rel_l2(out[s], want) <= ATTN_TOL
+            states = T.dn_tree(dn.x[s], dn.ring[slot], dn.conv1d, dn.a, dn.dt_bias, dn.state[slot, cur], int(pos[s]), dn.parent[s], rows, dn.hk, dn.hv, D, EPS)[-1]
+            assert O.rel_l2(state[slot, 1 - cur], states[way[-1]]) <= DN_TOL
+            at.kc[slot, pos[s]:pos[s] + n], at.vc[slot, pos[s]:pos[s] + n] = kx[s, way], vx[s, way]
+            for j in range(max(0, n - 3), n):
+                dn.ring[slot, (pos[s] + j) % dn.ring_slots, :dn.cw] = dn.x[s, way[j], :dn.cw]
+            pos[s] += n
+        dn.state = state
+        plane = plane + 1
+        assert np.array_equal(at.d_pos.read(np.int32, 4), pos)
+        assert np.array_equal(at.d_kc.read(np.float16, at.kc.size).reshape(at.kc.shape), at.kc)
+        assert np.array_equal(v_host(at.d_vc.read(np.uint16, at.vc.size).reshape(v_dev(at.vc).shape)).view(np.float16), at.vc)
+        assert np.array_equal(dn.d_ring.read(np.float32, dn.ring.size).reshape(dn.ring.shape), dn.ring)
+    assert rounds < full < 2 * rounds  # one from the start, one from some round on
     rec.destroy()
 
 

@@ -705,7 +705,7 @@ typedef struct {
  * pos and the next pass finds pos where it belongs.  max_cells > 0 (with pos and base): a sequence that shv_attn_tree leaves alone with as many cells
  * (pos < 0 or pos + rows in use > max_cells), whose logits are therefore of no pass, keeps nothing: path -1, n_keep 0, next -1, pos where it was; shv_attn_keep and
  * shv_dn_keep then leave its cells, state and ring as they are, and the other sequences of a recorded round go on.  0: the caller sees to the room itself.
- * At most SHV_TREE_ACCEPT_MAX_ROWS rows and 1024 sequences a call. */
+ * At most SHV_TREE_ACCEPT_MAX_ROWS rows, 1024 sequences and n = 2^30 a call. */
 #define SHV_TREE_ACCEPT_MAX_ROWS 16384
 typedef struct {
     const float *logits;

@@ -123,7 +123,8 @@ int shv_launch_tree_accept(shv_ctx *ctx, const shv_tree_accept_args *pa) {
         SHV_LAUNCH(ctx, tree_walk_kernel, dim3(a.n_seq), dim3(64), 0, a);
         return SHV_OK;
     }
-    SHV_REQUIRE(a.n >= 1 && a.logits_stride >= a.n, "tree_accept: rows of %d logits, stride %d", a.n, a.logits_stride);
+    // (indexes along a row are 32 bits and step past its end by up to a block's stride)
+    SHV_REQUIRE(a.n >= 1 && a.n <= 1 << 30 && a.logits_stride >= a.n, "tree_accept: rows of %d logits, at most %d; stride %d", a.n, 1 << 30, a.logits_stride);
     const int all = a.n_seq * a.rows;
     SHV_REQUIRE(all <= SHV_TREE_ACCEPT_MAX_ROWS, "tree_accept: %d rows; at most %d", all, SHV_TREE_ACCEPT_MAX_ROWS);
     int nb = (a.n + kPiece - 1) / kPiece;

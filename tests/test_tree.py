@@ -103,3 +103,8 @@ def test_argument_blocks_fit_the_op_record():
 @pytest.mark.parametrize("bad", [{"max_cells": -1}, {"max_cells": 64}, {"max_cells": -64, "pos": P, "base": P + 64}])
 def test_tree_accept_refuses_room_it_cannot_look_at(bad):
     _refused("shv_tree_accept", acc(**bad), "max_cells")
+
+
+@pytest.mark.parametrize("n", [2**31 - 1, 2**31 - 2048, 2**30 + 1])
+def test_tree_accept_refuses_rows_its_indexes_cannot_count(n):
+    _refused("shv_tree_accept", acc(n=n, logits_stride=2**31 - 1), "logits")

@@ -70,9 +70,11 @@ typedef __attribute__((address_space(3))) void *lds_ptr_t;
 
 constexpr int kChunk = 64 * 16;
 constexpr int kStages = 4, kAhead = kStages - 1;
-// Weights are e^(s - m) 2^kLift, and m stands until a score is more than 2^kSlack above it: up to 2^15, which the larger half holds, and down to
-// 2^-31 of the largest with the smaller half's last place (at a lift of 0 2^-24, 6e-6 of a weight of a hundredth).
-constexpr float kLift = 7.f, kSlack = 8.f;
+// Weights are e^(s - m) 2^kLift, and m stands until a score is more than kSlack powers of two above it: up to 2^15.9, which the larger half holds (2^16 is too
+// much), and down to 2^-35 of the largest with the smaller half's last place, to which it is rounded and not cut: behind a first cell that takes nearly all and has
+// no value, as models have it, the output is what small weights make of theirs (3000 cells of 2^-20 in one slice, cut off at 2^-31, 2.4e-4 low).
+// Behind 131000 cells / the windowed batch, us: lift 7 and slack 8 264 / 38.0, 11 and 4.9 264 / 37.9, 11 and 4 265 / 38.3, 12 and 3 269 / 39.6, 14 and 1 272 / 39.5.
+constexpr float kLift = 11.f, kSlack = 4.9f;
 constexpr int kLeastNarrow = 2, kLeastWide = 3;  // tiles a slice gets at least: launch_tree has the figures
 // Waves that join the slices of 256 dims' rows: one where there are many such pieces, eight where there are some, four where there are few.  us
 // by one / four / eight waves: 32 pieces of 13 slices 3.9 / 4.2 / 5.4 (of 130 slices one wave would go to memory nine times in a row), 192 of
@@ -717,12 +719,13 @@ __global__ __launch_bounds__(64 * W, W == 4 || D == 256 ? 2 : 4) void tree_attn_
                 continue;
             }
         }
-        // weights as two halves, the large one cut off and not rounded: the small one holds the rest either way
+        // weights as two halves, the large one cut off and not rounded: the small one holds the rest either way, and is rounded to nearest, so that what
+        // many cells lose cancels
         half8_t ph, pl;
 #pragma unroll
         for (int e = 0; e < 8; e += 2) {
             const half2_t h = __builtin_bit_cast(half2_t, __builtin_amdgcn_cvt_pkrtz(pv[e], pv[e + 1]));
-            const half2_t r = __builtin_bit_cast(half2_t, __builtin_amdgcn_cvt_pkrtz(fmaf(static_cast<float>(h[0]), -1.f, pv[e]), fmaf(static_cast<float>(h[1]), -1.f, pv[e + 1])));
+            const half2_t r = {static_cast<_Float16>(fmaf(static_cast<float>(h[0]), -1.f, pv[e])), static_cast<_Float16>(fmaf(static_cast<float>(h[1]), -1.f, pv[e + 1]))};
             ph[e] = h[0]; ph[e + 1] = h[1];
             pl[e] = r[0]; pl[e + 1] = r[1];
         }

@@ -136,6 +136,28 @@ def test_values_left_for_keeping_are_rounded_bit_by_bit(ctx, rows):
     assert np.array_equal(t.results()[2].view(np.uint16), want.view(np.uint16))
 
 
+@pytest.mark.parametrize("rows,cells,n_splits,lead", [(3, 3000, 16, 22), (3, 3000, 1, 20), (40, 5000, 9, 22), (40, 9000, 64, 21), (2, 20000, 40, 19)])
+def test_small_weights_beside_a_first_cell_that_takes_nearly_all(ctx, rows, cells, n_splits, lead):
+    """A first cell with 2^lead times the weight of any other and a value of nothing, as models that rest on their first token have it: the output is what the
+    small weights make of their values.  A weight is rounded to the nearest 2^-35 of the largest, by at most 2^-36: of one of 2^-22 that is 2^-14, no two cells alike,
+    and of a sum over thousands of them 2^-14 / sqrt(3 * 3000) = 6e-7 is left."""
+    t = AttnTree(340 + lead, "12/2x128", rows, [cells], kind="star")
+    u = np.sign(t.rng.standard_normal(t.d)).astype(np.float32)
+    t.q_norm[:] = t.k_norm[:] = 1
+    t.qkv[0, :, :2 * t.nh * t.d].reshape(rows, t.nh, 2, t.d)[:, :, 0] = 3 * u
+    away = 1 - lead * np.log(2) / np.sqrt(t.d)
+    t.kc[:] = (away * u + 0.05 * t.rng.standard_normal(t.kc.shape)).astype(np.float16)
+    t.kc[:, 0] = u
+    t.vc[:] = (1 + 0.1 * t.rng.standard_normal(t.vc.shape)).astype(np.float16)
+    t.vc[:, 0] = 0
+    own = t.qkv[0, :, 2 * t.nh * t.d:]
+    own[:, :t.nkv * t.d] = np.tile(-u, t.nkv)
+    own[:, t.nkv * t.d:2 * t.nkv * t.d] = 1
+    t.upload(ctx)
+    ctx.enqueue(A.OP_ATTN_TREE, t.args(ctx, n_splits))
+    t.check()
+
+
 @pytest.mark.parametrize("rows,n_splits,window", [(2, 16, 0), (9, 5, 0), (12, 16, 40)])
 def test_many_sequences_of_which_some_do_not_fit(ctx, rows, n_splits, window):
     """More sequences than a wave has lanes, of lengths from nothing to hundreds of cells, some without rows and some that do not fit the cache."""

@@ -200,23 +200,21 @@ __global__ __launch_bounds__(64 * kWaves, 2) void dn_tree_kernel(shv_dn_tree_arg
     };
     Taps even, odd;
     if (wave < rows) load(even, wave);
-    {
+    // One wave forms what all need of the gates, another leaves what shv_dn_keep does.
+    if (wave == 0 || (wave == kWaves - 1 && slab == 0)) {
         const float log_g = lane < rows ? softplus_ref(alpha + dt_bias) * decay : 0.f;
-        // A row of log g below kForgets, infinite perhaps, counts as kForgets: the rows' sums stay numbers whose differences say what lies between them.  What
-        // leaves the kernel is the sum as it is.
+        // Between rows a log g below kForgets, infinite perhaps, counts as kForgets: the sums stay numbers whose differences say what lies between them.
         const bool forgets = log_g < kForgets;
-        const double G = tree_sum(t, forgets ? kForgets : log_g, a.rows, lane);
+        const double G = tree_sum(t, forgets && wave == 0 ? kForgets : log_g, a.rows, lane);
         if (wave == 0) {
             L.G[lane] = G;
             L.beta[lane] = lane < rows ? sigmoid_exact(write) : 0.f;
             L.anc[lane] = t.ancestors;
             L.lost[lane] = 0;
-        }
-        if (wave == kWaves - 1 && slab == 0) {
-            const double sum = __ballot(forgets) == 0ull ? G : tree_sum(t, log_g, a.rows, lane);
+        } else if (lane < rows) {
             const size_t at = (static_cast<size_t>(seq) * a.rows + lane) * a.n_head_v + h;
-            if (lane < rows) a.decay[at] = static_cast<float>(sum);
-            if (lane < rows && a.log_g) a.log_g[at] = log_g;
+            a.decay[at] = static_cast<float>(G);
+            if (a.log_g) a.log_g[at] = log_g;
         }
     }
     const auto silu = [](float c) { return c * __builtin_amdgcn_rcpf(1.f + __expf(-c)); };

@@ -579,6 +579,8 @@ typedef struct {
  *   count [n_seq]: rows in use, 0 .. rows; a larger number means rows, a negative one 0.  NULL: all.  Rows past it may hold
  *     anything, and what would be theirs in an output stays as it was.
  *   pos, slot as in the other ops: sequence s has kept pos[s] tokens (NULL: none) and owns cache or state slot slot[s] (NULL: s).
+ *     A sequence that is not there, so that one recorded pass serves fewer, has count 0 and a slot below 0: nothing of it is read or written but what
+ *     shv_tree_accept says of it.  (A sequence that is there and has count 0 keeps its slot, since shv_dn_keep carries its state over to the next plane.)
  * A row sits at position pos + its depth.  The pass itself changes neither cache, ring nor state: shv_attn_tree and shv_dn_tree
  * leave beside their outputs what is needed to keep a branch, shv_tree_accept finds the branch, shv_attn_keep and
  * shv_dn_keep (one call a layer) write it into cache, ring and state.  A call's sequences have different slots, all ops take

@@ -440,7 +440,7 @@ __global__ __launch_bounds__(kBlock) void dn_keep_kernel(shv_dn_keep_args a) {
     __shared__ int used;
     const int tid = threadIdx.x, lane = tid & 63;
     const int slab = blockIdx.x, h = blockIdx.y, seq = blockIdx.z, hk = h % a.n_head_k;
-    const int slot = a.slot ? a.slot[seq] : seq;
+    const int where = a.slot ? a.slot[seq] : seq, slot = max(where, 0);  // (a sequence that is not there reads the first slot and writes nothing: no branch before the loads)
     const int planes = a.n_planes > 1 ? a.n_planes : 1;
     const int cur = a.plane ? static_cast<int>(static_cast<unsigned>(a.plane[slot]) % static_cast<unsigned>(planes)) : 0;
     const int next = cur + 1 < planes ? cur + 1 : 0;
@@ -482,6 +482,7 @@ __global__ __launch_bounds__(kBlock) void dn_keep_kernel(shv_dn_keep_args a) {
         }
     }
     __syncthreads();
+    if (where < 0) return;
     const int n = used;
     const float f = all;
     s0.x *= f; s0.y *= f; s0.z *= f; s0.w *= f;

@@ -961,6 +961,72 @@ def test_a_recorded_round_at_the_caches_end(ctx):
     rec.destroy()
 
 
+def test_sequences_that_are_not_there(ctx):
+    """One recording for five sequences of which two, then three others, then none are there: slots of -1 and counts of 0.  What belongs to the others is theirs, and
+    memory in front of caches, rings and states stays as it is."""
+    rows, vocab = 9, 300
+    c = ctx
+    at, dn = AttnTree(95, "16/2x256", rows, [40, 33, 70, 5, 64], count=[9, 0, 4, 0, 0]), DnTree(96, rows, [40, 33, 70, 5, 64], 2, 4, slots=5, count=[9, 0, 4, 0, 0])
+    ac = Accept(97, 5, rows, vocab)
+    dn.slot, dn.parent, ac.parent = at.slot, at.parent, at.parent
+    ac.settle(0.9)
+    at.slot[[1, 3, 4]] = -1
+    at.upload(c)
+    dn.upload(c)
+
+    def behind_a_wall(v):  # in memory with as much again in front
+        n = (v.nbytes + 15) // 16 * 16
+        b = c.upload(np.concatenate([np.full(n, 0xA5, np.uint8), np.frombuffer(v.tobytes(), np.uint8)]))
+        return b, b.ptr + n, n
+
+    walls = [behind_a_wall(v) for v in (at.kc, v_dev(at.vc), dn.ring, dn.state)]
+    (_, kc, _), (_, vc, _), (_, ring, _), (_, state, _) = walls
+    bufs = [c.upload(np.full(k, -7, np.int32)) for k in (45, 45, 5, 5, 5)]
+    best, path, n_keep, nxt, base = bufs
+    aa, da, ka = at.args(c, 6), dn.args(), dn.keep_args(path, n_keep)
+    aa.kcache, aa.vcache, da.ring, da.state, ka.ring, ka.state = kc, vc, ring, state, ring, state
+    da.slot = ka.slot = at.d_slot.ptr
+    da.count = at.d_count.ptr
+    da.pos, ka.pos = at.d_pos.ptr, base.ptr
+    rec = c.prerecord([A.make_op(A.OP_ATTN_TREE, aa), A.make_op(A.OP_DN_TREE, da),
+                       A.make_op(A.OP_TREE_ACCEPT, A.TreeAcceptArgs(c.upload(ac.logits).ptr, c.upload(ac.ids).ptr, at.d_parent.ptr, at.d_count.ptr, best.ptr, path.ptr, n_keep.ptr,
+                                                                    nxt.ptr, at.d_pos.ptr, base.ptr, 5, rows, vocab, vocab, at.max_cells)),
+                       A.make_op(A.OP_ATTN_KEEP, A.AttnKeepArgs(at.d_kx.ptr, at.d_vx.ptr, kc, vc, path.ptr, n_keep.ptr, base.ptr, at.d_slot.ptr, 5, rows, at.nkv, at.d, at.max_cells)),
+                       A.make_op(A.OP_DN_KEEP, ka)])
+    for count, slots in (([9, 0, 4, 0, 0], [3, -1, 0, -1, -1]), ([0, 7, 0, 2, 1], [-1, 2, -1, 1, 4]), ([0] * 5, [-1] * 5)):
+        pos = at.d_pos.read(np.int32, 5)
+        at.count, at.slot = np.array(count, np.int32), np.array(slots, np.int32)
+        at.d_count.write(at.count)
+        at.d_slot.write(at.slot)
+        rec.launch()
+        keep = n_keep.read(np.int32, 5)
+        kx, vx = at.results()[1:]
+        for s in range(5):
+            way, after = T.accept(ac.best[s], ac.ids[s], ac.parent[s], count[s])
+            assert path.read(np.int32, 45).reshape(5, 9)[s].tolist() == way + [-1] * (9 - len(way)) and keep[s] == len(way) and nxt.read(np.int32, 5)[s] == after
+            if slots[s] < 0:
+                continue
+            j = slots[s]
+            want = T.dn_tree(dn.x[s], dn.ring[j], dn.conv1d, dn.a, dn.dt_bias, dn.state[j, dn.plane[j]], int(pos[s]), dn.parent[s], count[s], 2, 4, D, EPS)
+            for r in range(count[s]):
+                assert O.rel_l2(dn.results()[0][s, r], want[0][r]) <= DN_TOL
+            dn.state[j, 1 - dn.plane[j]] = want[-1][way[-1]]
+            at.kc[j, pos[s]:pos[s] + len(way)], at.vc[j, pos[s]:pos[s] + len(way)] = kx[s, way], vx[s, way]
+            for e in range(max(0, len(way) - 3), len(way)):
+                dn.ring[j, (pos[s] + e) % dn.ring_slots, :dn.cw] = dn.x[s, way[e], :dn.cw]
+        got = [b.read(np.uint8, b.nbytes) for b, _, n in walls]
+        assert all((g[:n] == 0xA5).all() for g, (_, _, n) in zip(got, walls))
+        body = [g[n:].tobytes() for g, (_, _, n) in zip(got, walls)]
+        assert body[0] == at.kc.tobytes() and body[1] == v_dev(at.vc).tobytes() and body[2] == dn.ring.tobytes()
+        got_state = np.frombuffer(body[3], np.float32).reshape(dn.state.shape)
+        assert O.rel_l2(got_state.ravel(), dn.state.ravel()) <= DN_TOL
+        for j in range(5):
+            if j not in slots:
+                assert np.array_equal(got_state[j], dn.state[j]), j
+        dn.state = got_state.copy()
+    rec.destroy()
+
+
 def test_two_recorded_passes_share_a_context(ctx):
     """Two recordings of all five ops with inputs of their own, replayed in turn with eager calls of a third between them: the context's scratch
     carries nothing from one to another."""

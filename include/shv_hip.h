@@ -588,7 +588,8 @@ typedef struct {
 #define SHV_TREE_MAX_ROWS 64
 
 /* Gated full attention of a tree's rows over a sequence's cells and their own ancestors.  qkv rows, norms, rotary table and
- * caches as shv_attn_decode has them, for head_dim 64, 128 or 256, any number of query heads per KV head up to 64, and rope_dims
+ * caches as shv_attn_decode has them, but without its mask (layers that attend over cells selected by shv_qsa_index cannot be verified with it: it attends over all that
+ * the window leaves), for head_dim 64, 128 or 256, any number of query heads per KV head up to 64, and rope_dims
  * any multiple of head_dim / 32 up to head_dim; norms and rotary table 16-byte aligned.  A query's values, normed and rotated, lie within
  * binary16's range (norm weights up to 2000 keep them there; a larger value makes its row's result no number).  Row i sees cell c < pos and each row on its way to the root, itself included, and with window > 0
  * only those of them whose position p is below sinks (the first tokens, which stay visible) or within the last `window`

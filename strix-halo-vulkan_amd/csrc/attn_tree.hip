@@ -11,9 +11,9 @@
 // with a running maximum and sum.  Tiles go from memory to LDS past the registers, three ahead.  The rows' own keys and values never enter the
 // cache here: one more block of a KV head forms their cells, attends over them by the ancestors' bits, and leaves them for attn_keep.  A second
 // launch joins the slices.
-// What bounds it: one or two rows behind a long cache the cache's bytes (131000 cells 54 us, 5.0 TB/s of K and V); 64 rows products and their
+// What bounds it: one or two rows behind a long cache the cache's bytes (131000 cells 53 us, 5.1 TB/s of K and V, much of it from the last-level cache); 64 rows products and their
 // operands' reads from LDS, each half of the cycles at its rate, with the softmax on the vector units between them (64 rows of 16 heads behind 131000
-// cells 259 us, 1.06 PFLOP/s of binary16 products, where a large library product reaches 1.18); short
+// cells 258 us, 1.06 PFLOP/s of binary16 products, where a large library product reaches 1.18); short
 // caches the chain of trips to memory before the first product (2 rows behind 700 cells 9 us and 4 for the join).
 #include <atomic>
 
@@ -78,7 +78,8 @@ constexpr float kLift = 11.f, kSlack = 4.9f;
 constexpr int kLeastNarrow = 2, kLeastWide = 3;  // tiles a slice gets at least: launch_tree has the figures
 // Waves that join the slices of 256 dims' rows: one where there are many such pieces, eight where there are some, four where there are few.  us
 // by one / four / eight waves: 32 pieces of 13 slices 3.9 / 4.2 / 5.4 (of 130 slices one wave would go to memory nine times in a row), 192 of
-// 95 14.5 / 8.6 / 7.6, 1024 of 32 10.8 / 11.9 / 19, 2016 of 11 6.0 / 10.7 / 21.
+// 95 14.5 / 8.6 / 7.6, 1024 of 32 10.8 / 11.9 / 19, 2016 of 11 6.0 / 10.7 / 21.  Whole calls of 128 dims: 256 pieces 31.0 / 27.0 / 27.7, 1024 45.8 / 47.0 /
+// 53.6; of 64 dims: 64 pieces 28.4 / 21.7 / 20.8, 256 31.6 / 27.3 / 28.1, 1024 47.2 / 48.9 / 56.7 (one line for all widths costs their middle 0.8).
 constexpr int kMergeMany = 512, kMergeSome = 64;
 
 // Which tiles of 32 cells a sequence's rows look at: the sinks', then those the window of the first row reaches.
@@ -167,7 +168,7 @@ struct Cut {
 
 // The `work`-th slice of all the call's: whose it is and which of its own; seq -1: there are fewer.  The slices stand in a row, without gaps for
 // sequences that have fewer of them: blocks that find nothing to do and end, one in seven between those that work, leave the latter on
-// few compute units (six windows of 9 slices in a grid of 64 a sequence 66 us, of 72 40, in a row 24).
+// few compute units (six windows of 9 slices in a grid of 64 a sequence 66 us, of 72 40, in a row 24, and 27 with the count of all that makes them of like length).
 template <bool MANY>
 struct Slice {
     int seq, split;
@@ -372,7 +373,8 @@ struct TreeSmem {
 // without counting (one kernel for both costs a call of one 0.2 to 0.5 us).  Four waves: calls of up to 64 query rows a KV head, whose
 // rows every block norms and turns itself, the waves sharing the rows of however few groups there are.  Eight: wider ones, whose rows a
 // launch before (tree_prep_kernel) has left as operands.  There every block would have 128 rows to prepare, 5 us before its first product,
-// and the launch costs 4 (us of 12 rows behind 9000 cells so / with the launch 31.7 / 30.1, a batch of six windows 68 / 54).
+// and the launch costs 4 (us of 12 rows behind 9000 cells so / with the launch 31.7 / 30.1, a batch of six windows 68 / 54, before the steps that brought
+// these to 26 and 38).  Of 128 dims eight waves hold 128 registers each, so that two blocks share a unit, and 10 more stand in scratch memory, 36 bytes a lane.
 // Tried beside it: two groups a wave, so that an operand read serves both (512 registers a lane do not hold them: 1130 us where this takes
 // 260); a tile's keys multiplied under the weights of the one before (275 for 260); half of the waves half a tile behind the others (263, and a
 // batch of six windows 43 for 37).
@@ -845,12 +847,16 @@ int launch_tree(shv_ctx *ctx, const shv_attn_tree_args &a) {
     constexpr int kBlocksPerUnit = D == 256 ? 1 : 2;
     Plan plan;
     plan.q_blocks = (a.rows * rep + 16 * W - 1) / (16 * W);
-    // beside them every sequence has a slice for its rows and, of several, one that is not full
+    // Beside them every sequence has a slice for its rows and, of several, one that is not full.  Each counts as a block for the whole call, though it ends soon: from
+    // about ten wide sequences on part of the chip idles (64 rows behind 9000 cells each: eight sequences 201 us, ten 265, sixteen 494), and beside many
+    // sequences a long one gets too few slices (sixteen of 64 rows, one behind 131000 cells and the others behind 500, 3050 us, where that one alone takes 274).
     plan.slots = ctx->prop.multiProcessorCount * kBlocksPerUnit / (a.n_head_kv * plan.q_blocks) - (MANY ? 2 : 1) * a.n_seq;
     if (plan.slots < 1) plan.slots = 1;
     plan.len = ctx->tree_len;
     // us with slices of 1 / 2 / 3 / 4 / 6 tiles at least: 2 rows behind 700 cells 12.4 / 12.6 / 13.2 / 14.0 / 16.2, 8 behind 3000 25.4 / 22.2 / 22.1 /
-    // 22.9 / 24.0 (a slice more is a record more of every row to join); 32 behind 4000 (wide) - / 36.0 / 33.5 / 33.3 / 33.6
+    // 22.9 / 24.0 (a slice more is a record more of every row to join); 32 behind 4000 (wide) - / 36.0 / 33.5 / 33.3 / 33.6.  Of 128 dims (rep 4) 12.0 / 12.2 / 12.0 /
+    // 12.7 / 14.1, 18.0 / 18.1 / 17.9 / 18.0 / 18.9 and 32.8 / 32.7 / 31.1 / 31.9 / 32.0; of 64 (rep 8) 10.1 / 10.4 / 10.9 / 11.2 / 12.4, 17.2 / 15.1 / 15.3 / 16.1 / 17.4 and
+    // 24.5 / 20.7 / 20.5 / 20.7 / 22.3
     plan.least = W == 4 ? kLeastNarrow : kLeastWide;
     plan.rep_magic = ((1u << 20) + rep - 1) / rep;
     static std::atomic<uint64_t> raised{0};  // by device

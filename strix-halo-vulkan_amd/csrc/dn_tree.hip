@@ -6,9 +6,10 @@
 //     out_i   = (e^(G_i) S0^T q_i + sum over ancestors j and i itself of e^(G_i - G_j) (k_j . q_i) delta_j) / sqrt(d)
 // so no row needs a state of its own: S0 is read once, whatever the tree's shape, and the deltas are a triangular solve whose
 // matrix is masked by ancestry.
-// What bounds it, of 16 key and 32 value heads: a small tree its chain of steps, each waiting for the one before (parents, rows, products of
-// rows, inverse, solve: 5 rows 7.4 us, whose 2.5 MB would take 0.5); wide ones the preparing of rows, which every value head's block does for
-// itself on the vector units, and then the same chain (eight sequences of up to 64 rows 22.6 us, whose 36 MB would take 8).
+// What bounds it, of 16 key and 32 value heads: its chain of steps, each waiting for the one before.  In thousands of cycles of a block's first wave, 5
+// rows of one sequence / 64 of each of eight: the sequence's words and parents 4 / 6, gates 1.5 / 5, rows 1.5 / 13 and the wait for the slowest wave's 0.5 / 2,
+// products of rows 2.3 / 2.5, inverse and the products below the diagonal 0.1 / 3.3, products with the state 2.1 / 7.5, solve and outputs 2.1 / 10
+// (14 and 49: 7.0 us, whose 2.5 MB would take 0.5, and 26; with up to 64 rows 22, whose 36 MB would take 8).
 #include <atomic>
 
 #include "shv_device.hpp"
@@ -159,7 +160,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void dn_tree_kernel(shv_dn_tree_arg
     };
     // Where a lane's row's taps are: the row, its parent, grandparent and the one above it; behind the root the ring's rows.  Each is read as a buffer
     // of the conv's channels, and of none before the sequence's start, where loads give zeros: nothing waits to put them there, and a
-    // row's loads stay on their way under the row before (64 rows of one sequence 17.5 us, of eight 25.4; where a select put the zeros 19.5 and 27.3).
+    // row's loads stay on their way under the row before (where a select put the zeros, 64 rows of one sequence took 2 us more).
     const uint32_t width = static_cast<uint32_t>(2 * qk + vw) * 4;
     const float *from[3];
     uint64_t there[3];
@@ -428,8 +429,9 @@ int launch_tree(shv_ctx *ctx, const shv_dn_tree_args &a) {
     return SHV_OK;
 }
 
-// grid: (8 slabs of 16 state rows, n_head_v, n_seq): a thread holds eight values of one row.  HBM-bound: the state is read once
-// and written once (twelve sequences of 32 heads 12.9 us, 54 MB at 4.2 TB/s; one 4.1 us, the launch and two trips to memory).
+// grid: (8 slabs of 16 state rows, n_head_v, n_seq): a thread holds eight values of one row.  Memory-bound: the state is read once
+// and written once (twelve sequences of 32 heads, 54 MB: 13.8 us where the last-level cache still holds them, 19.1 from memory; one 3.9 us, the launch
+// and two trips to memory).
 constexpr int kKeepRows = 16;
 // OWN: the rows' own log decays are there.
 template <bool OWN>
@@ -528,8 +530,8 @@ int shv_launch_dn_tree(shv_ctx *ctx, const shv_dn_tree_args *pa) {
                     shv_aligned16(a.kn) && shv_aligned16(a.delta),
                 "dn_tree: x, ring, conv1d, state, out, kn and delta must be 16-byte aligned");
     // Columns cut in four, two or not at all: as far as every block still finds a compute unit of its own (a block's rows are prepared anew
-    // whatever its columns).  us of 5 / 64 rows of one sequence of 32 value heads cut in four 7.3 / 17.8, in two 7.9 / 17.7, whole
-    // 9.8 / 20.6; of four sequences 13.6 / 38, 8.3 / 20.8, 10.2 / 23.5.
+    // whatever its columns).  us of 5 / 64 rows of one sequence of 32 value heads cut in four 7.0 / 17.8, in two 7.4 / 17.8, whole
+    // 9.3 / 21.5; of four sequences 12.5 / 36, 7.5 / 19.8, 9.4 / 23.6.
     const int heads = a.n_seq * a.n_head_v, units = ctx->prop.multiProcessorCount;
     if (4 * heads <= units) return launch_tree<2>(ctx, a);
     if (2 * heads <= units) return launch_tree<4>(ctx, a);

@@ -1,7 +1,8 @@
 // The branch of a drafted tree that the model agrees with: the arg-max of every row's logits and the walk over them, one launch.
 //
-// HBM-bound on the logits, which are read once: a row is cut into as many pieces as fill the chip, each block leaves its
-// piece's best, the block of a row that finishes last joins the row's pieces, and the row of a sequence that does walks the tree.
+// Memory-bound on the logits, which are read once (97 rows of 151936 14.6 us where the last-level cache still holds them, 17.4 from memory, 3.4
+// TB/s): a row is cut into as many pieces as fill the chip, each block leaves its piece's best, the block of a row that finishes last joins the
+// row's pieces, and the row of a sequence that does walks the tree.
 // (Counted by sequence alone, 64 rows of 64 pieces wait 15 ns each for one counter: 60 us, now 9.6.)  The walk
 // is one wave: lane i holds row i, a step asks all lanes at once which of them follow the row it stands on with the token that row
 // wants, and takes the lowest.
@@ -14,7 +15,7 @@ namespace {
 using namespace shv;
 
 constexpr int kBlock = 256;
-// us of 5 / 64 / 192 rows of 151936: pieces of 1024 floats at least 6.4 / 9.7 / 21, of 2048 5.6 / 9.6 / 21 (5.6 TB/s), of 8192 6.3 / 9.7 / 21; cut for
+// us of 5 / 64 / 192 rows of 151936, the last-level cache holding them: pieces of 1024 floats at least 6.4 / 9.7 / 21, of 2048 5.6 / 9.6 / 21 (5.6 TB/s), of 8192 6.3 / 9.7 / 21; cut for
 // 4096 blocks 5.6 / 12.4 / 22.4, for 1024 5.6 / 9.6 / 20.9
 constexpr int kPiece = 2048;       // floats of a row a block takes at least
 constexpr int kBlocksWanted = 2048;

@@ -676,7 +676,7 @@ typedef struct {
 /* The state behind the kept branch, S' = e^(G_last) S + sum_j e^(G_last - G_j) k_j delta_j^T over the rows path[s][0 .. n_keep[s]), from what
  * shv_dn_tree left, into plane (plane[slot] + 1) % n_planes (in place with n_planes 0 or 1; with n_keep 0 the state as it is), and the conv
  * channels (2*hk*d + hv*d floats) of its last three rows from x into the ring's rows at their positions.  With planes the
- * caller makes the new one the committed one, plane[slot] = (plane[slot] + 1) % n_planes.  n_keep counts at most rows; path entries that
+ * caller makes the new one the committed one, plane[slot] = (plane[slot] + 1) % n_planes, of this call's slots and no others.  n_keep counts at most rows; path entries that
  * are no row are passed over.  With log_g, what lies between a row and the last is the sum of log g over the rows between and decay is not read (it may then be
  * NULL): the state is as shv_dn_step leaves it row after row, however far a row forgets.  Without it the difference of two sums G in float32 moves a
  * weight by up to |G| 2^-23: 2^-13 behind a row of log g = -1200. */

@@ -1027,6 +1027,45 @@ def test_sequences_that_are_not_there(ctx):
     rec.destroy()
 
 
+def test_recorded_rounds_in_place_on_some_of_the_slots(ctx):
+    """One state a slot, two sequences on two of five slots: rounds need nothing advanced, and the other slots' states and rings are not touched."""
+    rows, vocab, n_seq = 7, 200, 2
+    c = ctx
+    dn, ac = DnTree(98, rows, [20, 6, 1, 1, 1], 2, 4, planes=1, slots=4), Accept(99, n_seq, rows, vocab)
+    dn.n_seq, dn.pos, dn.slot = n_seq, dn.pos[:n_seq].copy(), np.array([4, 1], np.int32)
+    dn.x, dn.parent = dn.x[:n_seq], dn.parent[:n_seq]
+    ac.parent = dn.parent
+    dn.upload(c)
+    d_ids, d_logits, d_log = c.upload(ac.ids), c.upload(ac.logits), c.alloc(n_seq * rows * 4 * 4)
+    best, path, n_keep, nxt, base = (c.upload(np.zeros(k, np.int32)) for k in (14, 14, 2, 2, 2))
+    da, ka = dn.args(), dn.keep_args(path, n_keep)
+    da.log_g = ka.log_g = d_log.ptr
+    ka.pos, ka.decay = base.ptr, None
+    rec = c.prerecord([A.make_op(A.OP_DN_TREE, da),
+                       A.make_op(A.OP_TREE_ACCEPT, A.TreeAcceptArgs(d_logits.ptr, d_ids.ptr, dn.d_parent.ptr, None, best.ptr, path.ptr, n_keep.ptr, nxt.ptr, dn.d_pos.ptr,
+                                                                    base.ptr, n_seq, rows, vocab, vocab)),
+                       A.make_op(A.OP_DN_KEEP, ka)])
+    for _ in range(4):
+        dn.x = dn.rng.standard_normal(dn.x.shape).astype(np.float32)
+        ac.settle(0.9)
+        dn.d_x.write(dn.x)
+        d_ids.write(ac.ids)
+        rec.launch()
+        states = dn.check()
+        for s in range(n_seq):
+            way, _ = T.accept(ac.best[s], ac.ids[s], ac.parent[s], rows)
+            assert path.read(np.int32, 14).reshape(2, 7)[s].tolist() == way + [-1] * (7 - len(way))
+            got = dn.d_state.read(np.float32, dn.state.size).reshape(dn.state.shape)[dn.slot[s], 0]
+            assert O.rel_l2(got, states[s][way[-1]]) <= DN_TOL
+            dn.state[dn.slot[s], 0] = got
+            for e in range(max(0, len(way) - 3), len(way)):
+                dn.ring[dn.slot[s], (dn.pos[s] + e) % dn.ring_slots, :dn.cw] = dn.x[s, way[e], :dn.cw]
+            dn.pos[s] += len(way)
+        assert np.array_equal(dn.d_state.read(np.float32, dn.state.size), dn.state.ravel()) and np.array_equal(dn.d_ring.read(np.float32, dn.ring.size), dn.ring.ravel())
+        assert np.array_equal(dn.d_pos.read(np.int32, 2), dn.pos)
+    rec.destroy()
+
+
 def test_two_recorded_passes_share_a_context(ctx):
     """Two recordings of all five ops with inputs of their own, replayed in turn with eager calls of a third between them: the context's scratch
     carries nothing from one to another."""

@@ -136,6 +136,9 @@ enum {
     SHV_OP_DN_TREE = 23,
     SHV_OP_DN_KEEP = 24,
     SHV_OP_TREE_ACCEPT = 25,
+    SHV_OP_PAGE_PLAN = 26,
+    SHV_OP_ATTN_PAGED = 27,
+    SHV_OP_LOGPROBS = 28,
     SHV_OP__COUNT
 };
 
@@ -726,6 +729,94 @@ typedef struct {
     int32_t max_cells, reserved;
 } shv_tree_accept_args;
 
+/* ---- a serving batch over a paged cache --------------------------------------------------------
+ * A cache whose cells are handed out page by page, for many requests of uneven length.  (The reference gives a sequence its cells whole, one context
+ * after another, llm/graph.go:1004-1062.)  The pool is laid out as shv_attn_decode's caches are, a page of `page` cells in the place of a slot: kpages
+ * [n_pages][page][n_head_kv][head_dim] and vpages [n_pages][page/32][n_head_kv][head_dim][32], binary16; page is a power of two from 32 to 4096, a pool has fewer
+ * than 2^31 cells.  table [n_seq][max_pages] names a sequence's pages: its cell at position p is cell p % page of page table[s][p / page].  A table, like all
+ * that is planned, serves every layer.
+ * The rows of a pass are packed: sequence s has the rows start[s] .. start[s+1]-1 of every array by row, none where the two are equal.  Rows from start[n_seq] on are no
+ * sequence's, and what would be theirs in an output stays as it was.  Nothing an op writes may overlap anything it reads unless it is said to.
+ * At most SHV_PAGE_MAX_SEQS sequences a call. */
+#define SHV_PAGE_MAX_SEQS 2048
+
+/* The pages of a pass.  Sequence s has kept pos[s] tokens, holds held[s] pages, the first held[s] entries of its table row, and wants room for rows[s] more tokens:
+ *   rows >= 0: ceil((pos + rows) / page) pages.  Entries past those are given back, as after a branch that was not kept;
+ *   rows <  0: the sequence ends and gives all of them back.
+ * Its first shared[s] entries are another's (a common prefix), which are used and never given back; NULL: none.  A sequence whose pos is below 0, or whose
+ * tokens would not fit max_pages pages, is left as it is and gets no rows.
+ * free_pages [n_pages] is a stack of n_free[0] pages.  First every page given back is laid on it, sequence by sequence, a table row's lower entry first; then
+ * what is wanted is taken from its top, sequence by sequence.  What sequences want is counted up in order: from the first one on whose pages do not suffice, those that
+ * want any get none, keep what they hold and have no rows in this pass, and those that want none go on.  So do rows, counted up in order over all sequences: those by whom max_rows is passed have none.
+ * start [n_seq+1] receives where each sequence's rows begin; row_seq (or NULL), row_pos and row_cell [max_rows] each row's sequence, position and cell of the pool (page * `page` +
+ * cell of the page).  held, n_free, free_pages and table are brought up to date (table entries past held, and free_pages behind n_free, hold anything).
+ * base (or NULL) [n_seq] receives pos, and pos moves on by the rows that s has in this pass (to 0 where it ends), so that a recorded step can be replayed without the host. */
+typedef struct {
+    const int32_t *rows;
+    int32_t *pos;
+    int32_t *table;
+    int32_t *held;
+    int32_t *free_pages;
+    int32_t *n_free;
+    const int32_t *shared;
+    int32_t *start;
+    int32_t *row_seq;
+    int32_t *row_pos;
+    int32_t *row_cell;
+    int32_t *base;
+    int32_t n_seq, page, max_pages, n_pages, max_rows, reserved;
+} shv_page_plan_args;
+
+/* Gated full attention of a pass's packed rows over a paged cache: a chunk of a prompt, a single token, or many sequences' of either kind.  qkv rows, norms and
+ * rotary table as shv_attn_decode has them (rope: max_pages * page rows), for head_dim 64, 128 or 256, up to 64 query heads per KV head, and rope_dims any
+ * multiple of head_dim / 32 up to head_dim.  Row r's key (normed and rotated at row_pos[r]) and value are rounded to binary16 into cell row_cell[r] of the pool (no cell of the pool: they
+ * are left out), and the row then sees its sequence's cells at positions up to its own, with window > 0 only those of them below `sinks` or within the last `window` positions,
+ * row_pos[r] - p < window.  A sequence's rows are at consecutive positions, row_pos[start[s]] and on.  Cells of a table entry that is no page (below 0, n_pages and more) are not seen by anyone:
+ * pages that a window has passed may be taken out.  A row that sees nothing has zeros.  A cell that a row does not see may hold anything.
+ * out [max_rows][n_head*head_dim], before the sigmoid gate.  A query's values, normed and rotated, lie within binary16's range (norm weights up to 2000 keep them there).
+ * A sequence whose start is out of order or past max_rows, or whose positions are not within 0 .. max_pages * page - 1, gets no output.
+ * work: work_bytes of scratch, 16-byte aligned, as many as shv_attn_paged_work says for these sizes; a call uses it alone, calls of one stream may share it.
+ * max_rows * (n_head / n_head_kv) is at most 2^20. */
+typedef struct {
+    const float *qkv;
+    const float *q_norm;
+    const float *k_norm;
+    const float *rope;       /* row p: cos[rope_dims/2] then sin[rope_dims/2]; may be NULL with rope_dims 0 */
+    void *kpages;
+    void *vpages;
+    const int32_t *table;
+    const int32_t *start;
+    const int32_t *row_pos;
+    const int32_t *row_cell;
+    void *work;
+    float *out;
+    int64_t work_bytes;
+    int32_t n_seq, max_rows;
+    int32_t n_head, n_head_kv, head_dim, rope_dims;
+    int32_t page, max_pages, n_pages, qkv_stride;
+    int32_t window, sinks;
+    float eps;
+    int32_t reserved;
+} shv_attn_paged_args;
+
+/* What a server answers with beside a token, for n_rows rows of n logits, logits_stride floats apart: with log Z = log sum_i e^(x_i)
+ *   logprob [n_rows]: x - log Z of the row's token ids[r]; not a number where that is no token (below 0, n and more).  ids and logprob: both or neither;
+ *   entropy [n_rows] (or NULL): -sum_i p_i log p_i, in nats;
+ *   top_ids, top_logprobs [n_rows][n_top]: the n_top (at most SHV_LOGPROBS_MAX_TOP and n; 0: none) largest logits' places in falling order, of equal ones the lower place first,
+ *   and their log probabilities.  A logit that is not a number is never among them (where too few others are left, the place is -1 and the log probability -infinity).
+ * A logit of -infinity is a token that cannot come: it adds nothing.  Where a logit is +infinity or not a number, or all are -infinity, log Z is not a number, and nor is what is formed from it.
+ * (The reference's sampler leaves these to the host, llm/sample.go:359-367 and on.)  n at most 2^30. */
+#define SHV_LOGPROBS_MAX_TOP 64
+typedef struct {
+    const float *logits;
+    const int32_t *ids;
+    float *logprob;
+    float *entropy;
+    int32_t *top_ids;
+    float *top_logprobs;
+    int32_t n_rows, n, logits_stride, n_top;
+} shv_logprobs_args;
+
 typedef struct {
     uint32_t kind;
     uint32_t flags;          /* bit 0: may overlap the previous op (MultiDispatch.Overlap) */
@@ -782,6 +873,11 @@ int shv_attn_keep(shv_ctx *ctx, const shv_attn_keep_args *a);
 int shv_dn_tree(shv_ctx *ctx, const shv_dn_tree_args *a);
 int shv_dn_keep(shv_ctx *ctx, const shv_dn_keep_args *a);
 int shv_tree_accept(shv_ctx *ctx, const shv_tree_accept_args *a);
+int shv_page_plan(shv_ctx *ctx, const shv_page_plan_args *a);
+int shv_attn_paged(shv_ctx *ctx, const shv_attn_paged_args *a);
+int shv_logprobs(shv_ctx *ctx, const shv_logprobs_args *a);
+/* Bytes of scratch that a call of these sizes needs on this device (a's pointers are not looked at). */
+int shv_attn_paged_work(shv_ctx *ctx, const shv_attn_paged_args *a, int64_t *bytes);
 
 /* shv_argmax for callers that cannot allocate (code under HIP graph capture, tight serving loops,
  * harnesses that forbid hipMalloc).  No counterpart in the reference.  Same arguments and

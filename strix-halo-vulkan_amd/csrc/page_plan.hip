@@ -1,0 +1,186 @@
+// The pages of a serving batch's pass: what each sequence gives back, takes and where its new rows lie, one launch.
+//
+// With want = ceil((pos + rows) / page): back = held - max(want, shared), need = want - held, each where above zero.  The pages given back lie behind the
+// free ones, L = free | back in order, A = |L|; sequence s's j-th new page is L[A - 1 - (taken before it) - j].  All of that is two scans over the
+// sequences, of (back, need, rows) and of what is granted, and lookups by bisection from there on.
+// Bound by the chain of trips to memory (a sequence's words, then pages, then the stores) and the scans' barriers, not by bytes.  Every block makes the scans for
+// itself, which costs less than a launch between them and the rows; the words that others still read (held, pos, n_free) are written by the
+// block that arrives last.
+#include "shv_device.hpp"
+#include "shv_internal.hpp"
+
+namespace {
+
+using namespace shv;
+
+constexpr int kMaxSeqs = SHV_PAGE_MAX_SEQS;
+constexpr uint32_t kFull = 1u << 30;  // sums stop here: no count of pages or rows that matters is as large
+constexpr int kMaxRows = 1 << 20;
+
+__device__ __forceinline__ uint32_t add_up_to(uint32_t a, uint32_t b) { return min(a + b, kFull); }
+
+// N exclusive sums over a block of T threads, and the totals.
+template <int T, int N>
+__device__ __forceinline__ void block_scan(uint32_t (&v)[N], uint32_t (&total)[N], uint32_t (*waves)[T / 64]) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    uint32_t upto[N];
+#pragma unroll
+    for (int k = 0; k < N; k++) {
+        upto[k] = v[k];
+#pragma unroll
+        for (int off = 1; off < 64; off <<= 1) {
+            const uint32_t less = __shfl_up(upto[k], off, 64);
+            if (lane >= off) upto[k] = add_up_to(upto[k], less);
+        }
+        if (lane == 63) waves[k][wave] = upto[k];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < N; k++) {
+        uint32_t before = 0, all = 0;
+#pragma unroll
+        for (int w = 0; w < T / 64; w++) {
+            if (w == wave) before = all;
+            all = add_up_to(all, waves[k][w]);
+        }
+        const uint32_t less = __shfl_up(upto[k], 1, 64);
+        v[k] = lane == 0 ? before : add_up_to(before, less);
+        total[k] = all;
+    }
+    __syncthreads();  // `waves` is free again
+}
+
+// The last of n ascending values that is not above x; the first is not.
+__device__ __forceinline__ int last_not_above(const uint32_t *v, int n, uint32_t x) {
+    int lo = 0;
+    for (int hi = n; hi - lo > 1;) {
+        const int mid = (lo + hi) >> 1;
+        if (v[mid] <= x) lo = mid;
+        else hi = mid;
+    }
+    return lo;
+}
+
+template <int T>
+__global__ __launch_bounds__(T) void page_plan_kernel(shv_page_plan_args a, int shift, int32_t *counter) {
+    constexpr int kPer = T == 1024 ? kMaxSeqs / T : 1;  // sequences a thread, side by side
+    __shared__ uint32_t s_start[kPer * T + 1], s_taken[kPer * T + 1], s_back[kPer * T + 1];
+    __shared__ int s_held[kPer * T], s_pos[kPer * T];
+    __shared__ uint32_t waves[3][T / 64];
+    __shared__ int is_last;
+    const int tid = threadIdx.x;
+    const int first = tid * kPer;
+    int rows[kPer], pos[kPer], held[kPer], shared[kPer];
+#pragma unroll
+    for (int u = 0; u < kPer; u++) {
+        const int s = min(first + u, a.n_seq - 1);
+        rows[u] = a.rows[s], pos[u] = a.pos[s], held[u] = a.held[s], shared[u] = a.shared ? a.shared[s] : 0;
+    }
+    const uint32_t n_free = min(max(a.n_free[0], 0), a.n_pages);
+    uint32_t back[kPer], need[kPer], asked[kPer];
+    bool fits[kPer];
+    uint32_t sums[3] = {0, 0, 0}, total[3];
+#pragma unroll
+    for (int u = 0; u < kPer; u++) {
+        const bool there = first + u < a.n_seq, ends = rows[u] < 0;
+        held[u] = min(max(held[u], 0), a.max_pages);
+        shared[u] = min(max(shared[u], 0), held[u]);
+        const long long upto = static_cast<long long>(pos[u]) + max(rows[u], 0);
+        const long long want = ends ? 0 : (upto + a.page - 1) >> shift;
+        fits[u] = there && (ends || (pos[u] >= 0 && want <= a.max_pages));
+        const int w = fits[u] ? static_cast<int>(want) : held[u];
+        back[u] = fits[u] ? max(held[u] - max(w, shared[u]), 0) : 0;
+        need[u] = fits[u] ? max(w - held[u], 0) : 0;
+        asked[u] = fits[u] ? min(static_cast<uint32_t>(max(rows[u], 0)), kFull) : 0;
+        sums[0] = add_up_to(sums[0], back[u]), sums[1] = add_up_to(sums[1], need[u]), sums[2] = add_up_to(sums[2], asked[u]);
+    }
+    block_scan<T, 3>(sums, total, waves);
+    const uint32_t n_back = total[0], avail = n_free + n_back;
+    uint32_t take[kPer], gets[kPer], both[2] = {0, 0}, total2[2];
+    {
+        uint32_t b = sums[0], n = sums[1], r = sums[2];
+#pragma unroll
+        for (int u = 0; u < kPer; u++) {
+            s_back[first + u] = b;
+            b = add_up_to(b, back[u]), n = add_up_to(n, need[u]), r = add_up_to(r, asked[u]);
+            const bool granted = fits[u] && (need[u] == 0 || n <= avail) && r <= static_cast<uint32_t>(a.max_rows);
+            take[u] = granted ? need[u] : 0;
+            gets[u] = granted ? asked[u] : 0;
+            both[0] += take[u], both[1] += gets[u];  // (at most avail and max_rows together)
+        }
+    }
+    block_scan<T, 2>(both, total2, waves);
+    const uint32_t n_taken = total2[0], n_rows = total2[1];
+    {
+        uint32_t t = both[0], r = both[1];
+#pragma unroll
+        for (int u = 0; u < kPer; u++) {
+            s_taken[first + u] = t, s_start[first + u] = r;
+            s_held[first + u] = held[u], s_pos[first + u] = pos[u];
+            t += take[u], r += gets[u];
+        }
+    }
+    if (tid == 0) s_back[kPer * T] = n_back, s_taken[kPer * T] = n_taken, s_start[kPer * T] = n_rows;
+    __syncthreads();
+    if (blockIdx.x == 0) {
+        for (int s = tid; s < a.n_seq; s += T) {
+            a.start[s] = s_start[s];
+            if (a.base) a.base[s] = s_pos[s];
+        }
+        if (tid == 0) a.start[a.n_seq] = n_rows;
+    }
+    const auto given_back = [&](uint32_t r) {
+        const int s = last_not_above(s_back, a.n_seq, r);
+        const int low = s_held[s] - static_cast<int>((s + 1 < a.n_seq ? s_back[s + 1] : n_back) - s_back[s]);
+        return a.table[static_cast<size_t>(s) * a.max_pages + low + (r - s_back[s])];
+    };
+    const auto taken = [&](uint32_t e) {  // the e-th page from the top
+        const uint32_t i = avail - 1 - e;
+        return i < n_free ? a.free_pages[i] : given_back(i - n_free);
+    };
+    const uint32_t step = gridDim.x * T, me = blockIdx.x * T + tid;
+    for (uint32_t t = me; t < n_rows; t += step) {
+        const int s = last_not_above(s_start, a.n_seq, t);
+        const int p = s_pos[s] + static_cast<int>(t - s_start[s]), at = p >> shift;
+        const int page = at < s_held[s] ? a.table[static_cast<size_t>(s) * a.max_pages + at] : taken(s_taken[s] + at - s_held[s]);
+        if (a.row_seq) a.row_seq[t] = s;
+        a.row_pos[t] = p;
+        a.row_cell[t] = page >= 0 && page < a.n_pages ? (page << shift) + (p & (a.page - 1)) : -1;
+    }
+    // (what is written here is read by no block: entries past a growing sequence's, and behind the free pages)
+    for (uint32_t e = me; e < n_taken; e += step) {
+        const int s = last_not_above(s_taken, a.n_seq, e);
+        a.table[static_cast<size_t>(s) * a.max_pages + s_held[s] + (e - s_taken[s])] = taken(e);
+    }
+    for (uint32_t r = me; r < n_back && n_free + r < static_cast<uint32_t>(a.n_pages); r += step) a.free_pages[n_free + r] = given_back(r);
+    if (gridDim.x > 1 && !arrive_last(counter, gridDim.x, &is_last)) return;
+#pragma unroll
+    for (int u = 0; u < kPer; u++) {
+        if (!fits[u]) continue;  // left as it is, as behind the last
+        a.held[first + u] = rows[u] < 0 ? 0 : held[u] - back[u] + take[u];
+        if (a.base) a.pos[first + u] = rows[u] < 0 ? 0 : pos[u] + static_cast<int>(gets[u]);
+    }
+    if (tid == 0) a.n_free[0] = avail - n_taken;
+}
+
+}  // namespace
+
+int shv_launch_page_plan(shv_ctx *ctx, const shv_page_plan_args *pa) {
+    const shv_page_plan_args &a = *pa;
+    SHV_REQUIRE(a.rows && a.pos && a.table && a.held && a.free_pages && a.n_free && a.start && a.row_pos && a.row_cell, "page_plan: NULL argument");
+    SHV_REQUIRE(a.n_seq >= 1 && a.n_seq <= kMaxSeqs, "page_plan: %d sequences; 1..%d", a.n_seq, kMaxSeqs);
+    SHV_REQUIRE(a.page >= 32 && a.page <= 4096 && (a.page & (a.page - 1)) == 0, "page_plan: page %d; a power of two from 32 to 4096", a.page);
+    SHV_REQUIRE(a.n_pages >= 1 && static_cast<long long>(a.n_pages) * a.page < 1ll << 31, "page_plan: %d pages of %d cells; fewer than 2^31 cells", a.n_pages, a.page);
+    SHV_REQUIRE(a.max_pages >= 1 && static_cast<long long>(a.max_pages) * a.page < 1ll << 31, "page_plan: max_pages %d of %d cells; fewer than 2^31 cells", a.max_pages, a.page);
+    SHV_REQUIRE(a.max_rows >= 1 && a.max_rows <= kMaxRows, "page_plan: max_rows %d; 1..%d", a.max_rows, kMaxRows);
+    SHV_REQUIRE(a.rows != a.pos && a.rows != a.held && a.pos != a.held && a.base != a.pos, "page_plan: rows, pos, held and base are arrays of their own");
+    int shift = 0;
+    while (1 << shift < a.page) shift++;
+    int32_t *counter = ctx->lp_counters + shv_ctx::kLpPieces * shv_ctx::kLpCounterStep;
+    const int threads = a.n_seq <= 256 && a.max_rows <= 4096 ? 256 : 1024;
+    const int blocks = (a.max_rows + 4 * threads - 1) / (4 * threads);
+    const dim3 grid(blocks < 64 ? blocks : 64);
+    if (threads == 256) SHV_LAUNCH(ctx, page_plan_kernel<256>, grid, dim3(256), 0, a, shift, counter);
+    else SHV_LAUNCH(ctx, page_plan_kernel<1024>, grid, dim3(1024), 0, a, shift, counter);
+    return SHV_OK;
+}

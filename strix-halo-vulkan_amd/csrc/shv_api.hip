@@ -88,6 +88,9 @@ int shv_init(int device, shv_ctx **out) {
     if (e == hipSuccess) e = hipMalloc(reinterpret_cast<void **>(&ctx->tree_counters), shv_ctx::kTreeCounters * sizeof(int32_t));
     if (e == hipSuccess) e = hipMalloc(reinterpret_cast<void **>(&ctx->tree_len), sizeof(int32_t));
     if (e == hipSuccess) e = hipMemset(ctx->tree_counters, 0, shv_ctx::kTreeCounters * sizeof(int32_t));
+    if (e == hipSuccess) e = hipMalloc(reinterpret_cast<void **>(&ctx->lp_part), static_cast<size_t>(shv_ctx::kLpPieces) * shv_ctx::kLpPieceFloats * sizeof(float));
+    if (e == hipSuccess) e = hipMalloc(reinterpret_cast<void **>(&ctx->lp_counters), shv_ctx::kLpCounters * sizeof(int32_t));
+    if (e == hipSuccess) e = hipMemset(ctx->lp_counters, 0, shv_ctx::kLpCounters * sizeof(int32_t));
     if (e == hipSuccess) e = hipMalloc(reinterpret_cast<void **>(&ctx->gemv_amax_val), shv_ctx::kGemvAmaxBlocks * sizeof(float));
     if (e == hipSuccess) e = hipMalloc(reinterpret_cast<void **>(&ctx->gemv_amax_idx), shv_ctx::kGemvAmaxBlocks * sizeof(int32_t));
     if (e != hipSuccess) {
@@ -124,6 +127,8 @@ void shv_destroy(shv_ctx *ctx) {
     if (ctx->tree_idx) (void)hipFree(ctx->tree_idx);
     if (ctx->tree_counters) (void)hipFree(ctx->tree_counters);
     if (ctx->tree_len) (void)hipFree(ctx->tree_len);
+    if (ctx->lp_part) (void)hipFree(ctx->lp_part);
+    if (ctx->lp_counters) (void)hipFree(ctx->lp_counters);
     if (ctx->gemv_amax_val) (void)hipFree(ctx->gemv_amax_val);
     if (ctx->gemv_amax_idx) (void)hipFree(ctx->gemv_amax_idx);
     if (ctx->up_ring) (void)hipHostFree(ctx->up_ring);
@@ -324,6 +329,9 @@ static int dispatch_one(shv_ctx *ctx, uint32_t kind, const void *args, size_t by
         case SHV_OP_DN_TREE: return run_as<shv_dn_tree_args>(ctx, args, bytes, shv_launch_dn_tree, "dn_tree");
         case SHV_OP_DN_KEEP: return run_as<shv_dn_keep_args>(ctx, args, bytes, shv_launch_dn_keep, "dn_keep");
         case SHV_OP_TREE_ACCEPT: return run_as<shv_tree_accept_args>(ctx, args, bytes, shv_launch_tree_accept, "tree_accept");
+        case SHV_OP_PAGE_PLAN: return run_as<shv_page_plan_args>(ctx, args, bytes, shv_launch_page_plan, "page_plan");
+        case SHV_OP_ATTN_PAGED: return run_as<shv_attn_paged_args>(ctx, args, bytes, shv_launch_attn_paged, "attn_paged");
+        case SHV_OP_LOGPROBS: return run_as<shv_logprobs_args>(ctx, args, bytes, shv_launch_logprobs, "logprobs");
         default: return shv_set_error(SHV_E_INVALID, "shv_enqueue: unknown op kind %u", kind);
     }
 }
@@ -506,6 +514,9 @@ int shv_attn_tree(shv_ctx *ctx, const shv_attn_tree_args *a) { return dispatch_o
 int shv_attn_keep(shv_ctx *ctx, const shv_attn_keep_args *a) { return dispatch_one(ctx, SHV_OP_ATTN_KEEP, a, sizeof(*a)); }
 int shv_dn_tree(shv_ctx *ctx, const shv_dn_tree_args *a) { return dispatch_one(ctx, SHV_OP_DN_TREE, a, sizeof(*a)); }
 int shv_dn_keep(shv_ctx *ctx, const shv_dn_keep_args *a) { return dispatch_one(ctx, SHV_OP_DN_KEEP, a, sizeof(*a)); }
+int shv_page_plan(shv_ctx *ctx, const shv_page_plan_args *a) { return dispatch_one(ctx, SHV_OP_PAGE_PLAN, a, sizeof(*a)); }
+int shv_attn_paged(shv_ctx *ctx, const shv_attn_paged_args *a) { return dispatch_one(ctx, SHV_OP_ATTN_PAGED, a, sizeof(*a)); }
+int shv_logprobs(shv_ctx *ctx, const shv_logprobs_args *a) { return dispatch_one(ctx, SHV_OP_LOGPROBS, a, sizeof(*a)); }
 int shv_tree_accept(shv_ctx *ctx, const shv_tree_accept_args *a) { return dispatch_one(ctx, SHV_OP_TREE_ACCEPT, a, sizeof(*a)); }
 
 int shv_argmax_static(shv_ctx *ctx, const shv_argmax_args *a) {

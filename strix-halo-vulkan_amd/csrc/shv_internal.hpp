@@ -85,6 +85,11 @@ struct shv_ctx {
     int32_t *tree_counters = nullptr;
     int32_t *tree_len = nullptr;  // tiles of an attn_tree's slices, for its join
     enum { kTreePairs = SHV_TREE_ACCEPT_MAX_ROWS, kTreeSeqs = 1024, kTreeCounterStep = 32, kTreeCounters = (kTreeSeqs + SHV_TREE_ACCEPT_MAX_ROWS) * kTreeCounterStep };
+    // what the pieces of a row of logits leave for the block that joins them, and the rows' arrival counters, a line apart (logprobs);
+    // behind them the plan's own counter (page_plan)
+    float *lp_part = nullptr;
+    int32_t *lp_counters = nullptr;
+    enum { kLpPieces = 2048, kLpPieceFloats = 4 + 2 * SHV_LOGPROBS_MAX_TOP, kLpCounterStep = 32, kLpCounters = (kLpPieces + 1) * kLpCounterStep };
     // device address of this GPU's copy of the library's static scratch array (misc.hip), for the
     // entry point that allocates nothing
     void *static_scratch = nullptr;
@@ -225,6 +230,10 @@ int shv_launch_attn_keep(shv_ctx *ctx, const shv_attn_keep_args *a);
 int shv_launch_dn_tree(shv_ctx *ctx, const shv_dn_tree_args *a);
 int shv_launch_dn_keep(shv_ctx *ctx, const shv_dn_keep_args *a);
 int shv_launch_tree_accept(shv_ctx *ctx, const shv_tree_accept_args *a);
+// a serving batch over a paged cache (page_plan.hip, attn_paged.hip, logprobs.hip)
+int shv_launch_page_plan(shv_ctx *ctx, const shv_page_plan_args *a);
+int shv_launch_attn_paged(shv_ctx *ctx, const shv_attn_paged_args *a);
+int shv_launch_logprobs(shv_ctx *ctx, const shv_logprobs_args *a);
 bool shv_dn_chunk_covers(const shv_dn_step_args &a);
 int shv_launch_dn_chunk(shv_ctx *ctx, const shv_dn_step_args &a, float *hist, int hist_slots);
 int shv_launch_copy_spans(shv_ctx *ctx, const shv_span *spans, int n);

@@ -13,6 +13,8 @@ OP_MOE_ROUTER, OP_MOE_UP, OP_MOE_DOWN, OP_DN_STEP, OP_ATTN_DECODE = 5, 6, 7, 8, 
 OP_EMBED, OP_ARGMAX, OP_ADVANCE, OP_DEQUANT, OP_GEMV, OP_RING_ROWS, OP_ROUTER_FOLD, OP_QSA_INDEX = 10, 11, 12, 13, 14, 15, 16, 17
 OP_ARGMAX_STATIC, OP_ATTN_CELLS, OP_DN_PASS = 18, 19, 20
 OP_ATTN_TREE, OP_ATTN_KEEP, OP_DN_TREE, OP_DN_KEEP, OP_TREE_ACCEPT = 21, 22, 23, 24, 25
+OP_PAGE_PLAN, OP_ATTN_PAGED, OP_LOGPROBS = 26, 27, 28
+PAGE_MAX_SEQS, LOGPROBS_MAX_TOP = 2048, 64
 TREE_MAX_ROWS, TREE_ACCEPT_MAX_ROWS = 64, 16384
 PRO_NONE, PRO_RMSNORM, PRO_GATED_NORM, PRO_MUL_SIGMOID, PRO_RMSNORM_PAIR = 0, 1, 2, 3, 4
 
@@ -179,6 +181,27 @@ class EmbedArgs(C.Structure):
                 ("x_stride", C.c_int32), ("type", C.c_int32)]
 
 
+class PagePlanArgs(C.Structure):
+    _fields_ = [("rows", C.c_void_p), ("pos", C.c_void_p), ("table", C.c_void_p), ("held", C.c_void_p), ("free_pages", C.c_void_p),
+                ("n_free", C.c_void_p), ("shared", C.c_void_p), ("start", C.c_void_p), ("row_seq", C.c_void_p), ("row_pos", C.c_void_p),
+                ("row_cell", C.c_void_p), ("base", C.c_void_p), ("n_seq", C.c_int32), ("page", C.c_int32), ("max_pages", C.c_int32),
+                ("n_pages", C.c_int32), ("max_rows", C.c_int32), ("reserved", C.c_int32)]
+
+
+class AttnPagedArgs(C.Structure):
+    _fields_ = [("qkv", C.c_void_p), ("q_norm", C.c_void_p), ("k_norm", C.c_void_p), ("rope", C.c_void_p), ("kpages", C.c_void_p),
+                ("vpages", C.c_void_p), ("table", C.c_void_p), ("start", C.c_void_p), ("row_pos", C.c_void_p), ("row_cell", C.c_void_p),
+                ("work", C.c_void_p), ("out", C.c_void_p), ("work_bytes", C.c_int64), ("n_seq", C.c_int32), ("max_rows", C.c_int32),
+                ("n_head", C.c_int32), ("n_head_kv", C.c_int32), ("head_dim", C.c_int32), ("rope_dims", C.c_int32), ("page", C.c_int32),
+                ("max_pages", C.c_int32), ("n_pages", C.c_int32), ("qkv_stride", C.c_int32), ("window", C.c_int32), ("sinks", C.c_int32),
+                ("eps", C.c_float), ("reserved", C.c_int32)]
+
+
+class LogprobsArgs(C.Structure):
+    _fields_ = [("logits", C.c_void_p), ("ids", C.c_void_p), ("logprob", C.c_void_p), ("entropy", C.c_void_p), ("top_ids", C.c_void_p),
+                ("top_logprobs", C.c_void_p), ("n_rows", C.c_int32), ("n", C.c_int32), ("logits_stride", C.c_int32), ("n_top", C.c_int32)]
+
+
 class ArgmaxArgs(C.Structure):
     _fields_ = [("logits", C.c_void_p), ("best", C.c_void_p), ("ids", C.c_void_p),
                 ("pos", C.c_void_p), ("n_rows", C.c_int32), ("n", C.c_int32),
@@ -226,6 +249,7 @@ SYMBOLS = [
     "shv_fill_normal", "shv_moe_router", "shv_moe_up", "shv_moe_down", "shv_dn_step", "shv_dn_pass", "shv_attn_decode", "shv_embed", "shv_argmax", "shv_advance",
     "shv_argmax_static", "shv_ring_rows", "shv_router_fold", "shv_qsa_index",
     "shv_attn_tree", "shv_attn_keep", "shv_dn_tree", "shv_dn_keep", "shv_tree_accept",
+    "shv_page_plan", "shv_attn_paged", "shv_logprobs", "shv_attn_paged_work",
 ]
 
 _lib = None
@@ -298,6 +322,10 @@ def load():
     L.shv_dn_tree.argtypes = [vp, C.POINTER(DnTreeArgs)]
     L.shv_dn_keep.argtypes = [vp, C.POINTER(DnKeepArgs)]
     L.shv_tree_accept.argtypes = [vp, C.POINTER(TreeAcceptArgs)]
+    L.shv_page_plan.argtypes = [vp, C.POINTER(PagePlanArgs)]
+    L.shv_attn_paged.argtypes = [vp, C.POINTER(AttnPagedArgs)]
+    L.shv_logprobs.argtypes = [vp, C.POINTER(LogprobsArgs)]
+    L.shv_attn_paged_work.argtypes = [vp, C.POINTER(AttnPagedArgs), C.POINTER(C.c_int64)]
     _lib = L
     return L
 
@@ -433,6 +461,12 @@ class Context:
             self.h = None
 
     # ---- convenience wrappers over single ops ----
+    def attn_paged_work(self, args):
+        """Bytes of scratch that shv_attn_paged needs for the sizes in `args`."""
+        n = C.c_int64()
+        check(self.L.shv_attn_paged_work(self.h, C.byref(args), C.byref(n)))
+        return n.value
+
     def dequant(self, typ, src, dst, n):
         """n elements of ggml tensor type `typ` at src to float32 at dst."""
         a = DequantArgs(_ptr(src), _ptr(dst), n, typ)

@@ -6,6 +6,7 @@
 // Bound by the chain of trips to memory (a sequence's words, then pages, then the stores) and the scans' barriers, not by bytes.  Every block makes the scans for
 // itself, which costs less than a launch between them and the rows; the words that others still read (held, pos, n_free) are written by the
 // block that arrives last.
+#include "scan.hpp"
 #include "shv_device.hpp"
 #include "shv_internal.hpp"
 
@@ -14,52 +15,7 @@ namespace {
 using namespace shv;
 
 constexpr int kMaxSeqs = SHV_PAGE_MAX_SEQS;
-constexpr uint32_t kFull = 1u << 30;  // sums stop here: no count of pages or rows that matters is as large
 constexpr int kMaxRows = 1 << 20;
-
-__device__ __forceinline__ uint32_t add_up_to(uint32_t a, uint32_t b) { return min(a + b, kFull); }
-
-// N exclusive sums over a block of T threads, and the totals.
-template <int T, int N>
-__device__ __forceinline__ void block_scan(uint32_t (&v)[N], uint32_t (&total)[N], uint32_t (*waves)[T / 64]) {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    uint32_t upto[N];
-#pragma unroll
-    for (int k = 0; k < N; k++) {
-        upto[k] = v[k];
-#pragma unroll
-        for (int off = 1; off < 64; off <<= 1) {
-            const uint32_t less = __shfl_up(upto[k], off, 64);
-            if (lane >= off) upto[k] = add_up_to(upto[k], less);
-        }
-        if (lane == 63) waves[k][wave] = upto[k];
-    }
-    __syncthreads();
-#pragma unroll
-    for (int k = 0; k < N; k++) {
-        uint32_t before = 0, all = 0;
-#pragma unroll
-        for (int w = 0; w < T / 64; w++) {
-            if (w == wave) before = all;
-            all = add_up_to(all, waves[k][w]);
-        }
-        const uint32_t less = __shfl_up(upto[k], 1, 64);
-        v[k] = lane == 0 ? before : add_up_to(before, less);
-        total[k] = all;
-    }
-    __syncthreads();  // `waves` is free again
-}
-
-// The last of n ascending values that is not above x; the first is not.
-__device__ __forceinline__ int last_not_above(const uint32_t *v, int n, uint32_t x) {
-    int lo = 0;
-    for (int hi = n; hi - lo > 1;) {
-        const int mid = (lo + hi) >> 1;
-        if (v[mid] <= x) lo = mid;
-        else hi = mid;
-    }
-    return lo;
-}
 
 template <int T>
 __global__ __launch_bounds__(T) void page_plan_kernel(shv_page_plan_args a, int shift, int32_t *counter) {

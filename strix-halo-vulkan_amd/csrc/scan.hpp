@@ -9,6 +9,20 @@ constexpr uint32_t kFull = 1u << 30;  // sums stop here: no count of pages or ro
 
 __device__ __forceinline__ uint32_t add_up_to(uint32_t a, uint32_t b) { return min(a + b, kFull); }
 
+// Sum over a wave's lanes up to this one: four shifts within rows of 16 lanes, two carries between rows.  (By way of LDS six exchanges are a third of a microsecond.)
+template <int CTRL, int ROW_MASK = 0xF>
+__device__ __forceinline__ uint32_t shifted(uint32_t v) {
+    return static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(v), CTRL, ROW_MASK, 0xF, false));
+}
+__device__ __forceinline__ uint32_t wave_upto(uint32_t v) {
+    v = add_up_to(v, shifted<0x111>(v));
+    v = add_up_to(v, shifted<0x112>(v));
+    v = add_up_to(v, shifted<0x114>(v));
+    v = add_up_to(v, shifted<0x118>(v));
+    v = add_up_to(v, shifted<kDppBcast15, 0xA>(v));
+    return add_up_to(v, shifted<kDppBcast31, 0xC>(v));
+}
+
 // N exclusive sums over a block of T threads, and the totals.
 template <int T, int N>
 __device__ __forceinline__ void block_scan(uint32_t (&v)[N], uint32_t (&total)[N], uint32_t (*waves)[T / 64]) {
@@ -16,12 +30,7 @@ __device__ __forceinline__ void block_scan(uint32_t (&v)[N], uint32_t (&total)[N
     uint32_t upto[N];
 #pragma unroll
     for (int k = 0; k < N; k++) {
-        upto[k] = v[k];
-#pragma unroll
-        for (int off = 1; off < 64; off <<= 1) {
-            const uint32_t less = __shfl_up(upto[k], off, 64);
-            if (lane >= off) upto[k] = add_up_to(upto[k], less);
-        }
+        upto[k] = wave_upto(v[k]);
         if (lane == 63) waves[k][wave] = upto[k];
     }
     __syncthreads();
@@ -33,8 +42,7 @@ __device__ __forceinline__ void block_scan(uint32_t (&v)[N], uint32_t (&total)[N
             if (w == wave) before = all;
             all = add_up_to(all, waves[k][w]);
         }
-        const uint32_t less = __shfl_up(upto[k], 1, 64);
-        v[k] = lane == 0 ? before : add_up_to(before, less);
+        v[k] = add_up_to(before, shifted<0x138>(upto[k]));  // (the lane before's; of the first none)
         total[k] = all;
     }
     __syncthreads();  // `waves` is free again

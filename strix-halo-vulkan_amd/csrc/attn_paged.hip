@@ -3,13 +3,13 @@
 // Row r of a sequence, at position p_r, sees the sequence's cells c <= p_r that lie in a page (with a window those of them below `sinks` or above p_r - window):
 //     out_r = sum over them of softmax(q_r . k_c / sqrt(d)) v_c
 // q and k normed over a head and rotated at their positions.  Three launches:
-//   rows   the rows' keys and values into their cells, their queries into matrix-core operands, and, in a block of its own, the plan of the next;
-//   attn   a block takes one KV head and 128 query rows (query row r of a sequence is head r % rep of its row r / rep), 16 a wave, and a run of
+//   cells  the rows' keys and values into their cells, and, in a block of its own, the plan of the next;
+//   attn   a block takes one KV head and up to 128 query rows (256 of narrower heads; query row r of a sequence is head r % rep of its row r / rep), and a run of
 //          their tiles of 32 cells, on v_mfma_f32_16x16x32_f16:
 //              S^T = K Q^T   the cache's binary16 keys against the queries as two halves; a lane then holds eight cells of one query row, the operand
 //                            of the second product
 //              O  += P V     weights as two halves against values, which the cache holds by dim
-//          with a running maximum and sum.  Tiles go from memory to LDS past the registers, three ahead;
+//          with a running maximum and sum.  Tiles go from memory to LDS past the registers, 96 KB ahead;
 //   join   the records of query rows whose tiles several blocks have shared.
 #include <atomic>
 
@@ -23,17 +23,24 @@ namespace {
 using namespace shv;
 
 constexpr int kTile = 32;  // cells of a tile of V
-constexpr int kWaves = 8, kRows = 16 * kWaves;  // waves of a block and its query rows
+constexpr int kWaves = 8;
 constexpr int kMaxSeqs = SHV_PAGE_MAX_SEQS;
 constexpr int kChunk = 64 * 16;
-constexpr int kStages = 4, kAhead = kStages - 1;
+constexpr int kRingBytes = 128 << 10;
 // Weights are e^(s - m) 2^kLift, and m stands until a score is more than kSlack powers of two above it: up to 2^15.9, which the larger half holds, and down to
 // 2^-35 of the largest with the smaller half's last place, to which it is rounded.
 constexpr float kLift = 11.f, kSlack = 4.9f;
-constexpr int kLeast = 3;      // tiles a block gets at least
-constexpr int kFewBlocks = 1024;  // query blocks up to which the plan is made inside the launch of the rows
+constexpr int kLeast = 2;      // tiles a block gets at least
+constexpr int kShareFrom = 8;  // records of a query row from which waves share them
+constexpr int kFewBlocks = 1024;  // query blocks up to which the plan is made inside the launch of the cells
 
-// 128 query rows of a sequence and a run of the tiles they look at.
+// Groups of 16 query rows of a wave, and query rows of a block.  Of 256 dims a wave's registers hold one group; of fewer they hold two, which an operand read from LDS serves
+// both.
+template <int D>
+constexpr int kGroups = D == 256 ? 1 : 2;
+constexpr int rows_of(int D) { return 16 * kWaves * (D == 256 ? 1 : 2); }
+
+// A block's query rows of a sequence and a run of the tiles they look at.
 struct Piece {
     int seq, first;     // the sequence and its first packed row
     int r0, r_end;      // the first query row, and the sequence's number of them
@@ -41,24 +48,31 @@ struct Piece {
     int t0, t1;         // the run
     int rec;            // where its records go; -1: it is all there is
 };
-struct Join {
-    int first, r0, r_end, rec, n;
-    int pad[3];
+// What a block has: its first piece, and how many more lie from pieces[at] on; more -1: nothing.
+struct Block {
+    Piece piece;
+    int more, at;
+    int pad[6];
 };
-enum { kHeadBlocks = 0, kHeadCut = 1, kHeadJoins = 2, kHeadRecs = 3, kHeadWords = 16 };
+// Up to 16 query rows whose tiles several blocks share: rows r0 .. of a sequence, which are row `in` .. of their records.
+struct Join {
+    int first, r0, r_end, rec, n, in;
+    int pad[2];
+};
 
 // Where a call's scratch lies and what it can hold; worked out by the launcher from the sizes alone.
 struct Plan {
-    int32_t *head;
-    int32_t *first_of;  // a block's first piece; of the last block's end too
-    Piece *pieces;
+    int32_t *n_joins;
+    Block *blocks;
+    Piece *pieces;      // a query block's first piece, where a block has more than one
     Join *joins;
-    char *stage;        // queries: [KV head][packed row * rep + head of the group][large halves, small halves]
     float *sums;        // records: [record][KV head][slot_rows][D] unnormalised sums
     float2 *of;         // and their (maximum, sum)
     int slots;          // blocks a KV head that the chip holds at once
-    int slot_rows;      // query rows of a record
+    int rows;           // query rows of a block
+    int slot_rows;      // and of a record
     int most_blocks, most_q;
+    int dies, heads;    // dies that share a KV head, and KV heads of a die (place)
     int shift;          // log2 of the page
 };
 
@@ -90,42 +104,62 @@ struct Seq {
 };
 
 // ---- the plan: one block of T threads -----------------------------------------------------------
-// The query blocks of all sequences stand in a row with the tiles each looks at, P their running sum.  With as many query blocks as fill the chip evenly
-// each is a block's own, those with the most tiles first.  Otherwise block b takes the tiles b S .. (b + 1) S of the row, S = all / blocks, so that all blocks have
-// the same; a query block cut by that leaves a record of each piece.
+// What a block's work costs, in tenths of a microsecond: a tile of few query rows the time in which memory delivers it, of many that of the products; a piece
+// its way in and out, and its rows' bytes.
+struct Costs {
+    int few, group, piece, piece_group;
+    __host__ __device__ __forceinline__ int tile(int groups) const { return few > group * groups / 16 ? few : group * groups / 16; }
+    __host__ __device__ __forceinline__ int way(int groups) const { return piece + piece_group * groups / 16; }
+};
+__host__ __device__ constexpr Costs costs_of(int D) { return D == 256 ? Costs{16, 39, 30, 128} : D == 128 ? Costs{9, 20, 30, 64} : Costs{5, 12, 30, 32}; }
+
+// The query blocks of all sequences stand in a row, each with its cost, P their running sum.  Where they fill the chip evenly each is a block's own, those with the most
+// tiles first.  Otherwise block b takes what lies from b S to (b + 1) S in the row, S = all / blocks, so that all blocks have the same; a query block cut by that
+// leaves a record of each piece.
 template <int T, int SEQS, int NQ>
 struct PlanSmem {
-    uint32_t q0[SEQS + 1];      // query blocks before a sequence's
-    uint32_t p[NQ], at[NQ];     // tiles before a query block's; its first piece
+    uint32_t q0[SEQS];          // query blocks before a sequence's
+    int first[SEQS], n[SEQS], pos[SEQS];
+    uint32_t p[NQ], at[NQ];     // the cost before a query block; its first piece
     int rec[NQ];                // its first record, -1: it has one piece
-    uint32_t waves[4][T / 64];
+    uint32_t waves[3][T / 64];
     uint32_t bucket[64];
-    uint32_t most;
+    uint32_t most, most_way;
 };
 template <int T, int SEQS, int NQ>
 __device__ void make_plan(const shv_attn_paged_args &a, const Plan &plan, PlanSmem<T, SEQS, NQ> &sm) {
     const int tid = threadIdx.x, rep = a.n_head / a.n_head_kv;
+    const Costs costs = costs_of(a.head_dim);
     uint32_t nq = 0;
     for (int s0 = 0; s0 < a.n_seq; s0 += T) {
+        const int s = s0 + tid;
         uint32_t v[1] = {0}, all[1];
-        if (s0 + tid < a.n_seq) v[0] = (static_cast<uint32_t>(Seq(a, s0 + tid).n) * rep + kRows - 1) / kRows;
+        if (s < a.n_seq) {
+            const Seq seq(a, s);
+            sm.first[s] = seq.first, sm.n[s] = seq.n, sm.pos[s] = seq.pos;
+            v[0] = (static_cast<uint32_t>(seq.n) * rep + plan.rows - 1) / plan.rows;
+        }
         block_scan<T, 1>(v, all, sm.waves);
-        if (s0 + tid < a.n_seq) sm.q0[s0 + tid] = nq + v[0];
+        if (s < a.n_seq) sm.q0[s] = nq + v[0];
         nq += all[0];
     }
-    if (tid == 0) sm.most = 0;
+    if (tid == 0) sm.most = sm.most_way = 0;
     if (tid < 64) sm.bucket[tid] = 0;
     __syncthreads();
-    // query block i as a piece of all its tiles
+    // query block i as a piece of all its tiles; what a tile of it costs, and its way in and out (which the first one's block has in any case)
+    struct Whole : Piece {
+        uint32_t tile, way, groups;
+    };
     const auto whole = [&](uint32_t i) {
-        Piece p;
+        Whole p;
         p.seq = last_not_above(sm.q0, a.n_seq, i);
-        const Seq seq(a, p.seq);
-        p.first = seq.first, p.pos = seq.pos, p.r_end = seq.n * rep;
-        p.r0 = static_cast<int>(i - sm.q0[p.seq]) * kRows;
-        const int last = min(p.r0 + kRows, p.r_end) - 1;
-        p.t0 = 0, p.t1 = Tiles(a.window, a.sinks, p.pos + p.r0 / rep, p.pos + last / rep).all;
+        p.first = sm.first[p.seq], p.pos = sm.pos[p.seq], p.r_end = sm.n[p.seq] * rep;
+        p.r0 = static_cast<int>(i - sm.q0[p.seq]) * plan.rows;
+        const uint32_t last = min(p.r0 + plan.rows, p.r_end) - 1;
+        p.t0 = 0, p.t1 = Tiles(a.window, a.sinks, p.pos + static_cast<uint32_t>(p.r0) / static_cast<uint32_t>(rep), p.pos + last / static_cast<uint32_t>(rep)).all;
         p.rec = -1;
+        p.groups = (last - p.r0) / 16 + 1;
+        p.tile = costs.tile(p.groups), p.way = i == 0 ? 0 : costs.way(p.groups);
         return p;
     };
     nq = min(nq, static_cast<uint32_t>(min(plan.most_q, NQ)));
@@ -133,8 +167,10 @@ __device__ void make_plan(const shv_attn_paged_args &a, const Plan &plan, PlanSm
     for (uint32_t i0 = 0; i0 < nq; i0 += T) {
         uint32_t v[1] = {0}, all[1];
         if (i0 + tid < nq) {
-            v[0] = whole(i0 + tid).t1;
+            const Whole p = whole(i0 + tid);
+            v[0] = p.way + min(static_cast<uint64_t>(p.t1) * p.tile, static_cast<uint64_t>(kFull / 2));
             atomicMax(&sm.most, v[0]);
+            atomicMax(&sm.most_way, static_cast<uint32_t>(costs.way(p.groups)));
         }
         block_scan<T, 1>(v, all, sm.waves);
         if (i0 + tid < nq) sm.p[i0 + tid] = add_up_to(total, v[0]);
@@ -142,18 +178,18 @@ __device__ void make_plan(const shv_attn_paged_args &a, const Plan &plan, PlanSm
     }
     __syncthreads();
     const uint32_t most = sm.most, slots = plan.slots;
-    const uint32_t share = max((total + slots - 1) / slots, static_cast<uint32_t>(kLeast));
-    const bool cut = total < kFull && !((nq >= 2 * slots && most <= share) || (nq <= slots && most * 10 <= share * 11));
+    const uint32_t share = max((total + slots - 1) / slots, static_cast<uint32_t>(kLeast * costs.few));
+    // whole query blocks take as long as the longest, or as so many of the mean size one behind the other; a cut costs another way in and out, and the records' join
+    const uint32_t rounds = (nq + slots - 1) / slots;
+    const bool cut = total < kFull && max(most, nq > 0 ? total / nq * rounds : 0u) > share + sm.most_way + sm.most_way / 2;
     if (!cut) {
         for (int pass = 0; pass < 2; pass++) {
             for (uint32_t i = tid; i < nq; i += T) {
-                const Piece p = whole(i);
-                const uint32_t k = 63 - min(63u, static_cast<uint32_t>(static_cast<uint64_t>(p.t1) * 64 / (most + 1)));
+                const Whole p = whole(i);
+                const uint32_t cost = min(static_cast<uint64_t>(p.t1) * p.tile, static_cast<uint64_t>(kFull / 2));
+                const uint32_t k = 63 - min(63u, static_cast<uint32_t>(static_cast<uint64_t>(cost) * 64 / (most + 1)));
                 const uint32_t at = atomicAdd(&sm.bucket[k], 1u);
-                if (pass == 1) {
-                    plan.pieces[at] = p;
-                    plan.first_of[i] = i;
-                }
+                if (pass == 1) plan.blocks[at] = Block{p, 0, 0, {}};
             }
             __syncthreads();
             if (pass == 0) {
@@ -168,22 +204,29 @@ __device__ void make_plan(const shv_attn_paged_args &a, const Plan &plan, PlanSm
                 __syncthreads();
             }
         }
-        if (tid == 0) {
-            plan.first_of[nq] = nq;
-            plan.head[kHeadBlocks] = nq, plan.head[kHeadCut] = 0, plan.head[kHeadJoins] = 0, plan.head[kHeadRecs] = 0;
-        }
+        for (uint32_t b = nq + tid; b < static_cast<uint32_t>(plan.most_blocks); b += T) plan.blocks[b].more = -1;
+        if (tid == 0) *plan.n_joins = 0;
         return;
     }
+    // Cut c of the row, at c S, falls into query block i between two of its tiles or, on its way in or behind its last tile but one, on a border of query blocks.
+    // Piece k of query block i begins at its cut number first_cut + k.
+    const auto first_cut = [&](uint32_t i, const Whole &p) { return (sm.p[i] + p.way) / share; };
+    const auto piece_of = [&](uint32_t i, Whole p, uint32_t k) {
+        const uint32_t c = first_cut(i, p) + k, from = sm.p[i] + p.way, all = p.t1;
+        p.t0 = k == 0 ? 0 : (c * share - from + p.tile - 1) / p.tile;
+        p.t1 = min(all, ((c + 1) * share - from + p.tile - 1) / p.tile);
+        return p;
+    };
     const uint32_t blocks = (total + share - 1) / share;
     uint32_t before[3] = {0, 0, 0};  // pieces, records, joins
     for (uint32_t i0 = 0; i0 < nq; i0 += T) {
         const uint32_t i = i0 + tid;
         uint32_t v[3] = {0, 0, 0}, all[3], n = 0;
-        Piece p;
+        Whole p;
         if (i < nq) {
             p = whole(i);
-            n = (sm.p[i] + p.t1 + share - 1) / share - sm.p[i] / share;
-            v[0] = n, v[1] = n > 1 ? n : 0, v[2] = n > 1;
+            n = (sm.p[i] + p.way + (p.t1 - 1) * p.tile) / share - first_cut(i, p) + 1;
+            v[0] = n, v[1] = n > 1 ? n : 0, v[2] = n > 1 ? p.groups : 0;
         }
         block_scan<T, 3>(v, all, sm.waves);
         if (i < nq) {
@@ -191,8 +234,9 @@ __device__ void make_plan(const shv_attn_paged_args &a, const Plan &plan, PlanSm
             sm.at[i] = at;
             sm.rec[i] = n > 1 ? static_cast<int>(rec) : -1;
             if (n > 1) {
-                plan.joins[before[2] + v[2]] = Join{p.first, p.r0, p.r_end, static_cast<int>(rec), static_cast<int>(n), {}};
-                p.t1 = (sm.p[i] / share + 1) * share - sm.p[i];
+                for (uint32_t g = 0; g < p.groups; g++)
+                    plan.joins[before[2] + v[2] + g] = Join{p.first, p.r0 + 16 * static_cast<int>(g), p.r_end, static_cast<int>(rec), static_cast<int>(n), 16 * static_cast<int>(g), {}};
+                p = piece_of(i, p, 0);
                 p.rec = rec;
             }
             plan.pieces[at] = p;
@@ -200,18 +244,42 @@ __device__ void make_plan(const shv_attn_paged_args &a, const Plan &plan, PlanSm
         before[0] += all[0], before[1] += all[1], before[2] += all[2];
     }
     __syncthreads();
-    for (uint32_t b = tid; b < blocks; b += T) {
-        const uint32_t i = last_not_above(sm.p, nq, b * share), k = b - sm.p[i] / share, off = b * share - sm.p[i];
-        plan.first_of[b] = sm.at[i] + (off == 0 ? 0 : k);
-        if (off == 0) continue;
-        Piece p = whole(i);
-        p.t0 = off, p.t1 = min(static_cast<int>(off + share), p.t1), p.rec = sm.rec[i] + k;
-        plan.pieces[sm.at[i] + k] = p;
+    // the query block and which of its pieces that begin at or behind cut c
+    const auto piece_at = [&](uint32_t c, uint32_t &i, uint32_t &k) {
+        i = last_not_above(sm.p, nq, c * share);
+        const Whole p = whole(i);
+        const uint32_t x = c * share - sm.p[i];
+        k = 0;
+        if (x <= p.way) return p;
+        if (x > p.way + (p.t1 - 1) * p.tile) i++;
+        else k = c - first_cut(i, p);
+        return p;
+    };
+    const uint32_t dies = plan.dies, per = (blocks + dies - 1) / dies;
+    for (uint32_t slot = tid; slot < static_cast<uint32_t>(plan.most_blocks); slot += T) {
+        // neighbouring blocks lie on one die
+        const uint32_t row = slot / dies, b = (slot - row * dies) * per + row;
+        uint32_t i = 0, k = 0, at = 0, end = 0;
+        Whole p;
+        if (row < per && b < blocks) {
+            p = piece_at(b, i, k);
+            at = end = i < nq ? sm.at[i] + k : before[0];
+            if (i < nq) {
+                if (k == 0) p = whole(i);
+                uint32_t i2, k2;
+                piece_at(b + 1, i2, k2);
+                end = b + 1 < blocks && i2 < nq ? sm.at[i2] + k2 : before[0];
+            }
+        }
+        if (at == end) {
+            plan.blocks[slot].more = -1;
+            continue;
+        }
+        p = piece_of(i, p, k);
+        p.rec = sm.rec[i] < 0 ? -1 : sm.rec[i] + static_cast<int>(k);
+        plan.blocks[slot] = Block{p, static_cast<int>(end - at - 1), static_cast<int>(at + 1), {}};
     }
-    if (tid == 0) {
-        plan.first_of[blocks] = before[0];
-        plan.head[kHeadBlocks] = blocks, plan.head[kHeadCut] = 1, plan.head[kHeadJoins] = before[2], plan.head[kHeadRecs] = before[1];
-    }
+    if (tid == 0) *plan.n_joins = before[2];
 }
 
 __global__ __launch_bounds__(1024) void paged_plan_kernel(shv_attn_paged_args a, Plan plan) {
@@ -219,10 +287,10 @@ __global__ __launch_bounds__(1024) void paged_plan_kernel(shv_attn_paged_args a,
     make_plan(a, plan, *reinterpret_cast<PlanSmem<1024, kMaxSeqs, 8192 + kMaxSeqs> *>(raw));
 }
 
-// ---- the rows -----------------------------------------------------------------------------------
-// A wave a query row or a row's cell of a KV head; with PLAN the first block makes the plan.
+// ---- the rows' cells ----------------------------------------------------------------------------
+// A wave a row's cell of a KV head; with PLAN the first block makes the plan.
 template <int D, bool PLAN>
-__global__ __launch_bounds__(256) void paged_rows_kernel(shv_attn_paged_args a, Plan plan) {
+__global__ __launch_bounds__(256) void paged_cells_kernel(shv_attn_paged_args a, Plan plan) {
     constexpr int VEC = D / 64;
     if constexpr (PLAN) {
         __shared__ PlanSmem<256, kFewBlocks, kFewBlocks> sm;
@@ -232,50 +300,28 @@ __global__ __launch_bounds__(256) void paged_rows_kernel(shv_attn_paged_args a, 
         }
     }
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int rep = a.n_head / a.n_head_kv, per = a.n_head + a.n_head_kv;
     const uint32_t item = (blockIdx.x - (PLAN ? 1 : 0)) * 4 + wave;
-    const int r = static_cast<int>(item / static_cast<uint32_t>(per)), h = static_cast<int>(item) - r * per;
+    const int r = static_cast<int>(item / static_cast<uint32_t>(a.n_head_kv)), head = static_cast<int>(item) - r * a.n_head_kv;
     if (r >= a.max_rows) return;
-    const bool query = h < a.n_head;
-    const int head = query ? h : h - a.n_head;
-    const float *src = a.qkv + static_cast<size_t>(r) * a.qkv_stride + static_cast<size_t>(query ? head : a.n_head) * 2 * D + (query ? 0 : head * D);
+    const float *src = a.qkv + static_cast<size_t>(r) * a.qkv_stride + static_cast<size_t>(a.n_head) * 2 * D + head * D;
     Row<D> x, gamma, val;
     x.load(src, lane);
-    val.load(query ? src : src + static_cast<size_t>(a.n_head_kv) * D, lane);
-    gamma.load(query ? a.q_norm : a.k_norm, lane);
+    val.load(src + static_cast<size_t>(a.n_head_kv) * D, lane);
+    gamma.load(a.k_norm, lane);
     const int p = a.row_pos[r], cell = a.row_cell[r];
-    if (r >= a.start[a.n_seq] || p < 0 || p >= a.max_pages << plan.shift) return;
+    if (r >= a.start[a.n_seq] || p < 0 || p >= a.max_pages << plan.shift || cell < 0 || cell >= a.n_pages << plan.shift) return;
     Turn<D> turn(a.rope_dims, lane);
     if (a.rope_dims > 0) {
         turn.load(a.rope + static_cast<size_t>(p) * a.rope_dims, a.rope_dims);
         turn.settle();
     }
-    if (!query) {
-        if (cell < 0 || cell >= a.n_pages << plan.shift) return;
-        uint16_t kx[VEC];
-        cell_key<D>(x, gamma, turn, a.rope_dims, a.eps, kx);
-        const size_t kvw = static_cast<size_t>(a.n_head_kv) * D;
-        put_bytes<2 * VEC>(static_cast<uint16_t *>(a.kpages) + cell * kvw + head * D + VEC * lane, kx);
-        uint16_t *vd = static_cast<uint16_t *>(a.vpages) + (cell / kTile * kvw + static_cast<size_t>(head) * D + VEC * lane) * kTile + cell % kTile;
+    uint16_t kx[VEC];
+    cell_key<D>(x, gamma, turn, a.rope_dims, a.eps, kx);
+    const size_t kvw = static_cast<size_t>(a.n_head_kv) * D;
+    put_bytes<2 * VEC>(static_cast<uint16_t *>(a.kpages) + cell * kvw + head * D + VEC * lane, kx);
+    uint16_t *vd = static_cast<uint16_t *>(a.vpages) + (cell / kTile * kvw + static_cast<size_t>(head) * D + VEC * lane) * kTile + cell % kTile;
 #pragma unroll
-        for (int v = 0; v < VEC; v++) vd[v * kTile] = __half_as_ushort(__float2half_rn(val.x[v]));
-        return;
-    }
-    float ss = 0.f, y[VEC];
-#pragma unroll
-    for (int v = 0; v < VEC; v++) ss = fmaf(x.x[v], x.x[v], ss);
-    const float sc = __builtin_amdgcn_rsqf(fmaf(wave_sum_all(ss), 1.f / static_cast<float>(D), a.eps));
-#pragma unroll
-    for (int v = 0; v < VEC; v++) {
-        y[v] = x.x[v] * sc * gamma.x[v];
-        if (a.rope_dims > 0) y[v] = fmaf(__shfl(y[v], turn.partner, 64), turn.s.x[v], y[v] * turn.c.x[v]);
-    }
-    _Float16 hi[VEC], lo[VEC];
-    split_row<D>(y, hi, lo);
-    const int kvh = head / rep;
-    char *dst = plan.stage + ((static_cast<size_t>(kvh) * a.max_rows + r) * rep + head - kvh * rep) * D * 4 + 2 * VEC * lane;
-    put_bytes<2 * VEC>(dst, hi);
-    put_bytes<2 * VEC>(dst + 2 * D, lo);
+    for (int v = 0; v < VEC; v++) vd[v * kTile] = __half_as_ushort(__float2half_rn(val.x[v]));
 }
 
 // ---- attention ----------------------------------------------------------------------------------
@@ -284,62 +330,89 @@ __global__ __launch_bounds__(256) void paged_rows_kernel(shv_attn_paged_args a, 
 // scores of cells 8 q + 4 T + 0..3, T = 0, 1: the eight cells of its operand of the second product.
 template <int D>
 struct AttnSmem {
-    char ring[kStages][D / 8 * kChunk];
+    static constexpr int kStage = D / 8 * kChunk, kStages = kRingBytes / kStage;
+    char ring[kStages][kStage];
     float p[kWaves][16 * kTile / 2];  // a wave's weights of half a tile, where its values are not all finite
 };
 
-// Which block of the plan and KV head a workgroup has.  Workgroups go to the eight dies in turn; a die's KV heads are the same ones throughout, where their number
-// allows it, so that its L2 holds their cells, and neighbouring blocks of a plan that cuts lie on one die.
-struct Place {
-    int block, kvh;
-    __device__ __forceinline__ Place(int n_head_kv, int blocks, bool cut) {
-        const int g = n_head_kv & 7 ? n_head_kv & -n_head_kv : 8;  // dies share heads g apart
-        const int die = blockIdx.x & 7, nth = blockIdx.x >> 3, dies = 8 / g, heads = n_head_kv / g;
-        const int k = static_cast<int>(static_cast<uint32_t>(nth) / static_cast<uint32_t>(heads)), of = die / g, per = (blocks + dies - 1) / dies;
-        kvh = die % g + g * (nth - k * heads);
-        block = cut ? (k < per ? of * per + k : blocks) : k * dies + of;
+// Waits until no more than the youngest min(rounds, N) rounds' loads of a wave, PER each, are out: they complete in order.
+template <int PER, int N>
+__device__ __forceinline__ void wait_but(int rounds) {
+    if constexpr (N == 0) {
+        wait_loads<0>();
+    } else if (rounds >= N) {
+        wait_loads<PER * N>();
+    } else {
+        wait_but<PER, N - 1>(rounds);
     }
+}
+
+// What a block is to its pieces.
+struct Unit {
+    int kvh, rep;
+    size_t kvw;
+    const uint16_t *cells;  // the KV head's keys or values, whichever the wave loads
+    uint32_t from;          // of a lane's first chunk in a tile
+    bool keys;
 };
 
-// grid: 8 * ceil(blocks / dies) * heads (Place), blocks of 8 waves
-template <int D>
-__global__ __launch_bounds__(64 * kWaves, D == 256 ? 2 : 4) void paged_attn_kernel(shv_attn_paged_args a, Plan plan) {
+__device__ __forceinline__ void load_8(float (&to)[8], const float *from) {
+    const float4 a = *reinterpret_cast<const float4 *>(from), b = *reinterpret_cast<const float4 *>(from + 4);
+    to[0] = a.x, to[1] = a.y, to[2] = a.z, to[3] = a.w, to[4] = b.x, to[5] = b.y, to[6] = b.z, to[7] = b.w;
+}
+
+__device__ __forceinline__ void store_8(float *to, const float (&from)[8]) {
+    *reinterpret_cast<float4 *>(to) = make_float4(from[0], from[1], from[2], from[3]);
+    *reinterpret_cast<float4 *>(to + 4) = make_float4(from[4], from[5], from[6], from[7]);
+}
+
+// The rotation of a lane's dims where the two of a pair are 32 H apart, in one lane.
+template <int H, int KI>
+__device__ __forceinline__ void turn_in_lane(float (&x)[KI][8], const float *turn, int rope_dims, int dim0) {
+    if constexpr (2 * H <= KI) {
+        if (rope_dims != 64 * H) return;
+#pragma unroll
+        for (int i = 0; i < H; i++) {
+            float c[8], s[8];
+            load_8(c, turn + 32 * i + dim0);
+            load_8(s, turn + 32 * (H + i) + dim0);
+#pragma unroll
+            for (int t = 0; t < 8; t++) {
+                const float a = x[i][t], b = x[i + H][t];
+                x[i][t] = fmaf(-b, s[t], a * c[t]);
+                x[i + H][t] = fmaf(a, s[t], b * c[t]);
+            }
+        }
+    }
+}
+
+// One piece.  A wave takes G groups of query rows; TP waves share a group, each takes every TP-th tile, and their sums are joined in LDS at the end.
+template <int D, int G, int TP>
+__device__ __forceinline__ void run_piece(const shv_attn_paged_args &a, const Plan &plan, const Piece &piece, const Unit &unit, AttnSmem<D> &sm) {
     constexpr int KI = D / 32, DB = D / 16;
     constexpr int kPer = D / 8 / kWaves;  // chunks of a tile a wave asks for
-    extern __shared__ __align__(16) char raw[];
-    AttnSmem<D> &sm = *reinterpret_cast<AttnSmem<D> *>(raw);
+    constexpr int kStages = AttnSmem<D>::kStages, kRounds = kStages / TP;  // rounds of TP tiles in the ring: one is multiplied, the others are on their way
+    static_assert(G == 1 || TP == 1, "waves that share a group have one");
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int n = lane & 15, q = lane >> 4;
-    const int blocks = plan.head[kHeadBlocks];
-    const Place place(a.n_head_kv, blocks, plan.head[kHeadCut] != 0);
-    if (place.block >= blocks) return;
-    const int kvh = place.kvh, rep = a.n_head / a.n_head_kv;
-    const size_t kvw = static_cast<size_t>(a.n_head_kv) * D;
-    const bool keys = wave < kWaves / 2;
-    const int first = (keys ? wave : wave - kWaves / 2) * kPer;  // of the wave's chunks among K's or V's
-    const uint32_t from = keys ? static_cast<uint32_t>((8 * (n >> 2) + 4 * (first / KI) + (n & 3)) * kvw + 32 * (first % KI) + 8 * q) * 2
-                               : static_cast<uint32_t>((16 * first + n) * kTile + 8 * q) * 2;
-    const uint16_t *cells = keys ? static_cast<const uint16_t *>(a.kpages) + kvh * D : static_cast<const uint16_t *>(a.vpages) + static_cast<size_t>(kvh) * D * kTile;
+    const int n = lane & 15, q = lane >> 4, rep = unit.rep, kvh = unit.kvh;
+    const int mine_of = wave % TP;  // which tile of a round
+    const int r0 = piece.r0 + 16 * G * (wave / TP), r_end = piece.r_end;
+    const int last = min(piece.r0 + plan.rows, r_end) - 1;
+    const bool working = r0 <= last;
+    const int lo = piece.pos + static_cast<int>(static_cast<uint32_t>(piece.r0) / static_cast<uint32_t>(rep));
+    const int hi = piece.pos + static_cast<int>(static_cast<uint32_t>(last) / static_cast<uint32_t>(rep));  // the block's rows' positions
+    const Tiles tiles(a.window, a.sinks, lo, hi);
     const float c2 = 1.44269504088896f / sqrtf(static_cast<float>(D));
-    const int end = plan.first_of[place.block + 1];
-    for (int k = plan.first_of[place.block]; k < end; k++) {
-        const Piece piece = plan.pieces[k];
-        const int r0 = piece.r0 + 16 * wave, r_end = piece.r_end;
-        const bool working = r0 < r_end;
-        const int last = min(piece.r0 + kRows, r_end) - 1;
-        const int lo = piece.pos + piece.r0 / rep, hi = piece.pos + last / rep;  // the block's rows' positions
-        const Tiles tiles(a.window, a.sinks, lo, hi);
-        // a group that is not there is the last row again, and dropped
-        const int mine = min(r0 + n, r_end - 1);
-        const int my_pos = piece.pos + static_cast<int>(static_cast<uint32_t>(mine) / static_cast<uint32_t>(rep));
-        const int my_first = a.window > 0 ? my_pos - a.window + 1 : 0;  // the first position it sees, but for the sinks
-        // The table's entries around the tiles asked for last, one a lane.
-        const int32_t *table = a.table + static_cast<size_t>(piece.seq) * a.max_pages;
-        int held = 0, page0 = -64;
-        uint32_t valid = 0;  // of the stages: the tile lies in a page
-        const int n_tiles = piece.t1 - piece.t0;
-        const auto ask = [&](int j) {
-            const int tile = tiles.at(piece.t0 + j), entry = tile >> (plan.shift - 5);
+    int my_pos[G];  // (a row that is not there is the last one again, and dropped)
+    // The table's entries around the tiles asked for last, one a lane.
+    const int32_t *table = a.table + static_cast<size_t>(piece.seq) * a.max_pages;
+    int held = 0, page0 = -64;
+    uint32_t valid = 0;  // of the stages: the tile lies in a page
+    const int n_tiles = piece.t1 - piece.t0, rounds = (n_tiles + TP - 1) / TP;
+    const auto ask = [&](int round) {
+#pragma unroll
+        for (int t = 0; t < TP; t++) {
+            const int j = round * TP + t, tile = tiles.at(piece.t0 + min(j, n_tiles - 1)), entry = tile >> (plan.shift - 5);
             if (static_cast<uint32_t>(entry - page0) >= 64u) {
                 page0 = entry;
                 held = table[min(entry + lane, a.max_pages - 1)];
@@ -347,221 +420,379 @@ __global__ __launch_bounds__(64 * kWaves, D == 256 ? 2 : 4) void paged_attn_kern
             const int page = __builtin_amdgcn_readlane(held, entry - page0);
             const bool is = page >= 0 && page < a.n_pages;
             const uint32_t bit = 1u << (j & (kStages - 1));
-            valid = is ? valid | bit : valid & ~bit;
+            valid = is && j < n_tiles ? valid | bit : valid & ~bit;
             const size_t cell = (static_cast<size_t>(is ? page : 0) << plan.shift) + (tile * kTile & (a.page - 1));
-            const __amdgpu_buffer_rsrc_t bytes = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t *>(cells + cell * kvw), 0, static_cast<uint32_t>(kTile * kvw) * 2, 0x00027000);
+            const __amdgpu_buffer_rsrc_t bytes =
+                __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t *>(unit.cells + cell * unit.kvw), 0, static_cast<uint32_t>(kTile * unit.kvw) * 2, 0x00027000);
             char *to = sm.ring[j & (kStages - 1)] + (wave * kPer) * kChunk;
 #pragma unroll
             for (int u = 0; u < kPer; u++)
-                __builtin_amdgcn_raw_ptr_buffer_load_lds(bytes, (lds_ptr_t)(to + u * kChunk), 16, from, u * (keys ? 64 : 1024), 0, 0);
-        };
-        half8_t qh[KI], ql[KI];
-        {
-            const char *src = plan.stage + ((static_cast<size_t>(kvh) * a.max_rows + piece.first) * rep + mine) * D * 4 + q * 16;
-#pragma unroll
-            for (int i = 0; i < KI; i++) {
-                qh[i] = *reinterpret_cast<const half8_t *>(src + i * 64);
-                ql[i] = *reinterpret_cast<const half8_t *>(src + 2 * D + i * 64);
-            }
+                __builtin_amdgcn_raw_ptr_buffer_load_lds(bytes, (lds_ptr_t)(to + u * kChunk), 16, unit.from, u * (unit.keys ? 64 : 1024), 0, 0);
         }
-        float4_t o[DB];
-        float m_run = -INFINITY, l_run = 0.f;  // of the scores as they are, before their scale; the sums of a lane's own cells
+    };
+    // ---- queries: lane (n, q) holds dims 32 i + 8 q .. of its row from the load to the operand ----
+    int rope_dims = a.rope_dims, dim0 = 8 * q;
+    asm volatile("" : "+s"(rope_dims), "+v"(dim0));  // (what follows from them is formed here and not once for all pieces, which registers do not hold)
+    float x[G][KI][8];
+    const float *turn[G];
 #pragma unroll
-        for (int db = 0; db < DB; db++) o[db] = float4_t{0.f, 0.f, 0.f, 0.f};
-        bool saw = false;  // one of the lane's cells is one that its row sees
-        for (int j = 0; j < min(n_tiles, kAhead); j++) ask(j);
-        for (int j = 0; j < n_tiles; j++) {
-            const char *kt = sm.ring[j & (kStages - 1)];
-            // a wave's loads complete in order: this tile's have landed when no more are out than those behind it
-            if (j + 2 < n_tiles) wait_loads<2 * kPer>();
-            else if (j + 1 < n_tiles) wait_loads<kPer>();
-            else wait_loads<0>();
-            asm volatile("s_barrier" ::: "memory");  // everyone's: this tile is whole, and the stage of the one before is free
-            const bool is = valid >> (j & (kStages - 1)) & 1;
-            if (j + kAhead < n_tiles) ask(j + kAhead);
-            if (!is || !working) continue;
-            const int c0 = tiles.at(piece.t0 + j) * kTile;
-            uint32_t seen = 0xFF;  // which of the lane's eight cells its query row sees
-            const bool part = c0 + kTile - 1 > lo || (a.window > 0 && c0 + kTile - 1 >= a.sinks && c0 <= hi - a.window);
+    for (int g = 0; g < G; g++) {
+        const int mine = min(r0 + 16 * g + n, last), row = static_cast<int>(static_cast<uint32_t>(mine) / static_cast<uint32_t>(rep));
+        my_pos[g] = piece.pos + row;
+        turn[g] = a.rope + static_cast<size_t>(my_pos[g]) * rope_dims;
+        const float *src = a.qkv + static_cast<size_t>(piece.first + row) * a.qkv_stride + static_cast<size_t>(kvh * rep + mine - row * rep) * 2 * D + dim0;
+#pragma unroll
+        for (int i = 0; i < KI; i++) load_8(x[g][i], src + 32 * i);
+    }
+    const bool by_lds = rope_dims % 64 != 0 || rope_dims == 192;  // a rotated pair's dims lie in two lanes: they meet in the ring, before any tile is asked for
+    const int early = min(rounds, kRounds - 1);
+    if (!by_lds)
+        for (int r = 0; r < early; r++) ask(r);
+#pragma unroll
+    for (int g = 0; g < G; g++) {
+        float ss = 0.f;
+#pragma unroll
+        for (int i = 0; i < KI; i++)
+#pragma unroll
+            for (int t = 0; t < 8; t++) ss = fmaf(x[g][i][t], x[g][i][t], ss);
+        const float sc = __builtin_amdgcn_rsqf(fmaf(sum_over_q(ss), 1.f / static_cast<float>(D), a.eps));
+#pragma unroll
+        for (int i = 0; i < KI; i++) {
+            float gamma[8];
+            load_8(gamma, a.q_norm + 32 * i + dim0);
+#pragma unroll
+            for (int t = 0; t < 8; t++) x[g][i][t] *= sc * gamma[t];
+            if (i % 4 == 3) __builtin_amdgcn_sched_barrier(0);  // (not all loads at once: registers are short)
+        }
+        turn_in_lane<1>(x[g], turn[g], rope_dims, dim0);
+        turn_in_lane<2>(x[g], turn[g], rope_dims, dim0);
+        turn_in_lane<4>(x[g], turn[g], rope_dims, dim0);
+    }
+    if (by_lds) {
+        // (loops, and pairs turned where they lie: this path is for the layouts that are rare, and the instruction cache is shared with the one that is not)
+        const uint32_t half = rope_dims / 2;
+        float *rows = reinterpret_cast<float *>(sm.ring[0]) + wave * G * 16 * D;
+        static_assert(kWaves * G * 16 * D * 4 <= kRingBytes, "all rows in the ring");
+#pragma unroll
+        for (int g = 0; g < G; g++) {
+            float *own = rows + (16 * g + n) * D + dim0;
+#pragma unroll
+            for (int i = 0; i < KI; i++) store_8(own + 32 * i, x[g][i]);
+            __builtin_amdgcn_wave_barrier();
+#pragma unroll 1
+            for (uint32_t k = lane; k < 16 * half; k += 64) {
+                const uint32_t row = k / half, e = k - row * half;
+                const float *factors = a.rope + static_cast<size_t>(__shfl(my_pos[g], static_cast<int>(row), 64)) * rope_dims;
+                float *pair = rows + (16 * g + row) * D + e;
+                const float c = factors[e], s = factors[half + e], u = pair[0], v = pair[half];
+                pair[0] = fmaf(-v, s, u * c);
+                pair[half] = fmaf(u, s, v * c);
+            }
+            __builtin_amdgcn_wave_barrier();
+#pragma unroll
+            for (int i = 0; i < KI; i++) load_8(x[g][i], own + 32 * i);
+        }
+        __syncthreads();
+        for (int r = 0; r < early; r++) ask(r);
+    }
+    half8_t qh[G][KI], ql[G][KI];
+#pragma unroll
+    for (int g = 0; g < G; g++)
+#pragma unroll
+        for (int i = 0; i < KI; i++)
+#pragma unroll
+            for (int t = 0; t < 8; t++) {
+                qh[g][i][t] = static_cast<_Float16>(x[g][i][t]);
+                ql[g][i][t] = static_cast<_Float16>(fmaf(static_cast<float>(qh[g][i][t]), -1.f, x[g][i][t]));
+            }
+    __builtin_amdgcn_sched_barrier(0);
+    float4_t o[G][DB];
+    float m_run[G], l_run[G];  // of the scores as they are, before their scale; the sums of a lane's own cells
+    uint32_t saw = 0;          // bit g: one of the lane's cells is one that its row sees
+#pragma unroll
+    for (int g = 0; g < G; g++) {
+        m_run[g] = -INFINITY, l_run[g] = 0.f;
+#pragma unroll
+        for (int db = 0; db < DB; db++) o[g][db] = float4_t{0.f, 0.f, 0.f, 0.f};
+    }
+    for (int r = 0; r < rounds; r++) {
+        const int j = r * TP + mine_of;
+        const char *kt = sm.ring[j & (kStages - 1)];
+        wait_but<kPer * TP, kRounds - 2>(rounds - 1 - r);
+        asm volatile("s_barrier" ::: "memory");  // everyone's: this round is whole, and the stages of the one before are free
+        const bool is = valid >> (j & (kStages - 1)) & 1;
+        if (r + kRounds - 1 < rounds) ask(r + kRounds - 1);
+        if (!is || !working) continue;
+        const int c0 = tiles.at(piece.t0 + j) * kTile;
+        uint32_t seen[G];  // which of the lane's eight cells its query row sees
+        const bool part = c0 + kTile - 1 > lo || (a.window > 0 && c0 + kTile - 1 >= a.sinks && c0 <= hi - a.window);
+#pragma unroll
+        for (int g = 0; g < G; g++) {
+            seen[g] = 0xFF;
             if (part) {
-                seen = 0;
+                seen[g] = 0;
 #pragma unroll
                 for (int e = 0; e < 8; e++) {
                     const int c = c0 + 8 * q + e;
-                    seen |= c <= my_pos && (a.window == 0 || c < a.sinks || c >= my_first) ? 1u << e : 0u;
+                    seen[g] |= c <= my_pos[g] && (a.window == 0 || c < a.sinks || c > my_pos[g] - a.window) ? 1u << e : 0u;
                 }
             }
-            saw |= seen != 0;
-            const char *vt = kt + 2 * KI * kChunk;
-            // operands come from LDS four reads ahead of the products that use them
-            float4_t st[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}}, sl[2] = {st[0], st[0]};
-            half8_t kb[2][4];
-            const auto read_k = [&](half8_t(&to)[4], int g) {
+            saw |= seen[g] != 0 ? 1u << g : 0u;
+        }
+        const char *vt = kt + 2 * KI * kChunk;
+        // operands come from LDS four reads ahead of the products that use them
+        float4_t st[G][2], sl[G][2];
 #pragma unroll
-                for (int e = 0; e < 4; e++) to[e] = *reinterpret_cast<const half8_t *>(kt + ((e & 1) * KI + 2 * g + (e >> 1)) * kChunk + lane * 16);
-            };
-            read_k(kb[0], 0);
+        for (int g = 0; g < G; g++)
 #pragma unroll
-            for (int g = 0; g < KI / 2; g++) {
-                if (g + 1 < KI / 2) read_k(kb[(g + 1) & 1], g + 1);
-                __builtin_amdgcn_sched_barrier(0);
+            for (int T = 0; T < 2; T++) st[g][T] = sl[g][T] = float4_t{0.f, 0.f, 0.f, 0.f};
+        half8_t kb[2][4];
+        const auto read_k = [&](half8_t(&to)[4], int i) {
 #pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    st[e & 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kb[g & 1][e], qh[2 * g + (e >> 1)], st[e & 1], 0, 0, 0);
-                    sl[e & 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kb[g & 1][e], ql[2 * g + (e >> 1)], sl[e & 1], 0, 0, 0);
+            for (int e = 0; e < 4; e++) to[e] = *reinterpret_cast<const half8_t *>(kt + ((e & 1) * KI + 2 * i + (e >> 1)) * kChunk + lane * 16);
+        };
+        read_k(kb[0], 0);
+#pragma unroll
+        for (int i = 0; i < KI / 2; i++) {
+            if (i + 1 < KI / 2) read_k(kb[(i + 1) & 1], i + 1);
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int e = 0; e < 4; e++)
+#pragma unroll
+                for (int g = 0; g < G; g++) {
+                    st[g][e & 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kb[i & 1][e], qh[g][2 * i + (e >> 1)], st[g][e & 1], 0, 0, 0);
+                    sl[g][e & 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kb[i & 1][e], ql[g][2 * i + (e >> 1)], sl[g][e & 1], 0, 0, 0);
                 }
-            }
-            float mx = -INFINITY, s[8];
+        }
+        float pv[G][8];
+        bool by_hand = false;
 #pragma unroll
-            for (int e = 0; e < 8; e++) s[e] = st[e >> 2][e & 3] + sl[e >> 2][e & 3];
+        for (int g = 0; g < G; g++) {
+            float mx = -INFINITY;
+            float(&s)[8] = pv[g];
+#pragma unroll
+            for (int e = 0; e < 8; e++) s[e] = st[g][e >> 2][e & 3] + sl[g][e >> 2][e & 3];
             if (part) {
 #pragma unroll
-                for (int e = 0; e < 8; e++) s[e] = seen >> e & 1 ? s[e] : -INFINITY;
+                for (int e = 0; e < 8; e++) s[e] = seen[g] >> e & 1 ? s[e] : -INFINITY;
             }
 #pragma unroll
             for (int e = 0; e < 8; e++) mx = fmaxf(mx, s[e]);
             mx = max_over_q(mx);
             // the sums are rescaled a few times a run instead of whenever some row's maximum moves
-            const bool moves = mx * c2 > fmaf(m_run, c2, kSlack);
+            const bool moves = mx * c2 > fmaf(m_run[g], c2, kSlack);
             if (__ballot(moves) != 0ull) {
-                const float m_new = moves ? mx : m_run;
-                const float alpha = m_new == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((m_run - m_new) * c2);
-                l_run *= alpha;
-                m_run = m_new;
+                const float m_new = moves ? mx : m_run[g];
+                const float alpha = m_new == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((m_run[g] - m_new) * c2);
+                l_run[g] *= alpha;
+                m_run[g] = m_new;
                 float av[4];
 #pragma unroll
                 for (int e = 0; e < 4; e++) av[e] = __shfl(alpha, 4 * q + e, 64);
 #pragma unroll
                 for (int db = 0; db < DB; db++)
 #pragma unroll
-                    for (int e = 0; e < 4; e++) o[db][e] *= av[e];
+                    for (int e = 0; e < 4; e++) o[g][db][e] *= av[e];
             }
-            const float m2 = fmaf(m_run == -INFINITY ? 0.f : m_run, c2, -kLift);
-            float pv[8];
+            const float m2 = fmaf(m_run[g] == -INFINITY ? 0.f : m_run[g], c2, -kLift);
 #pragma unroll
             for (int e = 0; e < 8; e++) {
-                pv[e] = __builtin_amdgcn_exp2f(fmaf(s[e], c2, -m2));
-                l_run += pv[e];
-            }
-            if (part) {
-                // a value that is not finite would meet the weight 0 of rows that do not see it: such a tile is multiplied by hand
-                uint32_t odd = 0;
-#pragma unroll
-                for (int db = 0; db < DB; db++) {
-                    const uint4 v = *reinterpret_cast<const uint4 *>(vt + db * kChunk + lane * 16);
-                    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-                    for (int e = 0; e < 4; e++) odd |= ((w[e] & 0x7C007C00u) + 0x04000400u) & 0x80008000u;  // an exponent of ones carries into the sign
-                }
-                if (__ballot(odd != 0) != 0ull) {
-                    float *p = sm.p[wave];
-#pragma unroll 1
-                    for (int half = 0; half < 2; half++) {
-                        if ((q >> 1) == half) {
-#pragma unroll
-                            for (int e = 0; e < 8; e++) p[n * (kTile / 2) + 8 * (q & 1) + e] = seen >> e & 1 ? pv[e] : -1.f;
-                        }
-                        __builtin_amdgcn_wave_barrier();
-#pragma unroll 1
-                        for (int i = 0; i < kTile / 2; i++) {
-                            const int c = kTile / 2 * half + i;
-                            float w[4];
-#pragma unroll
-                            for (int e = 0; e < 4; e++) w[e] = p[(4 * q + e) * (kTile / 2) + i];
-#pragma unroll
-                            for (int db = 0; db < DB; db++) {
-                                const float v = static_cast<float>(*reinterpret_cast<const _Float16 *>(vt + db * kChunk + (16 * (c >> 3) + n) * 16 + (c & 7) * 2));
-#pragma unroll
-                                for (int e = 0; e < 4; e++) o[db][e] = w[e] < 0.f ? o[db][e] : fmaf(w[e], v, o[db][e]);
-                            }
-                        }
-                        __builtin_amdgcn_wave_barrier();
-                    }
-                    continue;
-                }
-            }
-            // weights as two halves, the large one cut off and not rounded: the small one holds the rest either way, and is rounded to nearest, so that what
-            // many cells lose cancels
-            half8_t ph, pl;
-#pragma unroll
-            for (int e = 0; e < 8; e += 2) {
-                const half2_t h = __builtin_bit_cast(half2_t, __builtin_amdgcn_cvt_pkrtz(pv[e], pv[e + 1]));
-                const half2_t r = {static_cast<_Float16>(fmaf(static_cast<float>(h[0]), -1.f, pv[e])), static_cast<_Float16>(fmaf(static_cast<float>(h[1]), -1.f, pv[e + 1]))};
-                ph[e] = h[0]; ph[e + 1] = h[1];
-                pl[e] = r[0]; pl[e + 1] = r[1];
-            }
-            half8_t vb[2][4];
-#pragma unroll
-            for (int e = 0; e < 4; e++) vb[0][e] = *reinterpret_cast<const half8_t *>(vt + e * kChunk + lane * 16);
-#pragma unroll
-            for (int g = 0; g < DB / 4; g++) {
-                if (g + 1 < DB / 4) {
-#pragma unroll
-                    for (int e = 0; e < 4; e++) vb[(g + 1) & 1][e] = *reinterpret_cast<const half8_t *>(vt + (4 * (g + 1) + e) * kChunk + lane * 16);
-                }
-                __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-                for (int e = 0; e < 4; e++) o[4 * g + e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ph, vb[g & 1][e], o[4 * g + e], 0, 0, 0);
-#pragma unroll
-                for (int e = 0; e < 4; e++) o[4 * g + e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(pl, vb[g & 1][e], o[4 * g + e], 0, 0, 0);
+                s[e] = __builtin_amdgcn_exp2f(fmaf(s[e], c2, -m2));
+                l_run[g] += s[e];
             }
         }
-        if (working) {
-            float sum = sum_over_q(l_run);
-            const uint64_t saws = __ballot(saw);
+        if (part) {
+            // a value that is not finite would meet the weight 0 of rows that do not see it: such a tile is multiplied by hand
+            uint32_t odd = 0;
+#pragma unroll
+            for (int db = 0; db < DB; db++) {
+                const uint4 v = *reinterpret_cast<const uint4 *>(vt + db * kChunk + lane * 16);
+                const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+                for (int e = 0; e < 4; e++) odd |= ((w[e] & 0x7C007C00u) + 0x04000400u) & 0x80008000u;  // an exponent of ones carries into the sign
+            }
+            by_hand = __ballot(odd != 0) != 0ull;
+        }
+        if (by_hand) {
+            float *p = sm.p[wave];
+#pragma unroll
+            for (int g = 0; g < G; g++)
+#pragma unroll 1
+                for (int half = 0; half < 2; half++) {
+                    if ((q >> 1) == half) {
+#pragma unroll
+                        for (int e = 0; e < 8; e++) p[n * (kTile / 2) + 8 * (q & 1) + e] = seen[g] >> e & 1 ? pv[g][e] : -1.f;
+                    }
+                    __builtin_amdgcn_wave_barrier();
+#pragma unroll 1
+                    for (int i = 0; i < kTile / 2; i++) {
+                        const int c = kTile / 2 * half + i;
+                        float w[4];
+#pragma unroll
+                        for (int e = 0; e < 4; e++) w[e] = p[(4 * q + e) * (kTile / 2) + i];
+#pragma unroll
+                        for (int db = 0; db < DB; db++) {
+                            const float v = static_cast<float>(*reinterpret_cast<const _Float16 *>(vt + db * kChunk + (16 * (c >> 3) + n) * 16 + (c & 7) * 2));
+#pragma unroll
+                            for (int e = 0; e < 4; e++) o[g][db][e] = w[e] < 0.f ? o[g][db][e] : fmaf(w[e], v, o[g][db][e]);
+                        }
+                    }
+                    __builtin_amdgcn_wave_barrier();
+                }
+            continue;
+        }
+        // weights as two halves, the large one cut off and not rounded: the small one holds the rest either way, and is rounded to nearest, so that what
+        // many cells lose cancels
+        half8_t ph[G], pl[G];
+#pragma unroll
+        for (int g = 0; g < G; g++)
+#pragma unroll
+            for (int e = 0; e < 8; e += 2) {
+                const half2_t h = __builtin_bit_cast(half2_t, __builtin_amdgcn_cvt_pkrtz(pv[g][e], pv[g][e + 1]));
+                const half2_t l = {static_cast<_Float16>(fmaf(static_cast<float>(h[0]), -1.f, pv[g][e])), static_cast<_Float16>(fmaf(static_cast<float>(h[1]), -1.f, pv[g][e + 1]))};
+                ph[g][e] = h[0]; ph[g][e + 1] = h[1];
+                pl[g][e] = l[0]; pl[g][e + 1] = l[1];
+            }
+        half8_t vb[2][4];
+#pragma unroll
+        for (int e = 0; e < 4; e++) vb[0][e] = *reinterpret_cast<const half8_t *>(vt + e * kChunk + lane * 16);
+#pragma unroll
+        for (int i = 0; i < DB / 4; i++) {
+            if (i + 1 < DB / 4) {
+#pragma unroll
+                for (int e = 0; e < 4; e++) vb[(i + 1) & 1][e] = *reinterpret_cast<const half8_t *>(vt + (4 * (i + 1) + e) * kChunk + lane * 16);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int g = 0; g < G; g++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) o[g][4 * i + e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ph[g], vb[i & 1][e], o[g][4 * i + e], 0, 0, 0);
+#pragma unroll
+            for (int g = 0; g < G; g++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) o[g][4 * i + e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(pl[g], vb[i & 1][e], o[g][4 * i + e], 0, 0, 0);
+        }
+    }
+    bool writes = working;
+    if constexpr (TP > 1) {
+        // the sums of a group's other waves, by way of the ring, which is free
+        static_assert(kWaves * (DB + 1) * 64 * 16 <= kRingBytes + (TP == 2 ? kRingBytes : 0), "half of the waves leave their sums");
+        float4_t *slot = reinterpret_cast<float4_t *>(sm.ring[0]) + (wave / 2) * (DB + 1) * 64 + lane;
+        __syncthreads();
+        if (working && mine_of == 1) {
+#pragma unroll
+            for (int db = 0; db < DB; db++) slot[db * 64] = o[0][db];
+            slot[DB * 64] = float4_t{m_run[0], l_run[0], __uint_as_float(saw), 0.f};
+        }
+        __syncthreads();
+        writes = working && mine_of == 0;
+        if (writes) {
+            const float4_t of = slot[DB * 64];
+            const float m = fmaxf(m_run[0], of[0]);
+            const float f1 = m_run[0] == m ? 1.f : __builtin_amdgcn_exp2f((m_run[0] - m) * c2), f2 = of[0] == m ? 1.f : __builtin_amdgcn_exp2f((of[0] - m) * c2);
+            l_run[0] = f1 * l_run[0] + f2 * of[1];
+            m_run[0] = m;
+            saw |= __float_as_uint(of[2]);
+            float a1[4], a2[4];
+#pragma unroll
+            for (int e = 0; e < 4; e++) a1[e] = __shfl(f1, 4 * q + e, 64), a2[e] = __shfl(f2, 4 * q + e, 64);
+#pragma unroll
+            for (int db = 0; db < DB; db++) {
+                const float4_t other = slot[db * 64];
+#pragma unroll
+                for (int e = 0; e < 4; e++) o[0][db][e] = a1[e] * o[0][db][e] + a2[e] * other[e];
+            }
+        }
+    }
+    if (writes) {
+#pragma unroll
+        for (int g = 0; g < G; g++) {
+            const int rg = r0 + 16 * g;
+            if (rg > last) break;
+            float sum = sum_over_q(l_run[g]);
             // a row whose scores are all -infinity has no weights; one that sees nothing has a sum of zero
-            if (m_run == -INFINITY && ((saws >> n) & 0x0001000100010001ull) != 0) sum = __int_as_float(0x7fc00000);
+            const uint64_t saws = __ballot(saw >> g & 1);
+            if (m_run[g] == -INFINITY && ((saws >> n) & 0x0001000100010001ull) != 0) sum = __int_as_float(0x7fc00000);
             if (piece.rec < 0) {
                 float lr[4];
 #pragma unroll
-                for (int i = 0; i < 4; i++) lr[i] = __shfl(sum, 4 * q + i, 64);
+                for (int i = 0; i < 4; i++) lr[i] = __shfl(sum == 0.f ? 0.f : 1.f / sum, 4 * q + i, 64);
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
-                    const int r = r0 + 4 * q + i, row = static_cast<int>(static_cast<uint32_t>(r) / static_cast<uint32_t>(rep));
-                    if (r >= r_end) continue;
+                    const int r = rg + 4 * q + i, row = static_cast<int>(static_cast<uint32_t>(r) / static_cast<uint32_t>(rep));
+                    if (r > last) continue;
                     float *dst = a.out + (static_cast<size_t>(piece.first + row) * a.n_head + kvh * rep + r - row * rep) * D;
 #pragma unroll
-                    for (int db = 0; db < DB; db++) dst[16 * db + n] = lr[i] == 0.f ? 0.f : o[db][i] / lr[i];
+                    for (int db = 0; db < DB; db++) dst[16 * db + n] = o[g][db][i] * lr[i];
                 }
             } else {
-                const size_t base = (static_cast<size_t>(piece.rec) * a.n_head_kv + kvh) * plan.slot_rows + 16 * wave;
+                const size_t base = (static_cast<size_t>(piece.rec) * a.n_head_kv + kvh) * plan.slot_rows + rg - piece.r0;
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
-                    if (r0 + 4 * q + i >= r_end) continue;
+                    if (rg + 4 * q + i > last) continue;
                     float *rec = plan.sums + (base + 4 * q + i) * D;
 #pragma unroll
-                    for (int db = 0; db < DB; db++) rec[16 * db + n] = o[db][i];
+                    for (int db = 0; db < DB; db++) rec[16 * db + n] = o[g][db][i];
                 }
-                if (q == 0 && r0 + n < r_end) plan.of[base + n] = make_float2(m_run, sum);
+                if (q == 0 && rg + n <= last) plan.of[base + n] = make_float2(m_run[g], sum);
             }
         }
-        __syncthreads();  // the stages are free for the next piece
+    }
+    __syncthreads();  // the stages are free for the next piece
+}
+
+// grid: 8 * ceil(blocks / dies) * heads, blocks of 8 waves.  Workgroups go to the eight dies in turn; a die's KV heads are the same ones throughout, where their number
+// allows it, so that its L2 holds their cells: die x has the heads x % g, x % g + g, .. for g the power of two in their number, up to 8.
+template <int D>
+__global__ __launch_bounds__(64 * kWaves, 2) void paged_attn_kernel(shv_attn_paged_args a, Plan plan) {
+    constexpr int KI = D / 32, kPer = D / 8 / kWaves;
+    extern __shared__ __align__(16) char raw[];
+    AttnSmem<D> &sm = *reinterpret_cast<AttnSmem<D> *>(raw);
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int n = lane & 15, q = lane >> 4;
+    const int die = blockIdx.x & 7, nth = blockIdx.x >> 3, g = 8 / plan.dies;
+    const int turn = static_cast<int>(static_cast<uint32_t>(nth) / static_cast<uint32_t>(plan.heads)), slot = turn * plan.dies + die / g;
+    if (slot >= plan.most_blocks) return;
+    const Block *block = plan.blocks + slot;
+    const int pieces = block->more + 1;
+    const Piece *at = &block->piece;
+    Unit unit;
+    unit.kvh = die % g + g * (nth - turn * plan.heads), unit.rep = a.n_head / a.n_head_kv;
+    unit.kvw = static_cast<size_t>(a.n_head_kv) * D;
+    unit.keys = wave < kWaves / 2;
+    const int first = (unit.keys ? wave : wave - kWaves / 2) * kPer;  // of the wave's chunks among K's or V's
+    unit.from = unit.keys ? static_cast<uint32_t>((8 * (n >> 2) + 4 * (first / KI) + (n & 3)) * unit.kvw + 32 * (first % KI) + 8 * q) * 2
+                          : static_cast<uint32_t>((16 * first + n) * kTile + 8 * q) * 2;
+    unit.cells = unit.keys ? static_cast<const uint16_t *>(a.kpages) + unit.kvh * D : static_cast<const uint16_t *>(a.vpages) + static_cast<size_t>(unit.kvh) * D * kTile;
+    for (int k = 0; k < pieces; k++) {
+        const Piece piece = *at;
+        at = k == 0 ? plan.pieces + block->at : at + 1;
+        const int groups = (min(piece.r_end - piece.r0, plan.rows) + 15) / 16;
+        if (groups <= kWaves / 2) run_piece<D, 1, 2>(a, plan, piece, unit, sm);
+        else run_piece<D, kGroups<D>, 1>(a, plan, piece, unit, sm);
     }
 }
 
 // ---- the join -----------------------------------------------------------------------------------
-// A unit is 256 / D query rows of a KV head, a lane four dims.  With many records a query row a block's four waves share them, otherwise each takes a unit of its own.
-constexpr int kShareFrom = 8;  // records a query row from which the waves share them
-template <int D>
+// A unit is 256 / D query rows of a KV head, a lane four dims.  SHARE, where a query row has many records: a block's four waves share them, otherwise each takes a unit
+// of its own.
+template <int D, bool SHARE>
 __global__ __launch_bounds__(256) void paged_join_kernel(shv_attn_paged_args a, Plan plan) {
     __shared__ float4_t sums[4][64];
     __shared__ float2 of[4][64];
-    constexpr int kLanes = D / 4, kUnit = 64 / kLanes;
+    constexpr int kLanes = D / 4, kUnit = 64 / kLanes, kPerHead = 16 / kUnit;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int n_joins = plan.head[kHeadJoins];
-    if (n_joins == 0) return;
     const int rep = a.n_head / a.n_head_kv;
     const float c2 = 1.44269504088896f / sqrtf(static_cast<float>(D));
-    const bool share = plan.head[kHeadRecs] >= kShareFrom * n_joins;
-    const uint32_t per_head = (plan.slot_rows + kUnit - 1) / kUnit, per = per_head * a.n_head_kv, units = per * n_joins;
-    const uint32_t step = share ? gridDim.x : gridDim.x * 4;
-    for (uint32_t unit = share ? blockIdx.x : blockIdx.x * 4 + wave; unit < units; unit += step) {
-        const uint32_t k = unit / per, in = unit - k * per, kvh = in / per_head, u = in - kvh * per_head;
+    const uint32_t per = kPerHead * a.n_head_kv, units = per * *plan.n_joins;
+    const uint32_t step = SHARE ? gridDim.x : gridDim.x * 4;
+    for (uint32_t unit = SHARE ? blockIdx.x : blockIdx.x * 4 + wave; unit < units; unit += step) {
+        const uint32_t k = unit / per, in = unit - k * per, kvh = in / kPerHead, u = in % kPerHead;
         const Join join = plan.joins[k];
         const int local = u * kUnit + lane / kLanes, r = join.r0 + local;
-        const bool there = local < plan.slot_rows && local < kRows && r < join.r_end;
+        const bool there = r < join.r_end;
         if (__ballot(there) == 0ull) continue;  // (the same in every wave that shares)
-        const size_t row = (static_cast<size_t>(join.rec) * a.n_head_kv + kvh) * plan.slot_rows + (there ? local : 0), stride = static_cast<size_t>(a.n_head_kv) * plan.slot_rows;
+        const size_t row = (static_cast<size_t>(join.rec) * a.n_head_kv + kvh) * plan.slot_rows + join.in + (there ? local : 0), stride = static_cast<size_t>(a.n_head_kv) * plan.slot_rows;
         const float4_t *from = reinterpret_cast<const float4_t *>(plan.sums + row * D) + lane % kLanes;
         const float2 *from_of = plan.of + row;
         constexpr int MB = 8;
@@ -576,7 +807,8 @@ __global__ __launch_bounds__(256) void paged_join_kernel(shv_attn_paged_args a, 
             for (int e = 0; e < 4; e++) num[e] = fmaf(num[e], shrink, w * v[e]);
             M = Mn;
         };
-        const int waves = share ? 4 : 1, me = share ? wave : 0;
+        constexpr int waves = SHARE ? 4 : 1;
+        const int me = SHARE ? wave : 0;
         for (int s0 = me; s0 < join.n; s0 += waves * MB) {
             float4_t v[MB];
             float2 ml[MB];
@@ -592,7 +824,7 @@ __global__ __launch_bounds__(256) void paged_join_kernel(shv_attn_paged_args a, 
             for (int i = 0; i < MB; i++)
                 if (s0 + waves * i < join.n) fold(v[i], ml[i]);
         }
-        if (share) {
+        if constexpr (SHARE) {
             __syncthreads();
             sums[wave][lane] = num;
             of[wave][lane] = make_float2(M, den);
@@ -628,29 +860,30 @@ int check_sizes(const shv_attn_paged_args &a) {
 // The scratch of a call of these sizes, laid out from `work` on; its end is the bytes that it takes.
 uintptr_t lay_out(const shv_ctx *ctx, const shv_attn_paged_args &a, Plan &plan) {
     const int rep = a.n_head / a.n_head_kv, D = a.head_dim;
-    const int per_unit = D == 256 ? 1 : 2;  // blocks a compute unit holds
-    plan.slots = ctx->prop.multiProcessorCount * per_unit / a.n_head_kv;
+    plan.slots = ctx->prop.multiProcessorCount / a.n_head_kv;
     if (plan.slots < 1) plan.slots = 1;
     const int query_rows = a.max_rows * rep;
-    plan.most_q = (a.n_seq < a.max_rows ? a.n_seq : a.max_rows) + query_rows / kRows;
-    plan.most_blocks = plan.most_q > plan.slots ? plan.most_q : plan.slots;
-    plan.slot_rows = query_rows < kRows ? (query_rows + 15) / 16 * 16 : kRows;
+    plan.rows = rows_of(D);
+    plan.most_q = (a.n_seq < a.max_rows ? a.n_seq : a.max_rows) + query_rows / plan.rows;
+    const int g = a.n_head_kv & 7 ? a.n_head_kv & -a.n_head_kv : 8;
+    plan.dies = 8 / g, plan.heads = a.n_head_kv / g;
+    plan.most_blocks = ((plan.most_q > plan.slots ? plan.most_q : plan.slots) + plan.dies - 1) / plan.dies * plan.dies;
+    plan.slot_rows = query_rows < plan.rows ? (query_rows + 15) / 16 * 16 : plan.rows;
     plan.shift = 0;
     while (1 << plan.shift < a.page) plan.shift++;
     // a cut query block has a piece more than cuts, and there are fewer cuts than slots
-    const size_t pieces = static_cast<size_t>(plan.most_q) + plan.slots, joins = plan.most_q < plan.slots ? plan.most_q : plan.slots, records = 2 * static_cast<size_t>(plan.slots) * a.n_head_kv * plan.slot_rows;
+    const size_t pieces = static_cast<size_t>(plan.most_q) + plan.slots, joins = plan.rows / 16 * static_cast<size_t>(plan.most_q < plan.slots ? plan.most_q : plan.slots), records = 2 * static_cast<size_t>(plan.slots) * a.n_head_kv * plan.slot_rows;
     uintptr_t at = reinterpret_cast<uintptr_t>(a.work);
     const auto take = [&](size_t bytes) {
         char *here = reinterpret_cast<char *>(at);
         at += (bytes + 255) / 256 * 256;
         return here;
     };
-    plan.head = reinterpret_cast<int32_t *>(take(kHeadWords * 4));
-    plan.first_of = reinterpret_cast<int32_t *>(take((plan.most_blocks + 1) * 4));
+    plan.n_joins = reinterpret_cast<int32_t *>(take(4));
+    plan.blocks = reinterpret_cast<Block *>(take(plan.most_blocks * sizeof(Block)));
     plan.pieces = reinterpret_cast<Piece *>(take(pieces * sizeof(Piece)));
     plan.joins = reinterpret_cast<Join *>(take(joins * sizeof(Join)));
     plan.of = reinterpret_cast<float2 *>(take(records * 8));
-    plan.stage = take(static_cast<size_t>(a.max_rows) * a.n_head * D * 4);
     plan.sums = reinterpret_cast<float *>(take(records * D * 4));
     return at;
 }
@@ -667,18 +900,18 @@ int launch_paged(shv_ctx *ctx, const shv_attn_paged_args &a) {
         SHV_HIP_CHECK(hipFuncSetAttribute(reinterpret_cast<const void *>(&paged_plan_kernel), hipFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(sizeof(BigSmem))));
         raised.fetch_or(bit, std::memory_order_release);
     }
-    const long long items = static_cast<long long>(a.max_rows) * (a.n_head + a.n_head_kv);
-    const unsigned row_blocks = static_cast<unsigned>((items + 3) / 4);
+    const unsigned row_blocks = static_cast<unsigned>((static_cast<long long>(a.max_rows) * a.n_head_kv + 3) / 4);
     if (plan.most_q <= kFewBlocks && a.n_seq <= kFewBlocks) {
-        SHV_LAUNCH(ctx, (paged_rows_kernel<D, true>), dim3(row_blocks + 1), dim3(256), 0, a, plan);
+        SHV_LAUNCH(ctx, (paged_cells_kernel<D, true>), dim3(row_blocks + 1), dim3(256), 0, a, plan);
     } else {
         SHV_LAUNCH(ctx, paged_plan_kernel, dim3(1), dim3(1024), sizeof(BigSmem), a, plan);
-        SHV_LAUNCH(ctx, (paged_rows_kernel<D, false>), dim3(row_blocks), dim3(256), 0, a, plan);
+        SHV_LAUNCH(ctx, (paged_cells_kernel<D, false>), dim3(row_blocks), dim3(256), 0, a, plan);
     }
-    const int g = a.n_head_kv & 7 ? a.n_head_kv & -a.n_head_kv : 8, dies = 8 / g, heads = a.n_head_kv / g;  // Place
-    SHV_LAUNCH(ctx, paged_attn_kernel<D>, dim3(static_cast<unsigned>((plan.most_blocks + dies - 1) / dies * heads * 8)), dim3(64 * kWaves), sizeof(AttnSmem<D>), a, plan);
-    const long long joins = plan.most_q < plan.slots ? plan.most_q : plan.slots, units = joins * a.n_head_kv * plan.slot_rows;
-    SHV_LAUNCH(ctx, paged_join_kernel<D>, dim3(static_cast<unsigned>(units < 2048 ? units : 2048)), dim3(256), 0, a, plan);
+    SHV_LAUNCH(ctx, paged_attn_kernel<D>, dim3(plan.most_blocks / plan.dies * plan.heads * 8), dim3(64 * kWaves), sizeof(AttnSmem<D>), a, plan);
+    const long long joins = plan.most_q < plan.slots ? plan.most_q : plan.slots, units = joins * a.n_head_kv * plan.slot_rows / (256 / D);
+    const dim3 grid(static_cast<unsigned>(units < 2048 ? units : 2048));
+    if (plan.slots >= kShareFrom * plan.most_q) SHV_LAUNCH(ctx, (paged_join_kernel<D, true>), grid, dim3(256), 0, a, plan);
+    else SHV_LAUNCH(ctx, (paged_join_kernel<D, false>), grid, dim3(256), 0, a, plan);
     return SHV_OK;
 }
 

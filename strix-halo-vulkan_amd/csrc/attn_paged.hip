@@ -38,6 +38,13 @@ constexpr int kFewBlocks = 1024;  // query blocks up to which the plan is made i
 // both.
 template <int D>
 constexpr int kGroups = D == 256 ? 1 : 2;
+// Waves that share a group of few query rows, each with tiles of its own.
+#ifndef MT128
+#define MT128 4
+#define MT64 8
+#endif
+template <int D>
+constexpr int kManyTurns = D == 256 ? 2 : D == 128 ? MT128 : MT64;
 constexpr int rows_of(int D) { return 16 * kWaves * (D == 256 ? 1 : 2); }
 
 // A block's query rows of a sequence and a run of the tiles they look at.
@@ -74,6 +81,10 @@ struct Plan {
     int most_blocks, most_q;
     int dies, heads;    // dies that share a KV head, and KV heads of a die (place)
     int shift;          // log2 of the page
+    uint32_t rep_magic; // 2^32 / rep, rounded up; 0 for rep 1
+    __device__ __forceinline__ int over_rep(int r) const {  // r / rep: exact for r < 2^20 and rep <= 64, which it is off by less than 1 / 64 before it is cut
+        return rep_magic == 0 ? r : static_cast<int>(__umulhi(static_cast<uint32_t>(r), rep_magic));
+    }
 };
 
 // Which tiles of 32 cells query rows of positions lo .. hi look at: the sinks', then those the window of the first row reaches.
@@ -116,20 +127,50 @@ __host__ __device__ constexpr Costs costs_of(int D) { return D == 256 ? Costs{16
 // The query blocks of all sequences stand in a row, each with its cost, P their running sum.  Where they fill the chip evenly each is a block's own, those with the most
 // tiles first.  Otherwise block b takes what lies from b S to (b + 1) S in the row, S = all / blocks, so that all blocks have the same; a query block cut by that
 // leaves a record of each piece.
+constexpr int kSeqBits = 11, kMaxSlots = 256;  // blocks that the chip holds at once: a unit one
+static_assert(kMaxSeqs <= 1 << kSeqBits, "a sequence's number");
 template <int T, int SEQS, int NQ>
 struct PlanSmem {
     uint32_t q0[SEQS];          // query blocks before a sequence's
     int first[SEQS], n[SEQS], pos[SEQS];
-    uint32_t p[NQ], at[NQ];     // the cost before a query block; its first piece
+    uint32_t p[NQ], of[NQ];     // the cost before a query block; its sequence, and above kSeqBits its first piece
     int rec[NQ];                // its first record, -1: it has one piece
+    uint16_t begins[kMaxSlots + 1];  // a block's first piece
     uint32_t waves[3][T / 64];
     uint32_t bucket[64];
     uint32_t most, most_way;
 };
+// A query block as a piece of all its tiles; what a tile of it costs, and its way in and out (which the first one's block has in any case).
+struct Whole : Piece {
+    uint32_t tile, way, groups;
+};
+__device__ __forceinline__ Whole whole_block(int window, int sinks, int D, int rows, uint32_t rep_magic, int seq, int first, int r_end, int pos, int r0, bool free_way) {
+    const auto over_rep = [&](int r) { return rep_magic == 0 ? r : static_cast<int>(__umulhi(static_cast<uint32_t>(r), rep_magic)); };
+    const Costs costs = costs_of(D);
+    Whole p;
+    p.seq = seq, p.first = first, p.r0 = r0, p.r_end = r_end, p.pos = pos;
+    const int last = min(r0 + rows, r_end) - 1;
+    p.t0 = 0, p.t1 = Tiles(window, sinks, pos + over_rep(r0), pos + over_rep(last)).all;
+    p.rec = -1;
+    p.groups = (last - r0) / 16 + 1;
+    p.tile = costs.tile(p.groups), p.way = free_way ? 0 : costs.way(p.groups);
+    return p;
+}
+
+// The largest of a wave, in every lane.
+__device__ __forceinline__ uint32_t wave_most(uint32_t v) {
+    v = max(v, static_cast<uint32_t>(dpp_or_own<kDppXor1>(v)));
+    v = max(v, static_cast<uint32_t>(dpp_or_own<kDppXor2>(v)));
+    v = max(v, static_cast<uint32_t>(dpp_or_own<kDppHalfMirror>(v)));
+    v = max(v, static_cast<uint32_t>(dpp_or_own<kDppMirror>(v)));
+    v = max(v, static_cast<uint32_t>(dpp_or_own<kDppBcast15>(v)));
+    v = max(v, static_cast<uint32_t>(dpp_or_own<kDppBcast31>(v)));
+    return __builtin_amdgcn_readlane(static_cast<int>(v), 63);
+}
+
 template <int T, int SEQS, int NQ>
 __device__ void make_plan(const shv_attn_paged_args &a, const Plan &plan, PlanSmem<T, SEQS, NQ> &sm) {
     const int tid = threadIdx.x, rep = a.n_head / a.n_head_kv;
-    const Costs costs = costs_of(a.head_dim);
     uint32_t nq = 0;
     for (int s0 = 0; s0 < a.n_seq; s0 += T) {
         const int s = s0 + tid;
@@ -146,42 +187,37 @@ __device__ void make_plan(const shv_attn_paged_args &a, const Plan &plan, PlanSm
     if (tid == 0) sm.most = sm.most_way = 0;
     if (tid < 64) sm.bucket[tid] = 0;
     __syncthreads();
-    // query block i as a piece of all its tiles; what a tile of it costs, and its way in and out (which the first one's block has in any case)
-    struct Whole : Piece {
-        uint32_t tile, way, groups;
+    const auto whole_of = [&](uint32_t i, int seq) {
+        return whole_block(a.window, a.sinks, a.head_dim, plan.rows, plan.rep_magic, seq, sm.first[seq], sm.n[seq] * rep, sm.pos[seq], static_cast<int>(i - sm.q0[seq]) * plan.rows, i == 0);
     };
-    const auto whole = [&](uint32_t i) {
-        Whole p;
-        p.seq = last_not_above(sm.q0, a.n_seq, i);
-        p.first = sm.first[p.seq], p.pos = sm.pos[p.seq], p.r_end = sm.n[p.seq] * rep;
-        p.r0 = static_cast<int>(i - sm.q0[p.seq]) * plan.rows;
-        const uint32_t last = min(p.r0 + plan.rows, p.r_end) - 1;
-        p.t0 = 0, p.t1 = Tiles(a.window, a.sinks, p.pos + static_cast<uint32_t>(p.r0) / static_cast<uint32_t>(rep), p.pos + last / static_cast<uint32_t>(rep)).all;
-        p.rec = -1;
-        p.groups = (last - p.r0) / 16 + 1;
-        p.tile = costs.tile(p.groups), p.way = i == 0 ? 0 : costs.way(p.groups);
-        return p;
-    };
+    const auto whole = [&](uint32_t i) { return whole_of(i, sm.of[i] & ((1 << kSeqBits) - 1)); };
     nq = min(nq, static_cast<uint32_t>(min(plan.most_q, NQ)));
-    uint32_t total = 0;
+    uint32_t total = 0, most = 0, most_way = 0;
     for (uint32_t i0 = 0; i0 < nq; i0 += T) {
         uint32_t v[1] = {0}, all[1];
         if (i0 + tid < nq) {
-            const Whole p = whole(i0 + tid);
+            const int seq = last_not_above(sm.q0, a.n_seq, i0 + tid);
+            sm.of[i0 + tid] = seq;
+            const Whole p = whole_of(i0 + tid, seq);
             v[0] = p.way + min(static_cast<uint64_t>(p.t1) * p.tile, static_cast<uint64_t>(kFull / 2));
-            atomicMax(&sm.most, v[0]);
-            atomicMax(&sm.most_way, static_cast<uint32_t>(costs.way(p.groups)));
+            most = max(most, v[0]), most_way = max(most_way, p.way);
         }
         block_scan<T, 1>(v, all, sm.waves);
         if (i0 + tid < nq) sm.p[i0 + tid] = add_up_to(total, v[0]);
         total = add_up_to(total, all[0]);
     }
+    most = wave_most(most), most_way = wave_most(most_way);
+    if ((tid & 63) == 0) {
+        atomicMax(&sm.most, most);
+        atomicMax(&sm.most_way, most_way);
+    }
     __syncthreads();
-    const uint32_t most = sm.most, slots = plan.slots;
-    const uint32_t share = max((total + slots - 1) / slots, static_cast<uint32_t>(kLeast * costs.few));
+    most = sm.most, most_way = sm.most_way;
+    const uint32_t slots = plan.slots;
+    const uint32_t share = max((total + slots - 1) / slots, static_cast<uint32_t>(kLeast * costs_of(a.head_dim).few));
     // whole query blocks take as long as the longest, or as so many of the mean size one behind the other; a cut costs another way in and out, and the records' join
     const uint32_t rounds = (nq + slots - 1) / slots;
-    const bool cut = total < kFull && max(most, nq > 0 ? total / nq * rounds : 0u) > share + sm.most_way + sm.most_way / 2;
+    const bool cut = total < kFull && max(most, nq > 0 ? total / nq * rounds : 0u) > share + most_way + most_way / 2;
     if (!cut) {
         for (int pass = 0; pass < 2; pass++) {
             for (uint32_t i = tid; i < nq; i += T) {
@@ -231,7 +267,7 @@ __device__ void make_plan(const shv_attn_paged_args &a, const Plan &plan, PlanSm
         block_scan<T, 3>(v, all, sm.waves);
         if (i < nq) {
             const uint32_t at = before[0] + v[0], rec = before[1] + v[1];
-            sm.at[i] = at;
+            sm.of[i] |= at << kSeqBits;
             sm.rec[i] = n > 1 ? static_cast<int>(rec) : -1;
             if (n > 1) {
                 for (uint32_t g = 0; g < p.groups; g++)
@@ -244,40 +280,35 @@ __device__ void make_plan(const shv_attn_paged_args &a, const Plan &plan, PlanSm
         before[0] += all[0], before[1] += all[1], before[2] += all[2];
     }
     __syncthreads();
-    // the query block and which of its pieces that begin at or behind cut c
+    // the query block and which of its pieces that begin at or behind cut c; i = nq: none
     const auto piece_at = [&](uint32_t c, uint32_t &i, uint32_t &k) {
         i = last_not_above(sm.p, nq, c * share);
+        k = 0;
         const Whole p = whole(i);
         const uint32_t x = c * share - sm.p[i];
-        k = 0;
-        if (x <= p.way) return p;
+        if (x <= p.way) return;
         if (x > p.way + (p.t1 - 1) * p.tile) i++;
         else k = c - first_cut(i, p);
-        return p;
     };
+    static_assert(kMaxSlots <= T, "a block a thread");
+    const uint32_t b = tid;
+    uint32_t i = nq, k = 0;
+    if (b < blocks) {
+        piece_at(b, i, k);
+        sm.begins[b] = i < nq ? (sm.of[i] >> kSeqBits) + k : before[0];
+    }
+    if (tid == 0) sm.begins[blocks] = before[0];
+    __syncthreads();
+    // neighbouring blocks lie on one die
     const uint32_t dies = plan.dies, per = (blocks + dies - 1) / dies;
     for (uint32_t slot = tid; slot < static_cast<uint32_t>(plan.most_blocks); slot += T) {
-        // neighbouring blocks lie on one die
-        const uint32_t row = slot / dies, b = (slot - row * dies) * per + row;
-        uint32_t i = 0, k = 0, at = 0, end = 0;
-        Whole p;
-        if (row < per && b < blocks) {
-            p = piece_at(b, i, k);
-            at = end = i < nq ? sm.at[i] + k : before[0];
-            if (i < nq) {
-                if (k == 0) p = whole(i);
-                uint32_t i2, k2;
-                piece_at(b + 1, i2, k2);
-                end = b + 1 < blocks && i2 < nq ? sm.at[i2] + k2 : before[0];
-            }
-        }
-        if (at == end) {
-            plan.blocks[slot].more = -1;
-            continue;
-        }
-        p = piece_of(i, p, k);
+        const uint32_t row = slot / dies, of = (slot - row * dies) * per + row;
+        if (row >= per || of >= blocks || sm.begins[of] == sm.begins[of + 1]) plan.blocks[slot].more = -1;
+    }
+    if (b < blocks && sm.begins[b] != sm.begins[b + 1]) {
+        Whole p = piece_of(i, whole(i), k);
         p.rec = sm.rec[i] < 0 ? -1 : sm.rec[i] + static_cast<int>(k);
-        plan.blocks[slot] = Block{p, static_cast<int>(end - at - 1), static_cast<int>(at + 1), {}};
+        plan.blocks[b % per * dies + b / per] = Block{p, sm.begins[b + 1] - sm.begins[b] - 1, sm.begins[b] + 1, {}};
     }
     if (tid == 0) *plan.n_joins = before[2];
 }
@@ -325,9 +356,15 @@ __global__ __launch_bounds__(256) void paged_cells_kernel(shv_attn_paged_args a,
 }
 
 // ---- attention ----------------------------------------------------------------------------------
-// A tile in LDS: 1 KB chunks that a wave reads 16 bytes a lane.  K chunk T * (D/32) + i: lane (n, q) = cell 8 (n / 4) + 4 T + n % 4, dims
-// 32 i + 8 q ..; V chunk db behind them: lane (n, q) = dim 16 db + n, cells 8 q ...  After S^T = K Q^T lane (n, q) then holds query row n's
+// A tile in LDS, as loads of 1 KB leave it.  K cell by cell, so that a load takes whole rows of a head (FIGURE); the 16-byte pieces of a cell's row lie in the order
+// piece ^ turn(cell), so that the lanes of a read, (n, q) = cell 8 (n / 4) + 4 T + n % 4, piece 4 i + q, ask for different banks, whichever sixteen of them go
+// together.  V chunk db behind them: lane (n, q) = dim 16 db + n, cells 8 q ...  After S^T = K Q^T lane (n, q) then holds query row n's
 // scores of cells 8 q + 4 T + 0..3, T = 0, 1: the eight cells of its operand of the second product.
+template <int D>
+__device__ __forceinline__ int turn_of(int cell) {
+    const int n = cell >> 3 << 2 | (cell & 3);
+    return D == 64 ? n >> 1 : n;  // (two cells' rows of 64 dims lie in one line of banks)
+}
 template <int D>
 struct AttnSmem {
     static constexpr int kStage = D / 8 * kChunk, kStages = kRingBytes / kStage;
@@ -352,7 +389,8 @@ struct Unit {
     int kvh, rep;
     size_t kvw;
     const uint16_t *cells;  // the KV head's keys or values, whichever the wave loads
-    uint32_t from;          // of a lane's first chunk in a tile
+    uint32_t from[2];       // where a lane's loads begin in a tile, of even and of odd ones
+    uint32_t step;          // and how far the next of the same kind is behind it
     bool keys;
 };
 
@@ -366,23 +404,30 @@ __device__ __forceinline__ void store_8(float *to, const float (&from)[8]) {
     *reinterpret_cast<float4 *>(to + 4) = make_float4(from[4], from[5], from[6], from[7]);
 }
 
+// Values as two halves, the large one cut off and not rounded (two in one instruction): the small one holds the rest either way, to 2^-22 of the value, and is rounded to
+// nearest, so that what many cells lose cancels.
+__device__ __forceinline__ void to_halves(const float (&x)[8], half8_t &hi, half8_t &lo) {
+#pragma unroll
+    for (int e = 0; e < 8; e += 2) {
+        const half2_t h = __builtin_bit_cast(half2_t, __builtin_amdgcn_cvt_pkrtz(x[e], x[e + 1]));
+        hi[e] = h[0], hi[e + 1] = h[1];
+        lo[e] = static_cast<_Float16>(fmaf(static_cast<float>(h[0]), -1.f, x[e])), lo[e + 1] = static_cast<_Float16>(fmaf(static_cast<float>(h[1]), -1.f, x[e + 1]));
+    }
+}
+
 // The rotation of a lane's dims where the two of a pair are 32 H apart, in one lane.
 template <int H, int KI>
-__device__ __forceinline__ void turn_in_lane(float (&x)[KI][8], const float *turn, int rope_dims, int dim0) {
+__device__ __forceinline__ void turn_in_lane(float (&x)[KI][8], const float (&c)[KI / 2][8], const float (&s)[KI / 2][8], int rope_dims) {
     if constexpr (2 * H <= KI) {
         if (rope_dims != 64 * H) return;
 #pragma unroll
-        for (int i = 0; i < H; i++) {
-            float c[8], s[8];
-            load_8(c, turn + 32 * i + dim0);
-            load_8(s, turn + 32 * (H + i) + dim0);
+        for (int i = 0; i < H; i++)
 #pragma unroll
             for (int t = 0; t < 8; t++) {
                 const float a = x[i][t], b = x[i + H][t];
-                x[i][t] = fmaf(-b, s[t], a * c[t]);
-                x[i + H][t] = fmaf(a, s[t], b * c[t]);
+                x[i][t] = fmaf(-b, s[i][t], a * c[i][t]);
+                x[i + H][t] = fmaf(a, s[i][t], b * c[i][t]);
             }
-        }
     }
 }
 
@@ -392,6 +437,7 @@ __device__ __forceinline__ void run_piece(const shv_attn_paged_args &a, const Pl
     constexpr int KI = D / 32, DB = D / 16;
     constexpr int kPer = D / 8 / kWaves;  // chunks of a tile a wave asks for
     constexpr int kStages = AttnSmem<D>::kStages, kRounds = kStages / TP;  // rounds of TP tiles in the ring: one is multiplied, the others are on their way
+    constexpr int kBatch = 4 / G;
     static_assert(G == 1 || TP == 1, "waves that share a group have one");
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int n = lane & 15, q = lane >> 4, rep = unit.rep, kvh = unit.kvh;
@@ -399,8 +445,7 @@ __device__ __forceinline__ void run_piece(const shv_attn_paged_args &a, const Pl
     const int r0 = piece.r0 + 16 * G * (wave / TP), r_end = piece.r_end;
     const int last = min(piece.r0 + plan.rows, r_end) - 1;
     const bool working = r0 <= last;
-    const int lo = piece.pos + static_cast<int>(static_cast<uint32_t>(piece.r0) / static_cast<uint32_t>(rep));
-    const int hi = piece.pos + static_cast<int>(static_cast<uint32_t>(last) / static_cast<uint32_t>(rep));  // the block's rows' positions
+    const int lo = piece.pos + plan.over_rep(piece.r0), hi = piece.pos + plan.over_rep(last);  // the block's rows' positions
     const Tiles tiles(a.window, a.sinks, lo, hi);
     const float c2 = 1.44269504088896f / sqrtf(static_cast<float>(D));
     int my_pos[G];  // (a row that is not there is the last one again, and dropped)
@@ -427,24 +472,39 @@ __device__ __forceinline__ void run_piece(const shv_attn_paged_args &a, const Pl
             char *to = sm.ring[j & (kStages - 1)] + (wave * kPer) * kChunk;
 #pragma unroll
             for (int u = 0; u < kPer; u++)
-                __builtin_amdgcn_raw_ptr_buffer_load_lds(bytes, (lds_ptr_t)(to + u * kChunk), 16, unit.from, u * (unit.keys ? 64 : 1024), 0, 0);
+                __builtin_amdgcn_raw_ptr_buffer_load_lds(bytes, (lds_ptr_t)(to + u * kChunk), 16, unit.from[u & 1], u / 2 * unit.step, 0, 0);
         }
     };
+    const int cell_of = 8 * (n >> 2) + (n & 3), key_at = cell_of * 2 * D + (q ^ turn_of<D>(cell_of)) * 16;
     // ---- queries: lane (n, q) holds dims 32 i + 8 q .. of its row from the load to the operand ----
     int rope_dims = a.rope_dims, dim0 = 8 * q;
     asm volatile("" : "+s"(rope_dims), "+v"(dim0));  // (what follows from them is formed here and not once for all pieces, which registers do not hold)
     float x[G][KI][8];
-    const float *turn[G];
+    const bool by_lds = rope_dims % 64 != 0 || rope_dims == 192;  // a rotated pair's dims lie in two lanes: they meet in the ring, before any tile is asked for
+    float gamma[KI][8], cosines[G][KI / 2][8], sines[G][KI / 2][8];
 #pragma unroll
     for (int g = 0; g < G; g++) {
-        const int mine = min(r0 + 16 * g + n, last), row = static_cast<int>(static_cast<uint32_t>(mine) / static_cast<uint32_t>(rep));
+        const int mine = min(r0 + 16 * g + n, last), row = plan.over_rep(mine);
         my_pos[g] = piece.pos + row;
-        turn[g] = a.rope + static_cast<size_t>(my_pos[g]) * rope_dims;
         const float *src = a.qkv + static_cast<size_t>(piece.first + row) * a.qkv_stride + static_cast<size_t>(kvh * rep + mine - row * rep) * 2 * D + dim0;
 #pragma unroll
         for (int i = 0; i < KI; i++) load_8(x[g][i], src + 32 * i);
     }
-    const bool by_lds = rope_dims % 64 != 0 || rope_dims == 192;  // a rotated pair's dims lie in two lanes: they meet in the ring, before any tile is asked for
+#pragma unroll
+    for (int i = 0; i < KI; i++) load_8(gamma[i], a.q_norm + 32 * i + dim0);
+    if (!by_lds) {
+        // (loads complete in order: all that the queries need goes out before the tiles do)
+#pragma unroll
+        for (int g = 0; g < G; g++) {
+            const float *turn = a.rope + static_cast<size_t>(my_pos[g]) * rope_dims + dim0;
+#pragma unroll
+            for (int i = 0; i < KI / 2; i++)
+                if (64 * i < rope_dims) {
+                    load_8(cosines[g][i], turn + 32 * i);
+                    load_8(sines[g][i], turn + rope_dims / 2 + 32 * i);
+                }
+        }
+    }
     const int early = min(rounds, kRounds - 1);
     if (!by_lds)
         for (int r = 0; r < early; r++) ask(r);
@@ -458,15 +518,12 @@ __device__ __forceinline__ void run_piece(const shv_attn_paged_args &a, const Pl
         const float sc = __builtin_amdgcn_rsqf(fmaf(sum_over_q(ss), 1.f / static_cast<float>(D), a.eps));
 #pragma unroll
         for (int i = 0; i < KI; i++) {
-            float gamma[8];
-            load_8(gamma, a.q_norm + 32 * i + dim0);
 #pragma unroll
-            for (int t = 0; t < 8; t++) x[g][i][t] *= sc * gamma[t];
-            if (i % 4 == 3) __builtin_amdgcn_sched_barrier(0);  // (not all loads at once: registers are short)
+            for (int t = 0; t < 8; t++) x[g][i][t] *= sc * gamma[i][t];
         }
-        turn_in_lane<1>(x[g], turn[g], rope_dims, dim0);
-        turn_in_lane<2>(x[g], turn[g], rope_dims, dim0);
-        turn_in_lane<4>(x[g], turn[g], rope_dims, dim0);
+        turn_in_lane<1>(x[g], cosines[g], sines[g], rope_dims);
+        turn_in_lane<2>(x[g], cosines[g], sines[g], rope_dims);
+        turn_in_lane<4>(x[g], cosines[g], sines[g], rope_dims);
     }
     if (by_lds) {
         // (loops, and pairs turned where they lie: this path is for the layouts that are rare, and the instruction cache is shared with the one that is not)
@@ -499,12 +556,7 @@ __device__ __forceinline__ void run_piece(const shv_attn_paged_args &a, const Pl
 #pragma unroll
     for (int g = 0; g < G; g++)
 #pragma unroll
-        for (int i = 0; i < KI; i++)
-#pragma unroll
-            for (int t = 0; t < 8; t++) {
-                qh[g][i][t] = static_cast<_Float16>(x[g][i][t]);
-                ql[g][i][t] = static_cast<_Float16>(fmaf(static_cast<float>(qh[g][i][t]), -1.f, x[g][i][t]));
-            }
+        for (int i = 0; i < KI; i++) to_halves(x[g][i], qh[g][i], ql[g][i]);
     __builtin_amdgcn_sched_barrier(0);
     float4_t o[G][DB];
     float m_run[G], l_run[G];  // of the scores as they are, before their scale; the sums of a lane's own cells
@@ -526,6 +578,9 @@ __device__ __forceinline__ void run_piece(const shv_attn_paged_args &a, const Pl
         const int c0 = tiles.at(piece.t0 + j) * kTile;
         uint32_t seen[G];  // which of the lane's eight cells its query row sees
         const bool part = c0 + kTile - 1 > lo || (a.window > 0 && c0 + kTile - 1 >= a.sinks && c0 <= hi - a.window);
+        int first_cell = lane;
+        asm volatile("" : "+v"(first_cell));  // (here and in what follows: what is seldom needed is not formed for all tiles, which registers do not hold)
+        first_cell = (first_cell >> 4) * 8;
 #pragma unroll
         for (int g = 0; g < G; g++) {
             seen[g] = 0xFF;
@@ -533,35 +588,40 @@ __device__ __forceinline__ void run_piece(const shv_attn_paged_args &a, const Pl
                 seen[g] = 0;
 #pragma unroll
                 for (int e = 0; e < 8; e++) {
-                    const int c = c0 + 8 * q + e;
+                    const int c = c0 + first_cell + e;
                     seen[g] |= c <= my_pos[g] && (a.window == 0 || c < a.sinks || c > my_pos[g] - a.window) ? 1u << e : 0u;
                 }
             }
             saw |= seen[g] != 0 ? 1u << g : 0u;
         }
         const char *vt = kt + 2 * KI * kChunk;
-        // operands come from LDS four reads ahead of the products that use them
+        // operands come from LDS eight products ahead of those that use them
         float4_t st[G][2], sl[G][2];
 #pragma unroll
         for (int g = 0; g < G; g++)
 #pragma unroll
             for (int T = 0; T < 2; T++) st[g][T] = sl[g][T] = float4_t{0.f, 0.f, 0.f, 0.f};
-        half8_t kb[2][4];
-        const auto read_k = [&](half8_t(&to)[4], int i) {
+        half8_t kb[2][kBatch];
+        int key0 = key_at;
+        asm volatile("" : "+v"(key0));
+        const auto read_k = [&](half8_t(&to)[kBatch], int i) {
 #pragma unroll
-            for (int e = 0; e < 4; e++) to[e] = *reinterpret_cast<const half8_t *>(kt + ((e & 1) * KI + 2 * i + (e >> 1)) * kChunk + lane * 16);
+            for (int e = 0; e < kBatch; e++) {
+                const int step = (kBatch * i + e) / 2;
+                to[e] = *reinterpret_cast<const half8_t *>(kt + (key0 ^ (step & 3) * 64) + (e & 1) * 8 * D + step / 4 * 256);
+            }
         };
         read_k(kb[0], 0);
 #pragma unroll
-        for (int i = 0; i < KI / 2; i++) {
-            if (i + 1 < KI / 2) read_k(kb[(i + 1) & 1], i + 1);
+        for (int i = 0; i < 2 * KI / kBatch; i++) {
+            if (i + 1 < 2 * KI / kBatch) read_k(kb[(i + 1) & 1], i + 1);
             __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-            for (int e = 0; e < 4; e++)
+            for (int e = 0; e < kBatch; e++)
 #pragma unroll
                 for (int g = 0; g < G; g++) {
-                    st[g][e & 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kb[i & 1][e], qh[g][2 * i + (e >> 1)], st[g][e & 1], 0, 0, 0);
-                    sl[g][e & 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kb[i & 1][e], ql[g][2 * i + (e >> 1)], sl[g][e & 1], 0, 0, 0);
+                    st[g][e & 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kb[i & 1][e], qh[g][(kBatch * i + e) / 2], st[g][e & 1], 0, 0, 0);
+                    sl[g][e & 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kb[i & 1][e], ql[g][(kBatch * i + e) / 2], sl[g][e & 1], 0, 0, 0);
                 }
         }
         float pv[G][8];
@@ -587,8 +647,10 @@ __device__ __forceinline__ void run_piece(const shv_attn_paged_args &a, const Pl
                 l_run[g] *= alpha;
                 m_run[g] = m_new;
                 float av[4];
+                int l = lane;
+                asm volatile("" : "+v"(l));
 #pragma unroll
-                for (int e = 0; e < 4; e++) av[e] = __shfl(alpha, 4 * q + e, 64);
+                for (int e = 0; e < 4; e++) av[e] = __shfl(alpha, (l >> 4) * 4 + e, 64);
 #pragma unroll
                 for (int db = 0; db < DB; db++)
 #pragma unroll
@@ -615,13 +677,16 @@ __device__ __forceinline__ void run_piece(const shv_attn_paged_args &a, const Pl
         }
         if (by_hand) {
             float *p = sm.p[wave];
+            int l = lane;
+            asm volatile("" : "+v"(l));
+            const int nn = l & 15, qq = l >> 4;
 #pragma unroll
             for (int g = 0; g < G; g++)
 #pragma unroll 1
                 for (int half = 0; half < 2; half++) {
-                    if ((q >> 1) == half) {
+                    if ((qq >> 1) == half) {
 #pragma unroll
-                        for (int e = 0; e < 8; e++) p[n * (kTile / 2) + 8 * (q & 1) + e] = seen[g] >> e & 1 ? pv[g][e] : -1.f;
+                        for (int e = 0; e < 8; e++) p[nn * (kTile / 2) + 8 * (qq & 1) + e] = seen[g] >> e & 1 ? pv[g][e] : -1.f;
                     }
                     __builtin_amdgcn_wave_barrier();
 #pragma unroll 1
@@ -629,10 +694,10 @@ __device__ __forceinline__ void run_piece(const shv_attn_paged_args &a, const Pl
                         const int c = kTile / 2 * half + i;
                         float w[4];
 #pragma unroll
-                        for (int e = 0; e < 4; e++) w[e] = p[(4 * q + e) * (kTile / 2) + i];
+                        for (int e = 0; e < 4; e++) w[e] = p[(4 * qq + e) * (kTile / 2) + i];
 #pragma unroll
                         for (int db = 0; db < DB; db++) {
-                            const float v = static_cast<float>(*reinterpret_cast<const _Float16 *>(vt + db * kChunk + (16 * (c >> 3) + n) * 16 + (c & 7) * 2));
+                            const float v = static_cast<float>(*reinterpret_cast<const _Float16 *>(vt + db * kChunk + (16 * (c >> 3) + nn) * 16 + (c & 7) * 2));
 #pragma unroll
                             for (int e = 0; e < 4; e++) o[g][db][e] = w[e] < 0.f ? o[g][db][e] : fmaf(w[e], v, o[g][db][e]);
                         }
@@ -641,45 +706,38 @@ __device__ __forceinline__ void run_piece(const shv_attn_paged_args &a, const Pl
                 }
             continue;
         }
-        // weights as two halves, the large one cut off and not rounded: the small one holds the rest either way, and is rounded to nearest, so that what
-        // many cells lose cancels
         half8_t ph[G], pl[G];
 #pragma unroll
-        for (int g = 0; g < G; g++)
+        for (int g = 0; g < G; g++) to_halves(pv[g], ph[g], pl[g]);
+        half8_t vb[2][kBatch];
 #pragma unroll
-            for (int e = 0; e < 8; e += 2) {
-                const half2_t h = __builtin_bit_cast(half2_t, __builtin_amdgcn_cvt_pkrtz(pv[g][e], pv[g][e + 1]));
-                const half2_t l = {static_cast<_Float16>(fmaf(static_cast<float>(h[0]), -1.f, pv[g][e])), static_cast<_Float16>(fmaf(static_cast<float>(h[1]), -1.f, pv[g][e + 1]))};
-                ph[g][e] = h[0]; ph[g][e + 1] = h[1];
-                pl[g][e] = l[0]; pl[g][e + 1] = l[1];
-            }
-        half8_t vb[2][4];
+        for (int e = 0; e < kBatch; e++) vb[0][e] = *reinterpret_cast<const half8_t *>(vt + e * kChunk + lane * 16);
 #pragma unroll
-        for (int e = 0; e < 4; e++) vb[0][e] = *reinterpret_cast<const half8_t *>(vt + e * kChunk + lane * 16);
+        for (int i = 0; i < DB / kBatch; i++) {
+            if (i + 1 < DB / kBatch) {
 #pragma unroll
-        for (int i = 0; i < DB / 4; i++) {
-            if (i + 1 < DB / 4) {
-#pragma unroll
-                for (int e = 0; e < 4; e++) vb[(i + 1) & 1][e] = *reinterpret_cast<const half8_t *>(vt + (4 * (i + 1) + e) * kChunk + lane * 16);
+                for (int e = 0; e < kBatch; e++) vb[(i + 1) & 1][e] = *reinterpret_cast<const half8_t *>(vt + (kBatch * (i + 1) + e) * kChunk + lane * 16);
             }
             __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
             for (int g = 0; g < G; g++)
 #pragma unroll
-                for (int e = 0; e < 4; e++) o[g][4 * i + e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ph[g], vb[i & 1][e], o[g][4 * i + e], 0, 0, 0);
+                for (int e = 0; e < kBatch; e++) o[g][kBatch * i + e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ph[g], vb[i & 1][e], o[g][kBatch * i + e], 0, 0, 0);
 #pragma unroll
             for (int g = 0; g < G; g++)
 #pragma unroll
-                for (int e = 0; e < 4; e++) o[g][4 * i + e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(pl[g], vb[i & 1][e], o[g][4 * i + e], 0, 0, 0);
+                for (int e = 0; e < kBatch; e++) o[g][kBatch * i + e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(pl[g], vb[i & 1][e], o[g][kBatch * i + e], 0, 0, 0);
         }
     }
     bool writes = working;
     if constexpr (TP > 1) {
         // the sums of a group's other waves, by way of the ring, which is free
-        static_assert(kWaves * (DB + 1) * 64 * 16 <= kRingBytes + (TP == 2 ? kRingBytes : 0), "half of the waves leave their sums");
-        float4_t *slot = reinterpret_cast<float4_t *>(sm.ring[0]) + (wave / 2) * (DB + 1) * 64 + lane;
+        constexpr int kOthers = kWaves / TP * (TP - 1);  // waves that leave theirs
+        static_assert(kOthers * (DB + 1) * kChunk <= kRingBytes, "they fit the ring");
+        float4_t *slots = reinterpret_cast<float4_t *>(sm.ring[0]) + wave / TP * (TP - 1) * (DB + 1) * 64 + lane;
         __syncthreads();
-        if (working && mine_of == 1) {
+        if (working && mine_of > 0) {
+            float4_t *slot = slots + (mine_of - 1) * (DB + 1) * 64;
 #pragma unroll
             for (int db = 0; db < DB; db++) slot[db * 64] = o[0][db];
             slot[DB * 64] = float4_t{m_run[0], l_run[0], __uint_as_float(saw), 0.f};
@@ -687,24 +745,31 @@ __device__ __forceinline__ void run_piece(const shv_attn_paged_args &a, const Pl
         __syncthreads();
         writes = working && mine_of == 0;
         if (writes) {
-            const float4_t of = slot[DB * 64];
-            const float m = fmaxf(m_run[0], of[0]);
-            const float f1 = m_run[0] == m ? 1.f : __builtin_amdgcn_exp2f((m_run[0] - m) * c2), f2 = of[0] == m ? 1.f : __builtin_amdgcn_exp2f((of[0] - m) * c2);
-            l_run[0] = f1 * l_run[0] + f2 * of[1];
-            m_run[0] = m;
-            saw |= __float_as_uint(of[2]);
-            float a1[4], a2[4];
+#pragma unroll 1
+            for (int k = 0; k < TP - 1; k++) {
+                const float4_t *slot = slots + k * (DB + 1) * 64;
+                const float4_t of = slot[DB * 64];
+                const float m = fmaxf(m_run[0], of[0]);
+                const float f1 = m_run[0] == m ? 1.f : __builtin_amdgcn_exp2f((m_run[0] - m) * c2), f2 = of[0] == m ? 1.f : __builtin_amdgcn_exp2f((of[0] - m) * c2);
+                l_run[0] = f1 * l_run[0] + f2 * of[1];
+                m_run[0] = m;
+                saw |= __float_as_uint(of[2]);
+                float a1[4], a2[4];
 #pragma unroll
-            for (int e = 0; e < 4; e++) a1[e] = __shfl(f1, 4 * q + e, 64), a2[e] = __shfl(f2, 4 * q + e, 64);
+                for (int e = 0; e < 4; e++) a1[e] = __shfl(f1, 4 * q + e, 64), a2[e] = __shfl(f2, 4 * q + e, 64);
 #pragma unroll
-            for (int db = 0; db < DB; db++) {
-                const float4_t other = slot[db * 64];
+                for (int db = 0; db < DB; db++) {
+                    const float4_t other = slot[db * 64];
 #pragma unroll
-                for (int e = 0; e < 4; e++) o[0][db][e] = a1[e] * o[0][db][e] + a2[e] * other[e];
+                    for (int e = 0; e < 4; e++) o[0][db][e] = a1[e] * o[0][db][e] + a2[e] * other[e];
+                }
             }
         }
     }
     if (writes) {
+        int l = lane;
+        asm volatile("" : "+v"(l));
+        const int nn = l & 15, qq = l >> 4;
 #pragma unroll
         for (int g = 0; g < G; g++) {
             const int rg = r0 + 16 * g;
@@ -712,29 +777,29 @@ __device__ __forceinline__ void run_piece(const shv_attn_paged_args &a, const Pl
             float sum = sum_over_q(l_run[g]);
             // a row whose scores are all -infinity has no weights; one that sees nothing has a sum of zero
             const uint64_t saws = __ballot(saw >> g & 1);
-            if (m_run[g] == -INFINITY && ((saws >> n) & 0x0001000100010001ull) != 0) sum = __int_as_float(0x7fc00000);
+            if (m_run[g] == -INFINITY && ((saws >> nn) & 0x0001000100010001ull) != 0) sum = __int_as_float(0x7fc00000);
             if (piece.rec < 0) {
                 float lr[4];
 #pragma unroll
-                for (int i = 0; i < 4; i++) lr[i] = __shfl(sum == 0.f ? 0.f : 1.f / sum, 4 * q + i, 64);
+                for (int i = 0; i < 4; i++) lr[i] = __shfl(sum == 0.f ? 0.f : 1.f / sum, 4 * qq + i, 64);
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
-                    const int r = rg + 4 * q + i, row = static_cast<int>(static_cast<uint32_t>(r) / static_cast<uint32_t>(rep));
+                    const int r = rg + 4 * qq + i, row = plan.over_rep(r);
                     if (r > last) continue;
                     float *dst = a.out + (static_cast<size_t>(piece.first + row) * a.n_head + kvh * rep + r - row * rep) * D;
 #pragma unroll
-                    for (int db = 0; db < DB; db++) dst[16 * db + n] = o[g][db][i] * lr[i];
+                    for (int db = 0; db < DB; db++) dst[16 * db + nn] = o[g][db][i] * lr[i];
                 }
             } else {
                 const size_t base = (static_cast<size_t>(piece.rec) * a.n_head_kv + kvh) * plan.slot_rows + rg - piece.r0;
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
-                    if (rg + 4 * q + i > last) continue;
-                    float *rec = plan.sums + (base + 4 * q + i) * D;
+                    if (rg + 4 * qq + i > last) continue;
+                    float *rec = plan.sums + (base + 4 * qq + i) * D;
 #pragma unroll
-                    for (int db = 0; db < DB; db++) rec[16 * db + n] = o[g][db][i];
+                    for (int db = 0; db < DB; db++) rec[16 * db + nn] = o[g][db][i];
                 }
-                if (q == 0 && rg + n <= last) plan.of[base + n] = make_float2(m_run[g], sum);
+                if (qq == 0 && rg + nn <= last) plan.of[base + nn] = make_float2(m_run[g], sum);
             }
         }
     }
@@ -745,7 +810,7 @@ __device__ __forceinline__ void run_piece(const shv_attn_paged_args &a, const Pl
 // allows it, so that its L2 holds their cells: die x has the heads x % g, x % g + g, .. for g the power of two in their number, up to 8.
 template <int D>
 __global__ __launch_bounds__(64 * kWaves, 2) void paged_attn_kernel(shv_attn_paged_args a, Plan plan) {
-    constexpr int KI = D / 32, kPer = D / 8 / kWaves;
+    constexpr int kPer = D / 8 / kWaves;
     extern __shared__ __align__(16) char raw[];
     AttnSmem<D> &sm = *reinterpret_cast<AttnSmem<D> *>(raw);
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -760,15 +825,22 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_attn_kernel(shv_attn_pag
     unit.kvh = die % g + g * (nth - turn * plan.heads), unit.rep = a.n_head / a.n_head_kv;
     unit.kvw = static_cast<size_t>(a.n_head_kv) * D;
     unit.keys = wave < kWaves / 2;
-    const int first = (unit.keys ? wave : wave - kWaves / 2) * kPer;  // of the wave's chunks among K's or V's
-    unit.from = unit.keys ? static_cast<uint32_t>((8 * (n >> 2) + 4 * (first / KI) + (n & 3)) * unit.kvw + 32 * (first % KI) + 8 * q) * 2
-                          : static_cast<uint32_t>((16 * first + n) * kTile + 8 * q) * 2;
+    // loads u of the wave: of keys 1024 / 2 D cells each, of values 16 dims
+    const int mine = unit.keys ? wave : wave - kWaves / 2;
+    constexpr int kPieces = D / 8, kCells = 64 / kPieces;
+#pragma unroll
+    for (int u = 0; u < 2; u++) {
+        const int cell = (mine * kPer + u) * kCells + lane / kPieces;
+        unit.from[u] = unit.keys ? static_cast<uint32_t>(cell * unit.kvw) * 2 + ((lane % kPieces) ^ turn_of<D>(cell)) * 16 : static_cast<uint32_t>((16 * (mine * kPer + u) + n) * kTile + 8 * q) * 2;
+    }
+    unit.step = unit.keys ? 2 * kCells * static_cast<uint32_t>(unit.kvw) * 2 : 2 * kChunk;
     unit.cells = unit.keys ? static_cast<const uint16_t *>(a.kpages) + unit.kvh * D : static_cast<const uint16_t *>(a.vpages) + static_cast<size_t>(unit.kvh) * D * kTile;
     for (int k = 0; k < pieces; k++) {
         const Piece piece = *at;
         at = k == 0 ? plan.pieces + block->at : at + 1;
         const int groups = (min(piece.r_end - piece.r0, plan.rows) + 15) / 16;
-        if (groups <= kWaves / 2) run_piece<D, 1, 2>(a, plan, piece, unit, sm);
+        if (kManyTurns<D> > 2 && groups <= kWaves / kManyTurns<D>) run_piece<D, 1, kManyTurns<D>>(a, plan, piece, unit, sm);
+        else if (groups <= kWaves / 2) run_piece<D, 1, 2>(a, plan, piece, unit, sm);
         else run_piece<D, kGroups<D>, 1>(a, plan, piece, unit, sm);
     }
 }
@@ -837,7 +909,7 @@ __global__ __launch_bounds__(256) void paged_join_kernel(shv_attn_paged_args a, 
             float4_t y;
 #pragma unroll
             for (int e = 0; e < 4; e++) y[e] = den == 0.f ? 0.f : num[e] / den;
-            const int t = r / rep;
+            const int t = plan.over_rep(r);
             *(reinterpret_cast<float4_t *>(a.out + (static_cast<size_t>(join.first + t) * a.n_head + kvh * rep + r - t * rep) * D) + lane % kLanes) = y;
         }
     }
@@ -862,6 +934,8 @@ uintptr_t lay_out(const shv_ctx *ctx, const shv_attn_paged_args &a, Plan &plan) 
     const int rep = a.n_head / a.n_head_kv, D = a.head_dim;
     plan.slots = ctx->prop.multiProcessorCount / a.n_head_kv;
     if (plan.slots < 1) plan.slots = 1;
+    if (plan.slots > kMaxSlots) plan.slots = kMaxSlots;
+    plan.rep_magic = rep == 1 ? 0 : static_cast<uint32_t>(((1ull << 32) + rep - 1) / rep);
     const int query_rows = a.max_rows * rep;
     plan.rows = rows_of(D);
     plan.most_q = (a.n_seq < a.max_rows ? a.n_seq : a.max_rows) + query_rows / plan.rows;

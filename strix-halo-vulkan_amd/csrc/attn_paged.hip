@@ -38,13 +38,11 @@ constexpr int kFewBlocks = 1024;  // query blocks up to which the plan is made i
 // both.
 template <int D>
 constexpr int kGroups = D == 256 ? 1 : 2;
-// Waves that share a group of few query rows, each with tiles of its own.
-#ifndef MT128
-#define MT128 4
-#define MT64 8
-#endif
+// Waves that share a group of few query rows, each with tiles of its own: a round of that many tiles costs one wait of the block's waves, and joining their sums the end of a
+// piece.  Of 128 dims 1 token behind 30000 takes 39.7 us with four and 41.5 with two, 96 in a window of 2048 the same; of 64 dims 48 tokens behind up to 6000 take 151 us with
+// eight, 145 with four and 153 with two, and one behind 900 20.2, 18.5 and 17.8.
 template <int D>
-constexpr int kManyTurns = D == 256 ? 2 : D == 128 ? MT128 : MT64;
+constexpr int kManyTurns = D == 256 ? 2 : 4;
 constexpr int rows_of(int D) { return 16 * kWaves * (D == 256 ? 1 : 2); }
 
 // A block's query rows of a sequence and a run of the tiles they look at.
@@ -115,14 +113,14 @@ struct Seq {
 };
 
 // ---- the plan: one block of T threads -----------------------------------------------------------
-// What a block's work costs, in tenths of a microsecond: a tile of few query rows the time in which memory delivers it, of many that of the products; a piece
-// its way in and out, and its rows' bytes.
+// What a block's work costs, in tenths of a microsecond: a tile of few query rows, by its block where memory has bandwidth to spare (few_least) and by memory where all units
+// ask for such tiles (few); one of many query rows by its products; a piece its way in and out, and its rows' bytes.
 struct Costs {
-    int few, group, piece, piece_group;
-    __host__ __device__ __forceinline__ int tile(int groups) const { return few > group * groups / 16 ? few : group * groups / 16; }
+    int few, few_least, group, piece, piece_group;
+    __host__ __device__ __forceinline__ int tile(int groups) const { return group * groups / 16; }
     __host__ __device__ __forceinline__ int way(int groups) const { return piece + piece_group * groups / 16; }
 };
-__host__ __device__ constexpr Costs costs_of(int D) { return D == 256 ? Costs{16, 39, 30, 128} : D == 128 ? Costs{9, 20, 30, 64} : Costs{5, 12, 30, 32}; }
+__host__ __device__ constexpr Costs costs_of(int D) { return D == 256 ? Costs{16, 12, 37, 90, 128} : D == 128 ? Costs{9, 8, 21, 60, 64} : Costs{5, 3, 12, 60, 32}; }
 
 // The query blocks of all sequences stand in a row, each with its cost, P their running sum.  Where they fill the chip evenly each is a block's own, those with the most
 // tiles first.  Otherwise block b takes what lies from b S to (b + 1) S in the row, S = all / blocks, so that all blocks have the same; a query block cut by that
@@ -144,7 +142,7 @@ struct PlanSmem {
 struct Whole : Piece {
     uint32_t tile, way, groups;
 };
-__device__ __forceinline__ Whole whole_block(int window, int sinks, int D, int rows, uint32_t rep_magic, int seq, int first, int r_end, int pos, int r0, bool free_way) {
+__device__ __forceinline__ Whole whole_block(int window, int sinks, int D, int rows, uint32_t rep_magic, int seq, int first, int r_end, int pos, int r0, bool free_way, uint32_t few) {
     const auto over_rep = [&](int r) { return rep_magic == 0 ? r : static_cast<int>(__umulhi(static_cast<uint32_t>(r), rep_magic)); };
     const Costs costs = costs_of(D);
     Whole p;
@@ -153,7 +151,7 @@ __device__ __forceinline__ Whole whole_block(int window, int sinks, int D, int r
     p.t0 = 0, p.t1 = Tiles(window, sinks, pos + over_rep(r0), pos + over_rep(last)).all;
     p.rec = -1;
     p.groups = (last - r0) / 16 + 1;
-    p.tile = costs.tile(p.groups), p.way = free_way ? 0 : costs.way(p.groups);
+    p.tile = max(static_cast<uint32_t>(costs.tile(p.groups)), few), p.way = free_way ? 0 : costs.way(p.groups);
     return p;
 }
 
@@ -187,18 +185,30 @@ __device__ void make_plan(const shv_attn_paged_args &a, const Plan &plan, PlanSm
     if (tid == 0) sm.most = sm.most_way = 0;
     if (tid < 64) sm.bucket[tid] = 0;
     __syncthreads();
+    const Costs costs = costs_of(a.head_dim);
+    uint32_t few = costs.few_least;
     const auto whole_of = [&](uint32_t i, int seq) {
-        return whole_block(a.window, a.sinks, a.head_dim, plan.rows, plan.rep_magic, seq, sm.first[seq], sm.n[seq] * rep, sm.pos[seq], static_cast<int>(i - sm.q0[seq]) * plan.rows, i == 0);
+        return whole_block(a.window, a.sinks, a.head_dim, plan.rows, plan.rep_magic, seq, sm.first[seq], sm.n[seq] * rep, sm.pos[seq], static_cast<int>(i - sm.q0[seq]) * plan.rows, i == 0, few);
     };
     const auto whole = [&](uint32_t i) { return whole_of(i, sm.of[i] & ((1 << kSeqBits) - 1)); };
     nq = min(nq, static_cast<uint32_t>(min(plan.most_q, NQ)));
+    // Tiles of few query rows, t of them, come as fast as memory gives them, few t / slots in all, or as their blocks take them beside those of many, whose cost is c:
+    // (few_least t + c) / slots.  Where the first is longer a tile costs what makes both alike.
+    uint32_t both[2] = {0, 0}, sums[2];
+    for (uint32_t i = tid; i < nq; i += T) {
+        const int seq = last_not_above(sm.q0, a.n_seq, i);
+        sm.of[i] = seq;
+        const Whole p = whole_of(i, seq);
+        const bool is_few = p.tile == few;
+        both[is_few] = add_up_to(both[is_few], is_few ? p.t1 : min(static_cast<uint64_t>(p.t1) * p.tile, static_cast<uint64_t>(kFull / 2)));
+    }
+    block_scan<T, 2>(both, sums, sm.waves);
+    if (sums[1] > 0) few = max(few, costs.few - min(sums[0] / sums[1], static_cast<uint32_t>(costs.few)));
     uint32_t total = 0, most = 0, most_way = 0;
     for (uint32_t i0 = 0; i0 < nq; i0 += T) {
         uint32_t v[1] = {0}, all[1];
         if (i0 + tid < nq) {
-            const int seq = last_not_above(sm.q0, a.n_seq, i0 + tid);
-            sm.of[i0 + tid] = seq;
-            const Whole p = whole_of(i0 + tid, seq);
+            const Whole p = whole(i0 + tid);
             v[0] = p.way + min(static_cast<uint64_t>(p.t1) * p.tile, static_cast<uint64_t>(kFull / 2));
             most = max(most, v[0]), most_way = max(most_way, p.way);
         }
@@ -214,7 +224,7 @@ __device__ void make_plan(const shv_attn_paged_args &a, const Plan &plan, PlanSm
     __syncthreads();
     most = sm.most, most_way = sm.most_way;
     const uint32_t slots = plan.slots;
-    const uint32_t share = max((total + slots - 1) / slots, static_cast<uint32_t>(kLeast * costs_of(a.head_dim).few));
+    const uint32_t share = max((total + slots - 1) / slots, static_cast<uint32_t>(kLeast * costs.few));
     // whole query blocks take as long as the longest, or as so many of the mean size one behind the other; a cut costs another way in and out, and the records' join
     const uint32_t rounds = (nq + slots - 1) / slots;
     const bool cut = total < kFull && max(most, nq > 0 ? total / nq * rounds : 0u) > share + most_way + most_way / 2;

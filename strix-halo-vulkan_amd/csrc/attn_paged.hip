@@ -4,12 +4,13 @@
 //     out_r = sum over them of softmax(q_r . k_c / sqrt(d)) v_c
 // q and k normed over a head and rotated at their positions.  Three launches:
 //   cells  the rows' keys and values into their cells, and, in a block of its own, the plan of the next;
-//   attn   a block takes one KV head and up to 128 query rows (256 of narrower heads; query row r of a sequence is head r % rep of its row r / rep), and a run of
+//   attn   a block takes one KV head and up to 64 query rows (128 of narrower heads; query row r of a sequence is head r % rep of its row r / rep), and a run of
 //          their tiles of 32 cells, on v_mfma_f32_16x16x32_f16:
 //              S^T = K Q^T   the cache's binary16 keys against the queries as two halves; a lane then holds eight cells of one query row, the operand
 //                            of the second product
 //              O  += P V     weights as two halves against values, which the cache holds by dim
-//          with a running maximum and sum.  Tiles go from memory to LDS past the registers, 96 KB ahead;
+//          with a running maximum and sum.  Tiles go from memory to LDS past the registers, and two blocks share a
+//          unit: while one begins a piece or ends it the other's tiles keep coming;
 //   join   the records of query rows whose tiles several blocks have shared.
 #include <atomic>
 
@@ -23,10 +24,12 @@ namespace {
 using namespace shv;
 
 constexpr int kTile = 32;  // cells of a tile of V
-constexpr int kWaves = 8;
 constexpr int kMaxSeqs = SHV_PAGE_MAX_SEQS;
 constexpr int kChunk = 64 * 16;
-constexpr int kRingBytes = 128 << 10;
+// Waves of a block: two of four share a unit, or one of eight has it (is_wide).  96 tokens in a window of 2048, 128 dims, take 170 us with two and 204 with one, 24 behind up to
+// 12000 147 and 169, a chunk of 512 among 23 tokens 235 and 275, 48 tokens of 64 dims behind up to 6000 101 and 144.
+constexpr int kWide = 8, kNarrow = 4;
+constexpr int ring_bytes(int waves) { return waves * (16 << 10); }
 // Weights are e^(s - m) 2^kLift, and m stands until a score is more than kSlack powers of two above it: up to 2^15.9, which the larger half holds, and down to
 // 2^-35 of the largest with the smaller half's last place, to which it is rounded.
 constexpr float kLift = 11.f, kSlack = 4.9f;
@@ -38,12 +41,11 @@ constexpr int kFewBlocks = 1024;  // query blocks up to which the plan is made i
 // both.
 template <int D>
 constexpr int kGroups = D == 256 ? 1 : 2;
-// Waves that share a group of few query rows, each with tiles of its own: a round of that many tiles costs one wait of the block's waves, and joining their sums the end of a
-// piece.  Of 128 dims 1 token behind 30000 takes 39.7 us with four and 41.5 with two, 96 in a window of 2048 the same; of 64 dims 48 tokens behind up to 6000 take 151 us with
-// eight, 145 with four and 153 with two, and one behind 900 20.2, 18.5 and 17.8.
-template <int D>
-constexpr int kManyTurns = D == 256 ? 2 : 4;
-constexpr int rows_of(int D) { return 16 * kWaves * (D == 256 ? 1 : 2); }
+// Waves that share a group of few query rows, each with tiles of its own, so that a round in the ring is 32 KB (64 in the wide block's): 24 tokens of 128 dims behind up to
+// 12000 take 147 us with two and 155 with one, 48 of 64 dims behind up to 6000 101 with two or four and 133 with one.
+template <int D, int WAVES>
+constexpr int kTurns = WAVES == kWide ? 2 : 256 / D;
+constexpr int rows_of(int D, int waves) { return 16 * waves * (D == 256 ? 1 : 2); }
 
 // A block's query rows of a sequence and a run of the tiles they look at.
 struct Piece {
@@ -74,7 +76,7 @@ struct Plan {
     float *sums;        // records: [record][KV head][slot_rows][D] unnormalised sums
     float2 *of;         // and their (maximum, sum)
     int slots;          // blocks a KV head that the chip holds at once
-    int rows;           // query rows of a block
+    int waves, rows;    // waves and query rows of a block
     int slot_rows;      // and of a record
     int most_blocks, most_q;
     int dies, heads;    // dies that share a KV head, and KV heads of a die (place)
@@ -120,12 +122,18 @@ struct Costs {
     __host__ __device__ __forceinline__ int tile(int groups) const { return group * groups / 16; }
     __host__ __device__ __forceinline__ int way(int groups) const { return piece + piece_group * groups / 16; }
 };
-__host__ __device__ constexpr Costs costs_of(int D) { return D == 256 ? Costs{16, 12, 37, 90, 128} : D == 128 ? Costs{9, 8, 21, 60, 64} : Costs{5, 3, 12, 60, 32}; }
+__host__ __device__ constexpr Costs wide_costs(int D) { return D == 256 ? Costs{16, 12, 37, 90, 128} : D == 128 ? Costs{9, 8, 21, 60, 64} : Costs{5, 3, 12, 60, 32}; }
+// (two narrow blocks share a unit)
+__host__ __device__ __forceinline__ Costs costs_of(int D, int waves) {
+    const Costs c = wide_costs(D);
+    const int by = kWide / waves;
+    return Costs{c.few * by, c.few_least * by, c.group * by, c.piece, c.piece_group};
+}
 
 // The query blocks of all sequences stand in a row, each with its cost, P their running sum.  Where they fill the chip evenly each is a block's own, those with the most
 // tiles first.  Otherwise block b takes what lies from b S to (b + 1) S in the row, S = all / blocks, so that all blocks have the same; a query block cut by that
 // leaves a record of each piece.
-constexpr int kSeqBits = 11, kMaxSlots = 256;  // blocks that the chip holds at once: a unit one
+constexpr int kSeqBits = 11, kMaxSlots = 512;  // blocks that the chip holds at once: a unit two
 static_assert(kMaxSeqs <= 1 << kSeqBits, "a sequence's number");
 template <int T, int SEQS, int NQ>
 struct PlanSmem {
@@ -142,9 +150,9 @@ struct PlanSmem {
 struct Whole : Piece {
     uint32_t tile, way, groups;
 };
-__device__ __forceinline__ Whole whole_block(int window, int sinks, int D, int rows, uint32_t rep_magic, int seq, int first, int r_end, int pos, int r0, bool free_way, uint32_t few) {
+__device__ __forceinline__ Whole whole_block(int window, int sinks, int D, int waves, int rows, uint32_t rep_magic, int seq, int first, int r_end, int pos, int r0, bool free_way, uint32_t few) {
     const auto over_rep = [&](int r) { return rep_magic == 0 ? r : static_cast<int>(__umulhi(static_cast<uint32_t>(r), rep_magic)); };
-    const Costs costs = costs_of(D);
+    const Costs costs = costs_of(D, waves);
     Whole p;
     p.seq = seq, p.first = first, p.r0 = r0, p.r_end = r_end, p.pos = pos;
     const int last = min(r0 + rows, r_end) - 1;
@@ -185,10 +193,10 @@ __device__ void make_plan(const shv_attn_paged_args &a, const Plan &plan, PlanSm
     if (tid == 0) sm.most = sm.most_way = 0;
     if (tid < 64) sm.bucket[tid] = 0;
     __syncthreads();
-    const Costs costs = costs_of(a.head_dim);
+    const Costs costs = costs_of(a.head_dim, plan.waves);
     uint32_t few = costs.few_least;
     const auto whole_of = [&](uint32_t i, int seq) {
-        return whole_block(a.window, a.sinks, a.head_dim, plan.rows, plan.rep_magic, seq, sm.first[seq], sm.n[seq] * rep, sm.pos[seq], static_cast<int>(i - sm.q0[seq]) * plan.rows, i == 0, few);
+        return whole_block(a.window, a.sinks, a.head_dim, plan.waves, plan.rows, plan.rep_magic, seq, sm.first[seq], sm.n[seq] * rep, sm.pos[seq], static_cast<int>(i - sm.q0[seq]) * plan.rows, i == 0, few);
     };
     const auto whole = [&](uint32_t i) { return whole_of(i, sm.of[i] & ((1 << kSeqBits) - 1)); };
     nq = min(nq, static_cast<uint32_t>(min(plan.most_q, NQ)));
@@ -300,12 +308,14 @@ __device__ void make_plan(const shv_attn_paged_args &a, const Plan &plan, PlanSm
         if (x > p.way + (p.t1 - 1) * p.tile) i++;
         else k = c - first_cut(i, p);
     };
-    static_assert(kMaxSlots <= T, "a block a thread");
-    const uint32_t b = tid;
-    uint32_t i = nq, k = 0;
-    if (b < blocks) {
-        piece_at(b, i, k);
-        sm.begins[b] = i < nq ? (sm.of[i] >> kSeqBits) + k : before[0];
+    constexpr int kBlocks = (kMaxSlots + T - 1) / T;  // of a thread
+    uint32_t i[kBlocks], k[kBlocks];
+#pragma unroll
+    for (int e = 0; e < kBlocks; e++) {
+        const uint32_t b = e * T + tid;
+        if (b >= blocks) break;
+        piece_at(b, i[e], k[e]);
+        sm.begins[b] = i[e] < nq ? (sm.of[i[e]] >> kSeqBits) + k[e] : before[0];
     }
     if (tid == 0) sm.begins[blocks] = before[0];
     __syncthreads();
@@ -315,9 +325,13 @@ __device__ void make_plan(const shv_attn_paged_args &a, const Plan &plan, PlanSm
         const uint32_t row = slot / dies, of = (slot - row * dies) * per + row;
         if (row >= per || of >= blocks || sm.begins[of] == sm.begins[of + 1]) plan.blocks[slot].more = -1;
     }
-    if (b < blocks && sm.begins[b] != sm.begins[b + 1]) {
-        Whole p = piece_of(i, whole(i), k);
-        p.rec = sm.rec[i] < 0 ? -1 : sm.rec[i] + static_cast<int>(k);
+#pragma unroll
+    for (int e = 0; e < kBlocks; e++) {
+        const uint32_t b = e * T + tid;
+        if (b >= blocks) break;
+        if (sm.begins[b] == sm.begins[b + 1]) continue;
+        Whole p = piece_of(i[e], whole(i[e]), k[e]);
+        p.rec = sm.rec[i[e]] < 0 ? -1 : sm.rec[i[e]] + static_cast<int>(k[e]);
         plan.blocks[b % per * dies + b / per] = Block{p, sm.begins[b + 1] - sm.begins[b] - 1, sm.begins[b] + 1, {}};
     }
     if (tid == 0) *plan.n_joins = before[2];
@@ -366,7 +380,8 @@ __global__ __launch_bounds__(256) void paged_cells_kernel(shv_attn_paged_args a,
 }
 
 // ---- attention ----------------------------------------------------------------------------------
-// A tile in LDS, as loads of 1 KB leave it.  K cell by cell, so that a load takes whole rows of a head (FIGURE); the 16-byte pieces of a cell's row lie in the order
+// A tile in LDS, as loads of 1 KB leave it.  K cell by cell, so that a load takes whole rows of a head (24 tokens of 128 dims behind up to
+// 12000: 175 us, and 181 where a load takes 64 bytes of sixteen rows); the 16-byte pieces of a cell's row lie in the order
 // piece ^ turn(cell), so that the lanes of a read, (n, q) = cell 8 (n / 4) + 4 T + n % 4, piece 4 i + q, ask for different banks, whichever sixteen of them go
 // together.  V chunk db behind them: lane (n, q) = dim 16 db + n, cells 8 q ...  After S^T = K Q^T lane (n, q) then holds query row n's
 // scores of cells 8 q + 4 T + 0..3, T = 0, 1: the eight cells of its operand of the second product.
@@ -375,11 +390,11 @@ __device__ __forceinline__ int turn_of(int cell) {
     const int n = cell >> 3 << 2 | (cell & 3);
     return D == 64 ? n >> 1 : n;  // (two cells' rows of 64 dims lie in one line of banks)
 }
-template <int D>
+template <int D, int WAVES>
 struct AttnSmem {
-    static constexpr int kStage = D / 8 * kChunk, kStages = kRingBytes / kStage;
+    static constexpr int kStage = D / 8 * kChunk, kStages = ring_bytes(WAVES) / kStage;
     char ring[kStages][kStage];
-    float p[kWaves][16 * kTile / 2];  // a wave's weights of half a tile, where its values are not all finite
+    float p[WAVES][16 * kTile / 2];  // a wave's weights of half a tile, where its values are not all finite
 };
 
 // Waits until no more than the youngest min(rounds, N) rounds' loads of a wave, PER each, are out: they complete in order.
@@ -400,7 +415,8 @@ struct Unit {
     size_t kvw;
     const uint16_t *cells;  // the KV head's keys or values, whichever the wave loads
     uint32_t from[2];       // where a lane's loads begin in a tile, of even and of odd ones
-    uint32_t step;          // and how far the next of the same kind is behind it
+    uint32_t step;          // how far the next of the same kind is behind it
+    uint32_t flip;          // and what the place of a key's pieces differs by, eight cells on
     bool keys;
 };
 
@@ -442,11 +458,11 @@ __device__ __forceinline__ void turn_in_lane(float (&x)[KI][8], const float (&c)
 }
 
 // One piece.  A wave takes G groups of query rows; TP waves share a group, each takes every TP-th tile, and their sums are joined in LDS at the end.
-template <int D, int G, int TP>
-__device__ __forceinline__ void run_piece(const shv_attn_paged_args &a, const Plan &plan, const Piece &piece, const Unit &unit, AttnSmem<D> &sm) {
+template <int D, int G, int TP, int WAVES>
+__device__ __forceinline__ void run_piece(const shv_attn_paged_args &a, const Plan &plan, const Piece &piece, const Unit &unit, AttnSmem<D, WAVES> &sm) {
     constexpr int KI = D / 32, DB = D / 16;
-    constexpr int kPer = D / 8 / kWaves;  // chunks of a tile a wave asks for
-    constexpr int kStages = AttnSmem<D>::kStages, kRounds = kStages / TP;  // rounds of TP tiles in the ring: one is multiplied, the others are on their way
+    constexpr int kPer = D / 8 / WAVES;  // chunks of a tile a wave asks for
+    constexpr int kStages = AttnSmem<D, WAVES>::kStages, kRounds = kStages / TP;  // rounds of TP tiles in the ring: one is multiplied, the others are on their way
     constexpr int kBatch = 4 / G;
     static_assert(G == 1 || TP == 1, "waves that share a group have one");
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -482,7 +498,7 @@ __device__ __forceinline__ void run_piece(const shv_attn_paged_args &a, const Pl
             char *to = sm.ring[j & (kStages - 1)] + (wave * kPer) * kChunk;
 #pragma unroll
             for (int u = 0; u < kPer; u++)
-                __builtin_amdgcn_raw_ptr_buffer_load_lds(bytes, (lds_ptr_t)(to + u * kChunk), 16, unit.from[u & 1], u / 2 * unit.step, 0, 0);
+                __builtin_amdgcn_raw_ptr_buffer_load_lds(bytes, (lds_ptr_t)(to + u * kChunk), 16, u / 2 * (1024 / D) & 8 ? unit.from[u & 1] ^ unit.flip : unit.from[u & 1], u / 2 * unit.step, 0, 0);
         }
     };
     const int cell_of = 8 * (n >> 2) + (n & 3), key_at = cell_of * 2 * D + (q ^ turn_of<D>(cell_of)) * 16;
@@ -539,7 +555,7 @@ __device__ __forceinline__ void run_piece(const shv_attn_paged_args &a, const Pl
         // (loops, and pairs turned where they lie: this path is for the layouts that are rare, and the instruction cache is shared with the one that is not)
         const uint32_t half = rope_dims / 2;
         float *rows = reinterpret_cast<float *>(sm.ring[0]) + wave * G * 16 * D;
-        static_assert(kWaves * G * 16 * D * 4 <= kRingBytes, "all rows in the ring");
+        static_assert(WAVES * G * 16 * D * 4 <= ring_bytes(WAVES), "all rows in the ring");
 #pragma unroll
         for (int g = 0; g < G; g++) {
             float *own = rows + (16 * g + n) * D + dim0;
@@ -581,7 +597,7 @@ __device__ __forceinline__ void run_piece(const shv_attn_paged_args &a, const Pl
         const int j = r * TP + mine_of;
         const char *kt = sm.ring[j & (kStages - 1)];
         wait_but<kPer * TP, kRounds - 2>(rounds - 1 - r);
-        asm volatile("s_barrier" ::: "memory");  // everyone's: this round is whole, and the stages of the one before are free
+        asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");  // everyone's: this round is whole, and the one before has been read
         const bool is = valid >> (j & (kStages - 1)) & 1;
         if (r + kRounds - 1 < rounds) ask(r + kRounds - 1);
         if (!is || !working) continue;
@@ -742,8 +758,8 @@ __device__ __forceinline__ void run_piece(const shv_attn_paged_args &a, const Pl
     bool writes = working;
     if constexpr (TP > 1) {
         // the sums of a group's other waves, by way of the ring, which is free
-        constexpr int kOthers = kWaves / TP * (TP - 1);  // waves that leave theirs
-        static_assert(kOthers * (DB + 1) * kChunk <= kRingBytes, "they fit the ring");
+        constexpr int kOthers = WAVES / TP * (TP - 1);  // waves that leave theirs
+        static_assert(kOthers * (DB + 1) * kChunk <= ring_bytes(WAVES), "they fit the ring");
         float4_t *slots = reinterpret_cast<float4_t *>(sm.ring[0]) + wave / TP * (TP - 1) * (DB + 1) * 64 + lane;
         __syncthreads();
         if (working && mine_of > 0) {
@@ -818,11 +834,11 @@ __device__ __forceinline__ void run_piece(const shv_attn_paged_args &a, const Pl
 
 // grid: 8 * ceil(blocks / dies) * heads, blocks of 8 waves.  Workgroups go to the eight dies in turn; a die's KV heads are the same ones throughout, where their number
 // allows it, so that its L2 holds their cells: die x has the heads x % g, x % g + g, .. for g the power of two in their number, up to 8.
-template <int D>
-__global__ __launch_bounds__(64 * kWaves, 2) void paged_attn_kernel(shv_attn_paged_args a, Plan plan) {
-    constexpr int kPer = D / 8 / kWaves;
+template <int D, int WAVES>
+__global__ __launch_bounds__(64 * WAVES, 2) void paged_attn_kernel(shv_attn_paged_args a, Plan plan) {
+    constexpr int kPer = D / 8 / WAVES;
     extern __shared__ __align__(16) char raw[];
-    AttnSmem<D> &sm = *reinterpret_cast<AttnSmem<D> *>(raw);
+    AttnSmem<D, WAVES> &sm = *reinterpret_cast<AttnSmem<D, WAVES> *>(raw);
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int n = lane & 15, q = lane >> 4;
     const int die = blockIdx.x & 7, nth = blockIdx.x >> 3, g = 8 / plan.dies;
@@ -834,9 +850,9 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_attn_kernel(shv_attn_pag
     Unit unit;
     unit.kvh = die % g + g * (nth - turn * plan.heads), unit.rep = a.n_head / a.n_head_kv;
     unit.kvw = static_cast<size_t>(a.n_head_kv) * D;
-    unit.keys = wave < kWaves / 2;
+    unit.keys = wave < WAVES / 2;
     // loads u of the wave: of keys 1024 / 2 D cells each, of values 16 dims
-    const int mine = unit.keys ? wave : wave - kWaves / 2;
+    const int mine = unit.keys ? wave : wave - WAVES / 2;
     constexpr int kPieces = D / 8, kCells = 64 / kPieces;
 #pragma unroll
     for (int u = 0; u < 2; u++) {
@@ -844,14 +860,21 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_attn_kernel(shv_attn_pag
         unit.from[u] = unit.keys ? static_cast<uint32_t>(cell * unit.kvw) * 2 + ((lane % kPieces) ^ turn_of<D>(cell)) * 16 : static_cast<uint32_t>((16 * (mine * kPer + u) + n) * kTile + 8 * q) * 2;
     }
     unit.step = unit.keys ? 2 * kCells * static_cast<uint32_t>(unit.kvw) * 2 : 2 * kChunk;
+    unit.flip = unit.keys ? 64 : 0;
+    static_assert(kPer <= 2 || (D > 64 && kPer * kCells <= 16), "eight cells on, turn_of differs by 4: 64 bytes");
     unit.cells = unit.keys ? static_cast<const uint16_t *>(a.kpages) + unit.kvh * D : static_cast<const uint16_t *>(a.vpages) + static_cast<size_t>(unit.kvh) * D * kTile;
     for (int k = 0; k < pieces; k++) {
         const Piece piece = *at;
         at = k == 0 ? plan.pieces + block->at : at + 1;
         const int groups = (min(piece.r_end - piece.r0, plan.rows) + 15) / 16;
-        if (kManyTurns<D> > 2 && groups <= kWaves / kManyTurns<D>) run_piece<D, 1, kManyTurns<D>>(a, plan, piece, unit, sm);
-        else if (groups <= kWaves / 2) run_piece<D, 1, 2>(a, plan, piece, unit, sm);
-        else run_piece<D, kGroups<D>, 1>(a, plan, piece, unit, sm);
+        constexpr int kShared = kTurns<D, WAVES>;
+        if constexpr (kShared > 1) {
+            if (groups <= WAVES / kShared) {
+                run_piece<D, 1, kShared, WAVES>(a, plan, piece, unit, sm);
+                continue;
+            }
+        }
+        run_piece<D, kGroups<D>, 1, WAVES>(a, plan, piece, unit, sm);
     }
 }
 
@@ -939,15 +962,22 @@ int check_sizes(const shv_attn_paged_args &a) {
     return SHV_OK;
 }
 
+// Blocks of eight waves read a tile for twice the query rows, which pays where a sequence has many of them and 256 dims: a chunk of 512 behind 7500, rep 8, takes 145 us
+// with them and 151 with blocks of four, 256 behind 3000 54.7 and 57.8, 100 behind 2000 39 and 38, one token behind 900 21 and 19.  Of 128 dims a block of four has as many
+// rows already: 2048 behind 8000 take 608 and 612, and all others are better with four.
+constexpr int kWideFrom = 2048;  // query rows of a KV head, on average over the sequences
+bool is_wide(const shv_attn_paged_args &a) { return a.head_dim == 256 && static_cast<long long>(a.max_rows) * (a.n_head / a.n_head_kv) >= static_cast<long long>(kWideFrom) * a.n_seq; }
+
 // The scratch of a call of these sizes, laid out from `work` on; its end is the bytes that it takes.
 uintptr_t lay_out(const shv_ctx *ctx, const shv_attn_paged_args &a, Plan &plan) {
     const int rep = a.n_head / a.n_head_kv, D = a.head_dim;
-    plan.slots = ctx->prop.multiProcessorCount / a.n_head_kv;
+    plan.waves = is_wide(a) ? kWide : kNarrow;
+    plan.slots = ctx->prop.multiProcessorCount * (kWide / plan.waves) / a.n_head_kv;
     if (plan.slots < 1) plan.slots = 1;
     if (plan.slots > kMaxSlots) plan.slots = kMaxSlots;
     plan.rep_magic = rep == 1 ? 0 : static_cast<uint32_t>(((1ull << 32) + rep - 1) / rep);
     const int query_rows = a.max_rows * rep;
-    plan.rows = rows_of(D);
+    plan.rows = rows_of(D, plan.waves);
     plan.most_q = (a.n_seq < a.max_rows ? a.n_seq : a.max_rows) + query_rows / plan.rows;
     const int g = a.n_head_kv & 7 ? a.n_head_kv & -a.n_head_kv : 8;
     plan.dies = 8 / g, plan.heads = a.n_head_kv / g;
@@ -980,7 +1010,9 @@ int launch_paged(shv_ctx *ctx, const shv_attn_paged_args &a) {
     static std::atomic<uint64_t> raised{0};  // by device
     const uint64_t bit = 1ull << (ctx->device & 63);
     if (!(raised.load(std::memory_order_acquire) & bit)) {
-        SHV_HIP_CHECK(hipFuncSetAttribute(reinterpret_cast<const void *>(&paged_attn_kernel<D>), hipFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(sizeof(AttnSmem<D>))));
+        if constexpr (D == 256)
+            SHV_HIP_CHECK(hipFuncSetAttribute(reinterpret_cast<const void *>(&paged_attn_kernel<D, kWide>), hipFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(sizeof(AttnSmem<D, kWide>))));
+        SHV_HIP_CHECK(hipFuncSetAttribute(reinterpret_cast<const void *>(&paged_attn_kernel<D, kNarrow>), hipFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(sizeof(AttnSmem<D, kNarrow>))));
         SHV_HIP_CHECK(hipFuncSetAttribute(reinterpret_cast<const void *>(&paged_plan_kernel), hipFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(sizeof(BigSmem))));
         raised.fetch_or(bit, std::memory_order_release);
     }
@@ -991,7 +1023,12 @@ int launch_paged(shv_ctx *ctx, const shv_attn_paged_args &a) {
         SHV_LAUNCH(ctx, paged_plan_kernel, dim3(1), dim3(1024), sizeof(BigSmem), a, plan);
         SHV_LAUNCH(ctx, (paged_cells_kernel<D, false>), dim3(row_blocks), dim3(256), 0, a, plan);
     }
-    SHV_LAUNCH(ctx, paged_attn_kernel<D>, dim3(plan.most_blocks / plan.dies * plan.heads * 8), dim3(64 * kWaves), sizeof(AttnSmem<D>), a, plan);
+    const dim3 blocks(plan.most_blocks / plan.dies * plan.heads * 8);
+    if (plan.waves == kNarrow) {
+        SHV_LAUNCH(ctx, (paged_attn_kernel<D, kNarrow>), blocks, dim3(64 * kNarrow), sizeof(AttnSmem<D, kNarrow>), a, plan);
+    } else if constexpr (D == 256) {
+        SHV_LAUNCH(ctx, (paged_attn_kernel<D, kWide>), blocks, dim3(64 * kWide), sizeof(AttnSmem<D, kWide>), a, plan);
+    }
     const long long joins = plan.most_q < plan.slots ? plan.most_q : plan.slots, units = joins * a.n_head_kv * plan.slot_rows / (256 / D);
     const dim3 grid(static_cast<unsigned>(units < 2048 ? units : 2048));
     if (plan.slots >= kShareFrom * plan.most_q) SHV_LAUNCH(ctx, (paged_join_kernel<D, true>), grid, dim3(256), 0, a, plan);

@@ -33,8 +33,13 @@ constexpr int ring_bytes(int waves) { return waves * (16 << 10); }
 // Weights are e^(s - m) 2^kLift, and m stands until a score is more than kSlack powers of two above it: up to 2^15.9, which the larger half holds, and down to
 // 2^-35 of the largest with the smaller half's last place, to which it is rounded.
 constexpr float kLift = 11.f, kSlack = 4.9f;
-constexpr int kLeast = 2;      // tiles a block gets at least
-constexpr int kShareFrom = 8;  // records of a query row from which waves share them
+// Tiles of few query rows whose cost a block gets at least, and quarters of a tile more by every further 16 query rows, whose records cost more than what their tiles' split gains:
+// one token of 256 dims behind 900 takes 19.4 us with two and 20.4 with three, 37 rows of rep 8 behind 3001 34.4 with two and 29.4 with the quarters, 64 of 128 dims behind
+// 3000 40.3 and 38.
+constexpr uint32_t kLeast = 2, kLeastMore = 3;
+// Records of a query row from which a block's waves share them, at most: 200 rows of 128 dims behind 100, which have up to 9, take 38.5 us with 8 and 32.5 with 16, 8 tokens of
+// 256 dims behind up to 16000, which have up to 32, 51.7 with 16 and 57.4 with 48.
+constexpr int kShareFrom = 16;
 constexpr int kFewBlocks = 1024;  // query blocks up to which the plan is made inside the launch of the cells
 
 // Groups of 16 query rows of a wave, and query rows of a block.  Of 256 dims a wave's registers hold one group; of fewer they hold two, which an operand read from LDS serves
@@ -144,7 +149,7 @@ struct PlanSmem {
     uint16_t begins[kMaxSlots + 1];  // a block's first piece
     uint32_t waves[3][T / 64];
     uint32_t bucket[64];
-    uint32_t most, most_way;
+    uint32_t most, most_way, most_groups;
 };
 // A query block as a piece of all its tiles; what a tile of it costs, and its way in and out (which the first one's block has in any case).
 struct Whole : Piece {
@@ -190,7 +195,7 @@ __device__ void make_plan(const shv_attn_paged_args &a, const Plan &plan, PlanSm
         if (s < a.n_seq) sm.q0[s] = nq + v[0];
         nq += all[0];
     }
-    if (tid == 0) sm.most = sm.most_way = 0;
+    if (tid == 0) sm.most = sm.most_way = sm.most_groups = 0;
     if (tid < 64) sm.bucket[tid] = 0;
     __syncthreads();
     const Costs costs = costs_of(a.head_dim, plan.waves);
@@ -212,27 +217,28 @@ __device__ void make_plan(const shv_attn_paged_args &a, const Plan &plan, PlanSm
     }
     block_scan<T, 2>(both, sums, sm.waves);
     if (sums[1] > 0) few = max(few, costs.few - min(sums[0] / sums[1], static_cast<uint32_t>(costs.few)));
-    uint32_t total = 0, most = 0, most_way = 0;
+    uint32_t total = 0, most = 0, most_way = 0, most_groups = 1;
     for (uint32_t i0 = 0; i0 < nq; i0 += T) {
         uint32_t v[1] = {0}, all[1];
         if (i0 + tid < nq) {
             const Whole p = whole(i0 + tid);
             v[0] = p.way + min(static_cast<uint64_t>(p.t1) * p.tile, static_cast<uint64_t>(kFull / 2));
-            most = max(most, v[0]), most_way = max(most_way, p.way);
+            most = max(most, v[0]), most_way = max(most_way, p.way), most_groups = max(most_groups, p.groups);
         }
         block_scan<T, 1>(v, all, sm.waves);
         if (i0 + tid < nq) sm.p[i0 + tid] = add_up_to(total, v[0]);
         total = add_up_to(total, all[0]);
     }
-    most = wave_most(most), most_way = wave_most(most_way);
+    most = wave_most(most), most_way = wave_most(most_way), most_groups = wave_most(most_groups);
     if ((tid & 63) == 0) {
         atomicMax(&sm.most, most);
         atomicMax(&sm.most_way, most_way);
+        atomicMax(&sm.most_groups, most_groups);
     }
     __syncthreads();
-    most = sm.most, most_way = sm.most_way;
+    most = sm.most, most_way = sm.most_way, most_groups = sm.most_groups;
     const uint32_t slots = plan.slots;
-    const uint32_t share = max((total + slots - 1) / slots, static_cast<uint32_t>(kLeast * costs.few));
+    const uint32_t share = max((total + slots - 1) / slots, (kLeast + (most_groups - 1) * kLeastMore / 4) * costs.few);
     // whole query blocks take as long as the longest, or as so many of the mean size one behind the other; a cut costs another way in and out, and the records' join
     const uint32_t rounds = (nq + slots - 1) / slots;
     const bool cut = total < kFull && max(most, nq > 0 ? total / nq * rounds : 0u) > share + most_way + most_way / 2;

@@ -487,6 +487,81 @@ def test_single_tokens_are_what_attn_decode_makes_of_them(ctx):
         assert O.rel_l2(got[r], ref[r]) <= 1e-4  # a key rounded to the other neighbour moves a score by 16 * 2^-12 / 16
 
 
+@pytest.mark.parametrize("d,dims", [(256, 8), (256, 16), (256, 32), (256, 128), (256, 192), (256, 200), (128, 0), (128, 4), (128, 32), (128, 96), (128, 124), (64, 0), (64, 2), (64, 48), (64, 64)])
+def test_rotations(ctx, monkeypatch, d, dims):
+    """Pairs of dims in one lane, in two lanes of a wave, and none, in chunks and single tokens."""
+    monkeypatch.setitem(LAYOUTS, "own", (6, 2, d, dims))
+    t = Paged(80 + dims, "own", [1, 23, 90], [77, 64, 3])
+    t.upload(ctx)
+    ctx.enqueue(A.OP_ATTN_PAGED, t.args(ctx))
+    t.check()
+
+
+@pytest.mark.parametrize("d,rep", [(256, 1), (256, 8), (128, 1), (128, 4), (64, 1), (64, 16)])
+def test_query_rows_about_the_blocks_sizes(ctx, monkeypatch, d, rep):
+    """Numbers of query rows that fill a wave's groups, the waves that share them and a block, one fewer and one more."""
+    monkeypatch.setitem(LAYOUTS, "own", (2 * rep, 2, d, 0))
+    lines = [max(1, x // rep + e) for x in (16, 32, 48, 64, 80, 128, 192) for e in (-1, 0, 1)]
+    t = Paged(90 + rep, "own", lines, [int(x) for x in np.random.default_rng(3).integers(0, 200, len(lines))], 64)
+    t.upload(ctx)
+    ctx.enqueue(A.OP_ATTN_PAGED, t.args(ctx))
+    t.check()
+
+
+@pytest.mark.parametrize("n,pos,window", [([255], [40], 0), ([256], [40], 0), ([257], [1000], 0), ([300, 1], [50, 900], 0), ([600, 1, 2], [0, 3000, 31], 0), ([600, 1, 40], [500, 700, 64], 300)])
+def test_rows_a_sequence_about_those_of_the_larger_blocks(ctx, n, pos, window):
+    t = Paged(100 + n[0], "16/2x256", n, pos, 64, spare_rows=0)
+    t.upload(ctx)
+    ctx.enqueue(A.OP_ATTN_PAGED, t.args(ctx, window, 3 if window else 0))
+    t.check(window, 3 if window else 0)
+
+
+@pytest.mark.parametrize("layout,n,pos", [("5/1x64", [1], [40000]), ("5/1x64", [1, 30, 1], [20000, 9000, 70]), ("16/2x256", [1, 1], [17000, 3]), ("12/2x128", [2, 1], [30000, 4000])])
+def test_few_rows_behind_much(ctx, layout, n, pos):
+    """A query row's tiles shared by as many blocks as there are, and by a few."""
+    t = Paged(110 + n[0], layout, n, pos, 128)
+    t.upload(ctx)
+    ctx.enqueue(A.OP_ATTN_PAGED, t.args(ctx))
+    t.check()
+
+
+def test_recorded_calls_that_share_scratch(ctx):
+    """Two recordings and an eager call, of sizes that lay the same scratch out differently, replayed in turn."""
+    sets = [Paged(120, "16/2x256", [1, 1, 1], [900, 5, 300]), Paged(121, "32/8x128", [70, 1, 3], [40, 800, 31], 64), Paged(122, "8/8x64", [1] * 9, [99 * i for i in range(9)])]
+    for t in sets:
+        t.upload(ctx)
+    args = [t.args(ctx) for t in sets]
+    work = max(args, key=lambda a: a.work_bytes)
+    for a in args:
+        a.work, a.work_bytes = work.work, work.work_bytes
+    recs = [ctx.prerecord([A.make_op(A.OP_ATTN_PAGED, a)]) for a in args[:2]]
+    for _ in range(3):
+        for t in sets:
+            t.d_out.write(np.full(t.max_rows * t.nh * t.d, 77.0, np.float32))
+        recs[0].launch()
+        ctx.enqueue(A.OP_ATTN_PAGED, args[2])
+        recs[1].launch()
+        recs[0].launch()
+        ctx.sync()
+        for t in sets:
+            t.check()
+    for rec in recs:
+        rec.destroy()
+
+
+def test_the_same_call_gives_the_same_bits(ctx):
+    """Which block takes what is planned, and records are joined in order: no result hangs on who comes first."""
+    for layout, n, pos in (("32/8x128", [150, 1, 1, 60], [300, 1500, 3, 100]), ("16/2x256", [1] * 20, [37 * i for i in range(20)]), ("8/8x64", [40, 1], [3000, 900])):
+        t = Paged(130, layout, n, pos, 64)
+        t.upload(ctx)
+        a = t.args(ctx)
+        seen = []
+        for _ in range(4):
+            ctx.enqueue(A.OP_ATTN_PAGED, a)
+            seen.append(t.results()[0].tobytes())
+        assert len(set(seen)) == 1
+
+
 # ---- log probabilities ---------------------------------------------------------------------------
 
 

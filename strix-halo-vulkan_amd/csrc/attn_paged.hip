@@ -40,7 +40,7 @@ constexpr uint32_t kLeast = 2, kLeastMore = 3;
 // Records of a query row from which a block's waves share them, at most: 200 rows of 128 dims behind 100, which have up to 9, take 38.5 us with 8 and 32.5 with 16, 8 tokens of
 // 256 dims behind up to 16000, which have up to 32, 51.7 with 16 and 57.4 with 48.
 constexpr int kShareFrom = 16;
-constexpr int kFewBlocks = 1024;  // query blocks up to which the plan is made inside the launch of the cells
+constexpr int kFewBlocks = 1024;  // query blocks up to which the plan is made inside the launch of the cells: a launch costs 3 us more, and more blocks more LDS than 256 threads should hold
 
 // Groups of 16 query rows of a wave, and query rows of a block.  Of 256 dims a wave's registers hold one group; of fewer they hold two, which an operand read from LDS serves
 // both.
@@ -120,15 +120,18 @@ struct Seq {
 };
 
 // ---- the plan: one block of T threads -----------------------------------------------------------
-// What a block's work costs, in tenths of a microsecond: a tile of few query rows, by its block where memory has bandwidth to spare (few_least) and by memory where all units
-// ask for such tiles (few); one of many query rows by its products; a piece its way in and out, and its rows' bytes.
+// What a block's work costs, in tenths of a microsecond of a unit: a tile of few query rows, by its block where memory has bandwidth to spare (few_least) and by memory where all units
+// ask for such tiles (few); one of many query rows by its products, here of 16 groups; a piece its way in and out, and its rows' bytes.  Fitted to the times of blocks, then
+// turned about: of 128 dims a chunk of 512 among 23 tokens behind up to 12000 took 275 us with group 21, 278 with 20,
+// 284 with 23, 291 with 18, and with few_least 7 283, with 9 293;
+// of 256 forty tokens behind up to 9000 105.8 with piece 90, 108.2 with 30, 107 with 120.
 struct Costs {
     int few, few_least, group, piece, piece_group;
     __host__ __device__ __forceinline__ int tile(int groups) const { return group * groups / 16; }
     __host__ __device__ __forceinline__ int way(int groups) const { return piece + piece_group * groups / 16; }
 };
 __host__ __device__ constexpr Costs wide_costs(int D) { return D == 256 ? Costs{16, 12, 37, 90, 128} : D == 128 ? Costs{9, 8, 21, 60, 64} : Costs{5, 3, 12, 60, 32}; }
-// (two narrow blocks share a unit)
+// Of a block's time: two narrow ones share a unit.
 __host__ __device__ __forceinline__ Costs costs_of(int D, int waves) {
     const Costs c = wide_costs(D);
     const int by = kWide / waves;
@@ -349,7 +352,9 @@ __global__ __launch_bounds__(1024) void paged_plan_kernel(shv_attn_paged_args a,
 }
 
 // ---- the rows' cells ----------------------------------------------------------------------------
-// A wave a row's cell of a KV head; with PLAN the first block makes the plan.
+// A wave a row's cell of a KV head; with PLAN the first block makes the plan, which takes longer than few rows' cells do: 5.8 us with one row, 8 with forty, a chain of the
+// sequences' words, three sums over them, a bisection and the stores.  Many rows are bound by the values' stores, two bytes in each of a cell's lines: 4096 rows of two heads of 256
+// dims take 17.5 us, for 25 MB.
 template <int D, bool PLAN>
 __global__ __launch_bounds__(256) void paged_cells_kernel(shv_attn_paged_args a, Plan plan) {
     constexpr int VEC = D / 64;
@@ -838,7 +843,10 @@ __device__ __forceinline__ void run_piece(const shv_attn_paged_args &a, const Pl
     __syncthreads();  // the stages are free for the next piece
 }
 
-// grid: 8 * ceil(blocks / dies) * heads, blocks of 8 waves.  Workgroups go to the eight dies in turn; a die's KV heads are the same ones throughout, where their number
+// Bound by memory where query rows are few (24 tokens of 128 dims behind up to 12000 read 5.5 TB/s, 40 of 256 behind up to 9000 5.0 while the kernel runs), by the
+// matrix units where they are many: a chunk of 2048 behind 8000, 128 dims, runs at 1040 TFLOP/s of products, both halves counted, where a large library product reaches 1295.
+//
+// grid: 8 * ceil(blocks / dies) * heads.  Workgroups go to the eight dies in turn; a die's KV heads are the same ones throughout, where their number
 // allows it, so that its L2 holds their cells: die x has the heads x % g, x % g + g, .. for g the power of two in their number, up to 8.
 template <int D, int WAVES>
 __global__ __launch_bounds__(64 * WAVES, 2) void paged_attn_kernel(shv_attn_paged_args a, Plan plan) {
@@ -885,7 +893,8 @@ __global__ __launch_bounds__(64 * WAVES, 2) void paged_attn_kernel(shv_attn_page
 }
 
 // ---- the join -----------------------------------------------------------------------------------
-// A unit is 256 / D query rows of a KV head, a lane four dims.  SHARE, where a query row has many records: a block's four waves share them, otherwise each takes a unit
+// Weighted sums of the records: bound by the trips to memory (plan, records, sums) where there are few, 3.2 us for one token behind 900, and by their bytes from the other dies' writes
+// otherwise, 4 to 12 us.  A unit is 256 / D query rows of a KV head, a lane four dims.  SHARE, where a query row has many records: a block's four waves share them, otherwise each takes a unit
 // of its own.
 template <int D, bool SHARE>
 __global__ __launch_bounds__(256) void paged_join_kernel(shv_attn_paged_args a, Plan plan) {
@@ -992,7 +1001,8 @@ uintptr_t lay_out(const shv_ctx *ctx, const shv_attn_paged_args &a, Plan &plan) 
     plan.shift = 0;
     while (1 << plan.shift < a.page) plan.shift++;
     // a cut query block has a piece more than cuts, and there are fewer cuts than slots
-    const size_t pieces = static_cast<size_t>(plan.most_q) + plan.slots, joins = plan.rows / 16 * static_cast<size_t>(plan.most_q < plan.slots ? plan.most_q : plan.slots), records = 2 * static_cast<size_t>(plan.slots) * a.n_head_kv * plan.slot_rows;
+    const size_t pieces = static_cast<size_t>(plan.most_q) + plan.slots, joins = plan.rows / 16 * static_cast<size_t>(plan.most_q < plan.slots ? plan.most_q : plan.slots);
+    const size_t records = 2 * static_cast<size_t>(plan.slots) * a.n_head_kv * plan.slot_rows;
     uintptr_t at = reinterpret_cast<uintptr_t>(a.work);
     const auto take = [&](size_t bytes) {
         char *here = reinterpret_cast<char *>(at);

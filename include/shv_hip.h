@@ -730,8 +730,8 @@ typedef struct {
 } shv_tree_accept_args;
 
 /* ---- a serving batch over a paged cache --------------------------------------------------------
- * A cache whose cells are handed out page by page, for many requests of uneven length.  (The reference gives a sequence its cells whole, one context
- * after another, llm/graph.go:1004-1062.)  The pool is laid out as shv_attn_decode's caches are, a page of `page` cells in the place of a slot: kpages
+ * A cache whose cells are handed out page by page, for many requests of uneven length.  (In the reference a sequence has a slot and all of
+ * its cells, and decodes beside others as rows of one pass, llm/graph.go:1383-1666.)  The pool is laid out as shv_attn_decode's caches are, a page of `page` cells in the place of a slot: kpages
  * [n_pages][page][n_head_kv][head_dim] and vpages [n_pages][page/32][n_head_kv][head_dim][32], binary16; page is a power of two from 32 to 4096, a pool has fewer
  * than 2^31 cells.  table [n_seq][max_pages] names a sequence's pages: its cell at position p is cell p % page of page table[s][p / page].  A table, like all
  * that is planned, serves every layer.
@@ -805,7 +805,7 @@ typedef struct {
  *   top_ids, top_logprobs [n_rows][n_top]: the n_top (at most SHV_LOGPROBS_MAX_TOP and n; 0: none) largest logits' places in falling order, of equal ones the lower place first,
  *   and their log probabilities.  A logit that is not a number is never among them (where too few others are left, the place is -1 and the log probability -infinity).
  * A logit of -infinity is a token that cannot come: it adds nothing.  Where a logit is +infinity or not a number, or all are -infinity, log Z is not a number, and nor is what is formed from it.
- * (The reference's sampler leaves these to the host, llm/sample.go:359-367 and on.)  n at most 2^30. */
+ * n at most 2^30. */
 #define SHV_LOGPROBS_MAX_TOP 64
 typedef struct {
     const float *logits;

@@ -152,11 +152,24 @@ struct PlanSmem {
     uint16_t begins[kMaxSlots + 1];  // a block's first piece
     uint32_t waves[3][T / 64];
     uint32_t bucket[64];
-    uint32_t most, most_way, most_groups;
+    uint32_t most[3][T / 64];
 };
 // A query block as a piece of all its tiles; what a tile of it costs, and its way in and out (which the first one's block has in any case).
 struct Whole : Piece {
     uint32_t tile, way, groups;
+    // What it costs but for its way; kFull, and no cut then, past 2^23 tiles, so that nothing below passes 32 bits (a tile costs less than 128).
+    __device__ __forceinline__ uint32_t cost() const { return static_cast<uint32_t>(t1) > kFull / 128 ? kFull : t1 * tile; }
+};
+// x / d by its reciprocal: exact for x < 2^31 and quotients to 2^21, which three roundings leave off by less than 1.  (The plan is a chain; a division's is twice as long.)
+struct Divisor {
+    uint32_t d;
+    float r;
+    __device__ __forceinline__ explicit Divisor(uint32_t by) : d(by), r(__builtin_amdgcn_rcpf(static_cast<float>(by))) {}
+    __device__ __forceinline__ uint32_t under(uint32_t x) const {
+        const uint32_t q = static_cast<uint32_t>(static_cast<float>(x) * r);
+        const int left = static_cast<int>(x - q * d);
+        return left < 0 ? q - 1 : left >= static_cast<int>(d) ? q + 1 : q;
+    }
 };
 __device__ __forceinline__ Whole whole_block(int window, int sinks, int D, int waves, int rows, uint32_t rep_magic, int seq, int first, int r_end, int pos, int r0, bool free_way, uint32_t few) {
     const auto over_rep = [&](int r) { return rep_magic == 0 ? r : static_cast<int>(__umulhi(static_cast<uint32_t>(r), rep_magic)); };
@@ -198,7 +211,6 @@ __device__ void make_plan(const shv_attn_paged_args &a, const Plan &plan, PlanSm
         if (s < a.n_seq) sm.q0[s] = nq + v[0];
         nq += all[0];
     }
-    if (tid == 0) sm.most = sm.most_way = sm.most_groups = 0;
     if (tid < 64) sm.bucket[tid] = 0;
     __syncthreads();
     const Costs costs = costs_of(a.head_dim, plan.waves);
@@ -211,35 +223,39 @@ __device__ void make_plan(const shv_attn_paged_args &a, const Plan &plan, PlanSm
     // Tiles of few query rows, t of them, come as fast as memory gives them, few t / slots in all, or as their blocks take them beside those of many, whose cost is c:
     // (few_least t + c) / slots.  Where the first is longer a tile costs what makes both alike.
     uint32_t both[2] = {0, 0}, sums[2];
+    Whole own = {};  // query block `tid`, which is all that a thread has in most calls
     for (uint32_t i = tid; i < nq; i += T) {
         const int seq = last_not_above(sm.q0, a.n_seq, i);
         sm.of[i] = seq;
         const Whole p = whole_of(i, seq);
+        if (i == tid) own = p;
         const bool is_few = p.tile == few;
-        both[is_few] = add_up_to(both[is_few], is_few ? p.t1 : min(static_cast<uint64_t>(p.t1) * p.tile, static_cast<uint64_t>(kFull / 2)));
+        both[is_few] = add_up_to(both[is_few], is_few ? min(static_cast<uint32_t>(p.t1), kFull) : p.cost());
     }
     block_scan<T, 2>(both, sums, sm.waves);
     if (sums[1] > 0) few = max(few, costs.few - min(sums[0] / sums[1], static_cast<uint32_t>(costs.few)));
+    own.tile = max(own.tile, few);
+    const auto mine = [&](uint32_t i) { return i == tid ? own : whole(i); };
     uint32_t total = 0, most = 0, most_way = 0, most_groups = 1;
     for (uint32_t i0 = 0; i0 < nq; i0 += T) {
         uint32_t v[1] = {0}, all[1];
         if (i0 + tid < nq) {
-            const Whole p = whole(i0 + tid);
-            v[0] = p.way + min(static_cast<uint64_t>(p.t1) * p.tile, static_cast<uint64_t>(kFull / 2));
+            const Whole p = mine(i0 + tid);
+            v[0] = p.way + p.cost();
             most = max(most, v[0]), most_way = max(most_way, p.way), most_groups = max(most_groups, p.groups);
+        }
+        if (i0 + T >= nq) {
+            const uint32_t of_wave[3] = {wave_most(most), wave_most(most_way), wave_most(most_groups)};
+            if ((tid & 63) == 0) sm.most[0][tid / 64] = of_wave[0], sm.most[1][tid / 64] = of_wave[1], sm.most[2][tid / 64] = of_wave[2];
         }
         block_scan<T, 1>(v, all, sm.waves);
         if (i0 + tid < nq) sm.p[i0 + tid] = add_up_to(total, v[0]);
         total = add_up_to(total, all[0]);
     }
-    most = wave_most(most), most_way = wave_most(most_way), most_groups = wave_most(most_groups);
-    if ((tid & 63) == 0) {
-        atomicMax(&sm.most, most);
-        atomicMax(&sm.most_way, most_way);
-        atomicMax(&sm.most_groups, most_groups);
-    }
     __syncthreads();
-    most = sm.most, most_way = sm.most_way, most_groups = sm.most_groups;
+    if (nq > 0)
+#pragma unroll
+        for (int w = 0; w < T / 64; w++) most = max(most, sm.most[0][w]), most_way = max(most_way, sm.most[1][w]), most_groups = max(most_groups, sm.most[2][w]);
     const uint32_t slots = plan.slots;
     const uint32_t share = max((total + slots - 1) / slots, (kLeast + (most_groups - 1) * kLeastMore / 4) * costs.few);
     // whole query blocks take as long as the longest, or as so many of the mean size one behind the other; a cut costs another way in and out, and the records' join
@@ -248,9 +264,8 @@ __device__ void make_plan(const shv_attn_paged_args &a, const Plan &plan, PlanSm
     if (!cut) {
         for (int pass = 0; pass < 2; pass++) {
             for (uint32_t i = tid; i < nq; i += T) {
-                const Whole p = whole(i);
-                const uint32_t cost = min(static_cast<uint64_t>(p.t1) * p.tile, static_cast<uint64_t>(kFull / 2));
-                const uint32_t k = 63 - min(63u, static_cast<uint32_t>(static_cast<uint64_t>(cost) * 64 / (most + 1)));
+                const Whole p = mine(i);
+                const uint32_t k = 63 - min(63u, static_cast<uint32_t>(static_cast<float>(p.cost()) * (64.f / static_cast<float>(most + 1))));
                 const uint32_t at = atomicAdd(&sm.bucket[k], 1u);
                 if (pass == 1) plan.blocks[at] = Block{p, 0, 0, {}};
             }
@@ -273,22 +288,23 @@ __device__ void make_plan(const shv_attn_paged_args &a, const Plan &plan, PlanSm
     }
     // Cut c of the row, at c S, falls into query block i between two of its tiles or, on its way in or behind its last tile but one, on a border of query blocks.
     // Piece k of query block i begins at its cut number first_cut + k.
-    const auto first_cut = [&](uint32_t i, const Whole &p) { return (sm.p[i] + p.way) / share; };
+    const Divisor by_share(share);
     const auto piece_of = [&](uint32_t i, Whole p, uint32_t k) {
-        const uint32_t c = first_cut(i, p) + k, from = sm.p[i] + p.way, all = p.t1;
+        const uint32_t from = sm.p[i] + p.way, c = by_share.under(from) + k, all = p.t1;
         p.t0 = k == 0 ? 0 : (c * share - from + p.tile - 1) / p.tile;
         p.t1 = min(all, ((c + 1) * share - from + p.tile - 1) / p.tile);
         return p;
     };
-    const uint32_t blocks = (total + share - 1) / share;
+    const uint32_t blocks = Divisor(share).under(total + share - 1);
     uint32_t before[3] = {0, 0, 0};  // pieces, records, joins
     for (uint32_t i0 = 0; i0 < nq; i0 += T) {
         const uint32_t i = i0 + tid;
         uint32_t v[3] = {0, 0, 0}, all[3], n = 0;
         Whole p;
         if (i < nq) {
-            p = whole(i);
-            n = (sm.p[i] + p.way + (p.t1 - 1) * p.tile) / share - first_cut(i, p) + 1;
+            p = mine(i);
+            const uint32_t from = sm.p[i] + p.way;
+            n = by_share.under(from + (p.t1 - 1) * p.tile) - by_share.under(from) + 1;
             v[0] = n, v[1] = n > 1 ? n : 0, v[2] = n > 1 ? p.groups : 0;
         }
         block_scan<T, 3>(v, all, sm.waves);
@@ -311,27 +327,34 @@ __device__ void make_plan(const shv_attn_paged_args &a, const Plan &plan, PlanSm
     const auto piece_at = [&](uint32_t c, uint32_t &i, uint32_t &k) {
         i = last_not_above(sm.p, nq, c * share);
         k = 0;
-        const Whole p = whole(i);
+        Whole p = whole(i);
         const uint32_t x = c * share - sm.p[i];
-        if (x <= p.way) return;
-        if (x > p.way + (p.t1 - 1) * p.tile) i++;
-        else k = c - first_cut(i, p);
+        if (x <= p.way) return p;
+        if (x <= p.way + (p.t1 - 1) * p.tile) {
+            k = c - by_share.under(sm.p[i] + p.way);
+            return p;
+        }
+        if (++i < nq) p = whole(i);
+        return p;
     };
     constexpr int kBlocks = (kMaxSlots + T - 1) / T;  // of a thread
     uint32_t i[kBlocks], k[kBlocks];
+    Whole of_block[kBlocks];
 #pragma unroll
     for (int e = 0; e < kBlocks; e++) {
         const uint32_t b = e * T + tid;
         if (b >= blocks) break;
-        piece_at(b, i[e], k[e]);
+        of_block[e] = piece_at(b, i[e], k[e]);
         sm.begins[b] = i[e] < nq ? (sm.of[i[e]] >> kSeqBits) + k[e] : before[0];
     }
     if (tid == 0) sm.begins[blocks] = before[0];
     __syncthreads();
     // neighbouring blocks lie on one die
-    const uint32_t dies = plan.dies, per = (blocks + dies - 1) / dies;
+    const uint32_t dies = plan.dies;  // a power of two
+    const int log_dies = __builtin_ctz(dies);
+    const uint32_t per = (blocks + dies - 1) >> log_dies;
     for (uint32_t slot = tid; slot < static_cast<uint32_t>(plan.most_blocks); slot += T) {
-        const uint32_t row = slot / dies, of = (slot - row * dies) * per + row;
+        const uint32_t row = slot >> log_dies, of = (slot & (dies - 1)) * per + row;
         if (row >= per || of >= blocks || sm.begins[of] == sm.begins[of + 1]) plan.blocks[slot].more = -1;
     }
 #pragma unroll
@@ -339,9 +362,10 @@ __device__ void make_plan(const shv_attn_paged_args &a, const Plan &plan, PlanSm
         const uint32_t b = e * T + tid;
         if (b >= blocks) break;
         if (sm.begins[b] == sm.begins[b + 1]) continue;
-        Whole p = piece_of(i[e], whole(i[e]), k[e]);
+        Whole p = piece_of(i[e], of_block[e], k[e]);
         p.rec = sm.rec[i[e]] < 0 ? -1 : sm.rec[i[e]] + static_cast<int>(k[e]);
-        plan.blocks[b % per * dies + b / per] = Block{p, sm.begins[b + 1] - sm.begins[b] - 1, sm.begins[b] + 1, {}};
+        const uint32_t die = Divisor(per).under(b);
+        plan.blocks[(b - die * per) * dies + die] = Block{p, sm.begins[b + 1] - sm.begins[b] - 1, sm.begins[b] + 1, {}};
     }
     if (tid == 0) *plan.n_joins = before[2];
 }

@@ -525,6 +525,30 @@ def test_few_rows_behind_much(ctx, layout, n, pos):
     t.check()
 
 
+def test_positions_near_the_largest(ctx, monkeypatch):
+    """A window at the last positions that 32 bits name, without rotation, gives what it gives at the first."""
+    monkeypatch.setitem(LAYOUTS, "own", (8, 2, 128, 0))
+    window, n, pos, page = 700, [1, 40], [1500, 900], 4096
+    t = Paged(140, "own", n, pos, page)
+    t.upload(ctx)
+    ctx.enqueue(A.OP_ATTN_PAGED, t.args(ctx, window))
+    near = t.check(window)
+    last = (1 << 31) // page - 1  # pages of the largest table, all but the last one taken out
+    table = np.full((2, last), -1, np.int32)
+    table[:, -1] = t.table[:, 0]
+    by = (last - 1) * page
+    t.upload(ctx)
+    a = t.args(ctx, window)
+    d_table, d_pos = ctx.upload(table), ctx.upload((t.row_pos.astype(np.int64) + by).clip(max=2**31 - 1).astype(np.int32))
+    a.table, a.row_pos, a.max_pages, a.rope = d_table.ptr, d_pos.ptr, last, None
+    a.work_bytes = ctx.attn_paged_work(a)
+    work = ctx.alloc(a.work_bytes)
+    a.work = work.ptr
+    ctx.enqueue(A.OP_ATTN_PAGED, a)
+    far = t.results()[0]
+    assert np.array_equal(far[:41], near[:41])
+
+
 def test_recorded_calls_that_share_scratch(ctx):
     """Two recordings and an eager call, of sizes that lay the same scratch out differently, replayed in turn."""
     sets = [Paged(120, "16/2x256", [1, 1, 1], [900, 5, 300]), Paged(121, "32/8x128", [70, 1, 3], [40, 800, 31], 64), Paged(122, "8/8x64", [1] * 9, [99 * i for i in range(9)])]

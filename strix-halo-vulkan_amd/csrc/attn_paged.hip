@@ -124,23 +124,24 @@ struct Seq {
 // ask for such tiles (few); one of many query rows by its products, here of 16 groups; a piece its way in and out, and its rows' bytes.  Fitted to the times of blocks, then
 // turned about: of 128 dims a chunk of 512 among 23 tokens behind up to 12000 took 275 us with group 21, 278 with 20,
 // 284 with 23, 291 with 18, and with few_least 7 283, with 9 293;
-// of 256 forty tokens behind up to 9000 105.8 with piece 90, 108.2 with 30, 107 with 120.
+// four chunks of 500 behind 3000 208 with few_beside 8, 197 with 10, 198 with 12; of 256 forty tokens behind up to 9000 105.8 with piece 90, 108.2 with 30, 107 with 120.
 struct Costs {
-    int few, few_least, group, piece, piece_group;
+    int few, few_least, few_beside, group, piece, piece_group;
     __host__ __device__ __forceinline__ int tile(int groups) const { return group * groups / 16; }
     __host__ __device__ __forceinline__ int way(int groups) const { return piece + piece_group * groups / 16; }
 };
-__host__ __device__ constexpr Costs wide_costs(int D) { return D == 256 ? Costs{16, 12, 37, 90, 128} : D == 128 ? Costs{9, 8, 21, 60, 64} : Costs{5, 3, 12, 60, 32}; }
+__host__ __device__ constexpr Costs wide_costs(int D) { return D == 256 ? Costs{16, 12, 16, 37, 90, 128} : D == 128 ? Costs{9, 8, 10, 21, 60, 64} : Costs{5, 3, 5, 12, 60, 32}; }
 // Of a block's time: two narrow ones share a unit.
 __host__ __device__ __forceinline__ Costs costs_of(int D, int waves) {
     const Costs c = wide_costs(D);
     const int by = kWide / waves;
-    return Costs{c.few * by, c.few_least * by, c.group * by, c.piece, c.piece_group};
+    return Costs{c.few * by, c.few_least * by, c.few_beside * by, c.group * by, c.piece, c.piece_group};
 }
 
 // The query blocks of all sequences stand in a row, each with its cost, P their running sum.  Where they fill the chip evenly each is a block's own, those with the most
 // tiles first.  Otherwise block b takes what lies from b S to (b + 1) S in the row, S = all / blocks, so that all blocks have the same; a query block cut by that
 // leaves a record of each piece.
+constexpr uint32_t kRare = 128;  // work of other blocks, tenths of a microsecond, for each tile of few query rows; 15 to 60 where a chunk comes with a batch's tokens, 600 in chunks alone
 constexpr int kSeqBits = 11, kMaxSlots = 512;  // blocks that the chip holds at once: a unit two
 static_assert(kMaxSeqs <= 1 << kSeqBits, "a sequence's number");
 template <int T, int SEQS, int NQ>
@@ -221,7 +222,8 @@ __device__ void make_plan(const shv_attn_paged_args &a, const Plan &plan, PlanSm
     const auto whole = [&](uint32_t i) { return whole_of(i, sm.of[i] & ((1 << kSeqBits) - 1)); };
     nq = min(nq, static_cast<uint32_t>(min(plan.most_q, NQ)));
     // Tiles of few query rows, t of them, come as fast as memory gives them, few t / slots in all, or as their blocks take them beside those of many, whose cost is c:
-    // (few_least t + c) / slots.  Where the first is longer a tile costs what makes both alike.
+    // (few_least t + c) / slots.  Where the first is longer a tile costs what makes both alike.  Where they are rare, the rests of chunks, each shares its unit with a block of
+    // products that was there first and is served first (few_beside).
     uint32_t both[2] = {0, 0}, sums[2];
     Whole own = {};  // query block `tid`, which is all that a thread has in most calls
     for (uint32_t i = tid; i < nq; i += T) {
@@ -233,7 +235,10 @@ __device__ void make_plan(const shv_attn_paged_args &a, const Plan &plan, PlanSm
         both[is_few] = add_up_to(both[is_few], is_few ? min(static_cast<uint32_t>(p.t1), kFull) : p.cost());
     }
     block_scan<T, 2>(both, sums, sm.waves);
-    if (sums[1] > 0) few = max(few, costs.few - min(sums[0] / sums[1], static_cast<uint32_t>(costs.few)));
+    if (sums[1] > 0) {
+        const uint32_t beside = sums[0] / sums[1];
+        few = beside > kRare ? costs.few_beside : max(few, costs.few - min(beside, static_cast<uint32_t>(costs.few)));
+    }
     own.tile = max(own.tile, few);
     const auto mine = [&](uint32_t i) { return i == tid ? own : whole(i); };
     uint32_t total = 0, most = 0, most_way = 0, most_groups = 1;

@@ -772,7 +772,8 @@ typedef struct {
  * multiple of head_dim / 32 up to head_dim.  Row r's key (normed and rotated at row_pos[r]) and value are rounded to binary16 into cell row_cell[r] of the pool (no cell of the pool: they
  * are left out), and the row then sees its sequence's cells at positions up to its own, with window > 0 only those of them below `sinks` or within the last `window` positions,
  * row_pos[r] - p < window.  A sequence's rows are at consecutive positions, row_pos[start[s]] and on.  Cells of a table entry that is no page (below 0, n_pages and more) are not seen by anyone:
- * pages that a window has passed may be taken out.  A row that sees nothing has zeros.  A cell that a row does not see may hold anything.
+ * pages that a window has passed may be taken out.  A row that sees nothing has zeros.  A cell that a row does not see may hold anything;
+ * of one that it sees an infinite key or value may leave not a number where the formula leaves an infinity or, of a weight of zero, nothing.
  * out [max_rows][n_head*head_dim], before the sigmoid gate.  A query's values, normed and rotated, lie within binary16's range (norm weights up to 2000 keep them there).
  * A sequence whose start is out of order or past max_rows, or whose positions are not within 0 .. max_pages * page - 1, gets no output.
  * work: work_bytes of scratch, 16-byte aligned, as many as shv_attn_paged_work says for these sizes; a call uses it alone, calls of one stream may share it.

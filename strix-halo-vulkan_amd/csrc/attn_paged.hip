@@ -637,7 +637,7 @@ __device__ __forceinline__ void run_piece(const shv_attn_paged_args &a, const Pl
         const int j = r * TP + mine_of;
         const char *kt = sm.ring[j & (kStages - 1)];
         wait_but<kPer * TP, kRounds - 2>(rounds - 1 - r);
-        asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");  // everyone's: this round is whole, and the one before has been read
+        asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");  // everyone's: these tiles are whole, and those before have been read
         const bool is = valid >> (j & (kStages - 1)) & 1;
         if (r + kRounds - 1 < rounds) ask(r + kRounds - 1);
         if (!is || !working) continue;

@@ -81,7 +81,7 @@ struct Plan {
     float *sums;        // records: [record][KV head][slot_rows][D] unnormalised sums
     float2 *of;         // and their (maximum, sum)
     int slots;          // blocks a KV head that the chip holds at once
-    int waves, rows;    // waves and query rows of a block
+    int waves, rows, rep; // waves and query rows of a block; query heads of a KV head
     int slot_rows;      // and of a record
     int most_blocks, most_q;
     int dies, heads;    // dies that share a KV head, and KV heads of a die (place)
@@ -154,6 +154,7 @@ struct PlanSmem {
     uint32_t waves[3][T / 64];
     uint32_t bucket[64];
     uint32_t most[3][T / 64];
+    uint32_t first_piece[64];   // WAVE: a query block's
 };
 // A query block as a piece of all its tiles; what a tile of it costs, and its way in and out (which the first one's block has in any case).
 struct Whole : Piece {
@@ -196,24 +197,37 @@ __device__ __forceinline__ uint32_t wave_most(uint32_t v) {
     return __builtin_amdgcn_readlane(static_cast<int>(v), 63);
 }
 
-template <int T, int SEQS, int NQ>
-__device__ void make_plan(const shv_attn_paged_args &a, const Plan &plan, PlanSmem<T, SEQS, NQ> &sm) {
-    const int tid = threadIdx.x, rep = a.n_head / a.n_head_kv;
+// WAVE, up to 64 sequences and query blocks: each wave makes all sums for itself and writes what the others write, without a barrier between them, up to where the blocks'
+// pieces are found.  (By a block's sums with two barriers each a call takes a microsecond more: 37 rows behind 3001 29.0
+// us for 28.0, 8 tokens behind up to 500 20.0 for 19.2.)
+template <bool WAVE, int T, int SEQS, int NQ>
+__device__ __forceinline__ void make_plan(const shv_attn_paged_args &a, const Plan &plan, PlanSmem<T, SEQS, NQ> &sm) {
+    const int tid = threadIdx.x, rep = plan.rep, log_rows = __builtin_ctz(plan.rows);
+    constexpr int STEP = WAVE ? 64 : T;
+    const int me = WAVE ? tid & 63 : tid;
+    const auto sums_before = [&](auto &v, auto &all) {
+        if constexpr (WAVE) wave_scan(v, all);
+        else block_scan<T>(v, all, sm.waves);
+    };
+    const auto sync = [] {
+        if constexpr (WAVE) __builtin_amdgcn_wave_barrier();
+        else __syncthreads();
+    };
     uint32_t nq = 0;
-    for (int s0 = 0; s0 < a.n_seq; s0 += T) {
-        const int s = s0 + tid;
+    for (int s0 = 0; s0 < a.n_seq; s0 += STEP) {
+        const int s = s0 + me;
         uint32_t v[1] = {0}, all[1];
         if (s < a.n_seq) {
             const Seq seq(a, s);
             sm.first[s] = seq.first, sm.n[s] = seq.n, sm.pos[s] = seq.pos;
-            v[0] = (static_cast<uint32_t>(seq.n) * rep + plan.rows - 1) / plan.rows;
+            v[0] = (static_cast<uint32_t>(seq.n) * rep + plan.rows - 1) >> log_rows;
         }
-        block_scan<T, 1>(v, all, sm.waves);
+        sums_before(v, all);
         if (s < a.n_seq) sm.q0[s] = nq + v[0];
         nq += all[0];
     }
     if (tid < 64) sm.bucket[tid] = 0;
-    __syncthreads();
+    sync();
     const Costs costs = costs_of(a.head_dim, plan.waves);
     uint32_t few = costs.few_least;
     const auto whole_of = [&](uint32_t i, int seq) {
@@ -225,48 +239,52 @@ __device__ void make_plan(const shv_attn_paged_args &a, const Plan &plan, PlanSm
     // (few_least t + c) / slots.  Where the first is longer a tile costs what makes both alike.  Where they are rare, the rests of chunks, each shares its unit with a block of
     // products that was there first and is served first (few_beside).
     uint32_t both[2] = {0, 0}, sums[2];
-    Whole own = {};  // query block `tid`, which is all that a thread has in most calls
-    for (uint32_t i = tid; i < nq; i += T) {
+    Whole own = {};  // query block `me`, which is all that a thread has in most calls
+    for (uint32_t i = me; i < nq; i += STEP) {
         const int seq = last_not_above(sm.q0, a.n_seq, i);
         sm.of[i] = seq;
         const Whole p = whole_of(i, seq);
-        if (i == tid) own = p;
+        if (i == me) own = p;
         const bool is_few = p.tile == few;
         both[is_few] = add_up_to(both[is_few], is_few ? min(static_cast<uint32_t>(p.t1), kFull) : p.cost());
     }
-    block_scan<T, 2>(both, sums, sm.waves);
+    sums_before(both, sums);
     if (sums[1] > 0) {
         const uint32_t beside = sums[0] / sums[1];
         few = beside > kRare ? costs.few_beside : max(few, costs.few - min(beside, static_cast<uint32_t>(costs.few)));
     }
     own.tile = max(own.tile, few);
-    const auto mine = [&](uint32_t i) { return i == tid ? own : whole(i); };
+    const auto mine = [&](uint32_t i) { return i == me ? own : whole(i); };
     uint32_t total = 0, most = 0, most_way = 0, most_groups = 1;
-    for (uint32_t i0 = 0; i0 < nq; i0 += T) {
+    for (uint32_t i0 = 0; i0 < nq; i0 += STEP) {
         uint32_t v[1] = {0}, all[1];
-        if (i0 + tid < nq) {
-            const Whole p = mine(i0 + tid);
+        if (i0 + me < nq) {
+            const Whole p = mine(i0 + me);
             v[0] = p.way + p.cost();
             most = max(most, v[0]), most_way = max(most_way, p.way), most_groups = max(most_groups, p.groups);
         }
-        if (i0 + T >= nq) {
+        if (!WAVE && i0 + T >= nq) {
             const uint32_t of_wave[3] = {wave_most(most), wave_most(most_way), wave_most(most_groups)};
             if ((tid & 63) == 0) sm.most[0][tid / 64] = of_wave[0], sm.most[1][tid / 64] = of_wave[1], sm.most[2][tid / 64] = of_wave[2];
         }
-        block_scan<T, 1>(v, all, sm.waves);
-        if (i0 + tid < nq) sm.p[i0 + tid] = add_up_to(total, v[0]);
+        sums_before(v, all);
+        if (i0 + me < nq) sm.p[i0 + me] = add_up_to(total, v[0]);
         total = add_up_to(total, all[0]);
     }
-    __syncthreads();
-    if (nq > 0)
+    sync();
+    if constexpr (WAVE) {
+        most = wave_most(most), most_way = wave_most(most_way), most_groups = wave_most(most_groups);
+    } else if (nq > 0) {
 #pragma unroll
         for (int w = 0; w < T / 64; w++) most = max(most, sm.most[0][w]), most_way = max(most_way, sm.most[1][w]), most_groups = max(most_groups, sm.most[2][w]);
+    }
     const uint32_t slots = plan.slots;
     const uint32_t share = max((total + slots - 1) / slots, (kLeast + (most_groups - 1) * kLeastMore / 4) * costs.few);
     // whole query blocks take as long as the longest, or as so many of the mean size one behind the other; a cut costs another way in and out, and the records' join
     const uint32_t rounds = (nq + slots - 1) / slots;
     const bool cut = total < kFull && max(most, nq > 0 ? total / nq * rounds : 0u) > share + most_way + most_way / 2;
     if (!cut) {
+        __syncthreads();
         for (int pass = 0; pass < 2; pass++) {
             for (uint32_t i = tid; i < nq; i += T) {
                 const Whole p = mine(i);
@@ -302,8 +320,8 @@ __device__ void make_plan(const shv_attn_paged_args &a, const Plan &plan, PlanSm
     };
     const uint32_t blocks = Divisor(share).under(total + share - 1);
     uint32_t before[3] = {0, 0, 0};  // pieces, records, joins
-    for (uint32_t i0 = 0; i0 < nq; i0 += T) {
-        const uint32_t i = i0 + tid;
+    for (uint32_t i0 = 0; i0 < nq; i0 += STEP) {
+        const uint32_t i = i0 + me;
         uint32_t v[3] = {0, 0, 0}, all[3], n = 0;
         Whole p;
         if (i < nq) {
@@ -312,22 +330,23 @@ __device__ void make_plan(const shv_attn_paged_args &a, const Plan &plan, PlanSm
             n = by_share.under(from + (p.t1 - 1) * p.tile) - by_share.under(from) + 1;
             v[0] = n, v[1] = n > 1 ? n : 0, v[2] = n > 1 ? p.groups : 0;
         }
-        block_scan<T, 3>(v, all, sm.waves);
+        sums_before(v, all);
         if (i < nq) {
             const uint32_t at = before[0] + v[0], rec = before[1] + v[1];
-            sm.of[i] |= at << kSeqBits;
+            if constexpr (WAVE) sm.first_piece[i] = at;
+            else sm.of[i] |= at << kSeqBits;
             sm.rec[i] = n > 1 ? static_cast<int>(rec) : -1;
             if (n > 1) {
-                for (uint32_t g = 0; g < p.groups; g++)
+                for (uint32_t g = 0; g < p.groups && (!WAVE || tid < 64); g++)
                     plan.joins[before[2] + v[2] + g] = Join{p.first, p.r0 + 16 * static_cast<int>(g), p.r_end, static_cast<int>(rec), static_cast<int>(n), 16 * static_cast<int>(g), {}};
                 p = piece_of(i, p, 0);
                 p.rec = rec;
             }
-            plan.pieces[at] = p;
+            if (!WAVE || tid < 64) plan.pieces[at] = p;
         }
         before[0] += all[0], before[1] += all[1], before[2] += all[2];
     }
-    __syncthreads();
+    sync();
     // the query block and which of its pieces that begin at or behind cut c; i = nq: none
     const auto piece_at = [&](uint32_t c, uint32_t &i, uint32_t &k) {
         i = last_not_above(sm.p, nq, c * share);
@@ -350,7 +369,7 @@ __device__ void make_plan(const shv_attn_paged_args &a, const Plan &plan, PlanSm
         const uint32_t b = e * T + tid;
         if (b >= blocks) break;
         of_block[e] = piece_at(b, i[e], k[e]);
-        sm.begins[b] = i[e] < nq ? (sm.of[i[e]] >> kSeqBits) + k[e] : before[0];
+        sm.begins[b] = i[e] < nq ? (WAVE ? sm.first_piece[i[e] & 63] : sm.of[i[e]] >> kSeqBits) + k[e] : before[0];
     }
     if (tid == 0) sm.begins[blocks] = before[0];
     __syncthreads();
@@ -377,7 +396,7 @@ __device__ void make_plan(const shv_attn_paged_args &a, const Plan &plan, PlanSm
 
 __global__ __launch_bounds__(1024) void paged_plan_kernel(shv_attn_paged_args a, Plan plan) {
     extern __shared__ __align__(16) char raw[];
-    make_plan(a, plan, *reinterpret_cast<PlanSmem<1024, kMaxSeqs, 8192 + kMaxSeqs> *>(raw));
+    make_plan<false>(a, plan, *reinterpret_cast<PlanSmem<1024, kMaxSeqs, 8192 + kMaxSeqs> *>(raw));
 }
 
 // ---- the rows' cells ----------------------------------------------------------------------------
@@ -390,7 +409,8 @@ __global__ __launch_bounds__(256) void paged_cells_kernel(shv_attn_paged_args a,
     if constexpr (PLAN) {
         __shared__ PlanSmem<256, kFewBlocks, kFewBlocks> sm;
         if (blockIdx.x == 0) {
-            make_plan(a, plan, sm);
+            if (a.n_seq <= 64 && plan.most_q <= 64) make_plan<true>(a, plan, sm);
+            else make_plan<false>(a, plan, sm);
             return;
         }
     }
@@ -891,7 +911,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void paged_attn_kernel(shv_attn_page
     const int pieces = block->more + 1;
     const Piece *at = &block->piece;
     Unit unit;
-    unit.kvh = die % g + g * (nth - turn * plan.heads), unit.rep = a.n_head / a.n_head_kv;
+    unit.kvh = die % g + g * (nth - turn * plan.heads), unit.rep = plan.rep;
     unit.kvw = static_cast<size_t>(a.n_head_kv) * D;
     unit.keys = wave < WAVES / 2;
     // loads u of the wave: of keys 1024 / 2 D cells each, of values 16 dims
@@ -931,7 +951,7 @@ __global__ __launch_bounds__(256) void paged_join_kernel(shv_attn_paged_args a, 
     __shared__ float2 of[4][64];
     constexpr int kLanes = D / 4, kUnit = 64 / kLanes, kPerHead = 16 / kUnit;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int rep = a.n_head / a.n_head_kv;
+    const int rep = plan.rep;
     const float c2 = 1.44269504088896f / sqrtf(static_cast<float>(D));
     const uint32_t per = kPerHead * a.n_head_kv, units = per * *plan.n_joins;
     const uint32_t step = SHARE ? gridDim.x : gridDim.x * 4;
@@ -1020,6 +1040,7 @@ uintptr_t lay_out(const shv_ctx *ctx, const shv_attn_paged_args &a, Plan &plan) 
     if (plan.slots < 1) plan.slots = 1;
     if (plan.slots > kMaxSlots) plan.slots = kMaxSlots;
     plan.rep_magic = rep == 1 ? 0 : static_cast<uint32_t>(((1ull << 32) + rep - 1) / rep);
+    plan.rep = rep;
     const int query_rows = a.max_rows * rep;
     plan.rows = rows_of(D, plan.waves);
     plan.most_q = (a.n_seq < a.max_rows ? a.n_seq : a.max_rows) + query_rows / plan.rows;

@@ -48,6 +48,17 @@ __device__ __forceinline__ void block_scan(uint32_t (&v)[N], uint32_t (&total)[N
     __syncthreads();  // `waves` is free again
 }
 
+// The same over the lanes of a wave.
+template <int N>
+__device__ __forceinline__ void wave_scan(uint32_t (&v)[N], uint32_t (&total)[N]) {
+#pragma unroll
+    for (int k = 0; k < N; k++) {
+        const uint32_t upto = wave_upto(v[k]);
+        total[k] = static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(upto), 63));
+        v[k] = shifted<0x138>(upto);
+    }
+}
+
 // The last of n ascending values that is not above x; the first is not.
 __device__ __forceinline__ int last_not_above(const uint32_t *v, int n, uint32_t x) {
     int lo = 0;

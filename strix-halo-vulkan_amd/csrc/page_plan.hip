@@ -21,15 +21,18 @@ constexpr int kMaxRows = 1 << 20;
 // one block; with 4, where a call of 48 sequences has two blocks, that takes 10.1 instead of 9.4.
 constexpr int kPagesFrom = 16;
 
-template <int T>
+// WAVE, up to 64 sequences: each wave makes the scans for itself and writes to LDS what the others write, without a barrier up to the last.  (48 sequences, two passes: 9.1 us, and 10.1 by a
+// block's scans with two barriers each.)
+template <int T, bool WAVE>
 __global__ __launch_bounds__(T) void page_plan_kernel(shv_page_plan_args a, int shift, int32_t *counter) {
     constexpr int kPer = T == 1024 ? kMaxSeqs / T : 1;  // sequences a thread, side by side
-    __shared__ uint32_t s_start[kPer * T + 1], s_taken[kPer * T + 1], s_back[kPer * T + 1];
+    __shared__ uint32_t s_start[kPer * T], s_taken[kPer * T], s_back[kPer * T];
     __shared__ int s_held[kPer * T], s_pos[kPer * T];
     __shared__ uint32_t waves[3][T / 64];
     __shared__ int is_last;
     const int tid = threadIdx.x;
-    const int first = tid * kPer;
+    static_assert(!WAVE || kPer == 1, "a lane a sequence");
+    const int first = WAVE ? tid & 63 : tid * kPer;
     int rows[kPer], pos[kPer], held[kPer], shared[kPer];
 #pragma unroll
     for (int u = 0; u < kPer; u++) {
@@ -54,7 +57,8 @@ __global__ __launch_bounds__(T) void page_plan_kernel(shv_page_plan_args a, int 
         asked[u] = fits[u] ? min(static_cast<uint32_t>(max(rows[u], 0)), kFull) : 0;
         sums[0] = add_up_to(sums[0], back[u]), sums[1] = add_up_to(sums[1], need[u]), sums[2] = add_up_to(sums[2], asked[u]);
     }
-    block_scan<T, 3>(sums, total, waves);
+    if constexpr (WAVE) wave_scan(sums, total);
+    else block_scan<T, 3>(sums, total, waves);
     const uint32_t n_back = total[0], avail = n_free + n_back;
     uint32_t take[kPer], gets[kPer], both[2] = {0, 0}, total2[2];
     {
@@ -69,7 +73,8 @@ __global__ __launch_bounds__(T) void page_plan_kernel(shv_page_plan_args a, int 
             both[0] += take[u], both[1] += gets[u];  // (at most avail and max_rows together)
         }
     }
-    block_scan<T, 2>(both, total2, waves);
+    if constexpr (WAVE) wave_scan(both, total2);
+    else block_scan<T, 2>(both, total2, waves);
     const uint32_t n_taken = total2[0], n_rows = total2[1];
     {
         uint32_t t = both[0], r = both[1];
@@ -80,8 +85,8 @@ __global__ __launch_bounds__(T) void page_plan_kernel(shv_page_plan_args a, int 
             t += take[u], r += gets[u];
         }
     }
-    if (tid == 0) s_back[kPer * T] = n_back, s_taken[kPer * T] = n_taken, s_start[kPer * T] = n_rows;
-    __syncthreads();
+    if constexpr (WAVE) __builtin_amdgcn_wave_barrier();
+    else __syncthreads();
     if (blockIdx.x == 0) {
         for (int s = tid; s < a.n_seq; s += T) {
             a.start[s] = s_start[s];
@@ -113,7 +118,12 @@ __global__ __launch_bounds__(T) void page_plan_kernel(shv_page_plan_args a, int 
         a.table[static_cast<size_t>(s) * a.max_pages + s_held[s] + (e - s_taken[s])] = taken(e);
     }
     for (uint32_t r = me; r < n_back && n_free + r < static_cast<uint32_t>(a.n_pages); r += step) a.free_pages[n_free + r] = given_back(r);
-    if (gridDim.x > 1 && !arrive_last(counter, gridDim.x, &is_last)) return;
+    if (gridDim.x > 1) {
+        if (!arrive_last(counter, gridDim.x, &is_last)) return;
+    } else if (WAVE) {
+        __syncthreads();  // every wave has read what is written now
+    }
+    if (WAVE && tid >= 64) return;
 #pragma unroll
     for (int u = 0; u < kPer; u++) {
         if (!fits[u]) continue;  // left as it is, as behind the last
@@ -142,7 +152,8 @@ int shv_launch_page_plan(shv_ctx *ctx, const shv_page_plan_args *pa) {
     const long long entries = static_cast<long long>(a.n_seq) * a.max_pages, pages = entries < a.n_pages ? entries : a.n_pages;
     const long long for_rows = (a.max_rows + threads - 1) / threads, for_pages = pages / (kPagesFrom * threads), blocks = for_rows > for_pages ? for_rows : for_pages;
     const dim3 grid(static_cast<unsigned>(blocks < 64 ? blocks : 64));
-    if (threads == 256) SHV_LAUNCH(ctx, page_plan_kernel<256>, grid, dim3(256), 0, a, shift, counter);
-    else SHV_LAUNCH(ctx, page_plan_kernel<1024>, grid, dim3(1024), 0, a, shift, counter);
+    if (threads == 256 && a.n_seq <= 64) SHV_LAUNCH(ctx, (page_plan_kernel<256, true>), grid, dim3(256), 0, a, shift, counter);
+    else if (threads == 256) SHV_LAUNCH(ctx, (page_plan_kernel<256, false>), grid, dim3(256), 0, a, shift, counter);
+    else SHV_LAUNCH(ctx, (page_plan_kernel<1024, false>), grid, dim3(1024), 0, a, shift, counter);
     return SHV_OK;
 }

@@ -400,7 +400,7 @@ __global__ __launch_bounds__(1024) void paged_plan_kernel(shv_attn_paged_args a,
 }
 
 // ---- the rows' cells ----------------------------------------------------------------------------
-// A wave a row's cell of a KV head; with PLAN the first block makes the plan, which takes longer than few rows' cells do: 5.8 us with one row, 8 with forty, a chain of the
+// A wave a row's cell of a KV head; with PLAN the first block makes the plan, which takes longer than few rows' cells do: 4.5 us with one row, 7 with forty, a chain of the
 // sequences' words, three sums over them, a bisection and the stores.  Many rows are bound by the values' stores, two bytes in each of a cell's lines: 4096 rows of two heads of 256
 // dims take 17.5 us, for 25 MB.
 template <int D, bool PLAN>

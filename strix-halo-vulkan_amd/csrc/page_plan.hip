@@ -3,8 +3,8 @@
 // With want = ceil((pos + rows) / page): back = held - max(want, shared), need = want - held, each where above zero.  The pages given back lie behind the
 // free ones, L = free | back in order, A = |L|; sequence s's j-th new page is L[A - 1 - (taken before it) - j].  All of that is two scans over the
 // sequences, of (back, need, rows) and of what is granted, and lookups by bisection from there on.
-// Bound by the chain of trips to memory (a sequence's words, then pages, then the stores) and the scans' barriers, not by bytes: 48 sequences of a token each take 3.3 to 4 us
-// of the kernel's own time, 900 with 12007 rows 8 to 9.4.  Every block makes the scans for itself, which costs less than a launch between them and the
+// Bound by the chain of trips to memory (a sequence's words, then pages, then the stores) and the scans' barriers, not by bytes: 48 sequences of a token each take 2.9 to 3.6 us
+// of the kernel's own time, 900 with 12007 rows 8 to 10.  Every block makes the scans for itself, which costs less than a launch between them and the
 // rows; a row a thread, since each is a bisection and two dependent loads (four a thread: 26 us for 19 of the 900 sequences' two passes).  The words that others
 // still read (held, pos, n_free) are written by the block that arrives last.
 #include "scan.hpp"

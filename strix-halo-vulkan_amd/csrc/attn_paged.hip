@@ -401,10 +401,54 @@ __global__ __launch_bounds__(1024) void paged_plan_kernel(shv_attn_paged_args a,
 
 // ---- the rows' cells ----------------------------------------------------------------------------
 // A wave a row's cell of a KV head; with PLAN the first block makes the plan, which takes longer than few rows' cells do: 4.5 us with one row, 7 with forty, a chain of the
-// sequences' words, three sums over them, a bisection and the stores.  Many rows are bound by the values' stores, two bytes in each of a cell's lines: 4096 rows of two heads of 256
-// dims take 17.5 us, for 25 MB.
+// sequences' words, three sums over them, a bisection and the stores.  Many rows would be bound by the values' stores, two
+// bytes in each of a cell's lines (17.5 us for 4096 rows of two heads of 256 dims, 25 MB).
+// Where rows are many, blocks from values_from on take the values of eight rows by 256 columns: a thread has a column, and cells side by side in a tile are one store.
+// A prompt of 2048 (two heads of 256 dims) takes 105 us with that and 108 without, one of 4096 (eight of 128) 306 and 316; four chunks whose cells begin anywhere 192 either
+// way, and 195 by 32 rows a block.
+constexpr int kValuesRows = 8;
+constexpr int kValuesFrom = 512;  // rows: below, the plan takes as long as the cells
+__device__ __forceinline__ bool has_cell(const shv_attn_paged_args &a, const Plan &plan, int r, int p, int cell) {
+    return r < a.start[a.n_seq] && p >= 0 && p < a.max_pages << plan.shift && cell >= 0 && cell < a.n_pages << plan.shift;
+}
+template <int D>
+__device__ __forceinline__ void put_values(const shv_attn_paged_args &a, const Plan &plan, uint32_t block) {
+    const uint32_t kvw = static_cast<uint32_t>(a.n_head_kv) * D, across = (kvw + 255) / 256, by = block / across;
+    const int r0 = static_cast<int>(by) * kValuesRows, lane = threadIdx.x & 63;
+    const uint32_t col = (block - by * across) * 256 + threadIdx.x;
+    const float *src = a.qkv + static_cast<size_t>(a.n_head) * 2 * D + kvw + min(col, kvw - 1);
+    float v[kValuesRows];
+#pragma unroll
+    for (int i = 0; i < kValuesRows; i++) v[i] = src[static_cast<size_t>(min(r0 + i, a.max_rows - 1)) * a.qkv_stride];
+    const int mine = r0 + lane % kValuesRows, r = min(mine, a.max_rows - 1);
+    int cell = a.row_cell[r];
+    if (mine >= a.max_rows || !has_cell(a, plan, r, a.row_pos[r], cell)) cell = -1;
+    const uint64_t follows = __ballot(cell >= 0 && __shfl_up(cell, 1, 64) == cell - 1 && cell % kTile != 0);  // it is in the row before's tile, behind it
+    if (col >= kvw) return;
+    uint16_t *const values = static_cast<uint16_t *>(a.vpages) + static_cast<size_t>(col) * kTile;
+    uint16_t h[kValuesRows];
+#pragma unroll
+    for (int i = 0; i < kValuesRows; i++) h[i] = __half_as_ushort(__float2half_rn(v[i]));
+    const auto at = [&](int i) {
+        const int c = __builtin_amdgcn_readlane(cell, i);
+        return values + static_cast<size_t>(c / kTile) * kvw * kTile + c % kTile;
+    };
+    const int c0 = __builtin_amdgcn_readlane(cell, 0);
+    const bool run = c0 >= 0 && (follows & 0xFE) == 0xFE;
+    if (run && c0 % 8 == 0) {
+        put_bytes<16>(at(0), h);
+    } else if (run && c0 % 4 == 0) {
+        put_bytes<8>(at(0), h);
+        put_bytes<8>(at(4), h + 4);
+    } else {
+#pragma unroll
+        for (int i = 0; i < kValuesRows; i++)
+            if (__builtin_amdgcn_readlane(cell, i) >= 0) *at(i) = h[i];
+    }
+}
+
 template <int D, bool PLAN>
-__global__ __launch_bounds__(256) void paged_cells_kernel(shv_attn_paged_args a, Plan plan) {
+__global__ __launch_bounds__(256) void paged_cells_kernel(shv_attn_paged_args a, Plan plan, uint32_t values_from) {
     constexpr int VEC = D / 64;
     if constexpr (PLAN) {
         __shared__ PlanSmem<256, kFewBlocks, kFewBlocks> sm;
@@ -414,6 +458,10 @@ __global__ __launch_bounds__(256) void paged_cells_kernel(shv_attn_paged_args a,
             return;
         }
     }
+    if (values_from > 0 && blockIdx.x >= values_from) {
+        put_values<D>(a, plan, blockIdx.x - values_from);
+        return;
+    }
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const uint32_t item = (blockIdx.x - (PLAN ? 1 : 0)) * 4 + wave;
     const int r = static_cast<int>(item / static_cast<uint32_t>(a.n_head_kv)), head = static_cast<int>(item) - r * a.n_head_kv;
@@ -421,10 +469,10 @@ __global__ __launch_bounds__(256) void paged_cells_kernel(shv_attn_paged_args a,
     const float *src = a.qkv + static_cast<size_t>(r) * a.qkv_stride + static_cast<size_t>(a.n_head) * 2 * D + head * D;
     Row<D> x, gamma, val;
     x.load(src, lane);
-    val.load(src + static_cast<size_t>(a.n_head_kv) * D, lane);
+    if (values_from == 0) val.load(src + static_cast<size_t>(a.n_head_kv) * D, lane);
     gamma.load(a.k_norm, lane);
     const int p = a.row_pos[r], cell = a.row_cell[r];
-    if (r >= a.start[a.n_seq] || p < 0 || p >= a.max_pages << plan.shift || cell < 0 || cell >= a.n_pages << plan.shift) return;
+    if (!has_cell(a, plan, r, p, cell)) return;
     Turn<D> turn(a.rope_dims, lane);
     if (a.rope_dims > 0) {
         turn.load(a.rope + static_cast<size_t>(p) * a.rope_dims, a.rope_dims);
@@ -434,6 +482,7 @@ __global__ __launch_bounds__(256) void paged_cells_kernel(shv_attn_paged_args a,
     cell_key<D>(x, gamma, turn, a.rope_dims, a.eps, kx);
     const size_t kvw = static_cast<size_t>(a.n_head_kv) * D;
     put_bytes<2 * VEC>(static_cast<uint16_t *>(a.kpages) + cell * kvw + head * D + VEC * lane, kx);
+    if (values_from > 0) return;
     uint16_t *vd = static_cast<uint16_t *>(a.vpages) + (cell / kTile * kvw + static_cast<size_t>(head) * D + VEC * lane) * kTile + cell % kTile;
 #pragma unroll
     for (int v = 0; v < VEC; v++) vd[v * kTile] = __half_as_ushort(__float2half_rn(val.x[v]));
@@ -1083,11 +1132,12 @@ int launch_paged(shv_ctx *ctx, const shv_attn_paged_args &a) {
         raised.fetch_or(bit, std::memory_order_release);
     }
     const unsigned row_blocks = static_cast<unsigned>((static_cast<long long>(a.max_rows) * a.n_head_kv + 3) / 4);
+    const unsigned value_blocks = a.max_rows >= kValuesFrom ? static_cast<unsigned>((a.max_rows + kValuesRows - 1) / kValuesRows * ((a.n_head_kv * D + 255) / 256)) : 0u;
     if (plan.most_q <= kFewBlocks && a.n_seq <= kFewBlocks) {
-        SHV_LAUNCH(ctx, (paged_cells_kernel<D, true>), dim3(row_blocks + 1), dim3(256), 0, a, plan);
+        SHV_LAUNCH(ctx, (paged_cells_kernel<D, true>), dim3(row_blocks + 1 + value_blocks), dim3(256), 0, a, plan, value_blocks > 0 ? row_blocks + 1 : 0u);
     } else {
         SHV_LAUNCH(ctx, paged_plan_kernel, dim3(1), dim3(1024), sizeof(BigSmem), a, plan);
-        SHV_LAUNCH(ctx, (paged_cells_kernel<D, false>), dim3(row_blocks), dim3(256), 0, a, plan);
+        SHV_LAUNCH(ctx, (paged_cells_kernel<D, false>), dim3(row_blocks + value_blocks), dim3(256), 0, a, plan, value_blocks > 0 ? row_blocks : 0u);
     }
     const dim3 blocks(plan.most_blocks / plan.dies * plan.heads * 8);
     if (plan.waves == kNarrow) {

@@ -525,6 +525,30 @@ def test_few_rows_behind_much(ctx, layout, n, pos):
     t.check()
 
 
+@pytest.mark.parametrize("layout", ["32/8x128", "5/1x64", "12/2x128", "7/7x256"])
+@pytest.mark.parametrize("first", [0, 1, 2, 4, 33])
+def test_many_rows_cells(ctx, layout, first):
+    """Values of rows whose cells begin anywhere in a tile, end with a page, skip a page that is none, and belong to nobody, where rows are many."""
+    n, pos = [203, 1, 0, 180, 77, 1, 64], [first, 5, 0, 62 + first, 501, 31, 64]
+    t = Paged(170 + first, layout, n, pos, 32, spare_rows=40)
+    t.table[3, 4] = -1
+    lost = t.row_pos[t.start[3]:t.start[4]] // 32 == 4
+    t.row_cell[t.start[3]:t.start[4]][lost] = -1
+    t.upload(ctx)
+    ctx.enqueue(A.OP_ATTN_PAGED, t.args(ctx))
+    t.check()
+
+
+@pytest.mark.parametrize("layout", [(1024, 1024, 64, 64), (257, 257, 64, 2), (1024, 16, 256, 64), (48, 24, 128, 32), (39, 13, 128, 128), (640, 10, 64, 0)])
+def test_numbers_of_heads(ctx, monkeypatch, layout):
+    """More KV heads than units, odd numbers of them, which do not divide the dies, and the most query heads there may be."""
+    monkeypatch.setitem(LAYOUTS, "own", layout)
+    t = Paged(150 + layout[1], "own", [1, 5, 1], [40, 0, 131])
+    t.upload(ctx)
+    ctx.enqueue(A.OP_ATTN_PAGED, t.args(ctx))
+    t.check()
+
+
 def test_positions_near_the_largest(ctx, monkeypatch):
     """A window at the last positions that 32 bits name, without rotation, gives what it gives at the first."""
     monkeypatch.setitem(LAYOUTS, "own", (8, 2, 128, 0))
@@ -763,3 +787,17 @@ def test_a_servers_passes(ctx):
                                            dv["tl"].read(np.float32, max_rows * top).reshape(max_rows, top)))
     assert waited > 0
     rec.destroy()
+
+
+def test_each_ops_time_is_told(ctx):
+    t, plan = Paged(160, "32/8x128", [1, 40], [300, 20]), Plan(161, 40, 32, 20, 300, 30, 400)
+    t.upload(ctx)
+    plan.upload(ctx)
+    plan.d["rows"].write(np.ones(40, np.int32))
+    logits = t.rng.standard_normal((5, 9001)).astype(np.float32)
+    a, got = _logprobs(ctx, logits, [1, 2, 3, 4, 5], 7)
+    total, each = ctx.dispatch_multi([A.make_op(A.OP_PAGE_PLAN, plan.args()), A.make_op(A.OP_ATTN_PAGED, t.args(ctx)), A.make_op(A.OP_LOGPROBS, a)], per_op=True)
+    assert len(each) == 3 and all(x > 0 for x in each) and total > 0
+    plan.check(np.ones(40, np.int32), [np.full(400, -5, np.int32) for _ in range(3)])
+    t.check()
+    _check_logprobs(logits, [1, 2, 3, 4, 5], 7, got())

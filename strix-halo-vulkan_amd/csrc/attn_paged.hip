@@ -40,6 +40,8 @@ constexpr uint32_t kLeast = 2, kLeastMore = 3;
 // Records of a query row from which a block's waves share them, at most: 200 rows of 128 dims behind 100, which have up to 9, take 38.5 us with 8 and 32.5 with 16, 8 tokens of
 // 256 dims behind up to 16000, which have up to 32, 51.7 with 16 and 57.4 with 48.
 constexpr int kShareFrom = 16;
+// Query blocks that a plan holds: 2^20 query rows by 128, and a rest of each sequence.
+constexpr int kMostBlocks = (1 << 20) / 128 + kMaxSeqs;
 constexpr int kFewBlocks = 1024;  // query blocks up to which the plan is made inside the launch of the cells: a launch costs 3 us more, and more blocks more LDS than 256 threads should hold
 
 // Groups of 16 query rows of a wave, and query rows of a block.  Of 256 dims a wave's registers hold one group; of fewer they hold two, which an operand read from LDS serves
@@ -396,7 +398,7 @@ __device__ __forceinline__ void make_plan(const shv_attn_paged_args &a, const Pl
 
 __global__ __launch_bounds__(1024) void paged_plan_kernel(shv_attn_paged_args a, Plan plan) {
     extern __shared__ __align__(16) char raw[];
-    make_plan<false>(a, plan, *reinterpret_cast<PlanSmem<1024, kMaxSeqs, 8192 + kMaxSeqs> *>(raw));
+    make_plan<false>(a, plan, *reinterpret_cast<PlanSmem<1024, kMaxSeqs, kMostBlocks> *>(raw));
 }
 
 // ---- the rows' cells ----------------------------------------------------------------------------
@@ -1077,9 +1079,14 @@ int check_sizes(const shv_attn_paged_args &a) {
 
 // Blocks of eight waves read a tile for twice the query rows, which pays where a sequence has many of them and 256 dims: a chunk of 512 behind 7500, rep 8, takes 145 us
 // with them and 151 with blocks of four, 256 behind 3000 54.7 and 57.8, 100 behind 2000 39 and 38, one token behind 900 21 and 19.  Of 128 dims a block of four has as many
-// rows already: 2048 behind 8000 take 608 and 612, and all others are better with four.
+// rows already: 2048 behind 8000 take 608 and 612, and all others are better with four.  And where blocks of four could be more than a plan holds, which those of eight never are.
 constexpr int kWideFrom = 2048;  // query rows of a KV head, on average over the sequences
-bool is_wide(const shv_attn_paged_args &a) { return a.head_dim == 256 && static_cast<long long>(a.max_rows) * (a.n_head / a.n_head_kv) >= static_cast<long long>(kWideFrom) * a.n_seq; }
+// Query blocks of `rows` query rows, at most: a sequence's last one may be short.
+int most_query_blocks(const shv_attn_paged_args &a, int rows) { return (a.n_seq < a.max_rows ? a.n_seq : a.max_rows) + a.max_rows * (a.n_head / a.n_head_kv) / rows; }
+bool is_wide(const shv_attn_paged_args &a) {
+    return a.head_dim == 256 && (static_cast<long long>(a.max_rows) * (a.n_head / a.n_head_kv) >= static_cast<long long>(kWideFrom) * a.n_seq ||
+                                 most_query_blocks(a, rows_of(256, kNarrow)) > kMostBlocks);
+}
 
 // The scratch of a call of these sizes, laid out from `work` on; its end is the bytes that it takes.
 uintptr_t lay_out(const shv_ctx *ctx, const shv_attn_paged_args &a, Plan &plan) {
@@ -1092,7 +1099,7 @@ uintptr_t lay_out(const shv_ctx *ctx, const shv_attn_paged_args &a, Plan &plan) 
     plan.rep = rep;
     const int query_rows = a.max_rows * rep;
     plan.rows = rows_of(D, plan.waves);
-    plan.most_q = (a.n_seq < a.max_rows ? a.n_seq : a.max_rows) + query_rows / plan.rows;
+    plan.most_q = most_query_blocks(a, plan.rows);
     const int g = a.n_head_kv & 7 ? a.n_head_kv & -a.n_head_kv : 8;
     plan.dies = 8 / g, plan.heads = a.n_head_kv / g;
     plan.most_blocks = ((plan.most_q > plan.slots ? plan.most_q : plan.slots) + plan.dies - 1) / plan.dies * plan.dies;
@@ -1121,7 +1128,7 @@ template <int D>
 int launch_paged(shv_ctx *ctx, const shv_attn_paged_args &a) {
     Plan plan;
     lay_out(ctx, a, plan);
-    using BigSmem = PlanSmem<1024, kMaxSeqs, 8192 + kMaxSeqs>;
+    using BigSmem = PlanSmem<1024, kMaxSeqs, kMostBlocks>;
     static std::atomic<uint64_t> raised{0};  // by device
     const uint64_t bit = 1ull << (ctx->device & 63);
     if (!(raised.load(std::memory_order_acquire) & bit)) {
@@ -1182,6 +1189,8 @@ extern "C" int shv_attn_paged_work(shv_ctx *ctx, const shv_attn_paged_args *a, i
     shv_attn_paged_args sizes = *a;
     sizes.work = nullptr;
     Plan plan;
-    *bytes = static_cast<int64_t>(lay_out(ctx, sizes, plan));
+    const int64_t need = static_cast<int64_t>(lay_out(ctx, sizes, plan));
+    SHV_REQUIRE(plan.most_q <= kMostBlocks, "attn_paged: up to %d blocks of query rows; a plan holds %d", plan.most_q, kMostBlocks);
+    *bytes = need;
     return SHV_OK;
 }

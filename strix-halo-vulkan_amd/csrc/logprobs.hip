@@ -276,7 +276,8 @@ __global__ __launch_bounds__(kBlock) void logprobs_kernel(shv_logprobs_args a, f
         const float v[2] = {before ? x[tid] : -INFINITY, behind ? x[tail + tid] : -INFINITY};
         add(v, std::integral_constant<int, 2>());
         if constexpr (TOP) {
-            // at most six
+            // at most six; every wave has read the list's length as the last selection left it
+            if (head > 0 || tail < a.n) __syncthreads();
             if (v[0] > -INFINITY) sm.list[atomicAdd(&sm.n, 1)] = token(v[0], tid);
             if (v[1] > -INFINITY) sm.list[atomicAdd(&sm.n, 1)] = token(v[1], tail + tid);
             if (head > 0 || tail < a.n) __syncthreads();

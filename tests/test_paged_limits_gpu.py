@@ -57,3 +57,17 @@ def test_more_query_rows_of_256_dims_than_small_blocks_hold(ctx, rep, n_seq, n):
             assert O.rel_l2(got[r], want[r]) <= G.ATTN_TOL, (s, r)
     for b in (qkv, out, work, *held):
         b.free()
+
+
+@pytest.mark.parametrize("top", [58, 59, 61, 64])
+@pytest.mark.parametrize("rows,n,offset", [(1, 65, 0), (40, 66, 3), (3, 67, 1), (200, 71, 2), (9, 8195, 0), (40, 8200, 1), (2, 16390, 3), (3, 151937, 2)])
+def test_lists_that_are_nearly_full_and_rows_that_begin_and_end_anywhere(ctx, rows, n, offset, top):
+    """The best of a row's body nearly fill the list before what stands before and behind it is added: the largest of them there, and the smallest."""
+    rng = np.random.default_rng(n + top)
+    logits = rng.standard_normal((rows, n)).astype(np.float32)
+    logits[::2, :4], logits[::2, -4:] = 9, 8
+    logits[1::2, :4] = logits[1::2, -4:] = -9
+    ids = rng.integers(0, n, rows)
+    a, got = G._logprobs(ctx, logits, ids, top, n + rows % 4, offset)
+    ctx.enqueue(A.OP_LOGPROBS, a)
+    G._check_logprobs(logits, ids, top, got())

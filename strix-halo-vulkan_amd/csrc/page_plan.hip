@@ -2,7 +2,8 @@
 //
 // With want = ceil((pos + rows) / page): back = held - max(want, shared), need = want - held, each where above zero.  The pages given back lie behind the
 // free ones, L = free | back in order, A = |L|; sequence s's j-th new page is L[A - 1 - (taken before it) - j].  All of that is two scans over the
-// sequences, of (back, need, rows) and of what is granted, and lookups by bisection from there on.
+// sequences, of (back, need, rows) and of what is granted, and lookups by bisection from there on.  Entries that come back and are no page are not in L: what comes back is looked at beside
+// the second scan (two passes of 48 sequences 8.6 us and 8.1 without it, of 900 22.1 and 19.0), and where some of it is none the grants are made again and places found by a scan over runs of entries.
 // Bound by the chain of trips to memory (a sequence's words, then pages, then the stores) and the scans' barriers, not by bytes: 48 sequences of a token each take 2.9 to 3.6 us
 // of the kernel's own time, 900 with 12007 rows 8 to 10.  Every block makes the scans for itself, which costs less than a launch between them and the
 // rows; a row a thread, since each is a bisection and two dependent loads (four a thread: 26 us for 19 of the 900 sequences' two passes).  The words that others
@@ -21,6 +22,8 @@ constexpr int kMaxRows = 1 << 20;
 // one block; with 4, where a call of 48 sequences has two blocks, that takes 10.1 instead of 9.4.
 constexpr int kPagesFrom = 16;
 
+constexpr int kOwn = 2, kAtOnce = 4;  // entries that come back: of a sequence by its own lane, and loads of a wave on their way of the others
+
 // WAVE, up to 64 sequences: each wave makes the scans for itself and writes to LDS what the others write, without a barrier up to the last.  (48 sequences, two passes: 9.1 us, and 10.1 by a
 // block's scans with two barriers each.)
 template <int T, bool WAVE>
@@ -28,11 +31,12 @@ __global__ __launch_bounds__(T) void page_plan_kernel(shv_page_plan_args a, int 
     constexpr int kPer = T == 1024 ? kMaxSeqs / T : 1;  // sequences a thread, side by side
     __shared__ uint32_t s_start[kPer * T], s_taken[kPer * T], s_back[kPer * T];
     __shared__ int s_held[kPer * T], s_pos[kPer * T];
-    __shared__ uint32_t waves[3][T / 64];
-    __shared__ int is_last;
+    __shared__ uint32_t waves[3][T / 64], s_run[T];
+    __shared__ int is_last, is_odd, n_many;
     const int tid = threadIdx.x;
     static_assert(!WAVE || kPer == 1, "a lane a sequence");
     const int first = WAVE ? tid & 63 : tid * kPer;
+    if (!WAVE && tid == 0) is_odd = n_many = 0;
     int rows[kPer], pos[kPer], held[kPer], shared[kPer];
 #pragma unroll
     for (int u = 0; u < kPer; u++) {
@@ -59,34 +63,122 @@ __global__ __launch_bounds__(T) void page_plan_kernel(shv_page_plan_args a, int 
     }
     if constexpr (WAVE) wave_scan(sums, total);
     else block_scan<T, 3>(sums, total, waves);
-    const uint32_t n_back = total[0], avail = n_free + n_back;
-    uint32_t take[kPer], gets[kPer], both[2] = {0, 0}, total2[2];
+    const uint32_t n_back = total[0];
     {
-        uint32_t b = sums[0], n = sums[1], r = sums[2];
+        uint32_t b = sums[0];
 #pragma unroll
         for (int u = 0; u < kPer; u++) {
             s_back[first + u] = b;
-            b = add_up_to(b, back[u]), n = add_up_to(n, need[u]), r = add_up_to(r, asked[u]);
-            const bool granted = fits[u] && (need[u] == 0 || n <= avail) && r <= static_cast<uint32_t>(a.max_rows);
-            take[u] = granted ? need[u] : 0;
-            gets[u] = granted ? asked[u] : 0;
-            both[0] += take[u], both[1] += gets[u];  // (at most avail and max_rows together)
+            b = add_up_to(b, back[u]);
+            s_held[first + u] = held[u], s_pos[first + u] = pos[u];
         }
     }
-    if constexpr (WAVE) wave_scan(both, total2);
-    else block_scan<T, 2>(both, total2, waves);
-    const uint32_t n_taken = total2[0], n_rows = total2[1];
-    {
-        uint32_t t = both[0], r = both[1];
+    // The r-th entry that comes back, one of sequence s.
+    const auto entry = [&](uint32_t r, int s) {
+        const int low = s_held[s] - static_cast<int>((s + 1 < a.n_seq ? s_back[s + 1] : n_back) - s_back[s]);
+        return a.table[static_cast<size_t>(s) * a.max_pages + low + (r - s_back[s])];
+    };
+    const auto is_page = [&](int e) { return e >= 0 && e < a.n_pages; };
+    // All of them are looked at: the first few of a sequence by its lane, the others by a wave, 64 a load.  The last loads are on their way while the grants are made.
+    int own[kPer][kOwn], others[kAtOnce];
+    bool odd = false;
+    if (n_back > 0) {
+        const int lane = tid & 63;
+#pragma unroll
+        for (int i = 0; i < kAtOnce; i++) others[i] = 0;
+        const auto look = [&](int s, int low, int n) {
+            const int32_t *of = a.table + static_cast<size_t>(s) * a.max_pages + low;
+            for (int at = kOwn + lane; __ballot(at < n) != 0ull; at += 64 * kAtOnce) {
+                int e[kAtOnce];
+#pragma unroll
+                for (int i = 0; i < kAtOnce; i++) e[i] = at + 64 * i < n ? of[at + 64 * i] : 0;
+#pragma unroll
+                for (int i = 0; i < kAtOnce; i++) {
+                    odd |= !is_page(others[i]);
+                    others[i] = e[i];
+                }
+            }
+        };
 #pragma unroll
         for (int u = 0; u < kPer; u++) {
-            s_taken[first + u] = t, s_start[first + u] = r;
-            s_held[first + u] = held[u], s_pos[first + u] = pos[u];
-            t += take[u], r += gets[u];
+            const int32_t *mine = a.table + static_cast<size_t>(first + u) * a.max_pages + (held[u] - back[u]);
+#pragma unroll
+            for (int i = 0; i < kOwn; i++) own[u][i] = i < back[u] ? mine[i] : 0;
+            if (!WAVE && back[u] > kOwn) s_taken[atomicAdd(&n_many, 1)] = first + u;
+        }
+        if constexpr (WAVE) {
+            for (uint64_t many = __ballot(back[0] > kOwn); many != 0; many &= many - 1) {
+                const int l = __ffsll(static_cast<unsigned long long>(many)) - 1, n = __builtin_amdgcn_readlane(back[0], l);
+                look(l, __builtin_amdgcn_readlane(held[0], l) - n, n);
+            }
+        } else {
+            __syncthreads();
+            for (int i = tid >> 6; i < n_many; i += T / 64) {
+                const int s = __builtin_amdgcn_readfirstlane(s_taken[i]), n = static_cast<int>((s + 1 < a.n_seq ? s_back[s + 1] : n_back) - s_back[s]);
+                look(s, s_held[s] - n, n);
+            }
         }
     }
-    if constexpr (WAVE) __builtin_amdgcn_wave_barrier();
-    else __syncthreads();
+    uint32_t run = 0;
+    uint32_t avail = n_free + n_back, n_given = n_back, n_taken, n_rows;
+    uint32_t take[kPer], gets[kPer];
+    for (bool again = false;; again = true) {
+        uint32_t both[2] = {0, 0}, total2[2];
+        {
+            uint32_t n = sums[1], r = sums[2];
+#pragma unroll
+            for (int u = 0; u < kPer; u++) {
+                n = add_up_to(n, need[u]), r = add_up_to(r, asked[u]);
+                const bool granted = fits[u] && (need[u] == 0 || n <= avail) && r <= static_cast<uint32_t>(a.max_rows);
+                take[u] = granted ? need[u] : 0;
+                gets[u] = granted ? asked[u] : 0;
+                both[0] += take[u], both[1] += gets[u];  // (at most avail and max_rows together)
+            }
+        }
+        if constexpr (WAVE) wave_scan(both, total2);
+        else block_scan<T, 2>(both, total2, waves);
+        n_taken = total2[0], n_rows = total2[1];
+        {
+            uint32_t t = both[0], r = both[1];
+#pragma unroll
+            for (int u = 0; u < kPer; u++) {
+                s_taken[first + u] = t, s_start[first + u] = r;
+                t += take[u], r += gets[u];
+            }
+        }
+        if (n_back > 0 && !again) {
+#pragma unroll
+            for (int u = 0; u < kPer; u++)
+#pragma unroll
+                for (int i = 0; i < kOwn; i++) odd |= !is_page(own[u][i]);
+#pragma unroll
+            for (int i = 0; i < kAtOnce; i++) odd |= !is_page(others[i]);
+            odd = __ballot(odd) != 0ull;
+            if (!WAVE && odd) is_odd = 1;
+        }
+        if constexpr (WAVE) {
+            if (again) __syncthreads();
+            else __builtin_amdgcn_wave_barrier();
+        } else {
+            __syncthreads();
+            odd = is_odd != 0;
+        }
+        if (!odd || again) break;
+        // what is a page among a run of them, a run a thread, and before it
+        run = (n_back + T - 1) / T;
+        uint32_t v[1] = {0}, all[1], end = 0;
+        int s = 0;
+        for (uint32_t r = min(tid * run, n_back); r < min((tid + 1) * run, n_back); r++) {
+            if (r >= end) {
+                s = last_not_above(s_back, a.n_seq, r);
+                end = s + 1 < a.n_seq ? s_back[s + 1] : n_back;
+            }
+            v[0] += is_page(entry(r, s));
+        }
+        block_scan<T, 1>(v, all, waves);
+        s_run[tid] = v[0];
+        n_given = all[0], avail = n_free + n_given;
+    }
     if (blockIdx.x == 0) {
         for (int s = tid; s < a.n_seq; s += T) {
             a.start[s] = s_start[s];
@@ -94,10 +186,14 @@ __global__ __launch_bounds__(T) void page_plan_kernel(shv_page_plan_args a, int 
         }
         if (tid == 0) a.start[a.n_seq] = n_rows;
     }
-    const auto given_back = [&](uint32_t r) {
-        const int s = last_not_above(s_back, a.n_seq, r);
-        const int low = s_held[s] - static_cast<int>((s + 1 < a.n_seq ? s_back[s + 1] : n_back) - s_back[s]);
-        return a.table[static_cast<size_t>(s) * a.max_pages + low + (r - s_back[s])];
+    const auto given_back = [&](uint32_t i) {
+        if (n_given == n_back) return entry(i, last_not_above(s_back, a.n_seq, i));
+        const int of = last_not_above(s_run, T, i);
+        uint32_t r = of * run, left = i - s_run[of];
+        for (;; r++) {
+            const int e = entry(r, last_not_above(s_back, a.n_seq, r));
+            if (r + 1 >= n_back || (is_page(e) && left-- == 0)) return e;
+        }
     };
     const auto taken = [&](uint32_t e) {  // the e-th page from the top
         const uint32_t i = avail - 1 - e;
@@ -117,7 +213,7 @@ __global__ __launch_bounds__(T) void page_plan_kernel(shv_page_plan_args a, int 
         const int s = last_not_above(s_taken, a.n_seq, e);
         a.table[static_cast<size_t>(s) * a.max_pages + s_held[s] + (e - s_taken[s])] = taken(e);
     }
-    for (uint32_t r = me; r < n_back && n_free + r < static_cast<uint32_t>(a.n_pages); r += step) a.free_pages[n_free + r] = given_back(r);
+    for (uint32_t r = me; r < n_given && n_free + r < static_cast<uint32_t>(a.n_pages); r += step) a.free_pages[n_free + r] = given_back(r);
     if (gridDim.x > 1) {
         if (!arrive_last(counter, gridDim.x, &is_last)) return;
     } else if (WAVE) {

@@ -71,3 +71,97 @@ def test_lists_that_are_nearly_full_and_rows_that_begin_and_end_anywhere(ctx, ro
     a, got = G._logprobs(ctx, logits, ids, top, n + rows % 4, offset)
     ctx.enqueue(A.OP_LOGPROBS, a)
     G._check_logprobs(logits, ids, top, got())
+
+
+# ---- pages that the host has taken out of a table ---------------------------------------------
+
+
+def plan_of_pages(rows, pos, table, held, free, n_free, shared, page, max_pages, max_rows, with_base):
+    """The plan, request by request, where entries that are no page are passed over as they are given back."""
+    n_pages, n = len(free), len(rows)
+    stack, table, held, pos = [int(x) for x in free[:n_free]], table.copy(), list(map(int, held)), list(map(int, pos))
+    base, want = list(pos), [0 if r < 0 else -(-(p + int(r)) // page) for r, p in zip(rows, pos)]
+    ok = [rows[s] < 0 or (pos[s] >= 0 and want[s] <= max_pages) for s in range(n)]
+    for s in range(n):
+        if ok[s]:
+            keep = min(held[s], max(want[s], min(int(shared[s]), held[s]) if shared is not None else 0))
+            stack += [int(e) for e in table[s, keep:held[s]] if 0 <= e < n_pages]
+            held[s] = 0 if rows[s] < 0 else keep
+    avail, wished, asked, start, maps = len(stack), 0, 0, [0], []
+    for s in range(n):
+        lot = max(0, int(rows[s])) if ok[s] else 0
+        if ok[s] and rows[s] >= 0:
+            need = max(0, want[s] - held[s])
+            wished, asked = wished + need, asked + lot
+            if (need and wished > avail) or asked > max_rows:
+                lot = 0
+            else:
+                for _ in range(need):
+                    table[s, held[s]] = stack.pop()
+                    held[s] += 1
+                for p in range(pos[s], pos[s] + lot):
+                    e = int(table[s, p // page])
+                    maps.append((s, p, e * page + p % page if 0 <= e < n_pages else -1))
+                if with_base:
+                    pos[s] += lot
+        else:
+            lot = 0
+            if ok[s] and with_base:
+                pos[s] = 0
+        start.append(start[-1] + lot)
+    after = free.copy()
+    after[:len(stack)] = stack
+    return dict(table=table, held=np.array(held), free=after, n_free=len(stack), pos=np.array(pos), start=np.array(start), maps=np.array(maps, np.int64).reshape(-1, 3), base=np.array(base))
+
+
+def take_out(t, chance):
+    """Entries of the host's tables that become no page, each at such a chance; what they named is lost, as to another pool."""
+    for s in range(t.n_seq):
+        out = t.rng.random(t.held[s]) < chance
+        t.table[s, :t.held[s]][out] = t.rng.choice([-1, -99, -2**31, t.n_pages, 2**31 - 1], int(out.sum()))
+
+
+@pytest.mark.parametrize("n_seq,page,max_pages,longest,spare,max_rows,kw", [
+    (1, 32, 4, 100, 0, 5, {}), (2, 32, 40, 1200, 1, 100, dict(shared=False)), (48, 64, 20, 900, 0, 48, {}), (64, 32, 190, 6000, 0, 200, dict(shared=False)), (65, 256, 9, 1000, 4, 500, {}),
+    (256, 32, 200, 6000, 10, 4000, dict(shared=False)), (900, 32, 200, 3000, 30, 12007, {}), (2048, 32, 12, 200, 100, 20000, dict(shared=False))])
+@pytest.mark.parametrize("chance", [0.05, 0.5, 1.0])
+def test_pages_that_were_taken_out_are_not_given_back(ctx, monkeypatch, n_seq, page, max_pages, longest, spare, max_rows, kw, chance):
+    """Sequences some of whose pages are out of their tables end, go back and grow, in one pass with others that take what came back."""
+    monkeypatch.setattr(P, "plan", plan_of_pages)
+    t = G.Plan(n_seq + page + 1, n_seq, page, max_pages, longest, spare, max_rows, **kw)
+    t.upload(ctx)
+    seen = [np.full(max_rows, -5, np.int32) for _ in range(3)]
+    for step in range(5):
+        take_out(t, chance)
+        t.d["table"].write(t.table)
+        rows = np.where(t.rng.random(n_seq) < 0.2, t.rng.integers(0, max(2, max_rows // 3), n_seq), t.rng.integers(0, 3, n_seq))
+        rows = np.where(t.rng.random(n_seq) < 0.3, -1, rows).astype(np.int32)
+        if step == 2:
+            t.pos = np.where(t.rng.random(n_seq) < 0.5, t.pos // 2, t.pos).astype(np.int32)
+            t.d["pos"].write(t.pos)
+        t.d["rows"].write(rows)
+        ctx.enqueue(A.OP_PAGE_PLAN, t.args())
+        w = t.check(rows, seen)
+        stack = w["free"][:w["n_free"]]
+        assert ((stack >= 0) & (stack < t.n_pages)).all() and len(set(stack.tolist())) == len(stack)
+
+
+def test_a_windows_pages_come_back_once(ctx, monkeypatch):
+    """A window's pages go from a table to the stack by the host's hand, the sequence ends, another takes all there is: every page is handed out once and no entry that is none."""
+    monkeypatch.setattr(P, "plan", plan_of_pages)
+    t = G.Plan(9, 2, 32, 20, 0, 0, 700, odd=False, shared=False)
+    t.pos[:] = [32 * 9 + 5, 0]
+    t.n_pages = 10
+    t.table[0, :10] = t.rng.permutation(10)
+    t.held[:] = [10, 0]
+    t.free = np.full(10, -77, np.int32)
+    out = t.table[0, 1:7].copy()
+    t.table[0, 1:7] = -1
+    t.free[:6], t.n_free = out, 6
+    t.upload(ctx)
+    rows = np.array([-1, 320], np.int32)
+    t.d["rows"].write(rows)
+    ctx.enqueue(A.OP_PAGE_PLAN, t.args())
+    w = t.check(rows, [np.full(700, -5, np.int32) for _ in range(3)])
+    assert list(w["start"]) == [0, 0, 320] and w["n_free"] == 0
+    assert sorted(t.table[1, :10].tolist()) == list(range(10)) and (w["maps"][:, 2] >= 0).all()

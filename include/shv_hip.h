@@ -742,9 +742,9 @@ typedef struct {
 
 /* The pages of a pass.  Sequence s has kept pos[s] tokens, holds held[s] pages, the first held[s] entries of its table row, and wants room for rows[s] more tokens:
  *   rows >= 0: ceil((pos + rows) / page) pages.  Entries past those are given back, as after a branch that was not kept;
- *   rows <  0: the sequence ends and gives all of them back.
+ *   rows <  0: the sequence ends and gives all of them back, whatever its pos.
  * Its first shared[s] entries are another's (a common prefix), which are used and never given back; NULL: none.  Entries among the held ones that are no page (below 0, n_pages and
- * more: the host has taken a page out that a window has passed, and laid it on the stack or kept it) are held as the others are and passed over where they would be given back: the stack holds pages alone.  A sequence whose pos is below 0, or whose
+ * more: the host has taken a page out that a window has passed, and laid it on the stack or kept it) are held as the others are and passed over where they would be given back: the stack holds pages alone.  A sequence that does not end and whose pos is below 0, or whose
  * tokens would not fit max_pages pages, is left as it is and gets no rows.
  * free_pages [n_pages] is a stack of n_free[0] pages.  First every page given back is laid on it, sequence by sequence, a table row's lower entry first; then
  * what is wanted is taken from its top, sequence by sequence.  What sequences want is counted up in order: from the first one on whose pages do not suffice, those that

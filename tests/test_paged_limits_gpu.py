@@ -165,3 +165,21 @@ def test_a_windows_pages_come_back_once(ctx, monkeypatch):
     w = t.check(rows, [np.full(700, -5, np.int32) for _ in range(3)])
     assert list(w["start"]) == [0, 0, 320] and w["n_free"] == 0
     assert sorted(t.table[1, :10].tolist()) == list(range(10)) and (w["maps"][:, 2] >= 0).all()
+
+
+@pytest.mark.parametrize("n_seq", [4, 70, 300])
+@pytest.mark.parametrize("base", [True, False])
+def test_a_sequence_without_a_position_ends_and_is_otherwise_left_alone(ctx, n_seq, base):
+    """pos below 0: with rows below 0 all its pages come back, with any other rows it keeps them and has no row."""
+    t = G.Plan(n_seq, n_seq, 32, 20, 500, 4, 900, odd=False, shared=False, base=base)
+    t.pos[::2] = -1 - np.arange(len(t.pos[::2]))
+    t.upload(ctx)
+    rows = np.ones(n_seq, np.int32)
+    rows[::4], rows[2::8] = -3, 0
+    t.d["rows"].write(rows)
+    held, free, pos = t.held.copy(), t.n_free, t.pos.copy()
+    ctx.enqueue(A.OP_PAGE_PLAN, t.args())
+    w = t.check(rows, [np.full(900, -5, np.int32) for _ in range(3)])
+    assert (w["held"][::4] == 0).all() and np.array_equal(w["held"][2::4], held[2::4]) and (np.diff(w["start"])[::2] == 0).all()
+    assert np.array_equal(w["pos"][2::4], pos[2::4])
+    assert w["n_free"] == free + held[::4].sum() - (w["held"][1::2] - held[1::2]).sum()

@@ -777,7 +777,7 @@ __device__ __forceinline__ void run_piece(const shv_attn_paged_args &a, const Pl
             for (int e = 0; e < 8; e++) mx = fmaxf(mx, s[e]);
             mx = max_over_q(mx);
             // the sums are rescaled a few times a run instead of whenever some row's maximum moves
-            const bool moves = mx * c2 > fmaf(m_run[g], c2, kSlack);
+            const bool moves = (mx - m_run[g]) * c2 > kSlack;  // (infinity less infinity: no)
             if (__ballot(moves) != 0ull) {
                 const float m_new = moves ? mx : m_run[g];
                 const float alpha = m_new == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((m_run[g] - m_new) * c2);
@@ -793,10 +793,11 @@ __device__ __forceinline__ void run_piece(const shv_attn_paged_args &a, const Pl
 #pragma unroll
                     for (int e = 0; e < 4; e++) o[g][db][e] *= av[e];
             }
-            const float m2 = fmaf(m_run[g] == -INFINITY ? 0.f : m_run[g], c2, -kLift);
+            // the difference first: of scores past 2^24 their scaled values' roundings alone would send a weight past binary16
+            const float m0 = m_run[g] == -INFINITY ? 0.f : m_run[g];
 #pragma unroll
             for (int e = 0; e < 8; e++) {
-                s[e] = __builtin_amdgcn_exp2f(fmaf(s[e], c2, -m2));
+                s[e] = __builtin_amdgcn_exp2f(fmaf(s[e] - m0, c2, kLift));
                 l_run[g] += s[e];
             }
         }

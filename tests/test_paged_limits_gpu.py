@@ -183,3 +183,41 @@ def test_a_sequence_without_a_position_ends_and_is_otherwise_left_alone(ctx, n_s
     assert (w["held"][::4] == 0).all() and np.array_equal(w["held"][2::4], held[2::4]) and (np.diff(w["start"])[::2] == 0).all()
     assert np.array_equal(w["pos"][2::4], pos[2::4])
     assert w["n_free"] == free + held[::4].sum() - (w["held"][1::2] - held[1::2]).sum()
+
+
+# ---- scores of any size --------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("leads", [False, True])
+@pytest.mark.parametrize("layout,norm,n,pos", [
+    ((16, 2, 256, 0), 1500, [1, 1, 1], [3000, 700, 40]), ((16, 2, 256, 0), 2000, [40, 1], [500, 2000]), ((16, 2, 256, 0), 2000, [300], [100]), ((12, 2, 128, 0), 2000, [1, 90], [2500, 300]),
+    ((8, 8, 64, 0), 2000, [1, 200], [2500, 30]), ((16, 2, 256, 0), 4000, [3, 50], [900, 77])])
+def test_scores_of_the_largest_norm_weights(ctx, monkeypatch, layout, norm, n, pos, leads):
+    """Queries and keys that point one way under large norm weights, scores past 2^24 powers of two, whose last places are several powers of two each: a row's output is a mean of the
+    values it sees whatever its weights are, so between their smallest and their largest; where one cell leads by more than all roundings it is that cell's value.  Weights enter to 22
+    bits and sums of at most a hundred tiles are float32: 2^-21 + 100 2^-24 < 1e-5 of the largest value."""
+    monkeypatch.setitem(G.LAYOUTS, "own", layout)
+    t = G.Paged(norm + n[0] + pos[0], "own", n, pos, 64)
+    u = np.sign(t.rng.standard_normal(t.d)).astype(np.float32)
+    t.q_norm[:] = t.k_norm[:] = norm
+    t.qkv[:, :2 * t.nh * t.d].reshape(-1, t.nh, 2, t.d)[:, :, 0] = u
+    t.qkv[:, 2 * t.nh * t.d:2 * t.nh * t.d + t.nkv * t.d] = np.tile(np.where(np.arange(t.d) < 8, 1e-3, 1) * u, t.nkv)
+    few = (0.03 * t.rng.standard_normal(t.kp.shape)).astype(np.float16)  # a few powers of two by the first dims
+    t.kp[:] = np.where(np.arange(t.d) < 8, few, (norm * u).astype(np.float16))
+    lead = [int(t.rng.integers(0, p)) for p in pos]
+    if leads:
+        for s, c in enumerate(lead):
+            where = tuple(int(x[0]) for x in t.cells(s, c, c + 1))
+            t.kp[where] = (norm * u).astype(np.float16)
+    t.upload(ctx)
+    ctx.enqueue(A.OP_ATTN_PAGED, t.args(ctx))
+    out, _, vp = t.results()
+    for s in range(len(n)):
+        seen = vp[t.cells(s, 0, pos[s] + n[s])].astype(np.float64)
+        for i in range(n[s]):
+            got = out[t.start[s] + i].reshape(t.nkv, -1, t.d)
+            v = seen[:pos[s] + i + 1]
+            tol = 1e-5 * np.abs(v).max()
+            low, high = (v[lead[s]], v[lead[s]]) if leads else (v.min(0), v.max(0))
+            assert np.isfinite(got).all(), (s, i)
+            assert (got >= low[:, None] - tol).all() and (got <= high[:, None] + tol).all(), (s, i)

@@ -537,9 +537,10 @@ __global__ __launch_bounds__(64 * W, W == 4 || D == 256 ? 2 : 4) void tree_attn_
         for (int e = 0; e < 8; e++) mx = fmaxf(mx, s[e]);
         mx = max_over_q(mx);
         // the sums are rescaled a few times a slice instead of whenever some row's maximum moves
-        const bool moves = mx * c2 > fmaf(m_run, c2, kSlack);
+        const bool moves = (mx - m_run) * c2 > kLift + kSlack;  // (infinity less infinity: no)
         if (__ballot(moves) != 0ull) {
-            const float m_new = moves ? mx : m_run;
+            // m_run stands kLift below the maximum, or where its last places are too large for that, at it
+            const float low = mx - kLift / c2, m_new = !moves ? m_run : (mx - low) * c2 > kLift + kSlack ? mx : low;
             const float alpha = m_new == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((m_run - m_new) * c2);
             l_run *= alpha;
             m_run = m_new;
@@ -551,11 +552,12 @@ __global__ __launch_bounds__(64 * W, W == 4 || D == 256 ? 2 : 4) void tree_attn_
 #pragma unroll
                 for (int e = 0; e < 4; e++) o[db][e] *= av[e];
         }
-        const float m2 = fmaf(m_run == -INFINITY ? 0.f : m_run, c2, -kLift);
+        // the difference first: of scores past 2^24 their scaled values' roundings alone would send a weight past binary16
+        const float m0 = m_run == -INFINITY ? 0.f : m_run;
         float pv[8];
 #pragma unroll
         for (int e = 0; e < 8; e++) {
-            pv[e] = __builtin_amdgcn_exp2f(fmaf(s[e], c2, -m2));
+            pv[e] = __builtin_amdgcn_exp2f((s[e] - m0) * c2);
             l_run += pv[e];
         }
         if (part) {

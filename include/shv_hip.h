@@ -778,7 +778,7 @@ typedef struct {
  * out [max_rows][n_head*head_dim], before the sigmoid gate.  A query's values, normed and rotated, lie within binary16's range (norm weights up to 2000 keep them there).
  * A sequence whose start is out of order or past max_rows, or whose positions are not within 0 .. max_pages * page - 1, gets no output.
  * work: work_bytes of scratch, 16-byte aligned, as many as shv_attn_paged_work says for these sizes; a call uses it alone, calls of one stream may share it.
- * max_rows * (n_head / n_head_kv) is at most 2^20. */
+ * max_rows * (n_head / n_head_kv) is at most 2^20, max_rows * n_head_kv at most 2^25. */
 typedef struct {
     const float *qkv;
     const float *q_norm;

@@ -1072,6 +1072,8 @@ int check_sizes(const shv_attn_paged_args &a) {
                 "attn_paged: %d query heads over %d KV heads; 1..64 per KV head, 1024 in all", a.n_head, a.n_head_kv);
     SHV_REQUIRE(a.max_rows >= 1 && static_cast<long long>(a.max_rows) * (a.n_head / a.n_head_kv) <= 1 << 20, "attn_paged: %d rows of %d query heads per KV head; at most 2^20 together",
                 a.max_rows, a.n_head / a.n_head_kv);
+    // (of the cells' launch: 96 threads at most for each, fewer than 2^32 in all)
+    SHV_REQUIRE(static_cast<long long>(a.max_rows) * a.n_head_kv <= 1 << 25, "attn_paged: %d rows of %d KV heads; at most 2^25 together", a.max_rows, a.n_head_kv);
     SHV_REQUIRE(a.page >= 32 && a.page <= 4096 && (a.page & (a.page - 1)) == 0, "attn_paged: page %d; a power of two from 32 to 4096", a.page);
     SHV_REQUIRE(a.n_pages >= 1 && static_cast<long long>(a.n_pages) * a.page < 1ll << 31, "attn_paged: %d pages of %d cells; fewer than 2^31 cells", a.n_pages, a.page);
     SHV_REQUIRE(a.max_pages >= 1 && static_cast<long long>(a.max_pages) * a.page < 1ll << 31, "attn_paged: max_pages %d of %d cells; fewer than 2^31 cells", a.max_pages, a.page);

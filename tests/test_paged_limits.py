@@ -21,3 +21,11 @@ def test_no_accepted_call_has_more_query_blocks_than_a_plan_holds(d, rep, n_seq,
     rc, got = _work(head_dim=d, n_head=rep, n_head_kv=1, n_seq=n_seq, max_rows=max_rows, rope_dims=0)
     assert rc == 0
     assert got <= MOST_BLOCKS * (64 + 32) + 2 * 128 * (d + 2) * 4 + 4096
+
+
+@pytest.mark.parametrize("heads,rows", [(1024, (1 << 15) + 1), (64, (1 << 19) + 1), (33, 1 << 20)])
+def test_more_cells_than_a_launch_has_threads_for_are_refused(heads, rows):
+    kw = dict(n_head=heads, n_head_kv=heads, head_dim=64, rope_dims=0, qkv_stride=heads * 256)
+    assert _work(**kw, max_rows=rows) == (-1, -5)
+    B._refused("shv_attn_paged", B.attn(**kw, max_rows=rows), "KV heads")
+    assert _work(**kw, max_rows=(1 << 25) // heads)[0] == 0

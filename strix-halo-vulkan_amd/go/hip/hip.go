@@ -469,7 +469,7 @@ type QSAArgs struct {
 func QSAIndex(d QSAArgs) Op {
 	var a C.shv_qsa_index_args
 	a.x, a.gamma, a.w, a.q_norm, a.k_norm, a.rope = fp(d.X), fp(d.Gamma), fp(d.W), fp(d.QNorm), fp(d.KNorm), fp(d.Rope)
-	a.idxcache, a.pooled = vp(d.IdxCache), fp(d.Pooled)
+	a.idxcache, a.pooled = (*C.uint16_t)(vp(d.IdxCache)), fp(d.Pooled)
 	a.pos, a.slot = ip(d.Rows.Pos), ip(d.Rows.Slot)
 	a.work, a.score, a.mask = fp(d.Work), fp(d.Score), (*C.uint32_t)(vp(d.Mask))
 	a.n_seq, a.seq_len, a.n_embd = C.int32_t(d.Rows.NSeq), C.int32_t(d.Rows.SeqLen), C.int32_t(d.NEmbd)

@@ -4,7 +4,7 @@
 // package llm what package vk offers it (vk/engine.go) for the token loop's ops.
 //
 // NOT COMPILED IN THIS REPOSITORY: the build image has no Go toolchain, so this file has been
-// checked by eye against the header only.  It is the binding a maintainer of the reference adds
+// checked by eye and as text against the header only.  It is the binding a maintainer of the reference adds
 // beside vk/ (build tag shv_hip); llm/gpu_moe_hip.go next to it shows one block's op list built
 // on it.  The C++ mirror in host/llm.cpp is the same code compiled and tested.
 package hip
@@ -451,6 +451,77 @@ func TreeAccept(logits, ids, best, path, nKeep, next, pos, base *Buffer, t Tree,
 	a.n_seq, a.rows, a.n, a.logits_stride = C.int32_t(t.NSeq), C.int32_t(t.Rows), C.int32_t(n), C.int32_t(stride)
 	a.max_cells = C.int32_t(t.MaxCells)
 	return mk(C.SHV_OP_TREE_ACCEPT, unsafe.Pointer(&a), C.sizeof_shv_tree_accept_args)
+}
+
+// PagedBatch names the packed rows of a batch's pass over a pool of cache pages: NSeq sequences of MaxPages table entries each, NPages pages of
+// Page cells, up to MaxRows rows.  Start, RowPos and RowCell are PagePlan's results, Table its state; one plan serves every layer.
+type PagedBatch struct {
+	NSeq, MaxRows                 int
+	Page, MaxPages, NPages        int
+	Table, Start, RowPos, RowCell *Buffer // device int32
+}
+
+// PagePlan settles which pages the pass's new tokens go to: rows holds how many each sequence brings, below 0 where it ends.  shared (pages of a
+// common prefix), rowSeq and base (takes the positions, which then move on by themselves) may be nil.
+func PagePlan(rows, pos, held, freePages, nFree, shared, rowSeq, base *Buffer, b PagedBatch) Op {
+	var a C.shv_page_plan_args
+	a.rows, a.pos, a.table, a.held = ip(rows), ip(pos), ip(b.Table), ip(held)
+	a.free_pages, a.n_free, a.shared = ip(freePages), ip(nFree), ip(shared)
+	a.start, a.row_seq, a.row_pos, a.row_cell, a.base = ip(b.Start), ip(rowSeq), ip(b.RowPos), ip(b.RowCell), ip(base)
+	a.n_seq, a.page, a.max_pages = C.int32_t(b.NSeq), C.int32_t(b.Page), C.int32_t(b.MaxPages)
+	a.n_pages, a.max_rows = C.int32_t(b.NPages), C.int32_t(b.MaxRows)
+	return mk(C.SHV_OP_PAGE_PLAN, unsafe.Pointer(&a), C.sizeof_shv_page_plan_args)
+}
+
+// AttnPagedArgs are the fields of shv_attn_paged_args a caller sets.
+type AttnPagedArgs struct {
+	QKV, QNorm, KNorm, Rope *Buffer
+	KPages, VPages          *Buffer // a layer's pool
+	Work, Out               *Buffer // scratch of AttnPagedWork bytes, which all layers share; before the sigmoid gate
+	Batch                   PagedBatch
+	NHead, NHeadKV, HeadDim int
+	RopeDims, QKVStride     int
+	Window, Sinks           int // Window 0: every cell
+	Eps                     float32
+}
+
+// AttnPaged writes the packed rows' cells and attends over each sequence's pages.
+func AttnPaged(d AttnPagedArgs) Op {
+	a := d.args()
+	return mk(C.SHV_OP_ATTN_PAGED, unsafe.Pointer(&a), C.sizeof_shv_attn_paged_args)
+}
+
+// AttnPagedWork is how many bytes of Work these sizes need on this device.
+func (d *Device) AttnPagedWork(p AttnPagedArgs) (uint64, error) {
+	a := p.args()
+	var n C.int64_t
+	err := call(func() C.int { return C.shv_attn_paged_work(d.ctx, &a, &n) })
+	return uint64(n), err
+}
+
+func (d AttnPagedArgs) args() C.shv_attn_paged_args {
+	var a C.shv_attn_paged_args
+	a.qkv, a.q_norm, a.k_norm, a.rope = fp(d.QKV), fp(d.QNorm), fp(d.KNorm), fp(d.Rope)
+	a.kpages, a.vpages, a.work, a.out = vp(d.KPages), vp(d.VPages), vp(d.Work), fp(d.Out)
+	a.table, a.start, a.row_pos, a.row_cell = ip(d.Batch.Table), ip(d.Batch.Start), ip(d.Batch.RowPos), ip(d.Batch.RowCell)
+	if d.Work != nil {
+		a.work_bytes = C.int64_t(d.Work.size)
+	}
+	a.n_seq, a.max_rows = C.int32_t(d.Batch.NSeq), C.int32_t(d.Batch.MaxRows)
+	a.n_head, a.n_head_kv, a.head_dim, a.rope_dims = C.int32_t(d.NHead), C.int32_t(d.NHeadKV), C.int32_t(d.HeadDim), C.int32_t(d.RopeDims)
+	a.page, a.max_pages, a.n_pages, a.qkv_stride = C.int32_t(d.Batch.Page), C.int32_t(d.Batch.MaxPages), C.int32_t(d.Batch.NPages), C.int32_t(d.QKVStride)
+	a.window, a.sinks, a.eps = C.int32_t(d.Window), C.int32_t(d.Sinks), C.float(d.Eps)
+	return a
+}
+
+// LogProbs answers rows of logits with the log probability of each row's token, the entropy and the top most likely tokens.  ids and logprob go
+// together, as do topIds, topLogprobs and top above 0; each may be nil.
+func LogProbs(logits, ids, logprob, entropy, topIds, topLogprobs *Buffer, rows, n, stride, top int) Op {
+	var a C.shv_logprobs_args
+	a.logits, a.ids, a.logprob, a.entropy = fp(logits), ip(ids), fp(logprob), fp(entropy)
+	a.top_ids, a.top_logprobs = ip(topIds), fp(topLogprobs)
+	a.n_rows, a.n, a.logits_stride, a.n_top = C.int32_t(rows), C.int32_t(n), C.int32_t(stride), C.int32_t(top)
+	return mk(C.SHV_OP_LOGPROBS, unsafe.Pointer(&a), C.sizeof_shv_logprobs_args)
 }
 
 // QSAArgs are the fields of shv_qsa_index_args (indexerAt / selected / topK, llm/attn.go:247-443).

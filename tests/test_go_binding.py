@@ -33,7 +33,7 @@ BLOCKS = re.findall(r"var a C\.(shv_\w+_args)\n(.*?)\n}", GO, re.S)
 
 def test_the_blocks_are_found():
     names = {n for n, _ in BLOCKS}
-    assert {"shv_gemv_q4k_args", "shv_attn_decode_args", "shv_qsa_index_args", "shv_attn_tree_args"} <= names
+    assert {"shv_page_plan_args", "shv_attn_paged_args", "shv_logprobs_args", "shv_gemv_q4k_args", "shv_attn_decode_args", "shv_qsa_index_args", "shv_attn_tree_args"} <= names
 
 
 @pytest.mark.parametrize("name,body", BLOCKS, ids=[n for n, _ in BLOCKS])
@@ -64,6 +64,13 @@ def test_what_a_constructor_sets_is_what_the_header_names(name, body):
             cast = re.match(r"C\.(int32_t|int64_t|uint32_t|float)\(", value)
             if cast:
                 assert fields[f] == cast.group(1), (name, f, fields[f], value)
+
+
+@pytest.mark.parametrize("name", ["shv_page_plan_args", "shv_attn_paged_args", "shv_logprobs_args"])
+def test_every_field_of_the_paged_ops_is_set(name):
+    body = dict(BLOCKS)[name]
+    missing = [f for f in _fields(name) if f != "reserved" and not re.search(r"\ba\.%s\b" % f, body)]
+    assert not missing
 
 
 def test_ops_named_in_go_are_the_headers():

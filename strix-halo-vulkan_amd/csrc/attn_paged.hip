@@ -33,6 +33,9 @@ constexpr int ring_bytes(int waves) { return waves * (16 << 10); }
 // Weights are e^(s - m) 2^kLift, and m stands until a score is more than kSlack powers of two above it: up to 2^15.9, which the larger half holds, and down to
 // 2^-35 of the largest with the smaller half's last place, to which it is rounded.
 constexpr float kLift = 11.f, kSlack = 4.9f;
+// Maxima, in powers of two, from which a weight is formed from the difference of the scores as they are: roundings of scaled scores past 2^24, which norm weights of 1500 reach with 256
+// dims, would send it past binary16.  Always formed so, a chunk of 512 among 23 tokens takes 306 us for 294, and a prompt of 4096 264 for 266: 128 dims have no registers for it.
+constexpr float kFar = 1024.f;
 // Tiles of few query rows whose cost a block gets at least, and quarters of a tile more by every further 16 query rows, whose records cost more than what their tiles' split gains:
 // one token of 256 dims behind 900 takes 19.4 us with two and 20.4 with three, 37 rows of rep 8 behind 3001 34.4 with two and 29.4 with the quarters, 64 of 128 dims behind
 // 3000 40.3 and 38.
@@ -697,6 +700,7 @@ __device__ __forceinline__ void run_piece(const shv_attn_paged_args &a, const Pl
     __builtin_amdgcn_sched_barrier(0);
     float4_t o[G][DB];
     float m_run[G], l_run[G];  // of the scores as they are, before their scale; the sums of a lane's own cells
+    bool far = false;          // a maximum is past kFar
     uint32_t saw = 0;          // bit g: one of the lane's cells is one that its row sees
 #pragma unroll
     for (int g = 0; g < G; g++) {
@@ -783,6 +787,7 @@ __device__ __forceinline__ void run_piece(const shv_attn_paged_args &a, const Pl
                 const float alpha = m_new == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((m_run[g] - m_new) * c2);
                 l_run[g] *= alpha;
                 m_run[g] = m_new;
+                far |= __ballot(moves && fabsf(mx) * c2 > kFar) != 0ull;
                 float av[4];
                 int l = lane;
                 asm volatile("" : "+v"(l));
@@ -793,14 +798,27 @@ __device__ __forceinline__ void run_piece(const shv_attn_paged_args &a, const Pl
 #pragma unroll
                     for (int e = 0; e < 4; e++) o[g][db][e] *= av[e];
             }
-            // the difference first: of scores past 2^24 their scaled values' roundings alone would send a weight past binary16
-            const float m0 = m_run[g] == -INFINITY ? 0.f : m_run[g];
+        }
+        if (__builtin_expect(far, 0)) {
+            // (the difference first)
 #pragma unroll
-            for (int e = 0; e < 8; e++) {
-                s[e] = __builtin_amdgcn_exp2f(fmaf(s[e] - m0, c2, kLift));
-                l_run[g] += s[e];
+            for (int g = 0; g < G; g++) {
+                const float m0 = m_run[g] == -INFINITY ? 0.f : m_run[g];
+#pragma unroll
+                for (int e = 0; e < 8; e++) pv[g][e] = __builtin_amdgcn_exp2f(fmaf(pv[g][e] - m0, c2, kLift));
+            }
+        } else {
+#pragma unroll
+            for (int g = 0; g < G; g++) {
+                const float m2 = fmaf(m_run[g] == -INFINITY ? 0.f : m_run[g], c2, -kLift);
+#pragma unroll
+                for (int e = 0; e < 8; e++) pv[g][e] = __builtin_amdgcn_exp2f(fmaf(pv[g][e], c2, -m2));
             }
         }
+#pragma unroll
+        for (int g = 0; g < G; g++)
+#pragma unroll
+            for (int e = 0; e < 8; e++) l_run[g] += pv[g][e];
         if (part) {
             // a value that is not finite would meet the weight 0 of rows that do not see it: such a tile is multiplied by hand
             uint32_t odd = 0;

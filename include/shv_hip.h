@@ -776,6 +776,8 @@ typedef struct {
  * pages that a window has passed may be taken out.  A row that sees nothing has zeros.  A cell that a row does not see may hold anything;
  * of one that it sees an infinite key or value may leave not a number where the formula leaves an infinity or, of a weight of zero, nothing.
  * out [max_rows][n_head*head_dim], before the sigmoid gate.  A query's values, normed and rotated, lie within binary16's range (norm weights up to 2000 keep them there).
+ * Queries enter to 22 bits, weights to 22 bits and no finer than 2^-35 of the largest: beside a cell that leads by 2^24 another's weight is off by up to 2^-12 of itself, and a mean of thousands
+ * of them by about 4e-6.
  * A sequence whose start is out of order or past max_rows, or whose positions are not within 0 .. max_pages * page - 1, gets no output.
  * work: work_bytes of scratch, 16-byte aligned, as many as shv_attn_paged_work says for these sizes; a call uses it alone, calls of one stream may share it.
  * max_rows * (n_head / n_head_kv) is at most 2^20, max_rows * n_head_kv at most 2^25. */
@@ -807,7 +809,7 @@ typedef struct {
  *   top_ids, top_logprobs [n_rows][n_top]: the n_top (at most SHV_LOGPROBS_MAX_TOP and n; 0: none) largest logits' places in falling order, of equal ones the lower place first,
  *   and their log probabilities.  A logit that is not a number is never among them (where too few others are left, the place is -1 and the log probability -infinity).
  * A logit of -infinity is a token that cannot come: it adds nothing.  Where a logit is +infinity or not a number, or all are -infinity, log Z is not a number, and nor is what is formed from it.
- * n at most 2^30. */
+ * All n_rows rows are read and answered: where fewer are in use the others' results mean nothing.  n at most 2^30. */
 #define SHV_LOGPROBS_MAX_TOP 64
 typedef struct {
     const float *logits;

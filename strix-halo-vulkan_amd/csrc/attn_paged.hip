@@ -26,8 +26,8 @@ using namespace shv;
 constexpr int kTile = 32;  // cells of a tile of V
 constexpr int kMaxSeqs = SHV_PAGE_MAX_SEQS;
 constexpr int kChunk = 64 * 16;
-// Waves of a block: two of four share a unit, or one of eight has it (is_wide).  96 tokens in a window of 2048, 128 dims, take 170 us with two and 204 with one, 24 behind up to
-// 12000 147 and 169, a chunk of 512 among 23 tokens 235 and 275, 48 tokens of 64 dims behind up to 6000 101 and 144.
+// Waves of a block: two of four share a unit, or one of eight has it (is_wide).  96 tokens in a window of 2048, 128 dims, take 170 us with two and 201 with one, 24 behind up to
+// 12000 146 and 166, a chunk of 512 among 23 tokens 230 and 280, 48 tokens of 64 dims behind up to 6000 100 and 154.
 constexpr int kWide = 8, kNarrow = 4;
 constexpr int ring_bytes(int waves) { return waves * (16 << 10); }
 // Weights are e^(s - m) 2^kLift, and m stands until a score is more than kSlack powers of two above it: up to 2^15.9, which the larger half holds, and down to
@@ -37,11 +37,11 @@ constexpr float kLift = 11.f, kSlack = 4.9f;
 // dims, would send it past binary16.  Always formed so, a chunk of 512 among 23 tokens takes 306 us for 294, and a prompt of 4096 264 for 266: 128 dims have no registers for it.
 constexpr float kFar = 1024.f;
 // Tiles of few query rows whose cost a block gets at least, and quarters of a tile more by every further 16 query rows, whose records cost more than what their tiles' split gains:
-// one token of 256 dims behind 900 takes 19.4 us with two and 20.4 with three, 37 rows of rep 8 behind 3001 34.4 with two and 29.4 with the quarters, 64 of 128 dims behind
-// 3000 40.3 and 38.
+// one token of 256 dims behind 900 takes 18.4 us with two and 19.4 with three, 37 rows of rep 8 behind 3001 33.9 with two and 29.1 with the quarters, 64 of 128 dims behind
+// 3000 38.8 and 37.0.
 constexpr uint32_t kLeast = 2, kLeastMore = 3;
-// Records of a query row from which a block's waves share them, at most: 200 rows of 128 dims behind 100, which have up to 9, take 38.5 us with 8 and 32.5 with 16, 8 tokens of
-// 256 dims behind up to 16000, which have up to 32, 51.7 with 16 and 57.4 with 48.
+// Records of a query row from which a block's waves share them, at most: 200 rows of 128 dims behind 100, which have up to 9, take 35.4 us with 8 and 31.4 with 16, 8 tokens of
+// 256 dims behind up to 16000, which have up to 32, 50.8 with 16 and 56.2 with 48.
 constexpr int kShareFrom = 16;
 // Query blocks that a plan holds: 2^20 query rows by 128, and a rest of each sequence.
 constexpr int kMostBlocks = (1 << 20) / 128 + kMaxSeqs;
@@ -52,7 +52,7 @@ constexpr int kFewBlocks = 1024;  // query blocks up to which the plan is made i
 template <int D>
 constexpr int kGroups = D == 256 ? 1 : 2;
 // Waves that share a group of few query rows, each with tiles of its own, so that a round in the ring is 32 KB (64 in the wide block's): 24 tokens of 128 dims behind up to
-// 12000 take 147 us with two and 155 with one, 48 of 64 dims behind up to 6000 101 with two or four and 133 with one.
+// 12000 take 146 us with two and 156 with one, 48 of 64 dims behind up to 6000 102 with two or four and 134 with one.
 template <int D, int WAVES>
 constexpr int kTurns = WAVES == kWide ? 2 : 256 / D;
 constexpr int rows_of(int D, int waves) { return 16 * waves * (D == 256 ? 1 : 2); }
@@ -127,9 +127,9 @@ struct Seq {
 // ---- the plan: one block of T threads -----------------------------------------------------------
 // What a block's work costs, in tenths of a microsecond of a unit: a tile of few query rows, by its block where memory has bandwidth to spare (few_least) and by memory where all units
 // ask for such tiles (few); one of many query rows by its products, here of 16 groups; a piece its way in and out, and its rows' bytes.  Fitted to the times of blocks, then
-// turned about: of 128 dims a chunk of 512 among 23 tokens behind up to 12000 took 275 us with group 21, 278 with 20,
-// 284 with 23, 291 with 18, and with few_least 7 283, with 9 293;
-// four chunks of 500 behind 3000 208 with few_beside 8, 197 with 10, 198 with 12; of 256 forty tokens behind up to 9000 105.8 with piece 90, 108.2 with 30, 107 with 120.
+// turned about on a few batches: of 128 dims a chunk of 512 among 23 tokens behind up to 12000 takes 230 us with group 21, 232 with 20, 239 with 23, 237 with 18, and with few_least 7 238,
+// with 9 236; four chunks of 500 behind 3000 203 with few_beside 8, 192 with 10, 194 with 12; of 256 forty tokens behind up to 9000 105.8 with piece 90, 106.9 with 30, 104.8
+// with 120.  Neighbouring values are within 4 %, and another batch may have another of them best.
 struct Costs {
     int few, few_least, few_beside, group, piece, piece_group;
     __host__ __device__ __forceinline__ int tile(int groups) const { return group * groups / 16; }
@@ -203,8 +203,8 @@ __device__ __forceinline__ uint32_t wave_most(uint32_t v) {
 }
 
 // WAVE, up to 64 sequences and query blocks: each wave makes all sums for itself and writes what the others write, without a barrier between them, up to where the blocks'
-// pieces are found.  (By a block's sums with two barriers each a call takes a microsecond more: 37 rows behind 3001 29.0
-// us for 28.0, 8 tokens behind up to 500 20.0 for 19.2.)
+// pieces are found.  (By a block's sums with two barriers each a call takes a microsecond more: 37 rows behind 3001 30.3
+// us for 29.1, 8 tokens behind up to 500 20.2 for 19.1.)
 template <bool WAVE, int T, int SEQS, int NQ>
 __device__ __forceinline__ void make_plan(const shv_attn_paged_args &a, const Plan &plan, PlanSmem<T, SEQS, NQ> &sm) {
     const int tid = threadIdx.x, rep = plan.rep, log_rows = __builtin_ctz(plan.rows);
@@ -407,10 +407,10 @@ __global__ __launch_bounds__(1024) void paged_plan_kernel(shv_attn_paged_args a,
 // ---- the rows' cells ----------------------------------------------------------------------------
 // A wave a row's cell of a KV head; with PLAN the first block makes the plan, which takes longer than few rows' cells do: 4.5 us with one row, 7 with forty, a chain of the
 // sequences' words, three sums over them, a bisection and the stores.  Many rows would be bound by the values' stores, two
-// bytes in each of a cell's lines (17.5 us for 4096 rows of two heads of 256 dims, 25 MB).
+// bytes in each of a cell's lines (18.2 us for 4096 rows of two heads of 256 dims, 25 MB, and 10 by columns).
 // Where rows are many, blocks from values_from on take the values of eight rows by 256 columns: a thread has a column, and cells side by side in a tile are one store.
-// A prompt of 2048 (two heads of 256 dims) takes 105 us with that and 108 without, one of 4096 (eight of 128) 306 and 316; four chunks whose cells begin anywhere 192 either
-// way, and 195 by 32 rows a block.
+// A prompt of 2048 (two heads of 256 dims) takes 113 us with that and 115.5 without, one of 4096 (eight of 128) 303 and 314; four chunks whose cells begin anywhere 191 either
+// way.
 constexpr int kValuesRows = 8;
 constexpr int kValuesFrom = 512;  // rows: below, the plan takes as long as the cells
 __device__ __forceinline__ bool has_cell(const shv_attn_paged_args &a, const Plan &plan, int r, int p, int cell) {
@@ -494,8 +494,8 @@ __global__ __launch_bounds__(256) void paged_cells_kernel(shv_attn_paged_args a,
 }
 
 // ---- attention ----------------------------------------------------------------------------------
-// A tile in LDS, as loads of 1 KB leave it.  K cell by cell, so that a load takes whole rows of a head (24 tokens of 128 dims behind up to
-// 12000: 175 us, and 181 where a load takes 64 bytes of sixteen rows); the 16-byte pieces of a cell's row lie in the order
+// A tile in LDS, as loads of 1 KB leave it.  K cell by cell, so that a load takes whole rows of a head (3 % less, when this
+// kernel came to it, for 24 tokens of 128 dims behind up to 12000 than where a load takes 64 bytes of sixteen rows); the 16-byte pieces of a cell's row lie in the order
 // piece ^ turn(cell), so that the lanes of a read, (n, q) = cell 8 (n / 4) + 4 T + n % 4, piece 4 i + q, ask for different banks, whichever sixteen of them go
 // together.  V chunk db behind them: lane (n, q) = dim 16 db + n, cells 8 q ...  After S^T = K Q^T lane (n, q) then holds query row n's
 // scores of cells 8 q + 4 T + 0..3, T = 0, 1: the eight cells of its operand of the second product.
@@ -963,7 +963,7 @@ __device__ __forceinline__ void run_piece(const shv_attn_paged_args &a, const Pl
 }
 
 // Bound by memory where query rows are few (24 tokens of 128 dims behind up to 12000 read 5.5 TB/s, 40 of 256 behind up to 9000 5.0 while the kernel runs), by the
-// matrix units where they are many: a chunk of 2048 behind 8000, 128 dims, runs at 1040 TFLOP/s of products, both halves counted, where a large library product reaches 1295.
+// matrix units where they are many: a chunk of 2048 behind 8000, 128 dims, runs at 1100 TFLOP/s of products, both halves counted, where a large library product reaches 1295.
 //
 // grid: 8 * ceil(blocks / dies) * heads.  Workgroups go to the eight dies in turn; a die's KV heads are the same ones throughout, where their number
 // allows it, so that its L2 holds their cells: die x has the heads x % g, x % g + g, .. for g the power of two in their number, up to 8.
@@ -1013,7 +1013,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void paged_attn_kernel(shv_attn_page
 
 // ---- the join -----------------------------------------------------------------------------------
 // Weighted sums of the records: bound by the trips to memory (plan, records, sums) where there are few, 3.2 us for one token behind 900, and by their bytes from the other dies' writes
-// otherwise, 4 to 12 us.  A unit is 256 / D query rows of a KV head, a lane four dims.  SHARE, where a query row has many records: a block's four waves share them, otherwise each takes a unit
+// otherwise, 4 to 25 us.  A unit is 256 / D query rows of a KV head, a lane four dims.  SHARE, where a query row has many records: a block's four waves share them, otherwise each takes a unit
 // of its own.
 template <int D, bool SHARE>
 __global__ __launch_bounds__(256) void paged_join_kernel(shv_attn_paged_args a, Plan plan) {
@@ -1098,9 +1098,9 @@ int check_sizes(const shv_attn_paged_args &a) {
     return SHV_OK;
 }
 
-// Blocks of eight waves read a tile for twice the query rows, which pays where a sequence has many of them and 256 dims: a chunk of 512 behind 7500, rep 8, takes 145 us
-// with them and 151 with blocks of four, 256 behind 3000 54.7 and 57.8, 100 behind 2000 39 and 38, one token behind 900 21 and 19.  Of 128 dims a block of four has as many
-// rows already: 2048 behind 8000 take 608 and 612, and all others are better with four.  And where blocks of four could be more than a plan holds, which those of eight never are.
+// Blocks of eight waves read a tile for twice the query rows, which pays where a sequence has many of them and 256 dims: a chunk of 512 behind 7500, rep 8, takes 137 us
+// with them and 146 with blocks of four, 256 behind 3000 52.7 and 55.6, 100 behind 2000 40.6 and 35.3, one token behind 900 19.8 and 18.  Of 128 dims a block of four has as many
+// rows already: 2048 behind 8000 take 584 and 592, and all others are better with four.  And where blocks of four could be more than a plan holds, which those of eight never are.
 constexpr int kWideFrom = 2048;  // query rows of a KV head, on average over the sequences
 // Query blocks of `rows` query rows, at most: a sequence's last one may be short.
 int most_query_blocks(const shv_attn_paged_args &a, int rows) { return (a.n_seq < a.max_rows ? a.n_seq : a.max_rows) + a.max_rows * (a.n_head / a.n_head_kv) / rows; }

@@ -3,10 +3,10 @@
 // With want = ceil((pos + rows) / page): back = held - max(want, shared), need = want - held, each where above zero.  The pages given back lie behind the
 // free ones, L = free | back in order, A = |L|; sequence s's j-th new page is L[A - 1 - (taken before it) - j].  All of that is two scans over the
 // sequences, of (back, need, rows) and of what is granted, and lookups by bisection from there on.  Entries that come back and are no page are not in L: what comes back is looked at beside
-// the second scan (two passes of 48 sequences 8.6 us and 8.1 without it, of 900 22.1 and 19.0), and where some of it is none the grants are made again and places found by a scan over runs of entries.
-// Bound by the chain of trips to memory (a sequence's words, then pages, then the stores) and the scans' barriers, not by bytes: 48 sequences of a token each take 2.9 to 3.6 us
-// of the kernel's own time, 900 with 12007 rows 8 to 10.  Every block makes the scans for itself, which costs less than a launch between them and the
-// rows; a row a thread, since each is a bisection and two dependent loads (four a thread: 26 us for 19 of the 900 sequences' two passes).  The words that others
+// the second scan (two passes of 48 sequences 9.9 us and 9.0 without it, of 900 with 12007 rows 22.1 and 18.9), and where some of it is none the grants are made again and places found by a scan over runs of entries.
+// Bound by the chain of trips to memory (a sequence's words, then pages, then the stores) and the scans' barriers, not by bytes: 48 sequences of a token each take 3.1 to 4.5 us
+// of the kernel's own time, 900 with 12007 rows 9.4 to 11.4.  Every block makes the scans for itself, which costs less than a launch between them and the
+// rows; a row a thread, since each is a bisection and two dependent loads (four a thread cost the 900 sequences' two passes 7 us).  The words that others
 // still read (held, pos, n_free) are written by the block that arrives last.
 #include "scan.hpp"
 #include "shv_device.hpp"
@@ -18,13 +18,13 @@ using namespace shv;
 
 constexpr int kMaxSeqs = SHV_PAGE_MAX_SEQS;
 constexpr int kMaxRows = 1 << 20;
-// Pages a thread that could be given back, from which a call gets a block more.  200 sequences of up to 188 pages, a row each, two passes: 11.7 us with 16, 13.4 with 32 and 17 by
-// one block; with 4, where a call of 48 sequences has two blocks, that takes 10.1 instead of 9.4.
+// Pages a thread that could be given back, from which a call gets a block more.  200 sequences of up to 188 pages, a row each, two passes: 14.2 us with 16, 16.0 with 32 and 18.6 by
+// one block; 4, with which a call of 48 sequences has two blocks, gains nothing there (10.3 and 10.3).
 constexpr int kPagesFrom = 16;
 
 constexpr int kOwn = 2, kAtOnce = 4;  // entries that come back: of a sequence by its own lane, and loads of a wave on their way of the others
 
-// WAVE, up to 64 sequences: each wave makes the scans for itself and writes to LDS what the others write, without a barrier up to the last.  (48 sequences, two passes: 9.1 us, and 10.1 by a
+// WAVE, up to 64 sequences: each wave makes the scans for itself and writes to LDS what the others write, without a barrier up to the last.  (48 sequences, two passes: 10.4 us, and 11.3 by a
 // block's scans with two barriers each.)
 template <int T, bool WAVE>
 __global__ __launch_bounds__(T) void page_plan_kernel(shv_page_plan_args a, int shift, int32_t *counter) {

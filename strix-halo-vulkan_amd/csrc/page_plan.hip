@@ -3,7 +3,8 @@
 // With want = ceil((pos + rows) / page): back = held - max(want, shared), need = want - held, each where above zero.  The pages given back lie behind the
 // free ones, L = free | back in order, A = |L|; sequence s's j-th new page is L[A - 1 - (taken before it) - j].  All of that is two scans over the
 // sequences, of (back, need, rows) and of what is granted, and lookups by bisection from there on.  Entries that come back and are no page are not in L: what comes back is looked at beside
-// the second scan (two passes of 48 sequences 9.9 us and 9.0 without it, of 900 with 12007 rows 22.1 and 18.9), and where some of it is none the grants are made again and places found by a scan over runs of entries.
+// the second scan (two passes of 48 sequences 9.9 us and 9.0 without it, of 900 with 12007 rows 22.1 and 18.9), and where some of it is none the pages among it are laid
+// on the stack first and the grants made again.
 // Bound by the chain of trips to memory (a sequence's words, then pages, then the stores) and the scans' barriers, not by bytes: 48 sequences of a token each take 3.1 to 4.5 us
 // of the kernel's own time, 900 with 12007 rows 9.4 to 11.4.  Every block makes the scans for itself, which costs less than a launch between them and the
 // rows; a row a thread, since each is a bisection and two dependent loads (four a thread cost the 900 sequences' two passes 7 us).  The words that others
@@ -31,7 +32,7 @@ __global__ __launch_bounds__(T) void page_plan_kernel(shv_page_plan_args a, int 
     constexpr int kPer = T == 1024 ? kMaxSeqs / T : 1;  // sequences a thread, side by side
     __shared__ uint32_t s_start[kPer * T], s_taken[kPer * T], s_back[kPer * T];
     __shared__ int s_held[kPer * T], s_pos[kPer * T];
-    __shared__ uint32_t waves[3][T / 64], s_run[T];
+    __shared__ uint32_t waves[3][T / 64];
     __shared__ int is_last, is_odd, n_many;
     const int tid = threadIdx.x;
     static_assert(!WAVE || kPer == 1, "a lane a sequence");
@@ -74,9 +75,9 @@ __global__ __launch_bounds__(T) void page_plan_kernel(shv_page_plan_args a, int 
         }
     }
     // The r-th entry that comes back, one of sequence s.
-    const auto entry = [&](uint32_t r, int s) {
+    const auto where = [&](uint32_t r, int s) {
         const int low = s_held[s] - static_cast<int>((s + 1 < a.n_seq ? s_back[s + 1] : n_back) - s_back[s]);
-        return a.table[static_cast<size_t>(s) * a.max_pages + low + (r - s_back[s])];
+        return a.table + static_cast<size_t>(s) * a.max_pages + low + (r - s_back[s]);
     };
     const auto is_page = [&](int e) { return e >= 0 && e < a.n_pages; };
     // All of them are looked at: the first few of a sequence by its lane, the others by a wave, 64 a load.  The last loads are on their way while the grants are made.
@@ -119,8 +120,8 @@ __global__ __launch_bounds__(T) void page_plan_kernel(shv_page_plan_args a, int 
             }
         }
     }
-    uint32_t run = 0;
-    uint32_t avail = n_free + n_back, n_given = n_back, n_taken, n_rows;
+    bool stacked = false;
+    uint32_t avail = n_free + n_back, n_taken, n_rows;
     uint32_t take[kPer], gets[kPer];
     for (bool again = false;; again = true) {
         uint32_t both[2] = {0, 0}, total2[2];
@@ -164,20 +165,33 @@ __global__ __launch_bounds__(T) void page_plan_kernel(shv_page_plan_args a, int 
             odd = is_odd != 0;
         }
         if (!odd || again) break;
-        // what is a page among a run of them, a run a thread, and before it
-        run = (n_back + T - 1) / T;
-        uint32_t v[1] = {0}, all[1], end = 0;
-        int s = 0;
-        for (uint32_t r = min(tid * run, n_back); r < min((tid + 1) * run, n_back); r++) {
-            if (r >= end) {
-                s = last_not_above(s_back, a.n_seq, r);
-                end = s + 1 < a.n_seq ? s_back[s + 1] : n_back;
+        // what is a page among a run of them, a run a thread, goes to the stack before any is taken (by every block, the same to the same place)
+        const uint32_t run = (n_back + T - 1) / T, r0 = min(tid * run, n_back), r1 = min(r0 + run, n_back);
+        uint32_t v[1], all[1], at = 0, n_given = 0;
+        for (bool put = false;; put = true) {
+            for (uint32_t r = r0; r < r1;) {
+                const int s = last_not_above(s_back, a.n_seq, r);
+                const int32_t *of = where(r, s);
+                const uint32_t n = min(r1, s + 1 < a.n_seq ? s_back[s + 1] : n_back) - r;
+                for (uint32_t i = 0; i < n; i += kAtOnce) {
+                    int e[kAtOnce];
+#pragma unroll
+                    for (int j = 0; j < kAtOnce; j++) e[j] = i + j < n ? of[i + j] : -1;
+#pragma unroll
+                    for (int j = 0; j < kAtOnce; j++)
+                        if (is_page(e[j])) {
+                            if (put && at < n_given) a.free_pages[n_free + at] = e[j];
+                            at++;
+                        }
+                }
+                r += n;
             }
-            v[0] += is_page(entry(r, s));
+            if (put) break;
+            v[0] = at;
+            block_scan<T, 1>(v, all, waves);
+            at = v[0], n_given = min(all[0], a.n_pages - n_free), avail = n_free + n_given;
         }
-        block_scan<T, 1>(v, all, waves);
-        s_run[tid] = v[0];
-        n_given = all[0], avail = n_free + n_given;
+        stacked = true;
     }
     if (blockIdx.x == 0) {
         for (int s = tid; s < a.n_seq; s += T) {
@@ -186,18 +200,9 @@ __global__ __launch_bounds__(T) void page_plan_kernel(shv_page_plan_args a, int 
         }
         if (tid == 0) a.start[a.n_seq] = n_rows;
     }
-    const auto given_back = [&](uint32_t i) {
-        if (n_given == n_back) return entry(i, last_not_above(s_back, a.n_seq, i));
-        const int of = last_not_above(s_run, T, i);
-        uint32_t r = of * run, left = i - s_run[of];
-        for (;; r++) {
-            const int e = entry(r, last_not_above(s_back, a.n_seq, r));
-            if (r + 1 >= n_back || (is_page(e) && left-- == 0)) return e;
-        }
-    };
     const auto taken = [&](uint32_t e) {  // the e-th page from the top
         const uint32_t i = avail - 1 - e;
-        return i < n_free ? a.free_pages[i] : given_back(i - n_free);
+        return i < n_free || stacked ? a.free_pages[i] : *where(i - n_free, last_not_above(s_back, a.n_seq, i - n_free));
     };
     const uint32_t step = gridDim.x * T, me = blockIdx.x * T + tid;
     for (uint32_t t = me; t < n_rows; t += step) {
@@ -213,7 +218,8 @@ __global__ __launch_bounds__(T) void page_plan_kernel(shv_page_plan_args a, int 
         const int s = last_not_above(s_taken, a.n_seq, e);
         a.table[static_cast<size_t>(s) * a.max_pages + s_held[s] + (e - s_taken[s])] = taken(e);
     }
-    for (uint32_t r = me; r < n_given && n_free + r < static_cast<uint32_t>(a.n_pages); r += step) a.free_pages[n_free + r] = given_back(r);
+    if (!stacked)
+        for (uint32_t r = me; r < n_back && n_free + r < static_cast<uint32_t>(a.n_pages); r += step) a.free_pages[n_free + r] = *where(r, last_not_above(s_back, a.n_seq, r));
     if (gridDim.x > 1) {
         if (!arrive_last(counter, gridDim.x, &is_last)) return;
     } else if (WAVE) {

@@ -221,3 +221,61 @@ def test_scores_of_the_largest_norm_weights(ctx, monkeypatch, layout, norm, n, p
             low, high = (v[lead[s]], v[lead[s]]) if leads else (v.min(0), v.max(0))
             assert np.isfinite(got).all(), (s, i)
             assert (got >= low[:, None] - tol).all() and (got <= high[:, None] + tol).all(), (s, i)
+
+
+@pytest.mark.parametrize("n_seq", [1, 3, 70])
+def test_long_sequences_of_a_window_end(ctx, monkeypatch, n_seq):
+    """Sequences of thirty thousand pages of which a window has left a few: as they end those come back, and others take them."""
+    monkeypatch.setattr(P, "plan", plan_of_pages)
+    t = G.Plan(n_seq + 3, n_seq, 32, 31000, 0, 3, 5000, odd=False, shared=False)
+    long = np.arange(n_seq) % 3 == 0
+    t.pos[long], t.held[long] = 32 * 30000 - 7, 30000
+    t.n_pages = 66 * n_seq + 20
+    order = t.rng.permutation(t.n_pages).astype(np.int32)
+    t.table[long] = -1
+    for k, s in enumerate(np.flatnonzero(long)):
+        t.table[s, [0, *range(30000 - 64, 30000)]] = order[65 * k:65 * k + 65]
+    t.free = np.concatenate([order[-3:], np.full(t.n_pages - 3, -77, np.int32)])
+    t.upload(ctx)
+    rows = np.where(long, -1, 5000 // max(1, int((~long).sum()))).astype(np.int32)
+    for step in range(2):
+        t.d["rows"].write(rows)
+        ctx.enqueue(A.OP_PAGE_PLAN, t.args())
+        w = t.check(rows, [np.full(5000, -5, np.int32) if step == 0 else t.d["maps"][k].read(np.int32, 5000) for k in range(3)])
+        rows = np.where(long, 40, -1).astype(np.int32)
+    assert w["n_free"] + w["held"].sum() == 65 * long.sum() + 3
+
+
+@pytest.mark.parametrize("layout", [(16, 2, 256, 0), (12, 2, 128, 0), (8, 8, 64, 0)])
+@pytest.mark.parametrize("n,pos", [([1, 1], [400, 31]), ([40, 1], [500, 90]), ([300], [480])])
+def test_rows_of_large_and_of_ordinary_scores_together(ctx, monkeypatch, layout, n, pos):
+    """Keys that grow along the sequence: rows of every second head meet ever larger scores, past 2^24 powers of two at the end, and take the last cell; the others, at right angles to
+    the keys, meet ordinary ones beside them in the same group of rows."""
+    monkeypatch.setitem(G.LAYOUTS, "own", layout)
+    t = G.Paged(900 + n[0], "own", n, pos, 64)
+    u = np.sign(t.rng.standard_normal(t.d)).astype(np.float32)
+    across = u.copy()
+    across[8 + (t.d - 8) // 2:] *= -1  # half of the dims behind the first eight
+    t.q_norm[:] = t.k_norm[:] = 2000
+    q = t.qkv[:, :2 * t.nh * t.d].reshape(-1, t.nh, 2, t.d)
+    q[:, ::2, 0], q[:, 1::2, 0] = u, across
+    own = t.qkv[:, 2 * t.nh * t.d:2 * t.nh * t.d + t.nkv * t.d].reshape(-1, t.nkv, t.d)
+    own[:] = -u
+    few = (0.03 * t.rng.standard_normal(t.kp.shape)).astype(np.float16)
+    for s in range(len(n)):
+        where = t.cells(s, 0, pos[s])
+        grown = (np.round(2000 * (np.arange(pos[s]) + 1) / pos[s])[:, None, None] * u).astype(np.float16)
+        t.kp[where] = np.where(np.arange(t.d) < 8, few[where], grown)
+    t.upload(ctx)
+    ctx.enqueue(A.OP_ATTN_PAGED, t.args(ctx))
+    out, _, vp = t.results()
+    for s in range(len(n)):
+        seen = vp[t.cells(s, 0, pos[s] + n[s])].astype(np.float64)
+        for i in range(n[s]):
+            v = seen[:pos[s] + i + 1]
+            got = out[t.start[s] + i].reshape(t.nh, t.d)
+            tol = 1e-5 * np.abs(v).max()
+            kv = np.arange(t.nh) // (t.nh // t.nkv)
+            assert np.isfinite(got).all(), (s, i)
+            assert (np.abs(got - v[pos[s] - 1][kv])[::2] <= tol).all(), (s, i)
+            assert (got >= v.min(0)[kv] - tol).all() and (got <= v.max(0)[kv] + tol).all(), (s, i)
